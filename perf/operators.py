@@ -223,8 +223,7 @@ def run(state):
 
 def _own_prompt(s):
     out = torch.empty(s["q"].shape, dtype=s["q"].dtype, device=DEV)
-    _bb().prompt_attention(s["q"], s["k"], s["v"], s["cu"], s["max_len"], out, scale=s["scale"],
-                           causal=s["case"]["causal"])
+    _bb().prompt_attention(s["q"], s["k"], s["v"], s["cu"], out, scale=s["scale"], causal=s["case"]["causal"])
     return out
 
 
@@ -232,8 +231,8 @@ def _own_paged(s):
     bb = _bb()
     out = torch.empty_like(s["q"])
     bb.paged_append(s["k"], s["v"], s["k_cache"], s["v_cache"], s["table"], s["cu"], s["ctx"])
-    bb.paged_attention(s["q"], s["k_cache"], s["v_cache"], s["table"], s["cu"], s["ctx"], s["max_q"], s["max_ctx"],
-                       out, scale=s["scale"])
+    bb.paged_attention(s["q"], s["k_cache"], s["v_cache"], s["table"], s["cu"], s["ctx"], s["max_ctx"], out,
+                       scale=s["scale"])
     return {"out": out, "k_cache": s["k_cache"], "v_cache": s["v_cache"]}
 
 
