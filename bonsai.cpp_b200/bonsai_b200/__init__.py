@@ -62,6 +62,12 @@ SIGNATURES = {
     "bonsai_ln_modulate_f32": (_c_int, [_vp, _c_int, _c_int, _vp, _vp, _fp, _vp, _vp]),
     "bonsai_joint_attention": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _fp, _vp, _c_ll, _vp]),
     "bonsai_qk_norm_rope": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _vp, _c_int, _fp, _vp, _vp, _vp]),
+    "bonsai_prompt_attention": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                         _c_int, _c_int, _fp, _vp, _vp]),
+    "bonsai_paged_append": (_c_int, [_vp, _vp, _vp, _vp, _vp, _c_ll, _c_int, _vp, _vp, _c_int, _c_int,
+                                     _c_int, _c_int, _vp]),
+    "bonsai_paged_attention": (_c_int, [_vp, _vp, _vp, _vp, _c_ll, _c_int, _vp, _vp, _c_int, _c_int,
+                                        _c_int, _c_int, _c_int, _c_int, _c_int, _fp, _vp, _vp]),
     "bonsai_dit_create": (_c_int, [_vp, ctypes.POINTER(_vp)]),
     "bonsai_dit_destroy": (_c_int, [_vp]),
     "bonsai_dit_forward": (_c_int, [_vp, _vp, _vp, _vp, _fp, _vp, _vp]),
@@ -252,6 +258,112 @@ def joint_attention(q, k, v, out, scale=None, stream=None) -> None:
                                        float(scale if scale is not None else D ** -0.5),
                                        out.data_ptr(), out.stride(0), stream_ptr(stream)),
           "bonsai_joint_attention")
+
+
+# ----------------------------------------------------------------- text stage
+class HeadsDesc(ctypes.Structure):
+    """bonsai_heads_t: a 16-bit [token][head][dim] tensor with strides."""
+    _fields_ = [("data", _vp), ("stride_token", _c_ll), ("stride_head", _c_ll)]
+
+
+class PagesDesc(ctypes.Structure):
+    """bonsai_pages_t: one side of a paged cache [page][slot][head][dim]."""
+    _fields_ = [("data", _vp), ("stride_page", _c_ll), ("stride_token", _c_ll), ("stride_head", _c_ll),
+                ("n_pages", _c_int), ("page_size", _c_int)]
+
+
+def _text_dtype(*tensors) -> int:
+    import torch
+    dt, dev = tensors[0].dtype, torch.device("cuda", torch.cuda.current_device())
+    if dt not in (torch.float16, torch.bfloat16):
+        raise BonsaiError(f"text attention takes f16 or bf16 tensors, got {dt}")
+    for t in tensors:
+        if t.dtype != dt or t.device != dev:
+            raise BonsaiError(f"tensors must all be {dt} on {dev}, got {t.dtype} on {t.device}")
+        if t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise BonsaiError("the last dimension of a tensor of heads must be contiguous")
+    return 1 if dt == torch.bfloat16 else 0
+
+
+def _text_ints(**tensors):
+    import torch
+    dev = torch.device("cuda", torch.cuda.current_device())
+    for name, t in tensors.items():
+        if t.dtype != torch.int32 or t.device != dev or (t.numel() > 1 and t.stride(-1) != 1):
+            raise BonsaiError(f"{name} must be int32 with unit stride on {dev}")
+
+
+def _heads(t) -> HeadsDesc:
+    return HeadsDesc(t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def _pages(t) -> PagesDesc:
+    return PagesDesc(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2), t.shape[0], t.shape[1])
+
+
+def _same(what, *shapes):
+    if any(s != shapes[0] for s in shapes):
+        raise BonsaiError(f"{what} do not match: {[tuple(s) for s in shapes]}")
+
+
+def prompt_attention(q, k, v, cu_seqlens, out, scale=None, causal=True, stream=None) -> None:
+    """Attention over packed prompts: q, out [T][H][D], k, v [T][Hkv][D] (f16 or
+    bf16, any token / head strides that are multiples of 8), cu_seqlens cuda
+    int32 [n + 1]; sequence s has the rows [cu_seqlens[s], cu_seqlens[s + 1])."""
+    dt = _text_dtype(q, k, v, out)
+    _text_ints(cu_seqlens=cu_seqlens)
+    _same("q and out", q.shape, out.shape)
+    _same("k and v", k.shape, v.shape)
+    if k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+        raise BonsaiError(f"k {tuple(k.shape)} does not fit q {tuple(q.shape)}")
+    T, H, D = q.shape
+    check(lib().bonsai_prompt_attention(
+        ctypes.byref(_heads(q)), ctypes.byref(_heads(k)), ctypes.byref(_heads(v)), cu_seqlens.data_ptr(),
+        cu_seqlens.numel() - 1, T, H, k.shape[1], D, dt, int(bool(causal)),
+        float(scale if scale is not None else D ** -0.5), ctypes.byref(_heads(out)), stream_ptr(stream)),
+        "bonsai_prompt_attention")
+
+
+def _table_args(page_table, cu_q, ctx_lens):
+    _text_ints(page_table=page_table, cu_q=cu_q, ctx_lens=ctx_lens)
+    n = ctx_lens.numel()
+    if cu_q.numel() != n + 1 or page_table.dim() != 2 or page_table.shape[0] != n:
+        raise BonsaiError(f"page_table {tuple(page_table.shape)}, cu_q [{cu_q.numel()}] and ctx_lens [{n}] do not match")
+    return n
+
+
+def paged_append(k, v, k_cache, v_cache, page_table, cu_q, ctx_lens, stream=None) -> None:
+    """Write new keys / values [T][Hkv][D] into the cache [pages][page_size][Hkv][D]:
+    token i of sequence s (rows [cu_q[s], cu_q[s + 1])) goes to place
+    ctx_lens[s] - q_len + i of its page_table row [n][width]."""
+    _text_dtype(k, v, k_cache, v_cache)
+    n = _table_args(page_table, cu_q, ctx_lens)
+    _same("k and v", k.shape, v.shape)
+    _same("heads of k and of the caches", k.shape[1:], k_cache.shape[2:], v_cache.shape[2:])
+    check(lib().bonsai_paged_append(
+        ctypes.byref(_heads(k)), ctypes.byref(_heads(v)), ctypes.byref(_pages(k_cache)),
+        ctypes.byref(_pages(v_cache)), page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
+        cu_q.data_ptr(), ctx_lens.data_ptr(), n, k.shape[0], k.shape[1], k.shape[2], stream_ptr(stream)),
+        "bonsai_paged_append")
+
+
+def paged_attention(q, k_cache, v_cache, page_table, cu_q, ctx_lens, max_ctx, out, scale=None,
+                    stream=None) -> None:
+    """Causal attention of new tokens q [T][H][D] over the paged cache
+    [pages][page_size][Hkv][D], the new tokens' own keys appended before;
+    max_ctx: an upper bound of ctx_lens (only sets how the work is split)."""
+    dt = _text_dtype(q, k_cache, v_cache, out)
+    n = _table_args(page_table, cu_q, ctx_lens)
+    _same("q and out", q.shape, out.shape)
+    T, H, D = q.shape
+    if k_cache.shape[3] != D or v_cache.shape[3] != D:
+        raise BonsaiError(f"caches of head_dim {k_cache.shape[3]} / {v_cache.shape[3]} do not fit q {tuple(q.shape)}")
+    _same("heads of the caches", k_cache.shape[2:3], v_cache.shape[2:3])
+    check(lib().bonsai_paged_attention(
+        ctypes.byref(_heads(q)), ctypes.byref(_pages(k_cache)), ctypes.byref(_pages(v_cache)),
+        page_table.data_ptr(), page_table.stride(0), page_table.shape[1], cu_q.data_ptr(), ctx_lens.data_ptr(),
+        n, T, int(max_ctx), H, k_cache.shape[2], D, dt, float(scale if scale is not None else D ** -0.5),
+        ctypes.byref(_heads(out)), stream_ptr(stream)), "bonsai_paged_attention")
 
 
 # ----------------------------------------------------------------- host side

@@ -164,6 +164,32 @@ int launch_attention(const __half* q, const __half* k, const __half* v, int n_he
                      int head_dim, float scale, __half* out, long long ld_out, cudaStream_t st,
                      const RowRoutes* routes = nullptr);
 
+// -------------------------------------------------------- text attention
+// A 16-bit tensor of heads: element (token, head, d) at data + token * token
+// stride + head * head stride + d (elements); `page`: stride of a page of a
+// paged cache.
+struct TextTensor {
+  void* data = nullptr;
+  long long page = 0, token = 0, head = 0;
+};
+struct TextAttention {
+  TextTensor q, k, v, out;
+  const int* cu = nullptr;     // device [n_seqs + 1]
+  const int* ctx = nullptr;    // device [n_seqs] (paged)
+  const int* table = nullptr;  // device [n_seqs][table_ld] (paged; null: packed k and v)
+  long long table_ld = 0;
+  int table_width = 0, page_shift = 0, n_pages = 0;
+  int n_seqs = 0, total_q = 0, max_ctx = 0;
+  int n_heads = 0, n_kv = 0, head_dim = 0;
+  bool bf16 = false, causal = true;
+  float scale = 0.f;
+};
+int launch_text_attention(const TextAttention& a, cudaStream_t st);
+int launch_paged_append(const TextTensor& k, const TextTensor& v, const TextTensor& kc, const TextTensor& vc,
+                        const int* table, long long table_ld, int table_width, int page_shift, int n_pages,
+                        const int* cu, const int* ctx, int n_seqs, int total, int n_kv, int head_dim,
+                        cudaStream_t st);
+
 // ------------------------------------------------------------ pointwise
 int launch_f32_to_f16(const float* src, __half* dst, long long n, cudaStream_t st);
 int launch_ln_modulate_f16(const float* x, int rows, int dim, const float* shift,

@@ -240,6 +240,80 @@ int bonsai_qk_norm_rope(uint16_t* qk, int n_heads, int seq, int head_dim, const 
                         const float* w_hi, int split, float eps, const float* cos_t,
                         const float* sin_t, void* stream);
 
+/* ------------------------------------------------------ text stage
+ * Attention for the decoder-style text encoder in front of the diffuser
+ * (the reference runs that stage through llama.cpp): whole prompts of many
+ * requests, and new tokens over a paged key/value cache. */
+
+#define BONSAI_DTYPE_F16 0
+#define BONSAI_DTYPE_BF16 1
+
+/* A 16-bit tensor of heads: element (token, head, d) is at
+ * data + token * stride_token + head * stride_head + d (strides in elements).
+ * data is 16-byte aligned; strides are positive multiples of 8 (the stride
+ * of a dimension of size one is not looked at). */
+typedef struct {
+  void* data;
+  long long stride_token, stride_head;
+} bonsai_heads_t;
+
+/* One side (keys or values) of a paged cache: n_pages pages of page_size
+ * tokens, element (page, slot, head, d) at data + page * stride_page +
+ * slot * stride_token + head * stride_head + d.  page_size is a power of two
+ * from 8 to 65536; alignment as in bonsai_heads_t. */
+typedef struct {
+  void* data;
+  long long stride_page, stride_token, stride_head;
+  int n_pages, page_size;
+} bonsai_pages_t;
+
+/* Attention over whole prompts, packed one after another: sequence s has the
+ * rows [cu_seqlens[s], cu_seqlens[s + 1]) of q, k, v and out (device int32
+ * [n_seqs + 1], ascending; lengths may be zero; at most 8192 sequences).
+ * Query head h reads key/value head h / (n_heads / n_kv_heads).  causal != 0:
+ * a token sees its own sequence up to itself; 0: all of its sequence.
+ *   out[t][h] = sum_j softmax_j(scale * q[t][h] . k[j]) v[j]
+ * f16 or bf16 (dtype), f32 scores, statistics and sums; P is rounded to the
+ * tensors' type for the tensor cores.  head_dim 64 or 128; n_heads a multiple
+ * of n_kv_heads, at most 128 query heads to one; scale > 0.  Rows of out that
+ * belong to no sequence are not written.  A non-finite value reaches only the
+ * rows that see its token. */
+int bonsai_prompt_attention(const bonsai_heads_t* q, const bonsai_heads_t* k,
+                            const bonsai_heads_t* v, const int* cu_seqlens, int n_seqs,
+                            int total_tokens, int n_heads, int n_kv_heads, int head_dim, int dtype,
+                            int causal, float scale, const bonsai_heads_t* out, void* stream);
+
+/* Write the packed new keys and values (rows [cu_q[s], cu_q[s + 1]) of k and
+ * v belong to sequence s) into the cache: with ctx_lens[s] tokens in the
+ * sequence, the new ones included, new token i goes to place
+ * ctx_lens[s] - q_len + i, which is slot place % page_size of page
+ * page_table[s][place / page_size].  page_table: device int32, rows
+ * table_ld apart, table_width entries each.  Places before 0 or past the
+ * table, and page indices outside [0, n_pages), are not written.  Works for
+ * any 16-bit type.  Two places of one call must not share a slot. */
+int bonsai_paged_append(const bonsai_heads_t* k, const bonsai_heads_t* v,
+                        const bonsai_pages_t* k_cache, const bonsai_pages_t* v_cache,
+                        const int* page_table, long long table_ld, int table_width,
+                        const int* cu_q, const int* ctx_lens, int n_seqs, int total_q,
+                        int n_kv_heads, int head_dim, void* stream);
+
+/* Causal attention of the new tokens of each sequence (packed as in
+ * bonsai_paged_append, one token or a chunk) over its ctx_lens[s] cached
+ * tokens, the new ones included (append them first): new token i sees the
+ * places up to ctx_lens[s] - q_len + i.  A row that sees nothing is zero.
+ * Cache contents past a sequence's length are never used, whatever they are;
+ * page indices outside [0, n_pages) read as zeros; ctx_lens past the table
+ * are cut to it.  max_ctx: an upper bound of ctx_lens, which only sets how
+ * the work is split (partial results in stream-ordered scratch, merged in a
+ * fixed order): a wrong one costs time, not correctness.  Types, heads and
+ * scale as in bonsai_prompt_attention. */
+int bonsai_paged_attention(const bonsai_heads_t* q, const bonsai_pages_t* k_cache,
+                           const bonsai_pages_t* v_cache, const int* page_table,
+                           long long table_ld, int table_width, const int* cu_q,
+                           const int* ctx_lens, int n_seqs, int total_q, int max_ctx, int n_heads,
+                           int n_kv_heads, int head_dim, int dtype, float scale,
+                           const bonsai_heads_t* out, void* stream);
+
 /* ------------------------------------------------------ whole model */
 
 /* Model presets.  KLEIN4B = the reference's compiled-in DiffuserParams
