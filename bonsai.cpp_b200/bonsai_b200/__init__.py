@@ -54,6 +54,10 @@ SIGNATURES = {
     "bonsai_b1_linear_f32": (_c_int, [_vp, _c_int, _vp, _vp, _vp]),
     "bonsai_b1_linear_f32_noalloc": (_c_int, [_vp, _c_int, _vp, _vp, _vp]),
     "bonsai_b1_gemm": (_c_int, [_vp, _c_ll, _c_int, _vp, _c_int, _vp, _c_ll, _vp, _vp]),
+    "bonsai_lora_create": (_c_int, [_c_int, _c_int, _c_int, _c_int, _c_int, ctypes.POINTER(_vp)]),
+    "bonsai_lora_set": (_c_int, [_vp, _c_int, _vp, _vp, _c_int, _fp, _vp]),
+    "bonsai_lora_free": (_c_int, [_vp]),
+    "bonsai_b1_gemm_lora": (_c_int, [_vp, _c_ll, _c_int, _vp, _c_int, _vp, _c_ll, _vp, _vp, _vp, _vp, _c_int, _vp]),
     "bonsai_rope_2d_f32": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _vp]),
     "bonsai_rope_tables": (_c_int, [_vp, _c_int, _c_int, _vp, _fp, _vp, _vp, _vp]),
     "bonsai_rms_norm_f32": (_c_int, [_vp, _vp, _c_int, _c_int, _fp, _vp, _vp]),
@@ -211,6 +215,59 @@ def b1_gemm(x16, w: B1Weight, mode: int, out, gate=None, stream=None) -> None:
                                out.data_ptr(), out.stride(0),
                                gate.data_ptr() if gate is not None else None,
                                stream_ptr(stream)), "bonsai_b1_gemm")
+
+
+class LoraSet:
+    """Low-rank adapters for one B1_0 projection of out_dim x in_dim: n_slots
+    slots of rank <= max_rank (swiglu_from as the B1Weight's)."""
+
+    def __init__(self, out_dim: int, in_dim: int, max_rank: int, n_slots: int, swiglu_from: int = -1):
+        h = _vp()
+        check(lib().bonsai_lora_create(out_dim, in_dim, max_rank, n_slots, swiglu_from, ctypes.byref(h)),
+              "bonsai_lora_create")
+        self.handle = h
+        self.out_dim, self.in_dim, self.max_rank, self.n_slots = out_dim, in_dim, max_rank, n_slots
+
+    def set(self, slot: int, down, up, scale: float, stream=None) -> None:
+        """down f16 [rank][in_dim], up f16 [out_dim][rank]: contiguous tensors, host
+        or cuda; y += scale * up (down x)."""
+        import torch
+        rank = down.shape[0]
+        if down.dtype != torch.float16 or up.dtype != torch.float16:
+            raise BonsaiError("adapters must be f16")
+        if tuple(down.shape) != (rank, self.in_dim) or tuple(up.shape) != (self.out_dim, rank):
+            raise BonsaiError(f"adapter {tuple(down.shape)}, {tuple(up.shape)} does not fit "
+                              f"{self.out_dim} x {self.in_dim}")
+        if not (down.is_contiguous() and up.is_contiguous()):
+            raise BonsaiError("adapters must be contiguous")
+        check(lib().bonsai_lora_set(self.handle, slot, down.data_ptr(), up.data_ptr(), rank, float(scale),
+                                    stream_ptr(stream)), "bonsai_lora_set")
+
+    def clear(self, slot: int, stream=None) -> None:
+        check(lib().bonsai_lora_set(self.handle, slot, None, None, 0, 0.0, stream_ptr(stream)), "bonsai_lora_set")
+
+    def free(self):
+        if getattr(self, "handle", None):
+            lib().bonsai_lora_free(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def b1_gemm_lora(x16, w: B1Weight, mode: int, out, lora: LoraSet, cu_tokens, slots, gate=None, stream=None) -> None:
+    """b1_gemm with each request's adapter beside it: request i has the tokens
+    [cu_tokens[i], cu_tokens[i + 1]) and the adapter slots[i] (-1: none); cuda int32."""
+    _text_ints(cu_tokens=cu_tokens, slots=slots)
+    if cu_tokens.numel() != slots.numel() + 1:
+        raise BonsaiError(f"cu_tokens [{cu_tokens.numel()}] and slots [{slots.numel()}] do not match")
+    check(lib().bonsai_b1_gemm_lora(x16.data_ptr(), x16.stride(0), x16.shape[0], w.handle, mode, out.data_ptr(),
+                                    out.stride(0), gate.data_ptr() if gate is not None else None, lora.handle,
+                                    cu_tokens.data_ptr(), slots.data_ptr(), slots.numel(), stream_ptr(stream)),
+          "bonsai_b1_gemm_lora")
 
 
 def linear_f32(x, W, bias, out, stream=None) -> None:

@@ -177,6 +177,39 @@ using namespace bonsai;
     if (_e != cudaSuccess) return cuda_status(_e, (what)); \
   } while (0)
 
+// The one segment of a b1_gemm call: its checks, and where its epilogue writes.
+static int b1_gemm_segment(const char* fn, bonsai_b1_t h, int mode, void* out, long long ld_out,
+                           const float* gate, EpiSeg* seg) {
+  const std::string at = std::string(fn) + ": ";
+  if (!out) return fail(BONSAI_ERR_ARG, at + "null output");
+  const B1Weight& w = h->w;
+  int dev = 0;
+  RC_CUDA(cudaGetDevice(&dev), (at + "cudaGetDevice").c_str());
+  if (dev != w.device)
+    return fail(BONSAI_ERR_ARG, at + "the weight lives on device " + std::to_string(w.device) +
+                                    ", the current device is " + std::to_string(dev));
+  seg->row_begin = 0;
+  seg->row_end = w.n_rows;
+  seg->dst = out;
+  seg->ld = ld_out;
+  seg->gate = gate;
+  switch (mode) {
+    case BONSAI_EPI_F32: seg->mode = EPI_F32; break;
+    case BONSAI_EPI_F16: seg->mode = EPI_F16; break;
+    case BONSAI_EPI_GELU: seg->mode = EPI_GELU_F16; break;
+    case BONSAI_EPI_RESID: seg->mode = EPI_RESID_F32; break;
+    case BONSAI_EPI_SWIGLU:
+      if (w.swiglu_from != 0)
+        return fail(BONSAI_ERR_ARG, at + "SWIGLU needs a weight uploaded with swiglu_from=0");
+      seg->mode = EPI_SWIGLU_F16;
+      break;
+    default: return fail(BONSAI_ERR_ARG, at + "unknown epilogue mode");
+  }
+  const long long need = (mode == BONSAI_EPI_SWIGLU) ? w.n_rows / 2 : w.n_rows;
+  if (ld_out < need) return fail(BONSAI_ERR_ARG, at + "ld_out smaller than the output width");
+  return 0;
+}
+
 extern "C" {
 
 const char* bonsai_last_error(void) { return g_last_error.c_str(); }
@@ -363,34 +396,30 @@ int bonsai_b1_gemm(const uint16_t* x, long long ldx, int tokens, bonsai_b1_t h, 
                    void* out, long long ld_out, const float* gate, void* stream) {
   if (!h) return fail(BONSAI_ERR_ARG, "b1_gemm: null weight handle");
   if (tokens == 0) return 0;
-  if (!out) return fail(BONSAI_ERR_ARG, "b1_gemm: null output");
-  const B1Weight& w = h->w;
-  int dev = 0;
-  RC_CUDA(cudaGetDevice(&dev), "b1_gemm: cudaGetDevice");
-  if (dev != w.device)
-    return fail(BONSAI_ERR_ARG, "b1_gemm: the weight lives on device " + std::to_string(w.device) +
-                                    ", the current device is " + std::to_string(dev));
   EpiSeg seg;
-  seg.row_begin = 0;
-  seg.row_end = w.n_rows;
-  seg.dst = out;
-  seg.ld = ld_out;
-  seg.gate = gate;
-  switch (mode) {
-    case BONSAI_EPI_F32: seg.mode = EPI_F32; break;
-    case BONSAI_EPI_F16: seg.mode = EPI_F16; break;
-    case BONSAI_EPI_GELU: seg.mode = EPI_GELU_F16; break;
-    case BONSAI_EPI_RESID: seg.mode = EPI_RESID_F32; break;
-    case BONSAI_EPI_SWIGLU:
-      if (w.swiglu_from != 0)
-        return fail(BONSAI_ERR_ARG, "b1_gemm: SWIGLU needs a weight uploaded with swiglu_from=0");
-      seg.mode = EPI_SWIGLU_F16;
-      break;
-    default: return fail(BONSAI_ERR_ARG, "b1_gemm: unknown epilogue mode");
-  }
-  const long long need = (mode == BONSAI_EPI_SWIGLU) ? w.n_rows / 2 : w.n_rows;
-  if (ld_out < need) return fail(BONSAI_ERR_ARG, "b1_gemm: ld_out smaller than the output width");
-  return launch_b1_gemm(x, ldx, tokens, w, &seg, 1, false, static_cast<cudaStream_t>(stream));
+  const int rc = b1_gemm_segment("b1_gemm", h, mode, out, ld_out, gate, &seg);
+  if (rc) return rc;
+  return launch_b1_gemm(x, ldx, tokens, h->w, &seg, 1, false, static_cast<cudaStream_t>(stream));
+}
+
+int bonsai_b1_gemm_lora(const uint16_t* x, long long ldx, int tokens, bonsai_b1_t h, int mode,
+                        void* out, long long ld_out, const float* gate, bonsai_lora_t set,
+                        const int* cu_tokens, const int* slots, int n_reqs, void* stream) {
+  if (!h || !set) return fail(BONSAI_ERR_ARG, "b1_gemm_lora: null weight or adapter handle");
+  const B1Weight& w = h->w;
+  const LoraDevice& s = set->set;
+  if (tokens < 0 || n_reqs < 0) return fail(BONSAI_ERR_ARG, "b1_gemm_lora: negative count");
+  if (s.n_rows != w.n_rows || s.k_in != w.k_in || s.swiglu_from != w.swiglu_from || s.device != w.device)
+    return fail(BONSAI_ERR_ARG, "b1_gemm_lora: the adapters were made for another shape, row order or device");
+  if (tokens == 0) return 0;
+  if (n_reqs > 0 && (!cu_tokens || !slots)) return fail(BONSAI_ERR_ARG, "b1_gemm_lora: null cu_tokens or slots");
+  if (!x || (reinterpret_cast<uintptr_t>(x) & 15) != 0 || (ldx % 8) != 0 || ldx < w.k_in)
+    return fail(BONSAI_ERR_ARG, "b1_gemm_lora: activation must be 16-byte aligned with ld % 8 == 0 and ld >= K");
+  EpiSeg seg;
+  const int rc = b1_gemm_segment("b1_gemm_lora", h, mode, out, ld_out, gate, &seg);
+  if (rc) return rc;
+  return launch_b1_gemm_lora(reinterpret_cast<const __half*>(x), ldx, tokens, w, seg, s, cu_tokens, slots, n_reqs,
+                             static_cast<cudaStream_t>(stream));
 }
 
 int bonsai_b1_linear_f32(const float* act, int tokens, bonsai_b1_t h, float* out, void* stream) {

@@ -1,0 +1,92 @@
+// C ABI of the adapter sets (include/bonsai_cuda.h).
+#include "../../include/bonsai_cuda.h"
+#include "internal.cuh"
+
+#include <cmath>
+
+using namespace bonsai;
+
+extern "C" {
+
+int bonsai_lora_create(int out_dim, int in_dim, int max_rank, int n_slots, int swiglu_from, bonsai_lora_t* out) {
+  if (!out) return fail(BONSAI_ERR_ARG, "lora_create: null output handle");
+  *out = nullptr;
+  if (out_dim <= 0 || in_dim <= 0 || n_slots <= 0) return fail(BONSAI_ERR_ARG, "lora_create: non-positive shape");
+  if (in_dim % BONSAI_B1_BLOCK_SIZE != 0) return fail(BONSAI_ERR_ARG, "lora_create: in_dim must be a multiple of 32");
+  if (max_rank < 1 || max_rank > 128) return fail(BONSAI_ERR_UNSUPPORTED, "lora_create: max_rank must be 1..128");
+  if (swiglu_from >= 0 && (swiglu_from >= out_dim || ((out_dim - swiglu_from) & 1) || (swiglu_from & 1)))
+    return fail(BONSAI_ERR_ARG, "lora_create: swiglu_from must be even and leave an even number of rows");
+  auto* h = new bonsai_lora();
+  LoraDevice& s = h->set;
+  s.n_rows = out_dim;
+  s.k_in = in_dim;
+  s.max_rank = max_rank;
+  s.r_pad = (max_rank + 15) / 16 * 16;
+  s.n_slots = n_slots;
+  s.swiglu_from = swiglu_from < 0 ? -1 : swiglu_from;
+  cudaGetDevice(&s.device);
+  const size_t down = (size_t)n_slots * s.r_pad * in_dim * sizeof(__half);
+  const size_t up = (size_t)n_slots * s.r_pad * out_dim * sizeof(__half);
+  if (cudaMalloc(reinterpret_cast<void**>(&s.down), down) != cudaSuccess ||
+      cudaMalloc(reinterpret_cast<void**>(&s.up), up) != cudaSuccess ||
+      cudaMalloc(reinterpret_cast<void**>(&s.info), n_slots * sizeof(LoraSlot)) != cudaSuccess) {
+    cudaGetLastError();
+    bonsai_lora_free(h);
+    return fail(BONSAI_ERR_NOMEM, "lora_create: device allocation failed");
+  }
+  cudaError_t e = cudaMemset(s.info, 0, n_slots * sizeof(LoraSlot));  // rank 0: every slot empty
+  if (e == cudaSuccess) e = cudaDeviceSynchronize();
+  if (e != cudaSuccess) {
+    bonsai_lora_free(h);
+    return cuda_status(e, "lora_create: clear");
+  }
+  *out = h;
+  return 0;
+}
+
+int bonsai_lora_set(bonsai_lora_t h, int slot, const uint16_t* down, const uint16_t* up, int rank, float scale,
+                    void* stream) {
+  if (!h) return fail(BONSAI_ERR_ARG, "lora_set: null handle");
+  const LoraDevice& s = h->set;
+  if (slot < 0 || slot >= s.n_slots) return fail(BONSAI_ERR_ARG, "lora_set: no such slot");
+  if (rank < 0 || rank > s.max_rank) return fail(BONSAI_ERR_ARG, "lora_set: rank outside [0, max_rank]");
+  if (rank > 0 && (!down || !up)) return fail(BONSAI_ERR_ARG, "lora_set: null adapter");
+  if (rank > 0 && !std::isfinite(scale)) return fail(BONSAI_ERR_ARG, "lora_set: scale must be finite");
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_status(e, "lora_set: cudaGetDevice");
+  if (dev != s.device) return fail(BONSAI_ERR_ARG, "lora_set: the adapters live on device " + std::to_string(s.device));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const size_t row = (size_t)s.r_pad * sizeof(__half), width = (size_t)rank * sizeof(__half);
+  __half* d = s.down + (size_t)slot * s.r_pad * s.k_in;
+  __half* u = s.up + (size_t)slot * s.r_pad * s.n_rows;
+  const LoraSlot info{rank, scale};
+  if (rank > 0) {
+    e = cudaMemsetAsync(d, 0, row * s.k_in, st);
+    if (e == cudaSuccess) e = cudaMemsetAsync(u, 0, row * s.n_rows, st);
+    if (e == cudaSuccess) e = cudaMemcpyAsync(d, down, width * s.k_in, cudaMemcpyDefault, st);
+    // rows [swiglu_from, out) go to alternating device rows: gate, value, gate, ...
+    const int plain = s.swiglu_from < 0 ? s.n_rows : s.swiglu_from, half = (s.n_rows - plain) / 2;
+    auto rows = [&](int dst_row, int dst_step, int src_row, int n) {
+      if (n > 0 && e == cudaSuccess)
+        e = cudaMemcpy2DAsync(u + (size_t)dst_row * s.r_pad, row * dst_step, up + (size_t)src_row * rank, width, width,
+                              n, cudaMemcpyDefault, st);
+    };
+    rows(0, 1, 0, plain);
+    rows(plain, 2, plain, half);
+    rows(plain + 1, 2, plain + half, half);
+  }
+  if (e == cudaSuccess) e = cudaMemcpyAsync(s.info + slot, &info, sizeof(info), cudaMemcpyDefault, st);
+  return cuda_status(e, "lora_set: copy");
+}
+
+int bonsai_lora_free(bonsai_lora_t h) {
+  if (!h) return 0;
+  cudaFree(h->set.down);
+  cudaFree(h->set.up);
+  cudaFree(h->set.info);
+  delete h;
+  return 0;
+}
+
+}  // extern "C"

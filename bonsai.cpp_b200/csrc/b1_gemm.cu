@@ -87,6 +87,7 @@ struct Params {
   // so every other role's first bounded wait expires and the kernel unwinds
   // through its abort path with no copy or MMA in flight.  0 in normal use.
   int idle_loads;
+  const float* delta;  // kDelta: f32 [tokens][n_rows] added to the accumulator
 };
 
 __device__ __forceinline__ float tanh_hw(float x) {
@@ -127,7 +128,18 @@ __device__ __forceinline__ uint32_t bf16_from_f16_scale(uint32_t s16) {
   }
 }
 
-template <bool kBF16>
+// acc[j] of weight row `row`, tokens t0 + j (j < nt) += delta.  Lanes hold
+// consecutive rows, so each token is one coalesced read per warp.
+__device__ __forceinline__ void add_delta(uint32_t (&v)[32], const float* delta, int n_rows, int row,
+                                          int t0, int nt) {
+  if (row >= n_rows) return;
+  const float* d = delta + (size_t)t0 * n_rows + row;
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    if (j < nt) v[j] = __float_as_uint(__uint_as_float(v[j]) + __ldg(d + (size_t)j * n_rows));
+}
+
+template <bool kBF16, bool kDelta>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
     b1_gemm_kernel(const __grid_constant__ CUtensorMap xmap, const Params p) {
   extern __shared__ uint8_t smem_raw[];
@@ -354,6 +366,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         tmem_wait_ld();
         const int t0 = ttile * BN + c * 32;
         const int nt = min(32, p.tokens - t0);
+        if constexpr (kDelta) add_delta(v, p.delta, p.n_rows, row, t0, nt);
         if (warp_swiglu) {
           // Rows are stored gate/value interleaved; the even lane owns the pair.
           __half* dst = reinterpret_cast<__half*>(sg.dst) + base + (size_t)t0 * stride;
@@ -452,9 +465,11 @@ struct Params {
   EpiSeg seg[kMaxSegs];
   int* err;
   int fence_sys;  // a segment stores to other GPUs: fence.sys after the epilogue's stores
+  int n_rows;
+  const float* delta;  // kDelta: f32 [tokens][n_rows] added to the accumulator
 };
 
-template <bool kBF16>
+template <bool kBF16, bool kDelta>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
     b1_gemm_pair_kernel(const __grid_constant__ CUtensorMap xmap, const Params p) {
   extern __shared__ uint8_t smem_raw[];
@@ -692,6 +707,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         tmem_wait_ld();
         const int t0 = ttile * BN + c * 32;
         const int nt = min(32, p.tokens - t0);
+        if constexpr (kDelta) {
+          if (si >= 0) add_delta(v, p.delta, p.n_rows, row, t0, nt);
+        }
         if (warp_swiglu) {
           __half* dst = reinterpret_cast<__half*>(sg.dst) + base + (size_t)t0 * stride;
           const bool own = mode == EPI_SWIGLU_F16 && (rr & 1) == 0;
@@ -998,18 +1016,24 @@ B1Kernel forced_kernel() {
   return B1Kernel::Auto;
 }
 
+auto pair_kernel(bool bf16, bool delta) {
+  return delta ? (bf16 ? gemm::pair::b1_gemm_pair_kernel<true, true> : gemm::pair::b1_gemm_pair_kernel<false, true>)
+               : (bf16 ? gemm::pair::b1_gemm_pair_kernel<true, false>
+                       : gemm::pair::b1_gemm_pair_kernel<false, false>);
+}
+
 // Largest number of co-resident pair clusters (one per TPC when every SM
 // takes one CTA of the pair kernel); 0 if the query fails.
-int pair_cluster_slots(bool bf16) {
+int pair_cluster_slots(bool bf16, bool delta) {
   struct Slots {
-    int n[2] = {-1, -1};
+    int n[4] = {-1, -1, -1, -1};
   };
   static Slots slots[64];
   static std::mutex mu;
   std::lock_guard<std::mutex> lock(mu);
-  int& n = slots[device_slot()].n[bf16 ? 1 : 0];
+  int& n = slots[device_slot()].n[(bf16 ? 1 : 0) + (delta ? 2 : 0)];
   if (n >= 0) return n;
-  auto k2 = bf16 ? gemm::pair::b1_gemm_pair_kernel<true> : gemm::pair::b1_gemm_pair_kernel<false>;
+  auto k2 = pair_kernel(bf16, delta);
   n = 0;
   if (cudaFuncSetAttribute(k2, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            gemm::pair::SMEM_BYTES) != cudaSuccess)
@@ -1080,7 +1104,7 @@ int launch_b1_gemv_f32(const float* x, const B1Weight& w, float* y, cudaStream_t
 }
 
 int launch_b1_gemm(const void* x, long long ldx, int tokens, const B1Weight& w, const EpiSeg* segs,
-                   int nseg, bool x_bf16, cudaStream_t st, const TileSel* sel) {
+                   int nseg, bool x_bf16, cudaStream_t st, const TileSel* sel, const float* delta) {
   if (tokens < 0) return fail(-1, "b1_gemm: negative token count");
   if (tokens == 0) return 0;
   if (!x || !w.chunks) return fail(-1, "b1_gemm: null activation or weight");
@@ -1116,7 +1140,7 @@ int launch_b1_gemm(const void* x, long long ldx, int tokens, const B1Weight& w, 
   // Kernel choice: estimated time = waves x tile time, with a 256x256 pair
   // tile (two SMs) taking kPairTileCost 128x128-tile times of one SM (about
   // 2 x 1255 / 1536 from isolated measurements of the two kernels).
-  const int slots = pair_cluster_slots(x_bf16);
+  const int slots = pair_cluster_slots(x_bf16, delta != nullptr);
   const int n_tt1 = (tokens + gemm::BN - 1) / gemm::BN;
   const int n_tt2 = (tokens + gemm::pair::BN - 1) / gemm::pair::BN;
   const long long tiles1 = (long long)nf * n_tt1;
@@ -1134,7 +1158,9 @@ int launch_b1_gemm(const void* x, long long ldx, int tokens, const B1Weight& w, 
     all_split_ok = all_split_ok && segs[i].mode == EPI_RESID_F32 && segs[i].split_ok;
   }
   int ksplit = 1;
-  if (const char* e = getenv("BONSAI_B1_SPLITK")) {
+  if (delta) {
+    // whole K: the parts of a split would each add the delta
+  } else if (const char* e = getenv("BONSAI_B1_SPLITK")) {
     if (all_resid) ksplit = std::max(1, std::min(atoi(e), std::max(1, w.k_blocks / 2)));
   } else if (all_split_ok && w.k_blocks >= 16 && slots >= 1 && tiles2 >= slots) {
     // (a launch below one wave -- the 512-token text stream -- keeps whole
@@ -1193,7 +1219,9 @@ int launch_b1_gemm(const void* x, long long ldx, int tokens, const B1Weight& w, 
     for (int i = 0; i < nseg; ++i) q.seg[i] = segs[i];
     q.err = device_error_word();
     q.fence_sys = routed ? 1 : 0;
-    auto k2 = x_bf16 ? gemm::pair::b1_gemm_pair_kernel<true> : gemm::pair::b1_gemm_pair_kernel<false>;
+    q.n_rows = w.n_rows;
+    q.delta = delta;
+    auto k2 = pair_kernel(x_bf16, delta != nullptr);
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1233,11 +1261,13 @@ int launch_b1_gemm(const void* x, long long ldx, int tokens, const B1Weight& w, 
   p.err = device_error_word();
   p.fence_sys = routed ? 1 : 0;
   p.idle_loads = stall ? 1 : 0;
+  p.delta = delta;
 
   const int grid = (int)std::min<long long>(tiles1, num_sms());
-  auto kern = x_bf16 ? gemm::b1_gemm_kernel<true> : gemm::b1_gemm_kernel<false>;
-  static bool attr_set[64][2] = {};
-  bool& attr_done = attr_set[device_slot()][x_bf16 ? 1 : 0];
+  auto kern = delta ? (x_bf16 ? gemm::b1_gemm_kernel<true, true> : gemm::b1_gemm_kernel<false, true>)
+                    : (x_bf16 ? gemm::b1_gemm_kernel<true, false> : gemm::b1_gemm_kernel<false, false>);
+  static bool attr_set[64][4] = {};
+  bool& attr_done = attr_set[device_slot()][(x_bf16 ? 1 : 0) + (delta ? 2 : 0)];
   if (!attr_done) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          gemm::SMEM_BYTES);

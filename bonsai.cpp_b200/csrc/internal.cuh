@@ -105,10 +105,30 @@ struct TileSel {
 // Launch the tcgen05 B1_0 GEMM: for every token t < tokens and weight row n,
 // acc[t][n] = sum_k x[t][k] * W[n][k]; acc is routed through the segment that
 // covers n.  x is f16 (or bf16 when x_bf16) row-major with leading dimension
-// ldx (elements); it must be 16-byte aligned with ldx % 8 == 0.
+// ldx (elements); it must be 16-byte aligned with ldx % 8 == 0.  delta
+// (optional): f32 [tokens][n_rows], added to acc before the epilogue's mode.
 int launch_b1_gemm(const void* x, long long ldx, int tokens, const B1Weight& w,
                    const EpiSeg* segs, int nseg, bool x_bf16, cudaStream_t st,
-                   const TileSel* sel = nullptr);
+                   const TileSel* sel = nullptr, const float* delta = nullptr);
+
+// ------------------------------------------------- low-rank adapters
+struct LoraSlot {
+  int rank = 0;  // 0: no adapter in this slot
+  float scale = 0.f;
+};
+// Adapters of one projection: A rows [slot][r_pad][in], B rows
+// [slot][out][r_pad] (device row order of the B1_0 weight), f16, zero beyond
+// a slot's rank; r_pad = max_rank rounded up to 16.
+struct LoraDevice {
+  int n_rows = 0, k_in = 0, max_rank = 0, r_pad = 0, n_slots = 0, swiglu_from = -1, device = 0;
+  __half* down = nullptr;
+  __half* up = nullptr;
+  LoraSlot* info = nullptr;
+};
+// cu: device [n_reqs + 1] first token of each request; slots: device
+// [n_reqs] its adapter (outside [0, n_slots): none).
+int launch_b1_gemm_lora(const __half* x, long long ldx, int tokens, const B1Weight& w, const EpiSeg& seg,
+                        const LoraDevice& set, const int* cu, const int* slots, int n_reqs, cudaStream_t st);
 
 // B1_0 matrix-vector product for one f32 activation row: y[n] = sum_k
 // W[n][k] x[k] (f32 x and accumulation), memory-bound, no tensor cores.
@@ -247,4 +267,8 @@ int launch_euler_stats(float* lat, const float* pred, long long n, float dt, flo
 // Opaque handle behind bonsai_b1_t (include/bonsai_cuda.h).
 struct bonsai_b1_weight {
   bonsai::B1Weight w;
+};
+// Opaque handle behind bonsai_lora_t.
+struct bonsai_lora {
+  bonsai::LoraDevice set;
 };

@@ -169,6 +169,37 @@ int bonsai_b1_linear_f32_noalloc(const float* act, int tokens, bonsai_b1_t w, fl
 int bonsai_b1_gemm(const uint16_t* x, long long ldx, int tokens, bonsai_b1_t w, int mode,
                    void* out, long long ld_out, const float* gate, void* stream);
 
+/* ------------------------------------------------- low-rank adapters
+ * A set of low-rank adapters for one B1_0 projection, and the projection with
+ * each request's adapter beside it.  A 1-bit weight cannot take an adapter
+ * in, so the low-rank product runs next to it. */
+typedef struct bonsai_lora* bonsai_lora_t;
+
+/* n_slots empty slots for adapters of rank <= max_rank (1..128) on a
+ * projection of out_dim x in_dim (in_dim % 32 == 0).  swiglu_from as in
+ * bonsai_b1_upload (-1, or the weight's value).  Device memory:
+ * n_slots * (in_dim + out_dim) * max_rank (rounded up to 16) f16 values. */
+int bonsai_lora_create(int out_dim, int in_dim, int max_rank, int n_slots, int swiglu_from,
+                       bonsai_lora_t* out);
+/* Put an adapter into a slot: down f16 [rank][in_dim], up f16
+ * [out_dim][rank] (host or device memory), y += scale * up (down x).
+ * rank 0 empties the slot (down, up may be NULL).  Ordered on the stream;
+ * host memory has been read when the call returns. */
+int bonsai_lora_set(bonsai_lora_t set, int slot, const uint16_t* down, const uint16_t* up, int rank,
+                    float scale, void* stream);
+int bonsai_lora_free(bonsai_lora_t set);
+
+/* bonsai_b1_gemm with the adapters of many requests: the accumulator of
+ * token t is W x[t] + scale_a * up_a (down_a x[t]), written by mode as there.
+ * Request i has the tokens [cu_tokens[i], cu_tokens[i + 1]) (device int32
+ * [n_reqs + 1], ascending) and the adapter slots[i] (device int32 [n_reqs]);
+ * a value outside [0, n_slots) or an empty slot is no adapter, as are tokens
+ * of no request.  The low-rank products are held in f32 up to the epilogue's
+ * own rounding; scratch is stream-ordered. */
+int bonsai_b1_gemm_lora(const uint16_t* x, long long ldx, int tokens, bonsai_b1_t w, int mode,
+                        void* out, long long ld_out, const float* gate, bonsai_lora_t set,
+                        const int* cu_tokens, const int* slots, int n_reqs, void* stream);
+
 /* ------------------------------------------------------ pointwise ops */
 
 /* Drop-in for rope_2d_fwd_f32 (src/b1_0_kernel.h:309-361): for every
