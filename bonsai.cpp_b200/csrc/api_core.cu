@@ -147,6 +147,42 @@ ProfScope::~ProfScope() {
   if (idx_ >= 0 && idx_ < (long long)g_prof.size()) cudaEventRecord(g_prof[idx_].e1, st_);
 }
 
+namespace {
+struct ScratchPool {
+  cudaMemPool_t pool = nullptr;
+};
+std::mutex g_pool_mu;
+ScratchPool g_pool[64];
+}  // namespace
+
+int scratch_alloc(void** ptr, size_t bytes, const char* what, cudaStream_t st) {
+  int d = 0;
+  cudaError_t e = cudaGetDevice(&d);
+  cudaMemPool_t pool = nullptr;
+  if (e == cudaSuccess) {
+    std::lock_guard<std::mutex> lk(g_pool_mu);
+    ScratchPool& p = g_pool[d & 63];
+    if (!p.pool) {
+      cudaMemPoolProps props = {};
+      props.allocType = cudaMemAllocationTypePinned;
+      props.location.type = cudaMemLocationTypeDevice;
+      props.location.id = d;
+      e = cudaMemPoolCreate(&p.pool, &props);
+      unsigned long long keep = ~0ull;
+      if (e == cudaSuccess) e = cudaMemPoolSetAttribute(p.pool, cudaMemPoolAttrReleaseThreshold, &keep);
+    }
+    pool = p.pool;
+  }
+  if (e == cudaSuccess) e = cudaMallocFromPoolAsync(ptr, bytes, pool, st);
+  if (e == cudaSuccess) return 0;
+  cudaGetLastError();
+  return fail(BONSAI_ERR_NOMEM, std::string(what) + ": scratch allocation failed: " + cudaGetErrorString(e));
+}
+
+void scratch_free(void* ptr, cudaStream_t st) {
+  if (ptr) cudaFreeAsync(ptr, st);
+}
+
 int* device_error_word() { return dev_info().err_word; }
 long long launch_counter() { return g_launches; }
 void launch_counter_add(long long n) { g_launches += n; }
@@ -239,7 +275,8 @@ int bonsai_init(int device) {
 int bonsai_shutdown(void) {
   // Waits for the device, then releases what the library allocated lazily for
   // this host thread on the current device (the f16 activation scratch of
-  // bonsai_b1_linear_f32) and any pending profiling events.  Weight handles
+  // bonsai_b1_linear_f32), the device's unused scratch pool, and any pending
+  // profiling events.  Weight handles
   // and models stay valid until their own free/destroy calls.
   int d = 0;
   cudaGetDevice(&d);
@@ -253,6 +290,10 @@ int bonsai_shutdown(void) {
     if (sc.ptr) cudaFree(sc.ptr);
     if (sc.done) cudaEventDestroy(sc.done);
     g_scratch.erase(g_scratch.begin() + i);
+  }
+  {
+    std::lock_guard<std::mutex> lk(g_pool_mu);
+    if (g_pool[d & 63].pool) cudaMemPoolTrimTo(g_pool[d & 63].pool, 0);
   }
   for (auto& r : g_prof) {
     cudaEventDestroy(r.e0);

@@ -28,6 +28,13 @@ class ProfScope {
   cudaStream_t st_;
   long long idx_ = -1;
 };
+// Stream-ordered scratch of one call: a memory pool of the library's own per
+// device that keeps what it has (a default pool gives it back at every
+// synchronisation, and mapping it again costs 0.1 ms to several ms);
+// bonsai_shutdown() returns it.  Inside a stream capture the allocation
+// belongs to the graph.
+int scratch_alloc(void** ptr, size_t bytes, const char* what, cudaStream_t st);
+void scratch_free(void* ptr, cudaStream_t st);
 int* device_error_word();
 long long launch_counter();           // launches counted on this thread so far
 void launch_counter_add(long long n);  // account for kernels replayed from a CUDA graph

@@ -289,12 +289,10 @@ int launch_b1_gemm_lora(const __half* x, long long ldx, int tokens, const B1Weig
   if (tokens == 0) return 0;
   if (n_reqs == 0) return launch_b1_gemm(x, ldx, tokens, w, &seg, 1, false, st);
   const size_t low_n = ((size_t)tokens * set.r_pad + 3) / 4 * 4;
-  float* scratch = nullptr;
-  if (cudaMallocAsync(reinterpret_cast<void**>(&scratch), (low_n + (size_t)tokens * w.n_rows) * sizeof(float), st) !=
-      cudaSuccess) {
-    cudaGetLastError();
-    return fail(-6, "b1_gemm_lora: scratch allocation failed");
-  }
+  void* mem = nullptr;
+  int rc = scratch_alloc(&mem, (low_n + (size_t)tokens * w.n_rows) * sizeof(float), "b1_gemm_lora", st);
+  if (rc) return rc;
+  float* scratch = static_cast<float*>(mem);
   float* delta = scratch + low_n;
   lora::ShrinkParams s{};
   s.x = x;
@@ -310,7 +308,7 @@ int launch_b1_gemm_lora(const __half* x, long long ldx, int tokens, const B1Weig
   s.n_reqs = n_reqs;
   s.low = scratch;
   // 64-token tiles where the requests are long enough to fill them
-  int rc = tokens >= 32ll * n_reqs ? lora::shrink_by_rank<4>(s, set.max_rank, st)
+  rc = tokens >= 32ll * n_reqs ? lora::shrink_by_rank<4>(s, set.max_rank, st)
                                    : lora::shrink_by_rank<1>(s, set.max_rank, st);
   if (rc == 0) {
     lora::ExpandParams e{};
@@ -331,7 +329,7 @@ int launch_b1_gemm_lora(const __half* x, long long ldx, int tokens, const B1Weig
     rc = launch_status("lora_expand_kernel launch");
   }
   if (rc == 0) rc = launch_b1_gemm(x, ldx, tokens, w, &seg, 1, false, st, nullptr, delta);
-  cudaFreeAsync(scratch, st);
+  scratch_free(mem, st);
   return rc;
 }
 

@@ -772,15 +772,13 @@ int launch_text_attention(const TextAttention& a, cudaStream_t st) {
   void* part = nullptr;
   if (p.splits > 1) {
     const size_t items = (size_t)p.splits * a.total_q * a.n_heads;
-    if (cudaMallocAsync(&part, items * (a.head_dim + 1) * sizeof(float), st) != cudaSuccess) {
-      cudaGetLastError();
-      return fail(-6, "text attention: partial-output allocation failed");
-    }
+    const int rc = scratch_alloc(&part, items * (a.head_dim + 1) * sizeof(float), "text attention", st);
+    if (rc) return rc;
     p.part_o = static_cast<float*>(part);
     p.part_lse = p.part_o + items * a.head_dim;
   }
   const int rc = paged ? dispatch<true>(a, qm, km, vm, p, ctas, st) : dispatch<false>(a, qm, km, vm, p, ctas, st);
-  if (part) cudaFreeAsync(part, st);
+  scratch_free(part, st);
   return rc;
 }
 

@@ -68,7 +68,8 @@ int bonsai_device_error(void);
 
 /* Wait for the current device and release what the library allocated
  * lazily for the calling thread on it (bonsai_b1_linear_f32's activation
- * scratch, pending profiling events).  Weight handles and models stay valid.
+ * scratch, pending profiling events) and the unused stream-ordered scratch
+ * that it keeps for the device.  Weight handles and models stay valid.
  * The counterpart of ggml_backend_free (src/diffuser.cpp:310). */
 int bonsai_shutdown(void);
 
