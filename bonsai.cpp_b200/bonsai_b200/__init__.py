@@ -261,13 +261,23 @@ class LoraSet:
 def b1_gemm_lora(x16, w: B1Weight, mode: int, out, lora: LoraSet, cu_tokens, slots, gate=None, stream=None) -> None:
     """b1_gemm with each request's adapter beside it: request i has the tokens
     [cu_tokens[i], cu_tokens[i + 1]) and the adapter slots[i] (-1: none); cuda int32."""
-    _text_ints(cu_tokens=cu_tokens, slots=slots)
-    if cu_tokens.numel() != slots.numel() + 1:
-        raise BonsaiError(f"cu_tokens [{cu_tokens.numel()}] and slots [{slots.numel()}] do not match")
-    check(lib().bonsai_b1_gemm_lora(x16.data_ptr(), x16.stride(0), x16.shape[0], w.handle, mode, out.data_ptr(),
-                                    out.stride(0), gate.data_ptr() if gate is not None else None, lora.handle,
-                                    cu_tokens.data_ptr(), slots.data_ptr(), slots.numel(), stream_ptr(stream)),
-          "bonsai_b1_gemm_lora")
+    dev, st = _text_place(x16)
+    n = slots.shape[0]
+    if cu_tokens.shape[0] != n + 1:
+        raise BonsaiError(f"cu_tokens {tuple(cu_tokens.shape)} and slots [{n}] do not match")
+    T, K = x16.shape
+    sx, so = x16.stride(), out.stride()
+    f16 = mode in (BONSAI_EPI_F16, BONSAI_EPI_GELU, BONSAI_EPI_SWIGLU)
+    if x16.dtype is not _text_torch.float16 or K != w.in_dim or K > 1 and sx[1] != 1:
+        raise BonsaiError(f"x must be f16 [tokens][{w.in_dim}] with contiguous rows, got {x16.dtype} {tuple(x16.shape)}")
+    width = w.out_dim // 2 if mode == BONSAI_EPI_SWIGLU else w.out_dim
+    if out.dtype is not (_text_torch.float16 if f16 else _text_torch.float32) or out.shape != (T, width) \
+            or out.get_device() != dev or width > 1 and so[1] != 1:
+        raise BonsaiError(f"out {out.dtype} {tuple(out.shape)} does not fit the mode, {T} tokens and {width} outputs")
+    check(lib().bonsai_b1_gemm_lora(
+        x16.data_ptr(), sx[0] if T > 1 else K, T, w.handle, mode, out.data_ptr(), so[0] if T > 1 else width,
+        gate.data_ptr() if gate is not None else None, lora.handle, _text_ints(dev, "cu_tokens", cu_tokens),
+        _text_ints(dev, "slots", slots), n, st if stream is None else stream.cuda_stream), "bonsai_b1_gemm_lora")
 
 
 def linear_f32(x, W, bias, out, stream=None) -> None:
@@ -329,79 +339,104 @@ class PagesDesc(ctypes.Structure):
                 ("n_pages", _c_int), ("page_size", _c_int)]
 
 
-def _text_dtype(*tensors) -> int:
-    import torch
-    dt, dev = tensors[0].dtype, torch.device("cuda", torch.cuda.current_device())
-    if dt not in (torch.float16, torch.bfloat16):
-        raise BonsaiError(f"text attention takes f16 or bf16 tensors, got {dt}")
-    for t in tensors:
-        if t.dtype != dt or t.device != dev:
-            raise BonsaiError(f"tensors must all be {dt} on {dev}, got {t.dtype} on {t.device}")
-        if t.shape[-1] > 1 and t.stride(-1) != 1:
-            raise BonsaiError("the last dimension of a tensor of heads must be contiguous")
-    return 1 if dt == torch.bfloat16 else 0
+# These calls run once per layer and token, so their checks are kept to a few
+# microseconds: plain comparisons of what the tensors say of themselves.
+_text_torch = None
 
 
-def _text_ints(**tensors):
-    import torch
-    dev = torch.device("cuda", torch.cuda.current_device())
-    for name, t in tensors.items():
-        if t.dtype != torch.int32 or t.device != dev or (t.numel() > 1 and t.stride(-1) != 1):
-            raise BonsaiError(f"{name} must be int32 with unit stride on {dev}")
+def _text_place(first):
+    """(device index of `first`, which has to be the current one, and its current stream)."""
+    global _text_torch
+    if _text_torch is None:
+        import torch
+        _text_torch = torch
+    dev = first.get_device()
+    if dev < 0 or dev != _text_torch._C._cuda_getDevice():
+        raise BonsaiError(f"tensors must be on the current cuda device, got {first.device}")
+    return dev, _text_torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _heads(t) -> HeadsDesc:
-    return HeadsDesc(t.data_ptr(), t.stride(0), t.stride(1))
+def _text_dtype(dtype) -> int:
+    if dtype is _text_torch.float16:
+        return 0
+    if dtype is _text_torch.bfloat16:
+        return 1
+    raise BonsaiError(f"text attention takes f16 or bf16 tensors, got {dtype}")
 
 
-def _pages(t) -> PagesDesc:
-    return PagesDesc(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2), t.shape[0], t.shape[1])
+def _text_ints(dev, name, t):
+    if t.dtype is not _text_torch.int32 or t.get_device() != dev or t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise BonsaiError(f"{name} must be int32 with unit stride on the current device")
+    return t.data_ptr()
 
 
-def _same(what, *shapes):
-    if any(s != shapes[0] for s in shapes):
-        raise BonsaiError(f"{what} do not match: {[tuple(s) for s in shapes]}")
+def _heads(t, dtype, dev, dim):
+    """bonsai_heads_t of a [token][head][dim] tensor."""
+    s = t.stride()
+    if len(s) != 3 or t.dtype is not dtype or t.get_device() != dev or s[2] != 1 and dim > 1:
+        raise BonsaiError(f"want a [token][head][dim] tensor of {dtype} with contiguous dims on the current device, "
+                          f"got {t.dtype} {tuple(t.shape)} {tuple(s)} on {t.device}")
+    return ctypes.byref(HeadsDesc(t.data_ptr(), s[0], s[1]))
+
+
+def _pages(t, dtype, dev, dim):
+    """bonsai_pages_t of a [page][slot][head][dim] tensor."""
+    s, n = t.stride(), t.shape
+    if len(s) != 4 or t.dtype is not dtype or t.get_device() != dev or s[3] != 1 and dim > 1:
+        raise BonsaiError(f"want a [page][slot][head][dim] cache of {dtype} with contiguous dims on the current device, "
+                          f"got {t.dtype} {tuple(n)} {tuple(s)} on {t.device}")
+    return ctypes.byref(PagesDesc(t.data_ptr(), s[0], s[1], s[2], n[0], n[1]))
+
+
+def _same(what, a, b):
+    if a != b:
+        raise BonsaiError(f"{what} do not match: {tuple(a)}, {tuple(b)}")
 
 
 def prompt_attention(q, k, v, cu_seqlens, out, scale=None, causal=True, stream=None) -> None:
     """Attention over packed prompts: q, out [T][H][D], k, v [T][Hkv][D] (f16 or
     bf16, any token / head strides that are multiples of 8), cu_seqlens cuda
     int32 [n + 1]; sequence s has the rows [cu_seqlens[s], cu_seqlens[s + 1])."""
-    dt = _text_dtype(q, k, v, out)
-    _text_ints(cu_seqlens=cu_seqlens)
-    _same("q and out", q.shape, out.shape)
-    _same("k and v", k.shape, v.shape)
-    if k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
-        raise BonsaiError(f"k {tuple(k.shape)} does not fit q {tuple(q.shape)}")
-    T, H, D = q.shape
+    dev, st = _text_place(q)
+    dtype, shape, kshape = q.dtype, q.shape, k.shape
+    _same("q and out", shape, out.shape)
+    _same("k and v", kshape, v.shape)
+    T, H, D = shape
+    if kshape[0] != T or kshape[2] != D:
+        raise BonsaiError(f"k {tuple(kshape)} does not fit q {tuple(shape)}")
     check(lib().bonsai_prompt_attention(
-        ctypes.byref(_heads(q)), ctypes.byref(_heads(k)), ctypes.byref(_heads(v)), cu_seqlens.data_ptr(),
-        cu_seqlens.numel() - 1, T, H, k.shape[1], D, dt, int(bool(causal)),
-        float(scale if scale is not None else D ** -0.5), ctypes.byref(_heads(out)), stream_ptr(stream)),
-        "bonsai_prompt_attention")
+        _heads(q, dtype, dev, D), _heads(k, dtype, dev, D), _heads(v, dtype, dev, D),
+        _text_ints(dev, "cu_seqlens", cu_seqlens), cu_seqlens.shape[0] - 1, T, H, kshape[1], D, _text_dtype(dtype),
+        1 if causal else 0, D ** -0.5 if scale is None else scale, _heads(out, dtype, dev, D),
+        st if stream is None else stream.cuda_stream), "bonsai_prompt_attention")
 
 
-def _table_args(page_table, cu_q, ctx_lens):
-    _text_ints(page_table=page_table, cu_q=cu_q, ctx_lens=ctx_lens)
-    n = ctx_lens.numel()
-    if cu_q.numel() != n + 1 or page_table.dim() != 2 or page_table.shape[0] != n:
-        raise BonsaiError(f"page_table {tuple(page_table.shape)}, cu_q [{cu_q.numel()}] and ctx_lens [{n}] do not match")
-    return n
+def _table_args(dev, page_table, cu_q, ctx_lens):
+    """(page_table, row stride, width, cu_q, ctx_lens, sequences) as the C calls take them."""
+    n = ctx_lens.shape[0]
+    if cu_q.shape[0] != n + 1 or page_table.dim() != 2 or page_table.shape[0] != n:
+        raise BonsaiError(f"page_table {tuple(page_table.shape)}, cu_q {tuple(cu_q.shape)} and ctx_lens [{n}] do not match")
+    width = page_table.shape[1]
+    return (_text_ints(dev, "page_table", page_table), page_table.stride(0) if n > 1 else width, width,
+            _text_ints(dev, "cu_q", cu_q), _text_ints(dev, "ctx_lens", ctx_lens), n)
 
 
 def paged_append(k, v, k_cache, v_cache, page_table, cu_q, ctx_lens, stream=None) -> None:
     """Write new keys / values [T][Hkv][D] into the cache [pages][page_size][Hkv][D]:
     token i of sequence s (rows [cu_q[s], cu_q[s + 1])) goes to place
     ctx_lens[s] - q_len + i of its page_table row [n][width]."""
-    _text_dtype(k, v, k_cache, v_cache)
-    n = _table_args(page_table, cu_q, ctx_lens)
-    _same("k and v", k.shape, v.shape)
-    _same("heads of k and of the caches", k.shape[1:], k_cache.shape[2:], v_cache.shape[2:])
+    dev, st = _text_place(k)
+    dtype, shape, cshape = k.dtype, k.shape, k_cache.shape
+    _text_dtype(dtype)
+    _same("k and v", shape, v.shape)
+    _same("the caches", cshape, v_cache.shape)
+    T, Hk, D = shape
+    if cshape[2] != Hk or cshape[3] != D:
+        raise BonsaiError(f"caches {tuple(cshape)} do not fit k {tuple(shape)}")
     check(lib().bonsai_paged_append(
-        ctypes.byref(_heads(k)), ctypes.byref(_heads(v)), ctypes.byref(_pages(k_cache)),
-        ctypes.byref(_pages(v_cache)), page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
-        cu_q.data_ptr(), ctx_lens.data_ptr(), n, k.shape[0], k.shape[1], k.shape[2], stream_ptr(stream)),
-        "bonsai_paged_append")
+        _heads(k, dtype, dev, D), _heads(v, dtype, dev, D), _pages(k_cache, dtype, dev, D),
+        _pages(v_cache, dtype, dev, D), *_table_args(dev, page_table, cu_q, ctx_lens), T, Hk, D,
+        st if stream is None else stream.cuda_stream), "bonsai_paged_append")
 
 
 def paged_attention(q, k_cache, v_cache, page_table, cu_q, ctx_lens, max_ctx, out, scale=None,
@@ -409,18 +444,18 @@ def paged_attention(q, k_cache, v_cache, page_table, cu_q, ctx_lens, max_ctx, ou
     """Causal attention of new tokens q [T][H][D] over the paged cache
     [pages][page_size][Hkv][D], the new tokens' own keys appended before;
     max_ctx: an upper bound of ctx_lens (only sets how the work is split)."""
-    dt = _text_dtype(q, k_cache, v_cache, out)
-    n = _table_args(page_table, cu_q, ctx_lens)
-    _same("q and out", q.shape, out.shape)
-    T, H, D = q.shape
-    if k_cache.shape[3] != D or v_cache.shape[3] != D:
-        raise BonsaiError(f"caches of head_dim {k_cache.shape[3]} / {v_cache.shape[3]} do not fit q {tuple(q.shape)}")
-    _same("heads of the caches", k_cache.shape[2:3], v_cache.shape[2:3])
+    dev, st = _text_place(q)
+    dtype, shape, cshape = q.dtype, q.shape, k_cache.shape
+    _same("q and out", shape, out.shape)
+    _same("the caches", cshape, v_cache.shape)
+    T, H, D = shape
+    if cshape[3] != D:
+        raise BonsaiError(f"caches {tuple(cshape)} do not fit q {tuple(shape)}")
     check(lib().bonsai_paged_attention(
-        ctypes.byref(_heads(q)), ctypes.byref(_pages(k_cache)), ctypes.byref(_pages(v_cache)),
-        page_table.data_ptr(), page_table.stride(0), page_table.shape[1], cu_q.data_ptr(), ctx_lens.data_ptr(),
-        n, T, int(max_ctx), H, k_cache.shape[2], D, dt, float(scale if scale is not None else D ** -0.5),
-        ctypes.byref(_heads(out)), stream_ptr(stream)), "bonsai_paged_attention")
+        _heads(q, dtype, dev, D), _pages(k_cache, dtype, dev, D), _pages(v_cache, dtype, dev, D),
+        *_table_args(dev, page_table, cu_q, ctx_lens), T, max_ctx, H, cshape[2], D, _text_dtype(dtype),
+        D ** -0.5 if scale is None else scale, _heads(out, dtype, dev, D),
+        st if stream is None else stream.cuda_stream), "bonsai_paged_attention")
 
 
 # ----------------------------------------------------------------- host side
