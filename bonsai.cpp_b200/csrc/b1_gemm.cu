@@ -87,7 +87,8 @@ struct Params {
   // so every other role's first bounded wait expires and the kernel unwinds
   // through its abort path with no copy or MMA in flight.  0 in normal use.
   int idle_loads;
-  const float* delta;  // kDelta: f32 [tokens][n_rows] added to the accumulator
+  LoraGemm lora;  // kLora
+  int kparts, kpart;  // kLora: the tile's k-blocks in kparts accumulations of kpart
 };
 
 __device__ __forceinline__ float tanh_hw(float x) {
@@ -128,6 +129,14 @@ __device__ __forceinline__ uint32_t bf16_from_f16_scale(uint32_t s16) {
   }
 }
 
+// kLora, the low-rank product beside W x: LORA_NONE; LORA_DELTA: an f32
+// matrix delta that the epilogue adds; LORA_BLOCKS: extra k-blocks whose
+// weight columns are columns of the adapters' B and whose activations are the
+// low-rank values of the tokens of one request (zero for the tile's others):
+//   [W | B_a B_a B_b ...] [x; low_a hi; low_a lo; low_b hi; ...].
+// The f32 low-rank values enter as two f16 (value and remainder), which keeps
+// 22 bits of them.
+
 // acc[j] of weight row `row`, tokens t0 + j (j < nt) += delta.  Lanes hold
 // consecutive rows, so each token is one coalesced read per warp.
 __device__ __forceinline__ void add_delta(uint32_t (&v)[32], const float* delta, int n_rows, int row,
@@ -139,7 +148,47 @@ __device__ __forceinline__ void add_delta(uint32_t (&v)[32], const float* delta,
     if (j < nt) v[j] = __float_as_uint(__uint_as_float(v[j]) + __ldg(d + (size_t)j * n_rows));
 }
 
-template <bool kBF16, bool kDelta>
+// 16-column groups of the extra k-blocks of token tile `ttile`.
+template <int kLora>
+__device__ __forceinline__ int lora_groups(const LoraGemm& l, int ttile) {
+  return kLora == LORA_BLOCKS ? __ldg(l.group_count + ttile) : 0;
+}
+// One 16-column group: this thread's weight row (8 words of two columns) and
+// its token's activations (8 words), zero where they are none of the group's.
+__device__ __forceinline__ void lora_group(const LoraGemm& l, const int4 e, int row, int n_rows, int tok,
+                                           uint32_t* w, uint32_t* x) {
+  const int slot = e.x & 0x3fffffff;
+  const bool lo = (e.x & 0x40000000) != 0;
+  uint4 b0 = make_uint4(0, 0, 0, 0), b1 = b0;
+  if (row < n_rows) {
+    const uint4* src = reinterpret_cast<const uint4*>(l.up + ((size_t)slot * n_rows + row) * l.r_pad + e.y);
+    b0 = __ldg(src);
+    b1 = __ldg(src + 1);
+  }
+  w[0] = b0.x; w[1] = b0.y; w[2] = b0.z; w[3] = b0.w;
+  w[4] = b1.x; w[5] = b1.y; w[6] = b1.z; w[7] = b1.w;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = 0u;
+  if (tok >= e.z && tok < e.w) {
+    const float4* src = reinterpret_cast<const float4*>(l.low + (size_t)tok * l.r_pad + e.y);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 f = __ldg(src + i);
+      const __half2 h0 = __floats2half2_rn(f.x, f.y), h1 = __floats2half2_rn(f.z, f.w);
+      if (!lo) {
+        x[2 * i] = *reinterpret_cast<const uint32_t*>(&h0);
+        x[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+      } else {
+        const float2 g0 = __half22float2(h0), g1 = __half22float2(h1);
+        const __half2 r0 = __floats2half2_rn(f.x - g0.x, f.y - g0.y), r1 = __floats2half2_rn(f.z - g1.x, f.w - g1.y);
+        x[2 * i] = *reinterpret_cast<const uint32_t*>(&r0);
+        x[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&r1);
+      }
+    }
+  }
+}
+
+template <bool kBF16, int kLora>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
     b1_gemm_kernel(const __grid_constant__ CUtensorMap xmap, const Params p) {
   extern __shared__ uint8_t smem_raw[];
@@ -193,12 +242,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         const int ttile = tile / p.nf;
         const int ftile = sel_ftile(tile - ttile * p.nf, p.fcount, p.fbase);
         const uint32_t* wsrc = p.chunks + (size_t)ftile * k_blocks * kChunkWords;
-        for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+        const int nkb = k_blocks + (lora_groups<kLora>(p.lora, ttile) + 3) / 4;
+        for (int kb = 0; kb < nkb; ++kb, ++it) {
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1;
           if (!wait_bar(&empty[s], ph ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_TMA)) {
             ok = false;
             break;
+          }
+          if (kLora == LORA_BLOCKS && kb >= k_blocks) {  // the expansion warps bring both operands
+            bar_arrive(&rawfull[s]);
+            bar_arrive(&full[s]);
+            continue;
           }
           bar_arrive_expect_tx(&rawfull[s], RAW_STAGE_BYTES);
           bulk_load(raw + s * kChunkWords, wsrc + (size_t)kb * kChunkWords, RAW_STAGE_BYTES,
@@ -219,7 +274,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       constexpr uint32_t idesc = make_idesc_f16(BM, BN, kBF16 ? 1 : 0, 0, 0);
       uint32_t it = 0, lt = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < p.num_tiles && ok; tile += gridDim.x, ++lt) {
+      for (int tile = blockIdx.x; tile < p.num_tiles && ok; tile += gridDim.x) {
+        const int groups = lora_groups<kLora>(p.lora, tile / p.nf);
+        const int nkb = k_blocks + (groups + 3) / 4;
+        const int parts = kLora != LORA_NONE ? p.kparts : 1;
+        for (int part = 0; part < parts && ok; ++part, ++lt) {
+        const int kb0 = part * p.kpart, kb1 = part + 1 < parts ? kb0 + p.kpart : nkb;
         const uint32_t b = lt & 1;
         const uint32_t dph = (lt >> 1) & 1;
         if (!wait_bar(&dempty[b], dph ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)) {
@@ -228,7 +288,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
         tc_fence_after();
         const uint32_t d_tmem = tmem + D_COL0 + b * BN;
-        for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1;
           if (!wait_bar(&full[s], ph, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)) {
@@ -239,14 +299,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           const uint32_t xaddr = smem_u32(xs + s * X_STAGE_BYTES);
 #pragma unroll
           for (int k16 = 0; k16 < BK / 16; ++k16) {
+            if (kLora == LORA_BLOCKS && kb >= k_blocks && (kb - k_blocks) * 4 + k16 >= groups) break;
             const uint32_t a_tmem = tmem + A_COL0 + s * 32 + k16 * 8;
             const uint64_t bdesc = make_smem_desc(xaddr + k16 * 32, 16, 1024);
-            mma_ts(d_tmem, a_tmem, bdesc, idesc, (kb | k16) != 0 ? 1u : 0u);
+            mma_ts(d_tmem, a_tmem, bdesc, idesc, kb != kb0 || k16 != 0 ? 1u : 0u);
           }
           tc_commit(&empty[s]);
         }
         if (!ok) break;
         tc_commit(&dfull[b]);
+        }
       }
       // Drain: wait until every MMA this thread issued has completed.
       tc_commit(drain);
@@ -272,7 +334,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     int pending = -1;  // stage whose tcgen05.st is in flight
     bool ok = true;
     for (int tile = blockIdx.x; tile < p.num_tiles && ok; tile += gridDim.x) {
-      for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+      const int ttile = tile / p.nf;
+      const int groups = lora_groups<kLora>(p.lora, ttile);
+      const int nkb = k_blocks + (groups + 3) / 4;
+      for (int kb = 0; kb < nkb; ++kb, ++it) {
         if (it % EXP_PER_Q != slot) continue;
         const int s = it % STAGES;
         const uint32_t ph = (it / STAGES) & 1;
@@ -283,13 +348,29 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           ok = false;
           break;
         }
-        const uint32_t* rs = raw + s * kChunkWords;
-        const uint32_t p0 = rs[r];
-        const uint32_t p1 = rs[128 + r];
-        const uint32_t sc = rs[256 + r];
         uint32_t v[32];
-        expand_group(p0, bf16_from_f16_scale<kBF16>(sc & 0xFFFFu), v);
-        expand_group(p1, bf16_from_f16_scale<kBF16>(sc >> 16), v + 16);
+        if (kLora == LORA_BLOCKS && kb >= k_blocks) {
+          const int row = sel_ftile(tile - ttile * p.nf, p.fcount, p.fbase) * BM + r;
+          const uint32_t xrow = smem_u32(xs + s * X_STAGE_BYTES) + (uint32_t)r * 128u;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int gi = (kb - k_blocks) * 4 + g;
+            if (gi >= groups) break;  // its columns are not multiplied
+            const int4 e = __ldg(p.lora.groups + (size_t)ttile * p.lora.max_groups + gi);
+            uint32_t x[8];
+            lora_group(p.lora, e, row, p.n_rows, ttile * BN + r, v + 8 * g, x);
+            st_shared_v4(xrow + (((2u * g) ^ (r & 7)) << 4), x[0], x[1], x[2], x[3]);
+            st_shared_v4(xrow + (((2u * g + 1u) ^ (r & 7)) << 4), x[4], x[5], x[6], x[7]);
+          }
+          fence_proxy_async_smem();
+        } else {
+          const uint32_t* rs = raw + s * kChunkWords;
+          const uint32_t p0 = rs[r];
+          const uint32_t p1 = rs[128 + r];
+          const uint32_t sc = rs[256 + r];
+          expand_group(p0, bf16_from_f16_scale<kBF16>(sc & 0xFFFFu), v);
+          expand_group(p1, bf16_from_f16_scale<kBF16>(sc >> 16), v + 16);
+        }
         if (pending >= 0) {
           tmem_wait_st();
           tc_fence_before();
@@ -313,13 +394,17 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const int eh = (warp - WARP_EPI0) >> 2;  // which half of the token columns
     const uint32_t lane_base = (uint32_t)(q * 32) << 16;
     uint32_t lt = 0;
-    for (int tile = blockIdx.x; tile < p.num_tiles; tile += gridDim.x, ++lt) {
+    const int parts = kLora != LORA_NONE ? p.kparts : 1;
+    bool up = true;  // no wait has expired
+    for (int tile = blockIdx.x; tile < p.num_tiles && up; tile += gridDim.x) {
       const int ttile = tile / p.nf;
       const int ftile = sel_ftile(tile - ttile * p.nf, p.fcount, p.fbase);
+      for (int part = 0; part < parts; ++part, ++lt) {
       const uint32_t b = lt & 1;
       const uint32_t dph = (lt >> 1) & 1;
       const bool good = wait_bar(&dfull[b], dph, abort_flag, p.err, DEV_ERR_TIMEOUT_EPILOGUE);
-      if (!__all_sync(0xffffffffu, good)) break;  // tcgen05.ld is warp-collective
+      up = __all_sync(0xffffffffu, good);  // tcgen05.ld is warp-collective
+      if (!up) break;
       tc_fence_after();
 
       const int row = ftile * BM + q * 32 + (int)lane;
@@ -366,7 +451,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         tmem_wait_ld();
         const int t0 = ttile * BN + c * 32;
         const int nt = min(32, p.tokens - t0);
-        if constexpr (kDelta) add_delta(v, p.delta, p.n_rows, row, t0, nt);
+        if constexpr (kLora == LORA_DELTA) {
+          if (part + 1 == parts) add_delta(v, p.lora.delta, p.n_rows, row, t0, nt);
+        }
         if (warp_swiglu) {
           // Rows are stored gate/value interleaved; the even lane owns the pair.
           __half* dst = reinterpret_cast<__half*>(sg.dst) + base + (size_t)t0 * stride;
@@ -401,6 +488,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             for (int j = 0; j < 16; ++j)
               if (h16 + j < nt) dst[(h16 + j) * stride] = fmaf(gate, __uint_as_float(v[h16 + j]), old[j]);
           }
+        } else if (kLora != LORA_NONE && mode == EPI_F32 && part > 0) {
+          // the sum of the k-parts before, by this same thread
+          float* dst = reinterpret_cast<float*>(sg.dst) + base + (size_t)t0 * stride;
+#pragma unroll
+          for (int h16 = 0; h16 < 32; h16 += 16) {
+            float old[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) old[j] = h16 + j < nt ? dst[(h16 + j) * stride] : 0.f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (h16 + j < nt) dst[(h16 + j) * stride] = old[j] + __uint_as_float(v[h16 + j]);
+          }
         } else if (mode == EPI_F32) {
           float* dst = reinterpret_cast<float*>(sg.dst) + base + (size_t)t0 * stride;
 #pragma unroll
@@ -411,6 +510,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) bar_arrive(&dempty[b]);
+      }
     }
     if (p.fence_sys) __threadfence_system();  // peer stores ordered before the kernel's end
   }
@@ -466,10 +566,11 @@ struct Params {
   int* err;
   int fence_sys;  // a segment stores to other GPUs: fence.sys after the epilogue's stores
   int n_rows;
-  const float* delta;  // kDelta: f32 [tokens][n_rows] added to the accumulator
+  LoraGemm lora;  // kLora (ksplit is 1)
+  int kparts, kpart;
 };
 
-template <bool kBF16, bool kDelta>
+template <bool kBF16, int kLora>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
     b1_gemm_pair_kernel(const __grid_constant__ CUtensorMap xmap, const Params p) {
   extern __shared__ uint8_t smem_raw[];
@@ -533,12 +634,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         const int fidx = min(2 * pf + (int)rank, p.nf - 1);
         const int ftile = sel_ftile(fidx, p.fcount, p.fbase);
         const uint32_t* wsrc = p.chunks + (size_t)ftile * k_blocks * kChunkWords;
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const int nkb = kb1 + (lora_groups<kLora>(p.lora, ttile) + 3) / 4;
+        for (int kb = kb0; kb < nkb; ++kb, ++it) {
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1;
           if (!wait_bar(&empty[s], ph ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_TMA)) {
             ok = false;
             break;
+          }
+          if (kLora == LORA_BLOCKS && kb >= k_blocks) {  // the expansion warps bring both operands
+            bar_arrive(&rawfull[s]);
+            if (rank == 0) bar_arrive(&full[s]);
+            continue;
           }
           bar_arrive_expect_tx(&rawfull[s], RAW_STAGE_BYTES);
           bulk_load(raw + s * kChunkWords, wsrc + (size_t)kb * kChunkWords, RAW_STAGE_BYTES,
@@ -560,7 +667,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         constexpr uint32_t idesc = make_idesc_f16(2 * BM, BN, kBF16 ? 1 : 0, 0, 0);
         uint32_t it = 0, lt = 0;
         bool ok = true;
-        for (int tile = cid; tile < p.num_tiles && ok; tile += ncl, ++lt) {
+        for (int tile = cid; tile < p.num_tiles && ok; tile += ncl) {
+          const int groups = lora_groups<kLora>(p.lora, tile / p.ksplit / p.npf);
+          const int parts = kLora != LORA_NONE ? p.kparts : 1;
+          for (int part = 0; part < parts && ok; ++part, ++lt) {
           const uint32_t b = lt & 1;
           const uint32_t dph = (lt >> 1) & 1;
           if (!wait_bar(&dempty[b], dph ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)) {
@@ -569,8 +679,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           }
           tc_fence_after();
           const uint32_t d_tmem = tmem + b * BN;
-          const int kb0 = (tile % p.ksplit) * p.kchunk;
-          const int kb1 = min(k_blocks, kb0 + p.kchunk);
+          int kb0, kb1;
+          if constexpr (kLora != LORA_NONE) {
+            kb0 = part * p.kpart;
+            kb1 = part + 1 < parts ? kb0 + p.kpart : k_blocks + (groups + 3) / 4;
+          } else {
+            kb0 = (tile % p.ksplit) * p.kchunk;
+            kb1 = min(k_blocks, kb0 + p.kchunk);
+          }
           for (int kb = kb0; kb < kb1; ++kb, ++it) {
             const int s = it % STAGES;
             const uint32_t ph = (it / STAGES) & 1;
@@ -583,6 +699,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             const uint32_t xaddr = smem_u32(xs + s * X_STAGE_BYTES);
 #pragma unroll
             for (int k16 = 0; k16 < BK / 16; ++k16) {
+              if (kLora == LORA_BLOCKS && kb >= k_blocks && (kb - k_blocks) * 4 + k16 >= groups) break;
               const uint64_t adesc = make_smem_desc(aaddr + k16 * 32, 16, 1024);
               const uint64_t bdesc = make_smem_desc(xaddr + k16 * 32, 16, 1024);
               mma_ss_pair(d_tmem, adesc, bdesc, idesc, (kb != kb0 || k16 != 0) ? 1u : 0u);
@@ -591,6 +708,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           }
           if (!ok) break;
           tc_commit_pair(&dfull[b], 0x3);
+          }
         }
         tc_commit_pair(drain, 0x3);
       }
@@ -617,7 +735,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     for (int tile = cid; tile < p.num_tiles && ok; tile += ncl) {
       const int kb0 = (tile % p.ksplit) * p.kchunk;
       const int kb1 = min(k_blocks, kb0 + p.kchunk);
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+      const int ttile = tile / p.ksplit / p.npf;
+      const int groups = lora_groups<kLora>(p.lora, ttile);
+      const int nkb = kb1 + (groups + 3) / 4;
+      for (int kb = kb0; kb < nkb; ++kb, ++it) {
         if (it % EXP_PER_G != slot) continue;
         const int s = it % STAGES;
         const uint32_t ph = (it / STAGES) & 1;
@@ -628,18 +749,38 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           ok = false;
           break;
         }
-        const uint32_t* rs = raw + s * kChunkWords;
-        const uint32_t p0 = rs[r];
-        const uint32_t p1 = rs[128 + r];
-        const uint32_t sc = rs[256 + r];
-        uint32_t v[32];
-        expand_group(p0, bf16_from_f16_scale<kBF16>(sc & 0xFFFFu), v);
-        expand_group(p1, bf16_from_f16_scale<kBF16>(sc >> 16), v + 16);
-        const uint32_t abase = smem_u32(as + s * A_STAGE_BYTES) + row_off;
+        if (kLora == LORA_BLOCKS && kb >= k_blocks) {
+          const int fidx = min(2 * (tile - ttile * p.npf) + (int)rank, p.nf - 1);
+          const int row = sel_ftile(fidx, p.fcount, p.fbase) * BM + r;
+          const uint32_t arow = smem_u32(as + s * A_STAGE_BYTES) + row_off;
+          const uint32_t xrow = smem_u32(xs + s * X_STAGE_BYTES) + row_off;
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-          st_shared_v4(abase + (((uint32_t)c ^ sw) << 4), v[4 * c], v[4 * c + 1], v[4 * c + 2],
-                       v[4 * c + 3]);
+          for (int q = 0; q < 4; ++q) {
+            const int gi = (kb - k_blocks) * 4 + q;
+            if (gi >= groups) break;  // its columns are not multiplied
+            const int4 e = __ldg(p.lora.groups + (size_t)ttile * p.lora.max_groups + gi);
+            uint32_t w[8], x[8];
+            lora_group(p.lora, e, row, p.n_rows, ttile * BN + (int)rank * BNH + r, w, x);
+            const uint32_t c0 = ((2u * q) ^ sw) << 4, c1 = ((2u * q + 1u) ^ sw) << 4;
+            st_shared_v4(arow + c0, w[0], w[1], w[2], w[3]);
+            st_shared_v4(arow + c1, w[4], w[5], w[6], w[7]);
+            st_shared_v4(xrow + c0, x[0], x[1], x[2], x[3]);
+            st_shared_v4(xrow + c1, x[4], x[5], x[6], x[7]);
+          }
+        } else {
+          const uint32_t* rs = raw + s * kChunkWords;
+          const uint32_t p0 = rs[r];
+          const uint32_t p1 = rs[128 + r];
+          const uint32_t sc = rs[256 + r];
+          uint32_t v[32];
+          expand_group(p0, bf16_from_f16_scale<kBF16>(sc & 0xFFFFu), v);
+          expand_group(p1, bf16_from_f16_scale<kBF16>(sc >> 16), v + 16);
+          const uint32_t abase = smem_u32(as + s * A_STAGE_BYTES) + row_off;
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            st_shared_v4(abase + (((uint32_t)c ^ sw) << 4), v[4 * c], v[4 * c + 1], v[4 * c + 2],
+                         v[4 * c + 3]);
+        }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) bar_arrive_remote(full0 + (uint32_t)s * 8u);
@@ -651,15 +792,19 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const uint32_t lane_base = (uint32_t)(q * 32) << 16;
     const uint32_t dempty0 = mapa_shared(smem_u32(&dempty[0]), 0);
     uint32_t lt = 0;
-    for (int tile = cid; tile < p.num_tiles; tile += ncl, ++lt) {
+    const int parts = kLora != LORA_NONE ? p.kparts : 1;
+    bool up = true;  // no wait has expired
+    for (int tile = cid; tile < p.num_tiles && up; tile += ncl) {
       const int t2 = tile / p.ksplit;
       const int ttile = t2 / p.npf;
       const int pf = t2 - ttile * p.npf;
       const int fidx = 2 * pf + (int)rank;
+      for (int part = 0; part < parts; ++part, ++lt) {
       const uint32_t b = lt & 1;
       const uint32_t dph = (lt >> 1) & 1;
       const bool good = wait_bar(&dfull[b], dph, abort_flag, p.err, DEV_ERR_TIMEOUT_EPILOGUE);
-      if (!__all_sync(0xffffffffu, good)) break;
+      up = __all_sync(0xffffffffu, good);
+      if (!up) break;
       tc_fence_after();
 
       int si = -1;
@@ -707,8 +852,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         tmem_wait_ld();
         const int t0 = ttile * BN + c * 32;
         const int nt = min(32, p.tokens - t0);
-        if constexpr (kDelta) {
-          if (si >= 0) add_delta(v, p.delta, p.n_rows, row, t0, nt);
+        if constexpr (kLora == LORA_DELTA) {
+          if (si >= 0 && part + 1 == parts) add_delta(v, p.lora.delta, p.n_rows, row, t0, nt);
         }
         if (warp_swiglu) {
           __half* dst = reinterpret_cast<__half*>(sg.dst) + base + (size_t)t0 * stride;
@@ -749,6 +894,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             for (int j = 0; j < 16; ++j)
               if (h16 + j < nt) dst[(h16 + j) * stride] = fmaf(gate, __uint_as_float(v[h16 + j]), old[j]);
           }
+        } else if (kLora != LORA_NONE && mode == EPI_F32 && part > 0) {
+          // the sum of the k-parts before, by this same thread
+          float* dst = reinterpret_cast<float*>(sg.dst) + base + (size_t)t0 * stride;
+#pragma unroll
+          for (int h16 = 0; h16 < 32; h16 += 16) {
+            float old[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) old[j] = h16 + j < nt ? dst[(h16 + j) * stride] : 0.f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (h16 + j < nt) dst[(h16 + j) * stride] = old[j] + __uint_as_float(v[h16 + j]);
+          }
         } else if (mode == EPI_F32) {
           float* dst = reinterpret_cast<float*>(sg.dst) + base + (size_t)t0 * stride;
 #pragma unroll
@@ -759,6 +916,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) bar_arrive_remote(dempty0 + b * 8u);
+      }
     }
     if (p.fence_sys) __threadfence_system();  // peer stores ordered before the kernel's end
   }
@@ -1016,24 +1174,32 @@ B1Kernel forced_kernel() {
   return B1Kernel::Auto;
 }
 
-auto pair_kernel(bool bf16, bool delta) {
-  return delta ? (bf16 ? gemm::pair::b1_gemm_pair_kernel<true, true> : gemm::pair::b1_gemm_pair_kernel<false, true>)
-               : (bf16 ? gemm::pair::b1_gemm_pair_kernel<true, false>
-                       : gemm::pair::b1_gemm_pair_kernel<false, false>);
+// The instantiation for a launch; low-rank products come with f16 activations only.
+auto pair_kernel(bool bf16, int lora) {
+  using namespace gemm::pair;
+  if (lora == LORA_DELTA) return b1_gemm_pair_kernel<false, LORA_DELTA>;
+  if (lora == LORA_BLOCKS) return b1_gemm_pair_kernel<false, LORA_BLOCKS>;
+  return bf16 ? b1_gemm_pair_kernel<true, LORA_NONE> : b1_gemm_pair_kernel<false, LORA_NONE>;
+}
+auto single_kernel(bool bf16, int lora) {
+  using namespace gemm;
+  if (lora == LORA_DELTA) return b1_gemm_kernel<false, LORA_DELTA>;
+  if (lora == LORA_BLOCKS) return b1_gemm_kernel<false, LORA_BLOCKS>;
+  return bf16 ? b1_gemm_kernel<true, LORA_NONE> : b1_gemm_kernel<false, LORA_NONE>;
 }
 
 // Largest number of co-resident pair clusters (one per TPC when every SM
 // takes one CTA of the pair kernel); 0 if the query fails.
-int pair_cluster_slots(bool bf16, bool delta) {
+int pair_cluster_slots(bool bf16, int lora) {
   struct Slots {
     int n[4] = {-1, -1, -1, -1};
   };
   static Slots slots[64];
   static std::mutex mu;
   std::lock_guard<std::mutex> lock(mu);
-  int& n = slots[device_slot()].n[(bf16 ? 1 : 0) + (delta ? 2 : 0)];
+  int& n = slots[device_slot()].n[lora == LORA_NONE ? (bf16 ? 1 : 0) : 1 + lora];
   if (n >= 0) return n;
-  auto k2 = pair_kernel(bf16, delta);
+  auto k2 = pair_kernel(bf16, lora);
   n = 0;
   if (cudaFuncSetAttribute(k2, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            gemm::pair::SMEM_BYTES) != cudaSuccess)
@@ -1071,6 +1237,27 @@ int launch_b1_unretile(const B1Weight& w, uint8_t* dev_packed, cudaStream_t st) 
   return launch_status("b1_unretile_kernel launch");
 }
 
+namespace {
+// Kernel choice: estimated time = waves x tile time, with a 256x256 pair
+// tile (two SMs) taking kPairTileCost 128x128-tile times of one SM (about
+// 2 x 1255 / 1536 from isolated measurements of the two kernels).
+bool prefer_pair(long long tiles1, long long tiles2, int ksplit, int slots) {
+  constexpr double kPairTileCost = 1.63;
+  const B1Kernel force = forced_kernel();
+  if (force != B1Kernel::Auto || slots < 1) return force == B1Kernel::Pair;
+  const double t1 = (double)((tiles1 + num_sms() - 1) / num_sms());
+  const double t2 = kPairTileCost * (double)((tiles2 * ksplit + slots - 1) / slots) / ksplit;
+  return t2 < t1;
+}
+}  // namespace
+
+int b1_gemm_tile_tokens(int tokens, const B1Weight& w, int lora_mode) {
+  const long long tt1 = (tokens + gemm::BN - 1) / gemm::BN, tt2 = (tokens + gemm::pair::BN - 1) / gemm::pair::BN;
+  return prefer_pair(w.n_ftiles * tt1, (w.n_ftiles + 1) / 2 * tt2, 1, pair_cluster_slots(false, lora_mode))
+             ? gemm::pair::BN
+             : gemm::BN;
+}
+
 // Set by bonsai_debug_stall_next_gemm, consumed by the next launch on the thread.
 thread_local bool g_stall_next_gemm = false;
 
@@ -1104,7 +1291,7 @@ int launch_b1_gemv_f32(const float* x, const B1Weight& w, float* y, cudaStream_t
 }
 
 int launch_b1_gemm(const void* x, long long ldx, int tokens, const B1Weight& w, const EpiSeg* segs,
-                   int nseg, bool x_bf16, cudaStream_t st, const TileSel* sel, const float* delta) {
+                   int nseg, bool x_bf16, cudaStream_t st, const TileSel* sel, const LoraGemm* lora) {
   if (tokens < 0) return fail(-1, "b1_gemm: negative token count");
   if (tokens == 0) return 0;
   if (!x || !w.chunks) return fail(-1, "b1_gemm: null activation or weight");
@@ -1137,15 +1324,13 @@ int launch_b1_gemm(const void* x, long long ldx, int tokens, const B1Weight& w, 
     routed = true;
   }
 
-  // Kernel choice: estimated time = waves x tile time, with a 256x256 pair
-  // tile (two SMs) taking kPairTileCost 128x128-tile times of one SM (about
-  // 2 x 1255 / 1536 from isolated measurements of the two kernels).
-  const int slots = pair_cluster_slots(x_bf16, delta != nullptr);
+  const int lmode = lora ? lora->mode : LORA_NONE;
+  if (lmode != LORA_NONE && (x_bf16 || sel)) return fail(-1, "b1_gemm: low-rank products need f16 activations and all rows");
+  const int slots = pair_cluster_slots(x_bf16, lmode);
   const int n_tt1 = (tokens + gemm::BN - 1) / gemm::BN;
   const int n_tt2 = (tokens + gemm::pair::BN - 1) / gemm::pair::BN;
   const long long tiles1 = (long long)nf * n_tt1;
   const long long tiles2 = (long long)((nf + 1) / 2) * n_tt2;
-  constexpr double kPairTileCost = 1.63;
   // K split of the pair kernel: only for launches whose every segment is a
   // gate-residual that allows it (split_ok: the partitioned multi-GPU step),
   // where doubling the work units fills the last wave of clusters better
@@ -1158,8 +1343,8 @@ int launch_b1_gemm(const void* x, long long ldx, int tokens, const B1Weight& w, 
     all_split_ok = all_split_ok && segs[i].mode == EPI_RESID_F32 && segs[i].split_ok;
   }
   int ksplit = 1;
-  if (delta) {
-    // whole K: the parts of a split would each add the delta
+  if (lmode != LORA_NONE) {
+    // whole K in one CTA (pair): the low-rank part is added once
   } else if (const char* e = getenv("BONSAI_B1_SPLITK")) {
     if (all_resid) ksplit = std::max(1, std::min(atoi(e), std::max(1, w.k_blocks / 2)));
   } else if (all_split_ok && w.k_blocks >= 16 && slots >= 1 && tiles2 >= slots) {
@@ -1172,19 +1357,31 @@ int launch_b1_gemm(const void* x, long long ldx, int tokens, const B1Weight& w, 
     // tiles keep the result bit-identical to the unpartitioned forward
     if (half < 0.8 * whole) ksplit = 2;
   }
-  bool use_pair = false;
-  const B1Kernel force = forced_kernel();
   const bool stall = g_stall_next_gemm;  // test hook: this launch runs the one-CTA kernel idle
   g_stall_next_gemm = false;
+  bool use_pair = false;
   if (stall) {
     use_pair = false;
-  } else if (force == B1Kernel::Pair) {
-    if (slots < 1) return fail(-3, "b1_gemm: the pair kernel cannot be scheduled on this device");
-    use_pair = true;
-  } else if (force == B1Kernel::Auto && slots >= 1) {
-    const double t1 = (double)((tiles1 + num_sms() - 1) / num_sms());
-    const double t2 = kPairTileCost * (double)((tiles2 * ksplit + slots - 1) / slots) / ksplit;
-    use_pair = t2 < t1;
+  } else if (lmode == LORA_BLOCKS) {
+    use_pair = lora->tile_tokens == gemm::pair::BN;  // the blocks were laid out for these tiles
+    if (use_pair && slots < 1) return fail(-3, "b1_gemm: the pair kernel cannot be scheduled on this device");
+  } else {
+    if (forced_kernel() == B1Kernel::Pair && slots < 1)
+      return fail(-3, "b1_gemm: the pair kernel cannot be scheduled on this device");
+    use_pair = prefer_pair(tiles1, tiles2, ksplit, slots);
+  }
+
+  // With a low-rank product, an f32 result of a long K is accumulated in
+  // parts of at most kPartBlocks k-blocks, summed in f32 by the epilogue: the
+  // tensor core's own f32 additions truncate, an error that grows with their
+  // number (K = 9216 in one part: 9.8e-6 of the result, against 1.7e-6 of a
+  // plain f32 product).  An f16 result is rounded at 2^-11 anyway: one part.
+  constexpr int kPartBlocks = 24;
+  int kparts = 1, kpart = w.k_blocks;
+  if (lmode != LORA_NONE && (segs[0].mode == EPI_F32 || segs[0].mode == EPI_RESID_F32)) {
+    kparts = (w.k_blocks + kPartBlocks - 1) / kPartBlocks;
+    kpart = (w.k_blocks + kparts - 1) / kparts;
+    kparts = (w.k_blocks + kpart - 1) / kpart;
   }
 
   double out_bytes = 0;
@@ -1220,8 +1417,10 @@ int launch_b1_gemm(const void* x, long long ldx, int tokens, const B1Weight& w, 
     q.err = device_error_word();
     q.fence_sys = routed ? 1 : 0;
     q.n_rows = w.n_rows;
-    q.delta = delta;
-    auto k2 = pair_kernel(x_bf16, delta != nullptr);
+    if (lora) q.lora = *lora;
+    q.kparts = kparts;
+    q.kpart = kpart;
+    auto k2 = pair_kernel(x_bf16, lmode);
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1261,13 +1460,14 @@ int launch_b1_gemm(const void* x, long long ldx, int tokens, const B1Weight& w, 
   p.err = device_error_word();
   p.fence_sys = routed ? 1 : 0;
   p.idle_loads = stall ? 1 : 0;
-  p.delta = delta;
+  if (lora) p.lora = *lora;
+  p.kparts = kparts;
+  p.kpart = kpart;
 
   const int grid = (int)std::min<long long>(tiles1, num_sms());
-  auto kern = delta ? (x_bf16 ? gemm::b1_gemm_kernel<true, true> : gemm::b1_gemm_kernel<false, true>)
-                    : (x_bf16 ? gemm::b1_gemm_kernel<true, false> : gemm::b1_gemm_kernel<false, false>);
+  auto kern = single_kernel(x_bf16, lmode);
   static bool attr_set[64][4] = {};
-  bool& attr_done = attr_set[device_slot()][(x_bf16 ? 1 : 0) + (delta ? 2 : 0)];
+  bool& attr_done = attr_set[device_slot()][lmode == LORA_NONE ? (x_bf16 ? 1 : 0) : 1 + lmode];
   if (!attr_done) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          gemm::SMEM_BYTES);

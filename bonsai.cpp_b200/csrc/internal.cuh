@@ -109,14 +109,34 @@ struct TileSel {
   int base[kMaxTileGroups] = {0, 0, 0};
 };
 
+// The low-rank product beside a B1_0 GEMM.
+enum LoraMode : int { LORA_NONE = 0, LORA_DELTA = 1, LORA_BLOCKS = 2 };
+struct LoraGemm {
+  int mode = LORA_NONE;
+  // LORA_DELTA: f32 [tokens][n_rows], added to the accumulator
+  const float* delta = nullptr;
+  // LORA_BLOCKS: extra k-blocks of four 16-column groups, laid out for tiles
+  // of tile_tokens (b1_gemm_tile_tokens).  Token tile i has
+  // group_count[i] groups {slot | remainder << 30, first rank, first token,
+  // end token} at groups + i * max_groups; weight columns from up
+  // [slot][n_rows][r_pad], activations from low f32 [tokens][r_pad].
+  const int* group_count = nullptr;
+  const int4* groups = nullptr;
+  int tile_tokens = 0, max_groups = 0, r_pad = 0;
+  const __half* up = nullptr;
+  const float* low = nullptr;
+};
+
 // Launch the tcgen05 B1_0 GEMM: for every token t < tokens and weight row n,
 // acc[t][n] = sum_k x[t][k] * W[n][k]; acc is routed through the segment that
 // covers n.  x is f16 (or bf16 when x_bf16) row-major with leading dimension
-// ldx (elements); it must be 16-byte aligned with ldx % 8 == 0.  delta
-// (optional): f32 [tokens][n_rows], added to acc before the epilogue's mode.
+// ldx (elements); it must be 16-byte aligned with ldx % 8 == 0.  lora
+// (optional): a low-rank product added to acc before the epilogue's mode.
 int launch_b1_gemm(const void* x, long long ldx, int tokens, const B1Weight& w,
                    const EpiSeg* segs, int nseg, bool x_bf16, cudaStream_t st,
-                   const TileSel* sel = nullptr, const float* delta = nullptr);
+                   const TileSel* sel = nullptr, const LoraGemm* lora = nullptr);
+// Tokens per tile of the launch that launch_b1_gemm would make (128 or 256).
+int b1_gemm_tile_tokens(int tokens, const B1Weight& w, int lora_mode);
 
 // ------------------------------------------------- low-rank adapters
 struct LoraSlot {

@@ -5,14 +5,23 @@
 //
 // A 1-bit weight cannot take an adapter in (its entries are +-scale), so the
 // low-rank product runs beside it.
-//   lora_shrink_kernel   low[t][r] = scale_a * sum_k A_a[r][k] x[t][k]   (f32)
-//   lora_expand_kernel   delta[t][n] = sum_r B_a[n][r] low[t][r]         (f32)
-//   B1_0 GEMM            acc += delta in the epilogue, before its mode
-// low and delta stay in f32: nothing between x and the epilogue's own
-// rounding is rounded.
+// Two forms, chosen by the tokens per request:
+//   few (decoding): low[t][r] = scale_a * sum_k A_a[r][k] x[t][k] by
+//     lora_shrink_kernel, delta[t][n] = sum_r B_a[n][r] low[t][r] by
+//     lora_expand_kernel, and the B1_0 GEMM's epilogue adds delta: both are
+//     bound by reading the adapters once.
+//   many (prompts, images): low by lora_shrink_tile_kernel (tcgen05), and
+//     the B1_0 GEMM takes scale_a B_a low as extra k-blocks of its own
+//     products, listed by lora_plan_kernel: no second pass over y.
+// low (and delta) stay in f32; as a tensor-core operand low is two f16 values
+// (22 bits), so nothing between x and the epilogue's own rounding is rounded
+// further.
 #include "internal.cuh"
 
+#include "ptx.cuh"
+
 #include <cooperative_groups.h>
+#include <cudaTypedefs.h>
 
 #include <algorithm>
 #include <mutex>
@@ -20,6 +29,8 @@
 namespace cg = cooperative_groups;
 
 namespace bonsai {
+int encode_tmap_2d_16b(CUtensorMap* map, const void* base, long long rows, long long cols, long long ld,
+                       int box_cols, int box_rows, bool bf16);
 namespace lora {
 
 constexpr int kThreads = 256;
@@ -77,20 +88,18 @@ __device__ bool find_request(const int* cu, int n, int tokens, int size, int u, 
   return false;
 }
 
-// A cluster of CTAs takes one tile of 16 * MW tokens of one request; the
-// CTAs split K between them, and the 8 / MW warps of each 16-token row of
-// warps split the CTA's share.  x and A go from global memory straight into
+// ---- the form for few tokens per request
+// A cluster of CTAs takes one tile of 16 tokens of one request; the CTAs split
+// K between them, and their warps split the CTA's share.  x and A go from global memory straight into
 // the fragments of mma.m16n8k16: the order of k within a step is free as long
 // as both operands share it, so each thread takes 8 consecutive k of its row
-// (one 16-byte load) for two steps.  Bound by reading A (few tokens) or x
-// (many).  Partial sums meet in shared memory, then across the cluster, in a
+// (one 16-byte load) for two steps.  Bound by reading A.  Partial sums meet in shared memory, then across the cluster, in a
 // fixed order.
-template <int NT, int MW>  // NT: 8-rank tiles held
+template <int NT>  // 8-rank tiles held
 __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const ShrinkParams p) {
-  constexpr int KW = kWarps / MW;
-  constexpr int TM = 16 * MW;
+  constexpr int TM = 16;
   constexpr int R = NT * 8;
-  extern __shared__ float red[];  // [KW][TM][R]
+  extern __shared__ float red[];  // [kWarps][TM][R]
   __shared__ int found[2];
   cg::cluster_group cluster = cg::this_cluster();
   const int csize = (int)cluster.num_blocks(), crank = (int)cluster.block_rank();
@@ -114,9 +123,8 @@ __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const ShrinkParam
   const int end = min(p.cu[req + 1], p.tokens);
   const int t0 = max(0, p.cu[req]) + found[1] * TM;
 
-  const int mw = warp % MW, kw = warp / MW;
   const int g = lane >> 2, c = lane & 3;
-  const int ta = t0 + mw * 16 + g, tb = ta + 8;
+  const int ta = t0 + g, tb = ta + 8;
   const __half* xa = p.x + (size_t)ta * p.ldx + c * 8;
   const __half* xb = p.x + (size_t)tb * p.ldx + c * 8;
   const __half* aw = p.down + ((size_t)slot * p.r_pad + g) * p.k_in + c * 8;
@@ -127,7 +135,7 @@ __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const ShrinkParam
   float acc[NT][4] = {};
   const uint4 zero = make_uint4(0, 0, 0, 0);
 #pragma unroll 2
-  for (int ch = c0 + kw; ch < c1; ch += KW) {
+  for (int ch = c0 + warp; ch < c1; ch += kWarps) {
     const uint4 va = ta < end ? *reinterpret_cast<const uint4*>(xa + ch * kChunk) : zero;
     const uint4 vb = tb < end ? *reinterpret_cast<const uint4*>(xb + ch * kChunk) : zero;
     uint4 w[NT];
@@ -140,10 +148,10 @@ __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const ShrinkParam
       mma_f16(acc[i], va.z, vb.z, va.w, vb.w, w[i].z, w[i].w);
     }
   }
-  // accumulator i: rows g, g + 8 of the warp's 16 tokens, ranks 8 i + 2 c, + 1
+  // accumulator i: tokens g, g + 8, ranks 8 i + 2 c, + 1
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
-    float* d = red + ((size_t)kw * TM + mw * 16 + g) * R + i * 8 + c * 2;
+    float* d = red + ((size_t)warp * TM + g) * R + i * 8 + c * 2;
     d[0] = acc[i][0];
     d[1] = acc[i][1];
     d[8 * R] = acc[i][2];
@@ -153,7 +161,7 @@ __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const ShrinkParam
   for (int e = threadIdx.x; e < TM * R; e += kThreads) {
     float s = red[e];
 #pragma unroll
-    for (int k = 1; k < KW; ++k) s += red[k * TM * R + e];
+    for (int k = 1; k < kWarps; ++k) s += red[k * TM * R + e];
     red[e] = s;
   }
   cluster.sync();
@@ -241,11 +249,243 @@ __global__ void __launch_bounds__(kThreads) lora_expand_kernel(const ExpandParam
     if (t0 + j < p.tokens) p.delta[(size_t)(t0 + j) * p.n_rows + n] = acc[j];
 }
 
-template <int NT, int MW>
+// ---- the form for many tokens per request
+namespace tile {
+constexpr int BM = 128;     // tokens
+constexpr int BK = 64;      // inputs per stage
+constexpr int STAGES = 4;
+constexpr int X_BYTES = BM * BK * 2;
+constexpr int NUM_THREADS = 192;  // TMA, MMA, 4 epilogue warps
+constexpr int TMEM_COLS = 128;
+constexpr int kMaxRank = 128;
+
+// Shared memory of a launch: stages of x and A; the partial sums (f32
+// [r_pad][128 tokens]) take the stages' place once the products are done.
+inline int smem_bytes(int r_pad) {
+  return 1024 + std::max(STAGES * (X_BYTES + r_pad * BK * 2), r_pad * BM * 4) + 256;
+}
+}  // namespace tile
+
+// low of one 128-token tile of one request: x (128 x K) times A^T (K x rank) on
+// the tensor cores.  A cluster's CTAs split K (the tiles of a batch of prompts
+// are too few to fill the GPU otherwise) and add their parts through
+// distributed shared memory in a fixed order.  Bound by reading x.
+__global__ void __launch_bounds__(tile::NUM_THREADS)
+    lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap amap,
+                            const ShrinkParams p, int* err) {
+  using namespace tile;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int stage_bytes = X_BYTES + p.r_pad * BK * 2;
+  const int ring = max(STAGES * stage_bytes, p.r_pad * BM * 4);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + ring);
+  uint64_t* empty = full + STAGES;
+  uint64_t* done = empty + STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* found = reinterpret_cast<int*>(tmem_slot + 2);
+  float* sums = reinterpret_cast<float*>(smem);
+
+  cg::cluster_group cluster = cg::this_cluster();
+  const int csize = (int)cluster.num_blocks(), crank = (int)cluster.block_rank();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  if (warp == 0) {
+    int req = -1, tl = 0;
+    if (!find_request(p.cu, p.n_reqs, p.tokens, BM, (int)blockIdx.x / csize, req, tl)) req = -1;
+    if (lane == 0) {
+      found[0] = req;
+      found[1] = tl;
+    }
+  }
+  __syncthreads();
+  const int req = found[0];
+  if (req < 0) return;  // the whole cluster
+  const int slot = p.slots[req];
+  if (slot < 0 || slot >= p.n_slots) return;
+  const LoraSlot info = p.slot_info[slot];
+  if (info.rank == 0) return;
+  const int n16 = (info.rank + 15) / 16;
+  const int end = min(p.cu[req + 1], p.tokens);
+  const int t0 = max(0, p.cu[req]) + found[1] * BM;
+  const int blocks = (p.k_in + BK - 1) / BK, per = (blocks + csize - 1) / csize;
+  const int b0 = min(blocks, crank * per), b1 = min(blocks, b0 + per);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      bar_init(&full[s], 1);
+      bar_init(&empty[s], 1);
+    }
+    bar_init(done, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      bool ok = true;
+      for (int b = b0; b < b1; ++b) {
+        const int it = b - b0, s = it % STAGES;
+        if (!wait_bar(&empty[s], ((it / STAGES) & 1) ^ 1, abort_flag, err, DEV_ERR_TIMEOUT_TMA)) {
+          ok = false;
+          break;
+        }
+        uint8_t* st = smem + s * stage_bytes;
+        bar_arrive_expect_tx(&full[s], (uint32_t)(X_BYTES + n16 * 16 * BK * 2));
+        tma_load_2d(st, &xmap, &full[s], b * BK, t0);
+        for (int i = 0; i < n16; ++i)  // 16 ranks per box: only the slot's own
+          tma_load_2d(st + X_BYTES + i * 16 * BK * 2, &amap, &full[s], b * BK, slot * p.r_pad + i * 16);
+      }
+      if (!ok) {
+        const unsigned long long w0 = globaltimer_ns();
+        while (globaltimer_ns() - w0 < 1000000ull) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t idesc = make_idesc_f16(BM, n16 * 16, 0, 0, 0);
+      for (int b = b0; b < b1; ++b) {
+        const int it = b - b0, s = it % STAGES;
+        if (!wait_bar(&full[s], (it / STAGES) & 1, abort_flag, err, DEV_ERR_TIMEOUT_MMA)) break;
+        tc_fence_after();
+        const uint32_t xa = smem_u32(smem + s * stage_bytes), aa = xa + X_BYTES;
+#pragma unroll
+        for (int k16 = 0; k16 < BK / 16; ++k16)
+          mma_ss(tmem, make_smem_desc(xa + k16 * 32, 16, 1024), make_smem_desc(aa + k16 * 32, 16, 1024), idesc,
+                 (it | k16) != 0 ? 1u : 0u);
+        tc_commit(&empty[s]);
+      }
+      tc_commit(done);
+      const uint32_t da = smem_u32(done);
+      const unsigned long long w0 = globaltimer_ns();
+      while (!bar_try_wait(da, 0)) {
+        if (globaltimer_ns() - w0 > kWaitLimitNs) {
+          if (err) atomicCAS(err, 0, DEV_ERR_TIMEOUT_MMA);
+          break;
+        }
+      }
+    }
+  } else {
+    const int q = warp & 3;
+    const bool good = wait_bar(done, 0, abort_flag, err, DEV_ERR_TIMEOUT_EPILOGUE);
+    if (__all_sync(0xffffffffu, good)) {
+      tc_fence_after();
+      for (int c = 0; c < n16 * 16; c += 16) {
+        uint32_t r[16];
+        tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + c, r);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sums[(c + i) * BM + q * 32 + lane] = b1 > b0 ? __uint_as_float(r[i]) : 0.f;
+      }
+    }
+    tc_fence_before();
+  }
+  cluster.sync();
+  const int n = n16 * 16;
+  for (int e = crank * NUM_THREADS + threadIdx.x; e < n * BM; e += csize * NUM_THREADS) {
+    const int t = t0 + e % BM, r = e / BM;
+    float s = 0.f;
+    for (int c = 0; c < csize; ++c) s += cluster.map_shared_rank(sums, c)[e];
+    if (t < end) p.low[(size_t)t * p.r_pad + r] = info.scale * s;
+  }
+  cluster.sync();  // no CTA ends while another reads its shared memory
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// Lists the extra k-blocks of each token tile of the GEMM (LoraGemm): for
+// every request with an adapter that has tokens in the tile, its ranks in
+// groups of 16, first the values, then the remainders.  One warp per tile.
+__global__ void lora_plan_kernel(const int* __restrict__ cu, const int* __restrict__ slots, int n_reqs, int tokens,
+                                 const LoraSlot* __restrict__ slot_info, int n_slots, int tile_tokens, int n_tiles,
+                                 int max_groups, int* __restrict__ group_count, int4* __restrict__ groups) {
+  const int tile = (int)(blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32), lane = threadIdx.x & 31;
+  if (tile >= n_tiles) return;
+  const int t0 = tile * tile_tokens, t1 = min(tokens, t0 + tile_tokens);
+  int lo = 0, hi = n_reqs;  // the last request that begins at or before t0
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (cu[mid] <= t0) lo = mid; else hi = mid;
+  }
+  int base = 0;
+  for (int i0 = lo; i0 < n_reqs; i0 += 32) {
+    const int i = i0 + lane;
+    int slot = -1, n16 = 0, a = t1, b = t1;
+    if (i < n_reqs) {
+      a = max(t0, cu[i]);
+      b = min(t1, cu[i + 1]);
+      slot = slots[i];
+      if (a < b && slot >= 0 && slot < n_slots) n16 = (slot_info[slot].rank + 15) / 16;
+    }
+    int incl = 2 * n16;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    const int at = base + incl - 2 * n16;
+    for (int j = 0; j < 2 * n16; ++j)
+      if (at + j < max_groups)
+        groups[(size_t)tile * max_groups + at + j] =
+            make_int4(j < n16 ? slot : slot | (1 << 30), (j < n16 ? j : j - n16) * 16, a, b);
+    base += __shfl_sync(0xffffffffu, incl, 31);
+    // past the tile once a request of this round begins at or after its end
+    if (__any_sync(0xffffffffu, i < n_reqs && cu[i] >= t1)) break;
+  }
+  if (lane == 0) group_count[tile] = min(base, max_groups);
+}
+
+int shrink_tiles(const ShrinkParams& p, cudaStream_t st) {
+  CUtensorMap xmap, amap;
+  int rc = encode_tmap_2d_16b(&xmap, p.x, p.tokens, p.k_in, p.ldx, tile::BK, tile::BM, false);
+  if (!rc)
+    rc = encode_tmap_2d_16b(&amap, p.down, (long long)p.n_slots * p.r_pad, p.k_in, p.k_in, tile::BK, 16, false);
+  if (rc) return rc;
+  static std::once_flag once[64];
+  cudaError_t e = cudaSuccess;
+  std::call_once(once[device_slot()], [&] {
+    e = cudaFuncSetAttribute(lora_shrink_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             tile::smem_bytes(tile::kMaxRank));
+  });
+  if (e != cudaSuccess) return cuda_status(e, "lora shrink set smem attribute");
+  const long long seqs = std::min(p.n_reqs, p.tokens);
+  const long long units = (p.tokens + seqs * (tile::BM - 1)) / tile::BM;
+  int c = 8;  // CTAs that split K: about one per SM, each at least two stages
+  while (c > 1 && (units * c > 1ll * num_sms() || p.k_in / tile::BK < 2 * c)) c /= 2;
+  if (units * c > 0x7fffffffll) return fail(-2, "b1_gemm_lora: too many tokens in one call");
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)c;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)(units * c));
+  cfg.blockDim = dim3(tile::NUM_THREADS);
+  cfg.dynamicSmemBytes = (size_t)tile::smem_bytes(p.r_pad);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, lora_shrink_tile_kernel, xmap, amap, p, device_error_word());
+  if (e != cudaSuccess) return cuda_status(e, "lora_shrink_tile_kernel launch");
+  return launch_status("lora_shrink_tile_kernel launch");
+}
+
+template <int NT>
 int shrink(const ShrinkParams& p, cudaStream_t st) {
-  auto kern = lora_shrink_kernel<NT, MW>;
-  constexpr int TM = 16 * MW;
-  constexpr int smem = (kWarps / MW) * TM * NT * 8 * (int)sizeof(float);
+  auto kern = lora_shrink_kernel<NT>;
+  constexpr int TM = 16;
+  constexpr int smem = kWarps * TM * NT * 8 * (int)sizeof(float);
   static std::once_flag once[64];
   cudaError_t e = cudaSuccess;
   std::call_once(once[device_slot()],
@@ -255,7 +495,7 @@ int shrink(const ShrinkParams& p, cudaStream_t st) {
   const long long units = (p.tokens + seqs * (TM - 1)) / TM;
   // CTAs of a cluster split K: about two CTAs per SM, each warp at least one chunk
   int c = 8;
-  while (c > 1 && (units * c > 2ll * num_sms() || (p.k_in / kChunk) / c < kWarps / MW)) c /= 2;
+  while (c > 1 && (units * c > 2ll * num_sms() || (p.k_in / kChunk) / c < kWarps)) c /= 2;
   if (units * c > 0x7fffffffll) return fail(-2, "b1_gemm_lora: too many tokens in one call");
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
@@ -274,12 +514,11 @@ int shrink(const ShrinkParams& p, cudaStream_t st) {
   return launch_status("lora_shrink_kernel launch");
 }
 
-template <int MW>
 int shrink_by_rank(const ShrinkParams& p, int max_rank, cudaStream_t st) {
-  if (max_rank <= 16) return shrink<2, MW>(p, st);
-  if (max_rank <= 32) return shrink<4, MW>(p, st);
-  if (max_rank <= 64) return shrink<8, MW>(p, st);
-  return shrink<16, MW>(p, st);
+  if (max_rank <= 16) return shrink<2>(p, st);
+  if (max_rank <= 32) return shrink<4>(p, st);
+  if (max_rank <= 64) return shrink<8>(p, st);
+  return shrink<16>(p, st);
 }
 
 }  // namespace lora
@@ -288,12 +527,24 @@ int launch_b1_gemm_lora(const __half* x, long long ldx, int tokens, const B1Weig
                         const LoraDevice& set, const int* cu, const int* slots, int n_reqs, cudaStream_t st) {
   if (tokens == 0) return 0;
   if (n_reqs == 0) return launch_b1_gemm(x, ldx, tokens, w, &seg, 1, false, st);
+  LoraGemm g;
+  g.mode = tokens >= 32ll * n_reqs ? LORA_BLOCKS : LORA_DELTA;
+  // scratch: low, then delta or the lists of extra blocks
   const size_t low_n = ((size_t)tokens * set.r_pad + 3) / 4 * 4;
+  size_t more;
+  int n_tiles = 0;
+  if (g.mode == LORA_BLOCKS) {
+    g.tile_tokens = b1_gemm_tile_tokens(tokens, w, g.mode);
+    n_tiles = (tokens + g.tile_tokens - 1) / g.tile_tokens;
+    g.max_groups = 2 * (set.r_pad / 16) * std::min(n_reqs, g.tile_tokens);
+    more = (size_t)n_tiles * (g.max_groups * sizeof(int4) + sizeof(int));
+  } else {
+    more = (size_t)tokens * w.n_rows * sizeof(float);
+  }
   void* mem = nullptr;
-  int rc = scratch_alloc(&mem, (low_n + (size_t)tokens * w.n_rows) * sizeof(float), "b1_gemm_lora", st);
+  int rc = scratch_alloc(&mem, low_n * sizeof(float) + more, "b1_gemm_lora", st);
   if (rc) return rc;
-  float* scratch = static_cast<float*>(mem);
-  float* delta = scratch + low_n;
+  float* low = static_cast<float*>(mem);
   lora::ShrinkParams s{};
   s.x = x;
   s.ldx = ldx;
@@ -306,29 +557,42 @@ int launch_b1_gemm_lora(const __half* x, long long ldx, int tokens, const B1Weig
   s.cu = cu;
   s.slots = slots;
   s.n_reqs = n_reqs;
-  s.low = scratch;
-  // 64-token tiles where the requests are long enough to fill them
-  rc = tokens >= 32ll * n_reqs ? lora::shrink_by_rank<4>(s, set.max_rank, st)
-                                   : lora::shrink_by_rank<1>(s, set.max_rank, st);
-  if (rc == 0) {
-    lora::ExpandParams e{};
-    e.up = set.up;
-    e.slot_info = set.info;
-    e.n_slots = set.n_slots;
-    e.r_pad = set.r_pad;
-    e.n_rows = w.n_rows;
-    e.tokens = tokens;
-    e.cu = cu;
-    e.slots = slots;
-    e.n_reqs = n_reqs;
-    e.low = scratch;
-    e.delta = delta;
-    const dim3 grid((unsigned)((tokens + lora::kExpandTokens - 1) / lora::kExpandTokens),
-                    (unsigned)((w.n_rows + lora::kThreads - 1) / lora::kThreads));
-    lora::lora_expand_kernel<<<grid, lora::kThreads, 0, st>>>(e);
-    rc = launch_status("lora_expand_kernel launch");
+  s.low = low;
+  if (g.mode == LORA_BLOCKS) {
+    int4* groups = reinterpret_cast<int4*>(low + low_n);
+    int* count = reinterpret_cast<int*>(groups + (size_t)n_tiles * g.max_groups);
+    g.groups = groups;
+    g.group_count = count;
+    g.r_pad = set.r_pad;
+    g.up = set.up;
+    g.low = low;
+    lora::lora_plan_kernel<<<(unsigned)((n_tiles + 7) / 8), 256, 0, st>>>(
+        cu, slots, n_reqs, tokens, set.info, set.n_slots, g.tile_tokens, n_tiles, g.max_groups, count, groups);
+    rc = launch_status("lora_plan_kernel launch");
+    if (rc == 0) rc = lora::shrink_tiles(s, st);
+  } else {
+    g.delta = low + low_n;
+    rc = lora::shrink_by_rank(s, set.max_rank, st);
+    if (rc == 0) {
+      lora::ExpandParams e{};
+      e.up = set.up;
+      e.slot_info = set.info;
+      e.n_slots = set.n_slots;
+      e.r_pad = set.r_pad;
+      e.n_rows = w.n_rows;
+      e.tokens = tokens;
+      e.cu = cu;
+      e.slots = slots;
+      e.n_reqs = n_reqs;
+      e.low = low;
+      e.delta = low + low_n;
+      const dim3 grid((unsigned)((tokens + lora::kExpandTokens - 1) / lora::kExpandTokens),
+                      (unsigned)((w.n_rows + lora::kThreads - 1) / lora::kThreads));
+      lora::lora_expand_kernel<<<grid, lora::kThreads, 0, st>>>(e);
+      rc = launch_status("lora_expand_kernel launch");
+    }
   }
-  if (rc == 0) rc = launch_b1_gemm(x, ldx, tokens, w, &seg, 1, false, st, nullptr, delta);
+  if (rc == 0) rc = launch_b1_gemm(x, ldx, tokens, w, &seg, 1, false, st, nullptr, &g);
   scratch_free(mem, st);
   return rc;
 }
