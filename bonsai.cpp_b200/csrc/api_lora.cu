@@ -23,10 +23,11 @@ int bonsai_lora_create(int out_dim, int in_dim, int max_rank, int n_slots, int s
   s.max_rank = max_rank;
   s.r_pad = (max_rank + 15) / 16 * 16;
   s.n_slots = n_slots;
+  s.n_ftiles = (out_dim + 127) / 128;
   s.swiglu_from = swiglu_from < 0 ? -1 : swiglu_from;
   cudaGetDevice(&s.device);
   const size_t down = (size_t)n_slots * s.r_pad * in_dim * sizeof(__half);
-  const size_t up = (size_t)n_slots * s.r_pad * out_dim * sizeof(__half);
+  const size_t up = (size_t)n_slots * s.r_pad * s.n_ftiles * 128 * sizeof(__half);
   if (cudaMalloc(reinterpret_cast<void**>(&s.down), down) != cudaSuccess ||
       cudaMalloc(reinterpret_cast<void**>(&s.up), up) != cudaSuccess ||
       cudaMalloc(reinterpret_cast<void**>(&s.info), n_slots * sizeof(LoraSlot)) != cudaSuccess) {
@@ -57,24 +58,21 @@ int bonsai_lora_set(bonsai_lora_t h, int slot, const uint16_t* down, const uint1
   if (e != cudaSuccess) return cuda_status(e, "lora_set: cudaGetDevice");
   if (dev != s.device) return fail(BONSAI_ERR_ARG, "lora_set: the adapters live on device " + std::to_string(s.device));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const size_t row = (size_t)s.r_pad * sizeof(__half), width = (size_t)rank * sizeof(__half);
-  __half* d = s.down + (size_t)slot * s.r_pad * s.k_in;
-  __half* u = s.up + (size_t)slot * s.r_pad * s.n_rows;
   const LoraSlot info{rank, scale};
   if (rank > 0) {
-    e = cudaMemsetAsync(d, 0, row * s.k_in, st);
-    if (e == cudaSuccess) e = cudaMemsetAsync(u, 0, row * s.n_rows, st);
-    if (e == cudaSuccess) e = cudaMemcpyAsync(d, down, width * s.k_in, cudaMemcpyDefault, st);
-    // rows [swiglu_from, out) go to alternating device rows: gate, value, gate, ...
-    const int plain = s.swiglu_from < 0 ? s.n_rows : s.swiglu_from, half = (s.n_rows - plain) / 2;
-    auto rows = [&](int dst_row, int dst_step, int src_row, int n) {
-      if (n > 0 && e == cudaSuccess)
-        e = cudaMemcpy2DAsync(u + (size_t)dst_row * s.r_pad, row * dst_step, up + (size_t)src_row * rank, width, width,
-                              n, cudaMemcpyDefault, st);
-    };
-    rows(0, 1, 0, plain);
-    rows(plain, 2, plain, half);
-    rows(plain + 1, 2, plain + half, half);
+    __half* d = s.down + (size_t)slot * s.r_pad * s.k_in;
+    const size_t d_bytes = (size_t)rank * s.k_in * sizeof(__half), u_bytes = (size_t)rank * s.n_rows * sizeof(__half);
+    e = cudaMemsetAsync(d, 0, (size_t)s.r_pad * s.k_in * sizeof(__half), st);
+    if (e == cudaSuccess) e = cudaMemcpyAsync(d, down, d_bytes, cudaMemcpyDefault, st);
+    if (e != cudaSuccess) return cuda_status(e, "lora_set: copy");
+    void* staged = nullptr;
+    int rc = scratch_alloc(&staged, u_bytes, "lora_set", st);
+    if (rc) return rc;
+    e = cudaMemcpyAsync(staged, up, u_bytes, cudaMemcpyDefault, st);
+    rc = e == cudaSuccess ? launch_lora_retile(static_cast<const __half*>(staged), rank, s, slot, st)
+                          : cuda_status(e, "lora_set: copy");
+    scratch_free(staged, st);
+    if (rc) return rc;
   }
   if (e == cudaSuccess) e = cudaMemcpyAsync(s.info + slot, &info, sizeof(info), cudaMemcpyDefault, st);
   return cuda_status(e, "lora_set: copy");

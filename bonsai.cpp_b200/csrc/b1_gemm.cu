@@ -64,6 +64,24 @@ constexpr int NUM_THREADS = (WARP_EPI0 + EPI_WARPS) * 32;
 constexpr int SMEM_BYTES = 1024 /*align slack*/ + STAGES * X_STAGE_BYTES +
                            STAGES * RAW_STAGE_BYTES + 256 /*barriers etc*/;
 
+// LORA_BLOCKS: + the sums of the k-parts.
+constexpr int SMEM_BLOCKS_BYTES = SMEM_BYTES + BN * BM * 4;
+// LORA_DELTA: tiles of 64 tokens and fewer stages (few tokens: short loops)
+// leave room for the sums, each token's adapter, the low-rank values of the
+// CTA's tokens and each epilogue warp's ring of adapter pieces (its 32 rows x
+// 16 ranks: 1 KB).
+constexpr int DELTA_BN = 64;
+constexpr int DELTA_STAGES = 4;
+constexpr int DELTA_AHEAD = 12;
+constexpr int SMEM_DELTA_BYTES = 1024 + DELTA_STAGES * (DELTA_BN * BK * 2 + RAW_STAGE_BYTES) + 256 +
+                                 DELTA_BN * BM * 4 + DELTA_BN * 8 + DELTA_BN * 128 * 4 +
+                                 EPI_WARPS * DELTA_AHEAD * 1024;
+static_assert(SMEM_DELTA_BYTES <= 232448 && SMEM_BLOCKS_BYTES <= 232448, "shared memory of one CTA");
+
+// Barrier of the epilogue warps alone.
+__device__ __forceinline__ void epi_sync() {
+  asm volatile("bar.sync 1, %0;" ::"n"(EPI_WARPS * 32) : "memory");
+}
 __device__ __forceinline__ int sel_ftile(int fidx, int fcount, const int* fbase) {
   const int g = fidx / fcount;
   return fbase[g] + (fidx - g * fcount);
@@ -88,7 +106,9 @@ struct Params {
   // through its abort path with no copy or MMA in flight.  0 in normal use.
   int idle_loads;
   LoraGemm lora;  // kLora
-  int kparts, kpart;  // kLora: the tile's k-blocks in kparts accumulations of kpart
+  // kLora: k-blocks per accumulation (see kPartBlocks); LORA_DELTA: the CTAs of
+  // a cluster take kper k-blocks of one tile each
+  int kpart, kper;
 };
 
 __device__ __forceinline__ float tanh_hw(float x) {
@@ -129,42 +149,36 @@ __device__ __forceinline__ uint32_t bf16_from_f16_scale(uint32_t s16) {
   }
 }
 
-// kLora, the low-rank product beside W x: LORA_NONE; LORA_DELTA: an f32
-// matrix delta that the epilogue adds; LORA_BLOCKS: extra k-blocks whose
-// weight columns are columns of the adapters' B and whose activations are the
-// low-rank values of the tokens of one request (zero for the tile's others):
+// kLora, the low-rank product beside W x:
+// LORA_BLOCKS (many tokens per request): extra k-blocks whose weight columns
+// are columns of the adapters' B and whose activations are the low-rank
+// values of the tokens of one request (zero for the tile's others):
 //   [W | B_a B_a B_b ...] [x; low_a hi; low_a lo; low_b hi; ...].
 // The f32 low-rank values enter as two f16 (value and remainder), which keeps
 // 22 bits of them.
-
-// acc[j] of weight row `row`, tokens t0 + j (j < nt) += delta.  Lanes hold
-// consecutive rows, so each token is one coalesced read per warp.
-__device__ __forceinline__ void add_delta(uint32_t (&v)[32], const float* delta, int n_rows, int row,
-                                          int t0, int nt) {
-  if (row >= n_rows) return;
-  const float* d = delta + (size_t)t0 * n_rows + row;
-#pragma unroll
-  for (int j = 0; j < 32; ++j)
-    if (j < nt) v[j] = __float_as_uint(__uint_as_float(v[j]) + __ldg(d + (size_t)j * n_rows));
-}
+// LORA_DELTA (few tokens per request): the epilogue warps compute B low for
+// their rows and tokens in f32 while the products of W x run, reading each
+// adapter's rows once; a tile's k-blocks are split between the CTAs of a
+// cluster, since few tokens make few tiles (128 weight rows x all tokens).
+// The parts meet in shared memory, token by token, in a fixed order.
 
 // 16-column groups of the extra k-blocks of token tile `ttile`.
 template <int kLora>
 __device__ __forceinline__ int lora_groups(const LoraGemm& l, int ttile) {
   return kLora == LORA_BLOCKS ? __ldg(l.group_count + ttile) : 0;
 }
+// 128 weight rows x 16 ranks of an adapter's B, contiguous (LoraDevice::up).
+__device__ __forceinline__ const __half* lora_chunk(const LoraGemm& l, int slot, int ftile, int r0) {
+  return l.up + (((size_t)slot * l.n_ftiles + ftile) * (l.r_pad / 16) + r0 / 16) * (BM * 16);
+}
 // One 16-column group: this thread's weight row (8 words of two columns) and
 // its token's activations (8 words), zero where they are none of the group's.
-__device__ __forceinline__ void lora_group(const LoraGemm& l, const int4 e, int row, int n_rows, int tok,
+__device__ __forceinline__ void lora_group(const LoraGemm& l, const int4 e, int ftile, int r, int tok,
                                            uint32_t* w, uint32_t* x) {
   const int slot = e.x & 0x3fffffff;
   const bool lo = (e.x & 0x40000000) != 0;
-  uint4 b0 = make_uint4(0, 0, 0, 0), b1 = b0;
-  if (row < n_rows) {
-    const uint4* src = reinterpret_cast<const uint4*>(l.up + ((size_t)slot * n_rows + row) * l.r_pad + e.y);
-    b0 = __ldg(src);
-    b1 = __ldg(src + 1);
-  }
+  const uint4* wsrc = reinterpret_cast<const uint4*>(lora_chunk(l, slot, ftile, e.y) + r * 16);
+  const uint4 b0 = __ldg(wsrc), b1 = __ldg(wsrc + 1);
   w[0] = b0.x; w[1] = b0.y; w[2] = b0.z; w[3] = b0.w;
   w[4] = b1.x; w[5] = b1.y; w[6] = b1.z; w[7] = b1.w;
 #pragma unroll
@@ -173,7 +187,7 @@ __device__ __forceinline__ void lora_group(const LoraGemm& l, const int4 e, int 
     const float4* src = reinterpret_cast<const float4*>(l.low + (size_t)tok * l.r_pad + e.y);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float4 f = __ldg(src + i);
+      const float4 f = __ldcg(src + i);
       const __half2 h0 = __floats2half2_rn(f.x, f.y), h1 = __floats2half2_rn(f.z, f.w);
       if (!lo) {
         x[2 * i] = *reinterpret_cast<const uint32_t*>(&h0);
@@ -188,9 +202,151 @@ __device__ __forceinline__ void lora_group(const LoraGemm& l, const int4 e, int 
   }
 }
 
+// Adapter slot of token t (-1: none).
+__device__ __forceinline__ int lora_slot(const LoraGemm& l, int t) {
+  int lo = 0, hi = l.n_reqs;  // the last request that begins at or before t
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (__ldg(l.cu + mid) <= t) lo = mid; else hi = mid;
+  }
+  if (t < __ldg(l.cu + lo) || t >= __ldg(l.cu + lo + 1)) return -1;
+  const int slot = __ldg(l.slots + lo);
+  return slot >= 0 && slot < l.n_slots ? slot : -1;
+}
+// LORA_DELTA's first half of the epilogue, for the tokens t = rank + ncta * i
+// of a tile that this CTA finishes: delta[t] = sum_r B[row][r] low[t][r] (f32)
+// into psum [token][128 rows], zeros for the tokens of other CTAs.  Each half
+// of the 256 threads (one row each) takes every second token.  Bound by
+// reading B: every warp keeps DELTA_AHEAD pieces (its rows, 16 ranks of one
+// token) in flight across tokens, as asynchronous copies into a ring of its
+// own.  (Loads into registers, four ahead, were waited for together and took
+// three times as long, and so did bulk copies issued by one thread.)
+__device__ __forceinline__ void lora_delta(const LoraGemm& l, float* psum, int2* adapter, float* low, uint8_t* ring,
+                                           int rank, int ncta, int et, int ftile, int t0, int nt) {
+  if (et < nt) {
+    const int slot = lora_slot(l, t0 + et);
+    adapter[et] = make_int2(slot, slot >= 0 ? __ldg(&l.info[slot].rank) : 0);
+  }
+  griddep_wait();  // the low-rank values
+  epi_sync();
+  const int r4 = l.r_pad / 4;
+  for (int e = et; e < (nt + ncta - 1) / ncta * r4; e += EPI_WARPS * 32) {
+    const int i = e / r4, t = rank + i * ncta, r = e % r4 * 4;
+    if (t < nt)
+      *reinterpret_cast<float4*>(low + i * l.r_pad + r) =
+          r < adapter[t].y ? __ldcg(reinterpret_cast<const float4*>(l.low + (size_t)(t0 + t) * l.r_pad + r))
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  const int half = et >> 7, row = et & 127, lane = et & 31;
+  for (int t = half; t < nt; t += 2) psum[t * 128 + row] = 0.f;
+  epi_sync();
+
+  ring += (et >> 5) * DELTA_AHEAD * 1024;
+  const int toks = (nt - rank + ncta - 1) / ncta;  // of this CTA
+  int gi = half, gr = 0, gs = 0;  // next piece to ask for: token gi, ranks gr.., slot gs
+  auto ask = [&]() {
+    while (gi < toks && gr >= adapter[rank + gi * ncta].y) {
+      gi += 2;
+      gr = 0;
+    }
+    if (gi < toks) {
+      const __half* src = lora_chunk(l, adapter[rank + gi * ncta].x, ftile, gr) + (row & 96) * 16 + lane * 8;
+      const uint32_t dst = smem_u32(ring + gs * 1024) + lane * 16;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 512u), "l"(src + 256) : "memory");
+      gr += 16;
+      gs = gs + 1 == DELTA_AHEAD ? 0 : gs + 1;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  for (int u = 0; u < DELTA_AHEAD; ++u) ask();
+  int us = 0;
+  for (int i = half; i < toks; i += 2) {
+    const int ranks = adapter[rank + i * ncta].y;
+    const float* x = low + i * l.r_pad;
+    float acc0 = 0.f, acc1 = 0.f;
+    for (int r0 = 0; r0 < ranks; r0 += 16) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(DELTA_AHEAD - 1) : "memory");
+      __syncwarp();
+      const uint4* b = reinterpret_cast<const uint4*>(ring + us * 1024 + lane * 32);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint4 v = b[k];
+        const float4 x0 = *reinterpret_cast<const float4*>(x + r0 + 8 * k);
+        const float4 x1 = *reinterpret_cast<const float4*>(x + r0 + 8 * k + 4);
+        const float2 b0 = __half22float2(*reinterpret_cast<const __half2*>(&v.x));
+        const float2 b1 = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+        const float2 b2 = __half22float2(*reinterpret_cast<const __half2*>(&v.z));
+        const float2 b3 = __half22float2(*reinterpret_cast<const __half2*>(&v.w));
+        acc0 = fmaf(b0.x, x0.x, acc0);
+        acc1 = fmaf(b0.y, x0.y, acc1);
+        acc0 = fmaf(b1.x, x0.z, acc0);
+        acc1 = fmaf(b1.y, x0.w, acc1);
+        acc0 = fmaf(b2.x, x1.x, acc0);
+        acc1 = fmaf(b2.y, x1.y, acc1);
+        acc0 = fmaf(b3.x, x1.z, acc0);
+        acc1 = fmaf(b3.y, x1.w, acc1);
+      }
+      __syncwarp();  // every lane has read the piece: its place may be filled again
+      us = us + 1 == DELTA_AHEAD ? 0 : us + 1;
+      ask();
+    }
+    psum[(rank + i * ncta) * 128 + row] = acc0 + acc1;
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// LORA_DELTA's second half of the epilogue: the tokens of this CTA (rank of
+// the cluster's CTAs), summed over the CTAs' partial sums [token][128 rows]
+// and written by mode.  256 threads: one row, every second of the tokens.
+__device__ __forceinline__ void lora_finish(const EpiSeg& sg, const float* psum, int rank, int ncta, int et,
+                                            int row0, int n_rows, int t0, int nt) {
+  const int row = row0 + (et & 127);
+  const uint32_t base = smem_u32(psum) + (uint32_t)(et & 127) * 4u;
+  const float gate = sg.mode == EPI_RESID_F32 && sg.gate && row < n_rows ? sg.gate[row] : 1.0f;
+  constexpr int kBatch = 8;  // tokens whose reads (other CTAs' shared memory) are in flight together
+  for (int tb = rank + ncta * (et >> 7); tb < nt; tb += 2 * ncta * kBatch) {
+    float sum[kBatch] = {};
+    for (int c = 0; c < ncta; ++c) {
+      const uint32_t peer = mapa_shared(base, (uint32_t)c);
+      float x[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int t = min(tb + 2 * ncta * i, nt - 1);
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x[i]) : "r"(peer + (uint32_t)t * 512u) : "memory");
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) sum[i] += x[i];
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int t = tb + 2 * ncta * i;
+      if (t >= nt) break;
+      const float v = sum[i];
+      const size_t at = (size_t)(t0 + t) * sg.ld;
+      if (sg.mode == EPI_SWIGLU_F16) {  // rows alternate gate, value
+        const float o = __shfl_xor_sync(0xffffffffu, v, 1);
+        if (row < n_rows && (row & 1) == 0)
+          reinterpret_cast<__half*>(sg.dst)[at + (row >> 1)] = __float2half_rn(silu(v) * o);
+      } else if (row < n_rows) {
+        if (sg.mode == EPI_F32) reinterpret_cast<float*>(sg.dst)[at + row] = v;
+        if (sg.mode == EPI_F16) reinterpret_cast<__half*>(sg.dst)[at + row] = __float2half_rn(v);
+        if (sg.mode == EPI_GELU_F16) reinterpret_cast<__half*>(sg.dst)[at + row] = __float2half_rn(gelu_tanh(v));
+        if (sg.mode == EPI_RESID_F32) {
+          float* d = reinterpret_cast<float*>(sg.dst) + at + row;
+          *d = fmaf(gate, v, *d);
+        }
+      }
+    }
+  }
+}
+
 template <bool kBF16, int kLora>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
     b1_gemm_kernel(const __grid_constant__ CUtensorMap xmap, const Params p) {
+  constexpr int STAGES = kLora == LORA_DELTA ? DELTA_STAGES : gemm::STAGES;
+  constexpr int BN = kLora == LORA_DELTA ? DELTA_BN : gemm::BN;
+  constexpr int X_STAGE_BYTES = BN * BK * 2;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
@@ -204,6 +360,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   uint64_t* drain = dempty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  // Sums of the k-parts, [token][128 rows] (kLora); LORA_DELTA: then the
+  // tokens' adapters (slot, rank; rank 0: none) and low-rank values
+  float* psum = reinterpret_cast<float*>(smem + STAGES * (X_STAGE_BYTES + RAW_STAGE_BYTES) + 256);
+  int2* adapter = reinterpret_cast<int2*>(psum + BN * BM);
+  float* low = reinterpret_cast<float*>(adapter + BN);
+  uint8_t* ring = reinterpret_cast<uint8_t*>(low + BN * 128);
 
   const int warp = threadIdx.x / 32;
   const uint32_t lane = lane_id();
@@ -232,18 +395,28 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const uint32_t tmem = *tmem_slot;
 
   const int k_blocks = p.k_blocks;
+  // LORA_DELTA: this CTA's tile step and k-blocks [kr0, kr1) of it
+  constexpr bool kSplit = kLora == LORA_DELTA;
+  const int ncta = kSplit ? (k_blocks + p.kper - 1) / p.kper : 1;
+  const int crank = kSplit ? (int)cluster_ctarank() : 0;
+  const int tile0 = kSplit ? (int)blockIdx.x / ncta : (int)blockIdx.x;
+  const int tstep = kSplit ? (int)gridDim.x / ncta : (int)gridDim.x;
+  const int kr0 = kSplit ? crank * p.kper : 0;
+  const int kr1 = kSplit ? min(k_blocks, kr0 + p.kper) : k_blocks;
+  const int parts = kLora != LORA_NONE ? (kr1 - kr0 + p.kpart - 1) / p.kpart : 1;
+  if constexpr (kLora != LORA_NONE) griddep_launch();
 
   if (warp == WARP_TMA) {
     if (elect_one() && !p.idle_loads) {
       tma_prefetch_desc(&xmap);
       uint32_t it = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < p.num_tiles && ok; tile += gridDim.x) {
+      for (int tile = tile0; tile < p.num_tiles && ok; tile += tstep) {
         const int ttile = tile / p.nf;
         const int ftile = sel_ftile(tile - ttile * p.nf, p.fcount, p.fbase);
         const uint32_t* wsrc = p.chunks + (size_t)ftile * k_blocks * kChunkWords;
-        const int nkb = k_blocks + (lora_groups<kLora>(p.lora, ttile) + 3) / 4;
-        for (int kb = 0; kb < nkb; ++kb, ++it) {
+        const int nkb = kr1 + (lora_groups<kLora>(p.lora, ttile) + 3) / 4;
+        for (int kb = kr0; kb < nkb; ++kb, ++it) {
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1;
           if (!wait_bar(&empty[s], ph ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_TMA)) {
@@ -274,12 +447,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       constexpr uint32_t idesc = make_idesc_f16(BM, BN, kBF16 ? 1 : 0, 0, 0);
       uint32_t it = 0, lt = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < p.num_tiles && ok; tile += gridDim.x) {
+      for (int tile = tile0; tile < p.num_tiles && ok; tile += tstep) {
         const int groups = lora_groups<kLora>(p.lora, tile / p.nf);
-        const int nkb = k_blocks + (groups + 3) / 4;
-        const int parts = kLora != LORA_NONE ? p.kparts : 1;
+        const int nkb = kr1 + (groups + 3) / 4;
         for (int part = 0; part < parts && ok; ++part, ++lt) {
-        const int kb0 = part * p.kpart, kb1 = part + 1 < parts ? kb0 + p.kpart : nkb;
+        const int kb0 = kr0 + (kLora != LORA_NONE ? part * p.kpart : 0);
+        const int kb1 = part + 1 < parts ? kb0 + p.kpart : nkb;
         const uint32_t b = lt & 1;
         const uint32_t dph = (lt >> 1) & 1;
         if (!wait_bar(&dempty[b], dph ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)) {
@@ -333,11 +506,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     uint32_t it = 0;
     int pending = -1;  // stage whose tcgen05.st is in flight
     bool ok = true;
-    for (int tile = blockIdx.x; tile < p.num_tiles && ok; tile += gridDim.x) {
+    for (int tile = tile0; tile < p.num_tiles && ok; tile += tstep) {
       const int ttile = tile / p.nf;
       const int groups = lora_groups<kLora>(p.lora, ttile);
-      const int nkb = k_blocks + (groups + 3) / 4;
-      for (int kb = 0; kb < nkb; ++kb, ++it) {
+      const int nkb = kr1 + (groups + 3) / 4;
+      for (int kb = kr0; kb < nkb; ++kb, ++it) {
         if (it % EXP_PER_Q != slot) continue;
         const int s = it % STAGES;
         const uint32_t ph = (it / STAGES) & 1;
@@ -350,7 +523,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
         uint32_t v[32];
         if (kLora == LORA_BLOCKS && kb >= k_blocks) {
-          const int row = sel_ftile(tile - ttile * p.nf, p.fcount, p.fbase) * BM + r;
+          griddep_wait();  // the low-rank values
+          const int ftile = sel_ftile(tile - ttile * p.nf, p.fcount, p.fbase);
           const uint32_t xrow = smem_u32(xs + s * X_STAGE_BYTES) + (uint32_t)r * 128u;
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
@@ -358,7 +532,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             if (gi >= groups) break;  // its columns are not multiplied
             const int4 e = __ldg(p.lora.groups + (size_t)ttile * p.lora.max_groups + gi);
             uint32_t x[8];
-            lora_group(p.lora, e, row, p.n_rows, ttile * BN + r, v + 8 * g, x);
+            lora_group(p.lora, e, ftile, r, ttile * BN + r, v + 8 * g, x);
             st_shared_v4(xrow + (((2u * g) ^ (r & 7)) << 4), x[0], x[1], x[2], x[3]);
             st_shared_v4(xrow + (((2u * g + 1u) ^ (r & 7)) << 4), x[4], x[5], x[6], x[7]);
           }
@@ -389,14 +563,52 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       __syncwarp();
       if (lane == 0) bar_arrive(&full[pending]);
     }
+    if constexpr (kLora != LORA_NONE) griddep_wait();  // the grid ends after the ones before it
   } else if (warp >= WARP_EPI0 && warp < WARP_EPI0 + EPI_WARPS) {
     const int q = warp & 3;
     const int eh = (warp - WARP_EPI0) >> 2;  // which half of the token columns
     const uint32_t lane_base = (uint32_t)(q * 32) << 16;
     uint32_t lt = 0;
-    const int parts = kLora != LORA_NONE ? p.kparts : 1;
     bool up = true;  // no wait has expired
-    for (int tile = blockIdx.x; tile < p.num_tiles && up; tile += gridDim.x) {
+    if constexpr (kSplit) {
+      const int et = (int)threadIdx.x - WARP_EPI0 * 32;
+      for (int tile = tile0; tile < p.num_tiles; tile += tstep) {
+        const int ttile = tile / p.nf, t0 = ttile * BN, nt = min(BN, p.tokens - t0);
+        const int row0 = sel_ftile(tile - ttile * p.nf, p.fcount, p.fbase) * BM;
+        // B low of this CTA's tokens, while the products run
+        lora_delta(p.lora, psum, adapter, low, ring, crank, ncta, et, row0 / BM, t0, nt);
+        epi_sync();
+        for (int part = 0; part < parts; ++part, ++lt) {
+          const uint32_t b = lt & 1;
+          const bool good =
+              up && wait_bar(&dfull[b], (lt >> 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_EPILOGUE);
+          up = __all_sync(0xffffffffu, good);  // tcgen05.ld is warp-collective
+          if (!up) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int cc = 0; cc < BN / 32 / EPI_PER_Q; ++cc) {
+            const int c = eh * (BN / 32 / EPI_PER_Q) + cc;
+            if (c * 32 >= nt) break;
+            uint32_t v[32];
+            tmem_ld32(tmem + lane_base + D_COL0 + b * BN + c * 32, v);
+            tmem_wait_ld();
+            float* ps = psum + c * 32 * 128 + q * 32 + lane;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c * 32 + j < nt) ps[j * 128] += __uint_as_float(v[j]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(&dempty[b]);
+        }
+        if (ncta > 1) break;  // one tile per cluster: it goes on after the cluster's barrier
+        epi_sync();
+        if (*abort_flag) break;  // seen by every warp: it was set before the barrier
+        lora_finish(p.seg[0], psum, 0, 1, et, row0, p.n_rows, t0, nt);
+        epi_sync();
+      }
+    } else {
+    for (int tile = tile0; tile < p.num_tiles && up; tile += tstep) {
       const int ttile = tile / p.nf;
       const int ftile = sel_ftile(tile - ttile * p.nf, p.fcount, p.fbase);
       for (int part = 0; part < parts; ++part, ++lt) {
@@ -451,8 +663,17 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         tmem_wait_ld();
         const int t0 = ttile * BN + c * 32;
         const int nt = min(32, p.tokens - t0);
-        if constexpr (kLora == LORA_DELTA) {
-          if (part + 1 == parts) add_delta(v, p.lora.delta, p.n_rows, row, t0, nt);
+        if constexpr (kLora == LORA_BLOCKS) {
+          if (parts > 1) {  // this thread's own sums of the k-parts
+            float* ps = psum + c * 32 * 128 + q * 32 + lane;
+            if (part + 1 < parts) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) ps[j * 128] = __uint_as_float(v[j]) + (part > 0 ? ps[j * 128] : 0.f);
+              continue;
+            }
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + ps[j * 128]);
+          }
         }
         if (warp_swiglu) {
           // Rows are stored gate/value interleaved; the even lane owns the pair.
@@ -488,18 +709,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             for (int j = 0; j < 16; ++j)
               if (h16 + j < nt) dst[(h16 + j) * stride] = fmaf(gate, __uint_as_float(v[h16 + j]), old[j]);
           }
-        } else if (kLora != LORA_NONE && mode == EPI_F32 && part > 0) {
-          // the sum of the k-parts before, by this same thread
-          float* dst = reinterpret_cast<float*>(sg.dst) + base + (size_t)t0 * stride;
-#pragma unroll
-          for (int h16 = 0; h16 < 32; h16 += 16) {
-            float old[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) old[j] = h16 + j < nt ? dst[(h16 + j) * stride] : 0.f;
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (h16 + j < nt) dst[(h16 + j) * stride] = old[j] + __uint_as_float(v[h16 + j]);
-          }
         } else if (mode == EPI_F32) {
           float* dst = reinterpret_cast<float*>(sg.dst) + base + (size_t)t0 * stride;
 #pragma unroll
@@ -513,8 +722,20 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       }
     }
     if (p.fence_sys) __threadfence_system();  // peer stores ordered before the kernel's end
+    }
   }
 
+  if constexpr (kSplit) {
+    if (ncta > 1) {
+      cluster_sync_all();  // every CTA's partial sums are in its shared memory
+      if (warp >= WARP_EPI0 && !*abort_flag) {
+        const int ttile = tile0 / p.nf, t0 = ttile * BN;
+        lora_finish(p.seg[0], psum, crank, ncta, (int)threadIdx.x - WARP_EPI0 * 32,
+                    sel_ftile(tile0 - ttile * p.nf, p.fcount, p.fbase) * BM, p.n_rows, t0, min(BN, p.tokens - t0));
+      }
+      cluster_sync_all();  // no CTA ends while another reads its sums
+    }
+  }
   __syncthreads();
   if (warp == WARP_MMA) {
     tc_fence_after();
@@ -566,11 +787,10 @@ struct Params {
   int* err;
   int fence_sys;  // a segment stores to other GPUs: fence.sys after the epilogue's stores
   int n_rows;
-  LoraGemm lora;  // kLora (ksplit is 1)
-  int kparts, kpart;
+  LoraGemm lora;  // LORA_BLOCKS (ksplit is 1)
 };
 
-template <bool kBF16, int kLora>
+template <bool kBF16, int kLora>  // LORA_NONE or LORA_BLOCKS
 __global__ void __launch_bounds__(NUM_THREADS, 1)
     b1_gemm_pair_kernel(const __grid_constant__ CUtensorMap xmap, const Params p) {
   extern __shared__ uint8_t smem_raw[];
@@ -619,6 +839,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int k_blocks = p.k_blocks;
+  if constexpr (kLora != LORA_NONE) griddep_launch();
 
   if (warp == WARP_TMA) {
     if (elect_one()) {
@@ -667,10 +888,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         constexpr uint32_t idesc = make_idesc_f16(2 * BM, BN, kBF16 ? 1 : 0, 0, 0);
         uint32_t it = 0, lt = 0;
         bool ok = true;
-        for (int tile = cid; tile < p.num_tiles && ok; tile += ncl) {
+        for (int tile = cid; tile < p.num_tiles && ok; tile += ncl, ++lt) {
           const int groups = lora_groups<kLora>(p.lora, tile / p.ksplit / p.npf);
-          const int parts = kLora != LORA_NONE ? p.kparts : 1;
-          for (int part = 0; part < parts && ok; ++part, ++lt) {
           const uint32_t b = lt & 1;
           const uint32_t dph = (lt >> 1) & 1;
           if (!wait_bar(&dempty[b], dph ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)) {
@@ -679,14 +898,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           }
           tc_fence_after();
           const uint32_t d_tmem = tmem + b * BN;
-          int kb0, kb1;
-          if constexpr (kLora != LORA_NONE) {
-            kb0 = part * p.kpart;
-            kb1 = part + 1 < parts ? kb0 + p.kpart : k_blocks + (groups + 3) / 4;
-          } else {
-            kb0 = (tile % p.ksplit) * p.kchunk;
-            kb1 = min(k_blocks, kb0 + p.kchunk);
-          }
+          const int kb0 = (tile % p.ksplit) * p.kchunk;
+          const int kb1 = min(k_blocks, kb0 + p.kchunk) + (groups + 3) / 4;
           for (int kb = kb0; kb < kb1; ++kb, ++it) {
             const int s = it % STAGES;
             const uint32_t ph = (it / STAGES) & 1;
@@ -708,7 +921,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           }
           if (!ok) break;
           tc_commit_pair(&dfull[b], 0x3);
-          }
         }
         tc_commit_pair(drain, 0x3);
       }
@@ -750,8 +962,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           break;
         }
         if (kLora == LORA_BLOCKS && kb >= k_blocks) {
+          griddep_wait();  // the low-rank values
           const int fidx = min(2 * (tile - ttile * p.npf) + (int)rank, p.nf - 1);
-          const int row = sel_ftile(fidx, p.fcount, p.fbase) * BM + r;
+          const int ftile = sel_ftile(fidx, p.fcount, p.fbase);
           const uint32_t arow = smem_u32(as + s * A_STAGE_BYTES) + row_off;
           const uint32_t xrow = smem_u32(xs + s * X_STAGE_BYTES) + row_off;
 #pragma unroll
@@ -760,7 +973,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             if (gi >= groups) break;  // its columns are not multiplied
             const int4 e = __ldg(p.lora.groups + (size_t)ttile * p.lora.max_groups + gi);
             uint32_t w[8], x[8];
-            lora_group(p.lora, e, row, p.n_rows, ttile * BN + (int)rank * BNH + r, w, x);
+            lora_group(p.lora, e, ftile, r, ttile * BN + (int)rank * BNH + r, w, x);
             const uint32_t c0 = ((2u * q) ^ sw) << 4, c1 = ((2u * q + 1u) ^ sw) << 4;
             st_shared_v4(arow + c0, w[0], w[1], w[2], w[3]);
             st_shared_v4(arow + c1, w[4], w[5], w[6], w[7]);
@@ -786,25 +999,22 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if (lane == 0) bar_arrive_remote(full0 + (uint32_t)s * 8u);
       }
     }
+    if constexpr (kLora != LORA_NONE) griddep_wait();  // the grid ends after the ones before it
   } else if (warp >= WARP_EPI0 && warp < WARP_EPI0 + EPI_WARPS) {
     const int q = warp & 3;
     const int eh = (warp - WARP_EPI0) >> 2;
     const uint32_t lane_base = (uint32_t)(q * 32) << 16;
     const uint32_t dempty0 = mapa_shared(smem_u32(&dempty[0]), 0);
     uint32_t lt = 0;
-    const int parts = kLora != LORA_NONE ? p.kparts : 1;
-    bool up = true;  // no wait has expired
-    for (int tile = cid; tile < p.num_tiles && up; tile += ncl) {
+    for (int tile = cid; tile < p.num_tiles; tile += ncl, ++lt) {
       const int t2 = tile / p.ksplit;
       const int ttile = t2 / p.npf;
       const int pf = t2 - ttile * p.npf;
       const int fidx = 2 * pf + (int)rank;
-      for (int part = 0; part < parts; ++part, ++lt) {
       const uint32_t b = lt & 1;
       const uint32_t dph = (lt >> 1) & 1;
       const bool good = wait_bar(&dfull[b], dph, abort_flag, p.err, DEV_ERR_TIMEOUT_EPILOGUE);
-      up = __all_sync(0xffffffffu, good);
-      if (!up) break;
+      if (!__all_sync(0xffffffffu, good)) break;
       tc_fence_after();
 
       int si = -1;
@@ -852,9 +1062,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         tmem_wait_ld();
         const int t0 = ttile * BN + c * 32;
         const int nt = min(32, p.tokens - t0);
-        if constexpr (kLora == LORA_DELTA) {
-          if (si >= 0 && part + 1 == parts) add_delta(v, p.lora.delta, p.n_rows, row, t0, nt);
-        }
         if (warp_swiglu) {
           __half* dst = reinterpret_cast<__half*>(sg.dst) + base + (size_t)t0 * stride;
           const bool own = mode == EPI_SWIGLU_F16 && (rr & 1) == 0;
@@ -894,18 +1101,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             for (int j = 0; j < 16; ++j)
               if (h16 + j < nt) dst[(h16 + j) * stride] = fmaf(gate, __uint_as_float(v[h16 + j]), old[j]);
           }
-        } else if (kLora != LORA_NONE && mode == EPI_F32 && part > 0) {
-          // the sum of the k-parts before, by this same thread
-          float* dst = reinterpret_cast<float*>(sg.dst) + base + (size_t)t0 * stride;
-#pragma unroll
-          for (int h16 = 0; h16 < 32; h16 += 16) {
-            float old[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) old[j] = h16 + j < nt ? dst[(h16 + j) * stride] : 0.f;
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (h16 + j < nt) dst[(h16 + j) * stride] = old[j] + __uint_as_float(v[h16 + j]);
-          }
         } else if (mode == EPI_F32) {
           float* dst = reinterpret_cast<float*>(sg.dst) + base + (size_t)t0 * stride;
 #pragma unroll
@@ -916,7 +1111,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) bar_arrive_remote(dempty0 + b * 8u);
-      }
     }
     if (p.fence_sys) __threadfence_system();  // peer stores ordered before the kernel's end
   }
@@ -1177,7 +1371,6 @@ B1Kernel forced_kernel() {
 // The instantiation for a launch; low-rank products come with f16 activations only.
 auto pair_kernel(bool bf16, int lora) {
   using namespace gemm::pair;
-  if (lora == LORA_DELTA) return b1_gemm_pair_kernel<false, LORA_DELTA>;
   if (lora == LORA_BLOCKS) return b1_gemm_pair_kernel<false, LORA_BLOCKS>;
   return bf16 ? b1_gemm_pair_kernel<true, LORA_NONE> : b1_gemm_pair_kernel<false, LORA_NONE>;
 }
@@ -1188,16 +1381,58 @@ auto single_kernel(bool bf16, int lora) {
   return bf16 ? b1_gemm_kernel<true, LORA_NONE> : b1_gemm_kernel<false, LORA_NONE>;
 }
 
+// Largest number of co-resident clusters of `size` CTAs of the LORA_DELTA
+// kernel (a cluster lies within one GPC); 0 if the query fails.
+int delta_cluster_slots(int size) {
+  static int slots[64][9];
+  static bool known[64][9];
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lock(mu);
+  const int d = device_slot();
+  if (known[d][size]) return slots[d][size];
+  known[d][size] = true;
+  auto kern = single_kernel(false, LORA_DELTA);
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, gemm::SMEM_DELTA_BYTES) == cudaSuccess) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)size;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)size);
+    cfg.blockDim = dim3(gemm::NUM_THREADS);
+    cfg.dynamicSmemBytes = gemm::SMEM_DELTA_BYTES;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int c = 0;
+    if (cudaOccupancyMaxActiveClusters(&c, kern, &cfg) == cudaSuccess) slots[d][size] = c;
+  }
+  cudaGetLastError();
+  return slots[d][size];
+}
+
+// With a low-rank product, an f32 result of a long K is accumulated in parts
+// of at most kPartBlocks k-blocks, summed in f32 by the epilogue: the tensor
+// core's own f32 additions truncate, an error that grows with their number
+// (K = 9216 in one part: 9.8e-6 of the result, against 1.7e-6 of a plain f32
+// product).  An f16 result is rounded at 2^-11 anyway: one part.
+constexpr int kPartBlocks = 16;
+int lora_part(const B1Weight& w, int epi_mode) {
+  if ((epi_mode != EPI_F32 && epi_mode != EPI_RESID_F32) || w.k_blocks <= kPartBlocks) return w.k_blocks;
+  const int parts = (w.k_blocks + kPartBlocks - 1) / kPartBlocks;
+  return (w.k_blocks + parts - 1) / parts;
+}
+
 // Largest number of co-resident pair clusters (one per TPC when every SM
 // takes one CTA of the pair kernel); 0 if the query fails.
 int pair_cluster_slots(bool bf16, int lora) {
   struct Slots {
-    int n[4] = {-1, -1, -1, -1};
+    int n[3] = {-1, -1, -1};
   };
   static Slots slots[64];
   static std::mutex mu;
   std::lock_guard<std::mutex> lock(mu);
-  int& n = slots[device_slot()].n[lora == LORA_NONE ? (bf16 ? 1 : 0) : 1 + lora];
+  int& n = slots[device_slot()].n[lora == LORA_BLOCKS ? 2 : bf16 ? 1 : 0];
   if (n >= 0) return n;
   auto k2 = pair_kernel(bf16, lora);
   n = 0;
@@ -1251,9 +1486,12 @@ bool prefer_pair(long long tiles1, long long tiles2, int ksplit, int slots) {
 }
 }  // namespace
 
-int b1_gemm_tile_tokens(int tokens, const B1Weight& w, int lora_mode) {
+int b1_gemm_tile_tokens(int tokens, const B1Weight& w, int epi_mode) {
+  // sums in parts take the one-CTA kernel: a pair's 256-token tile leaves no
+  // shared memory for them
+  if (lora_part(w, epi_mode) < w.k_blocks) return gemm::BN;
   const long long tt1 = (tokens + gemm::BN - 1) / gemm::BN, tt2 = (tokens + gemm::pair::BN - 1) / gemm::pair::BN;
-  return prefer_pair(w.n_ftiles * tt1, (w.n_ftiles + 1) / 2 * tt2, 1, pair_cluster_slots(false, lora_mode))
+  return prefer_pair(w.n_ftiles * tt1, (w.n_ftiles + 1) / 2 * tt2, 1, pair_cluster_slots(false, LORA_BLOCKS))
              ? gemm::pair::BN
              : gemm::BN;
 }
@@ -1327,7 +1565,8 @@ int launch_b1_gemm(const void* x, long long ldx, int tokens, const B1Weight& w, 
   const int lmode = lora ? lora->mode : LORA_NONE;
   if (lmode != LORA_NONE && (x_bf16 || sel)) return fail(-1, "b1_gemm: low-rank products need f16 activations and all rows");
   const int slots = pair_cluster_slots(x_bf16, lmode);
-  const int n_tt1 = (tokens + gemm::BN - 1) / gemm::BN;
+  const int bn1 = lmode == LORA_DELTA ? gemm::DELTA_BN : gemm::BN;
+  const int n_tt1 = (tokens + bn1 - 1) / bn1;
   const int n_tt2 = (tokens + gemm::pair::BN - 1) / gemm::pair::BN;
   const long long tiles1 = (long long)nf * n_tt1;
   const long long tiles2 = (long long)((nf + 1) / 2) * n_tt2;
@@ -1362,6 +1601,8 @@ int launch_b1_gemm(const void* x, long long ldx, int tokens, const B1Weight& w, 
   bool use_pair = false;
   if (stall) {
     use_pair = false;
+  } else if (lmode == LORA_DELTA) {
+    use_pair = false;
   } else if (lmode == LORA_BLOCKS) {
     use_pair = lora->tile_tokens == gemm::pair::BN;  // the blocks were laid out for these tiles
     if (use_pair && slots < 1) return fail(-3, "b1_gemm: the pair kernel cannot be scheduled on this device");
@@ -1369,19 +1610,6 @@ int launch_b1_gemm(const void* x, long long ldx, int tokens, const B1Weight& w, 
     if (forced_kernel() == B1Kernel::Pair && slots < 1)
       return fail(-3, "b1_gemm: the pair kernel cannot be scheduled on this device");
     use_pair = prefer_pair(tiles1, tiles2, ksplit, slots);
-  }
-
-  // With a low-rank product, an f32 result of a long K is accumulated in
-  // parts of at most kPartBlocks k-blocks, summed in f32 by the epilogue: the
-  // tensor core's own f32 additions truncate, an error that grows with their
-  // number (K = 9216 in one part: 9.8e-6 of the result, against 1.7e-6 of a
-  // plain f32 product).  An f16 result is rounded at 2^-11 anyway: one part.
-  constexpr int kPartBlocks = 24;
-  int kparts = 1, kpart = w.k_blocks;
-  if (lmode != LORA_NONE && (segs[0].mode == EPI_F32 || segs[0].mode == EPI_RESID_F32)) {
-    kparts = (w.k_blocks + kPartBlocks - 1) / kPartBlocks;
-    kpart = (w.k_blocks + kparts - 1) / kparts;
-    kparts = (w.k_blocks + kpart - 1) / kpart;
   }
 
   double out_bytes = 0;
@@ -1418,8 +1646,6 @@ int launch_b1_gemm(const void* x, long long ldx, int tokens, const B1Weight& w, 
     q.fence_sys = routed ? 1 : 0;
     q.n_rows = w.n_rows;
     if (lora) q.lora = *lora;
-    q.kparts = kparts;
-    q.kpart = kpart;
     auto k2 = pair_kernel(x_bf16, lmode);
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
@@ -1435,13 +1661,16 @@ int launch_b1_gemm(const void* x, long long ldx, int tokens, const B1Weight& w, 
     cfg.numAttrs = 1;
     ProfScope prof("b1_gemm", 2.0 * tokens * rows_done * (double)w.k_in,
                    (double)tokens * w.k_in * 2 + rows_done * w.k_in * 6 / 32 + out_bytes, st);
+    if (lmode != LORA_NONE)
+      return launch_after("b1_gemm_pair_kernel launch", k2, cfg.gridDim, cfg.blockDim, gemm::pair::SMEM_BYTES, 2, st,
+                          xmap, q);
     const cudaError_t e = cudaLaunchKernelEx(&cfg, k2, xmap, q);
     if (e != cudaSuccess) return cuda_status(e, "b1_gemm_pair_kernel launch");
     return launch_status("b1_gemm_pair_kernel launch");
   }
 
   CUtensorMap xmap;
-  int rc = encode_tmap_2d_16b(&xmap, x, tokens, w.k_in, ldx, gemm::BK, gemm::BN, x_bf16);
+  int rc = encode_tmap_2d_16b(&xmap, x, tokens, w.k_in, ldx, gemm::BK, bn1, x_bf16);
   if (rc) return rc;
   gemm::Params p{};
   p.tokens = tokens;
@@ -1461,22 +1690,36 @@ int launch_b1_gemm(const void* x, long long ldx, int tokens, const B1Weight& w, 
   p.fence_sys = routed ? 1 : 0;
   p.idle_loads = stall ? 1 : 0;
   if (lora) p.lora = *lora;
-  p.kparts = kparts;
-  p.kpart = kpart;
+  p.kpart = lmode == LORA_NONE ? w.k_blocks : lora_part(w, segs[0].mode);
+  p.kper = w.k_blocks;
+  int cluster = 1;
+  if (lmode == LORA_DELTA) {
+    // Few tiles: as many CTAs per tile as the GPU holds at once, up to a
+    // cluster of 8 and down to 4 k-blocks each.
+    cluster = 8;
+    while (cluster > 1 && (w.k_blocks < 4 * cluster || delta_cluster_slots(cluster) < tiles1)) --cluster;
+    p.kper = (w.k_blocks + cluster - 1) / cluster;
+    cluster = (w.k_blocks + p.kper - 1) / p.kper;
+  }
 
-  const int grid = (int)std::min<long long>(tiles1, num_sms());
+  const int grid = (int)std::min<long long>(tiles1, num_sms()) * cluster;
   auto kern = single_kernel(x_bf16, lmode);
   static bool attr_set[64][4] = {};
   bool& attr_done = attr_set[device_slot()][lmode == LORA_NONE ? (x_bf16 ? 1 : 0) : 1 + lmode];
+  const int smem = lmode == LORA_DELTA    ? gemm::SMEM_DELTA_BYTES
+                   : lmode == LORA_BLOCKS ? gemm::SMEM_BLOCKS_BYTES
+                                          : gemm::SMEM_BYTES;
   if (!attr_done) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         gemm::SMEM_BYTES);
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return cuda_status(e, "b1_gemm set smem attribute");
     attr_done = true;
   }
   ProfScope prof("b1_gemm", 2.0 * tokens * rows_done * (double)w.k_in,
                  (double)tokens * w.k_in * 2 + rows_done * w.k_in * 6 / 32 + out_bytes, st);
-  kern<<<grid, gemm::NUM_THREADS, gemm::SMEM_BYTES, st>>>(xmap, p);
+  if (lmode != LORA_NONE)
+    return launch_after("b1_gemm_kernel launch", kern, dim3(grid),
+                        dim3(gemm::NUM_THREADS), smem, cluster, st, xmap, p);
+  kern<<<grid, gemm::NUM_THREADS, smem, st>>>(xmap, p);
   return launch_status("b1_gemm_kernel launch");
 }
 

@@ -18,6 +18,32 @@ void set_error(const std::string& msg);  // stores the message for bonsai_last_e
 int fail(int code, const std::string& msg);  // set_error + return code
 int cuda_status(cudaError_t e, const char* what);  // 0 or BONSAI_ERR_CUDA
 int launch_status(const char* what);  // checks cudaGetLastError() and counts the launch
+// Launch with programmatic dependent launch: the grid may start while the one
+// before it in the stream still runs, once all of that one's CTAs have called
+// griddep_launch() or ended.  The kernel calls griddep_wait() before it reads
+// or writes what earlier grids write or read, and in every CTA, so that its
+// own end also means theirs; and griddep_launch() only where what its
+// dependents read before their wait is already complete.
+template <typename... P, typename... A>
+int launch_after(const char* what, void (*kern)(P...), dim3 grid, dim3 block, size_t smem, int cluster,
+                 cudaStream_t st, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
+  return e == cudaSuccess ? launch_status(what) : cuda_status(e, what);
+}
 // RAII per-launch timer used by bonsai_profile_start/stop: records a CUDA
 // event before and after the launch on its stream when profiling is on.
 class ProfScope {
@@ -110,19 +136,27 @@ struct TileSel {
 };
 
 // The low-rank product beside a B1_0 GEMM.
+struct LoraSlot {
+  int rank = 0;  // 0: no adapter in this slot
+  float scale = 0.f;
+};
 enum LoraMode : int { LORA_NONE = 0, LORA_DELTA = 1, LORA_BLOCKS = 2 };
 struct LoraGemm {
   int mode = LORA_NONE;
-  // LORA_DELTA: f32 [tokens][n_rows], added to the accumulator
-  const float* delta = nullptr;
   // LORA_BLOCKS: extra k-blocks of four 16-column groups, laid out for tiles
   // of tile_tokens (b1_gemm_tile_tokens).  Token tile i has
   // group_count[i] groups {slot | remainder << 30, first rank, first token,
-  // end token} at groups + i * max_groups; weight columns from up
-  // [slot][n_rows][r_pad], activations from low f32 [tokens][r_pad].
+  // end token} at groups + i * max_groups.
   const int* group_count = nullptr;
   const int4* groups = nullptr;
-  int tile_tokens = 0, max_groups = 0, r_pad = 0;
+  int tile_tokens = 0, max_groups = 0;
+  // LORA_DELTA: the requests, as bonsai_b1_gemm_lora takes them
+  const int* cu = nullptr;
+  const int* slots = nullptr;
+  const LoraSlot* info = nullptr;
+  int n_reqs = 0, n_slots = 0;
+  // both: the adapters' B (LoraDevice::up), low-rank values f32 [tokens][r_pad]
+  int r_pad = 0, n_ftiles = 0;
   const __half* up = nullptr;
   const float* low = nullptr;
 };
@@ -135,23 +169,22 @@ struct LoraGemm {
 int launch_b1_gemm(const void* x, long long ldx, int tokens, const B1Weight& w,
                    const EpiSeg* segs, int nseg, bool x_bf16, cudaStream_t st,
                    const TileSel* sel = nullptr, const LoraGemm* lora = nullptr);
-// Tokens per tile of the launch that launch_b1_gemm would make (128 or 256).
-int b1_gemm_tile_tokens(int tokens, const B1Weight& w, int lora_mode);
+// Tokens per tile (128 or 256) that suit a launch with LORA_BLOCKS.
+int b1_gemm_tile_tokens(int tokens, const B1Weight& w, int epi_mode);
 
 // ------------------------------------------------- low-rank adapters
-struct LoraSlot {
-  int rank = 0;  // 0: no adapter in this slot
-  float scale = 0.f;
-};
-// Adapters of one projection: A rows [slot][r_pad][in], B rows
-// [slot][out][r_pad] (device row order of the B1_0 weight), f16, zero beyond
-// a slot's rank; r_pad = max_rank rounded up to 16.
+// Adapters of one projection, f16, zero beyond a slot's rank: A rows
+// [slot][r_pad][in]; B in chunks [slot][n_ftiles][r_pad / 16] of 128 rows
+// (device row order of the B1_0 weight) x 16 ranks, the layout the GEMM's
+// tiles read; r_pad = max_rank rounded up to 16.
 struct LoraDevice {
-  int n_rows = 0, k_in = 0, max_rank = 0, r_pad = 0, n_slots = 0, swiglu_from = -1, device = 0;
+  int n_rows = 0, k_in = 0, max_rank = 0, r_pad = 0, n_slots = 0, n_ftiles = 0, swiglu_from = -1, device = 0;
   __half* down = nullptr;
   __half* up = nullptr;
   LoraSlot* info = nullptr;
 };
+// B [out][rank] (device memory) into the chunks of a slot.
+int launch_lora_retile(const __half* up, int rank, const LoraDevice& set, int slot, cudaStream_t st);
 // cu: device [n_reqs + 1] first token of each request; slots: device
 // [n_reqs] its adapter (outside [0, n_slots): none).
 int launch_b1_gemm_lora(const __half* x, long long ldx, int tokens, const B1Weight& w, const EpiSeg& seg,

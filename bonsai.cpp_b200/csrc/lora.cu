@@ -7,13 +7,13 @@
 // low-rank product runs beside it.
 // Two forms, chosen by the tokens per request:
 //   few (decoding): low[t][r] = scale_a * sum_k A_a[r][k] x[t][k] by
-//     lora_shrink_kernel, delta[t][n] = sum_r B_a[n][r] low[t][r] by
-//     lora_expand_kernel, and the B1_0 GEMM's epilogue adds delta: both are
-//     bound by reading the adapters once.
+//     lora_shrink_kernel, and the B1_0 GEMM's epilogue warps compute
+//     B_a low while its products run (LORA_DELTA): both are bound by reading
+//     the adapters once.
 //   many (prompts, images): low by lora_shrink_tile_kernel (tcgen05), and
 //     the B1_0 GEMM takes scale_a B_a low as extra k-blocks of its own
 //     products, listed by lora_plan_kernel: no second pass over y.
-// low (and delta) stay in f32; as a tensor-core operand low is two f16 values
+// low stays in f32; as a tensor-core operand low is two f16 values
 // (22 bits), so nothing between x and the epilogue's own rounding is rounded
 // further.
 #include "internal.cuh"
@@ -96,7 +96,7 @@ __device__ bool find_request(const int* cu, int n, int tokens, int size, int u, 
 // (one 16-byte load) for two steps.  Bound by reading A.  Partial sums meet in shared memory, then across the cluster, in a
 // fixed order.
 template <int NT>  // 8-rank tiles held
-__global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const ShrinkParams p) {
+__global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const ShrinkParams p) {
   constexpr int TM = 16;
   constexpr int R = NT * 8;
   extern __shared__ float red[];  // [kWarps][TM][R]
@@ -104,6 +104,8 @@ __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const ShrinkParam
   cg::cluster_group cluster = cg::this_cluster();
   const int csize = (int)cluster.num_blocks(), crank = (int)cluster.block_rank();
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  griddep_wait();
+  griddep_launch();
   if (warp == 0) {
     int req = -1, tile = 0;
     if (!find_request(p.cu, p.n_reqs, p.tokens, TM, (int)blockIdx.x / csize, req, tile)) req = -1;
@@ -134,7 +136,7 @@ __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const ShrinkParam
 
   float acc[NT][4] = {};
   const uint4 zero = make_uint4(0, 0, 0, 0);
-#pragma unroll 2
+#pragma unroll NT <= 4 ? 4 : NT <= 8 ? 2 : 1
   for (int ch = c0 + warp; ch < c1; ch += kWarps) {
     const uint4 va = ta < end ? *reinterpret_cast<const uint4*>(xa + ch * kChunk) : zero;
     const uint4 vb = tb < end ? *reinterpret_cast<const uint4*>(xb + ch * kChunk) : zero;
@@ -158,95 +160,21 @@ __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const ShrinkParam
     d[8 * R + 1] = acc[i][3];
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < TM * R; e += kThreads) {
+  const int used = min(TM, end - t0) * R;  // of the tile's tokens
+  for (int e = threadIdx.x; e < used; e += kThreads) {
     float s = red[e];
 #pragma unroll
     for (int k = 1; k < kWarps; ++k) s += red[k * TM * R + e];
     red[e] = s;
   }
   cluster.sync();
-  for (int e = crank * kThreads + threadIdx.x; e < TM * R; e += csize * kThreads) {
+  for (int e = crank * kThreads + threadIdx.x; e < used; e += csize * kThreads) {
     const int t = t0 + e / R, r = e % R;
     float s = 0.f;
     for (int q = 0; q < csize; ++q) s += cluster.map_shared_rank(red, q)[e];
-    if (t < end && r < p.r_pad) p.low[(size_t)t * p.r_pad + r] = info.scale * s;
+    if (r < p.r_pad) p.low[(size_t)t * p.r_pad + r] = info.scale * s;
   }
   cluster.sync();  // no CTA ends while another reads its shared memory
-}
-
-struct ExpandParams {
-  const __half* up;           // [slots][n_rows][r_pad]
-  const LoraSlot* slot_info;
-  int n_slots, r_pad, n_rows, tokens;
-  const int* cu;
-  const int* slots;
-  int n_reqs;
-  const float* low;           // [tokens][r_pad]
-  float* delta;               // [tokens][n_rows]
-};
-
-constexpr int kExpandTokens = 4;
-
-// One thread per output row of 4 tokens: B rows are read once per run of
-// tokens with the same adapter, low from shared memory.  Bound by reading B.
-__global__ void __launch_bounds__(kThreads) lora_expand_kernel(const ExpandParams p) {
-  __shared__ float low[kExpandTokens][128];
-  __shared__ int slot_of[kExpandTokens];
-  const int t0 = (int)blockIdx.x * kExpandTokens;
-  const int n = (int)blockIdx.y * kThreads + threadIdx.x;
-  if (threadIdx.x < kExpandTokens) {
-    const int t = t0 + threadIdx.x;
-    int slot = -1;
-    if (t < p.tokens) {
-      int lo = 0, hi = p.n_reqs;  // the last request that begins at or before t
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (p.cu[mid] <= t) lo = mid; else hi = mid;
-      }
-      if (t >= p.cu[lo] && t < p.cu[lo + 1]) slot = p.slots[lo];
-      if (slot >= p.n_slots || (slot >= 0 && p.slot_info[slot].rank == 0)) slot = -1;
-    }
-    slot_of[threadIdx.x] = slot;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < kExpandTokens * p.r_pad; i += kThreads) {
-    const int j = i / p.r_pad, r = i % p.r_pad;
-    low[j][r] = slot_of[j] >= 0 ? p.low[(size_t)(t0 + j) * p.r_pad + r] : 0.f;
-  }
-  __syncthreads();
-  if (n >= p.n_rows) return;
-  float acc[kExpandTokens] = {};
-  for (int j0 = 0; j0 < kExpandTokens;) {
-    const int slot = slot_of[j0];
-    int j1 = j0 + 1;
-    while (j1 < kExpandTokens && slot_of[j1] == slot) ++j1;
-    if (slot >= 0) {
-      const int rank = p.slot_info[slot].rank;
-      const uint4* row = reinterpret_cast<const uint4*>(p.up + ((size_t)slot * p.n_rows + n) * p.r_pad);
-#pragma unroll 4
-      for (int r8 = 0; r8 < (rank + 7) / 8; ++r8) {
-        const uint4 v = __ldg(row + r8);
-        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-        float b[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-          b[2 * i] = f.x;
-          b[2 * i + 1] = f.y;
-        }
-#pragma unroll
-        for (int j = 0; j < kExpandTokens; ++j)
-          if (j >= j0 && j < j1) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) acc[j] = fmaf(b[i], low[j][r8 * 8 + i], acc[j]);
-          }
-      }
-    }
-    j0 = j1;
-  }
-#pragma unroll
-  for (int j = 0; j < kExpandTokens; ++j)
-    if (t0 + j < p.tokens) p.delta[(size_t)(t0 + j) * p.n_rows + n] = acc[j];
 }
 
 // ---- the form for many tokens per request
@@ -256,8 +184,9 @@ constexpr int BK = 64;      // inputs per stage
 constexpr int STAGES = 4;
 constexpr int X_BYTES = BM * BK * 2;
 constexpr int NUM_THREADS = 192;  // TMA, MMA, 4 epilogue warps
-constexpr int TMEM_COLS = 128;
+constexpr int ACCS = 4;     // accumulators, taken in turn: short chains of f32 additions (the tensor core's truncate)
 constexpr int kMaxRank = 128;
+inline __host__ __device__ int tmem_cols(int r_pad) { return r_pad <= 16 ? 64 : r_pad <= 32 ? 128 : r_pad <= 64 ? 256 : 512; }
 
 // Shared memory of a launch: stages of x and A; the partial sums (f32
 // [r_pad][128 tokens]) take the stages' place once the products are done.
@@ -289,6 +218,8 @@ __global__ void __launch_bounds__(tile::NUM_THREADS)
   cg::cluster_group cluster = cg::this_cluster();
   const int csize = (int)cluster.num_blocks(), crank = (int)cluster.block_rank();
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  griddep_wait();
+  griddep_launch();
   if (warp == 0) {
     int req = -1, tl = 0;
     if (!find_request(p.cu, p.n_reqs, p.tokens, BM, (int)blockIdx.x / csize, req, tl)) req = -1;
@@ -320,7 +251,7 @@ __global__ void __launch_bounds__(tile::NUM_THREADS)
     fence_barrier_init();
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, TMEM_COLS);
+    tmem_alloc(tmem_slot, tmem_cols(p.r_pad));
     tmem_relinquish();
   }
   tc_fence_before();
@@ -359,8 +290,8 @@ __global__ void __launch_bounds__(tile::NUM_THREADS)
         const uint32_t xa = smem_u32(smem + s * stage_bytes), aa = xa + X_BYTES;
 #pragma unroll
         for (int k16 = 0; k16 < BK / 16; ++k16)
-          mma_ss(tmem, make_smem_desc(xa + k16 * 32, 16, 1024), make_smem_desc(aa + k16 * 32, 16, 1024), idesc,
-                 (it | k16) != 0 ? 1u : 0u);
+          mma_ss(tmem + (it % ACCS) * p.r_pad, make_smem_desc(xa + k16 * 32, 16, 1024),
+                 make_smem_desc(aa + k16 * 32, 16, 1024), idesc, it >= ACCS || k16 != 0 ? 1u : 0u);
         tc_commit(&empty[s]);
       }
       tc_commit(done);
@@ -379,11 +310,16 @@ __global__ void __launch_bounds__(tile::NUM_THREADS)
     if (__all_sync(0xffffffffu, good)) {
       tc_fence_after();
       for (int c = 0; c < n16 * 16; c += 16) {
-        uint32_t r[16];
-        tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + c, r);
-        tmem_wait_ld();
+        float v[16] = {};
+        for (int a = 0; a < min(ACCS, b1 - b0); ++a) {
+          uint32_t r[16];
+          tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + a * p.r_pad + c, r);
+          tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sums[(c + i) * BM + q * 32 + lane] = b1 > b0 ? __uint_as_float(r[i]) : 0.f;
+          for (int i = 0; i < 16; ++i) v[i] += __uint_as_float(r[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sums[(c + i) * BM + q * 32 + lane] = v[i];
       }
     }
     tc_fence_before();
@@ -400,7 +336,31 @@ __global__ void __launch_bounds__(tile::NUM_THREADS)
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tmem, TMEM_COLS);
+    tmem_dealloc(tmem, tmem_cols(p.r_pad));
+  }
+}
+
+// B [out][rank] into the chunks of a slot (LoraDevice::up).  Rows
+// [swiglu_from, out) go to alternating device rows, gate then value, as those
+// of the B1_0 weight.
+__global__ void lora_retile_kernel(const __half* __restrict__ src, int rank, int n_rows, int n_ftiles, int r_pad,
+                                   int swiglu_from, __half* __restrict__ dst) {
+  const long long total = (long long)n_ftiles * 128 * r_pad;
+  for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total;
+       i += (long long)gridDim.x * blockDim.x) {
+    const int r16 = (int)(i % 16), row = (int)(i / 16 % 128);
+    const int g = (int)(i / 2048 % (r_pad / 16)), ft = (int)(i / 2048 / (r_pad / 16));
+    const int n = ft * 128 + row, r = g * 16 + r16;
+    __half v = __float2half_rn(0.f);
+    if (n < n_rows && r < rank) {
+      int s = n;
+      if (swiglu_from >= 0 && n >= swiglu_from) {
+        const int j = n - swiglu_from;
+        s = swiglu_from + ((j & 1) ? (n_rows - swiglu_from) / 2 + (j >> 1) : (j >> 1));
+      }
+      v = src[(size_t)s * rank + r];
+    }
+    dst[i] = v;
   }
 }
 
@@ -411,6 +371,8 @@ __global__ void lora_plan_kernel(const int* __restrict__ cu, const int* __restri
                                  const LoraSlot* __restrict__ slot_info, int n_slots, int tile_tokens, int n_tiles,
                                  int max_groups, int* __restrict__ group_count, int4* __restrict__ groups) {
   const int tile = (int)(blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32), lane = threadIdx.x & 31;
+  griddep_wait();
+  griddep_launch();
   if (tile >= n_tiles) return;
   const int t0 = tile * tile_tokens, t1 = min(tokens, t0 + tile_tokens);
   int lo = 0, hi = n_reqs;  // the last request that begins at or before t0
@@ -461,24 +423,12 @@ int shrink_tiles(const ShrinkParams& p, cudaStream_t st) {
   if (e != cudaSuccess) return cuda_status(e, "lora shrink set smem attribute");
   const long long seqs = std::min(p.n_reqs, p.tokens);
   const long long units = (p.tokens + seqs * (tile::BM - 1)) / tile::BM;
-  int c = 8;  // CTAs that split K: about one per SM, each at least two stages
-  while (c > 1 && (units * c > 1ll * num_sms() || p.k_in / tile::BK < 2 * c)) c /= 2;
+  int c = 8;  // CTAs that split K: up to three per SM, each at least two stages
+  while (c > 1 && (units * c > 3ll * num_sms() || p.k_in / tile::BK < 2 * c)) c /= 2;
   if (units * c > 0x7fffffffll) return fail(-2, "b1_gemm_lora: too many tokens in one call");
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)c;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)(units * c));
-  cfg.blockDim = dim3(tile::NUM_THREADS);
-  cfg.dynamicSmemBytes = (size_t)tile::smem_bytes(p.r_pad);
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, lora_shrink_tile_kernel, xmap, amap, p, device_error_word());
-  if (e != cudaSuccess) return cuda_status(e, "lora_shrink_tile_kernel launch");
-  return launch_status("lora_shrink_tile_kernel launch");
+  return launch_after("lora_shrink_tile_kernel launch", lora_shrink_tile_kernel, dim3((unsigned)(units * c)),
+                      dim3(tile::NUM_THREADS), (size_t)tile::smem_bytes(p.r_pad), c, st, xmap, amap, p,
+                      device_error_word());
 }
 
 template <int NT>
@@ -497,21 +447,7 @@ int shrink(const ShrinkParams& p, cudaStream_t st) {
   int c = 8;
   while (c > 1 && (units * c > 2ll * num_sms() || (p.k_in / kChunk) / c < kWarps)) c /= 2;
   if (units * c > 0x7fffffffll) return fail(-2, "b1_gemm_lora: too many tokens in one call");
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)c;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)(units * c));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kern, p);
-  if (e != cudaSuccess) return cuda_status(e, "lora_shrink_kernel launch");
-  return launch_status("lora_shrink_kernel launch");
+  return launch_after("lora_shrink_kernel launch", kern, dim3((unsigned)(units * c)), dim3(kThreads), smem, c, st, p);
 }
 
 int shrink_by_rank(const ShrinkParams& p, int max_rank, cudaStream_t st) {
@@ -523,23 +459,28 @@ int shrink_by_rank(const ShrinkParams& p, int max_rank, cudaStream_t st) {
 
 }  // namespace lora
 
+int launch_lora_retile(const __half* up, int rank, const LoraDevice& set, int slot, cudaStream_t st) {
+  const size_t n = (size_t)set.n_ftiles * 128 * set.r_pad;
+  lora::lora_retile_kernel<<<(unsigned)std::min<size_t>((n + 255) / 256, 148 * 16), 256, 0, st>>>(
+      up, rank, set.n_rows, set.n_ftiles, set.r_pad, set.swiglu_from, set.up + (size_t)slot * n);
+  return launch_status("lora_retile_kernel launch");
+}
+
 int launch_b1_gemm_lora(const __half* x, long long ldx, int tokens, const B1Weight& w, const EpiSeg& seg,
                         const LoraDevice& set, const int* cu, const int* slots, int n_reqs, cudaStream_t st) {
   if (tokens == 0) return 0;
   if (n_reqs == 0) return launch_b1_gemm(x, ldx, tokens, w, &seg, 1, false, st);
   LoraGemm g;
   g.mode = tokens >= 32ll * n_reqs ? LORA_BLOCKS : LORA_DELTA;
-  // scratch: low, then delta or the lists of extra blocks
+  // scratch: low, then the lists of extra blocks
   const size_t low_n = ((size_t)tokens * set.r_pad + 3) / 4 * 4;
-  size_t more;
+  size_t more = 0;
   int n_tiles = 0;
   if (g.mode == LORA_BLOCKS) {
-    g.tile_tokens = b1_gemm_tile_tokens(tokens, w, g.mode);
+    g.tile_tokens = b1_gemm_tile_tokens(tokens, w, seg.mode);
     n_tiles = (tokens + g.tile_tokens - 1) / g.tile_tokens;
     g.max_groups = 2 * (set.r_pad / 16) * std::min(n_reqs, g.tile_tokens);
     more = (size_t)n_tiles * (g.max_groups * sizeof(int4) + sizeof(int));
-  } else {
-    more = (size_t)tokens * w.n_rows * sizeof(float);
   }
   void* mem = nullptr;
   int rc = scratch_alloc(&mem, low_n * sizeof(float) + more, "b1_gemm_lora", st);
@@ -558,39 +499,26 @@ int launch_b1_gemm_lora(const __half* x, long long ldx, int tokens, const B1Weig
   s.slots = slots;
   s.n_reqs = n_reqs;
   s.low = low;
+  g.cu = cu;
+  g.slots = slots;
+  g.info = set.info;
+  g.n_reqs = n_reqs;
+  g.n_slots = set.n_slots;
+  g.r_pad = set.r_pad;
+  g.n_ftiles = set.n_ftiles;
+  g.up = set.up;
+  g.low = low;
   if (g.mode == LORA_BLOCKS) {
     int4* groups = reinterpret_cast<int4*>(low + low_n);
     int* count = reinterpret_cast<int*>(groups + (size_t)n_tiles * g.max_groups);
     g.groups = groups;
     g.group_count = count;
-    g.r_pad = set.r_pad;
-    g.up = set.up;
-    g.low = low;
-    lora::lora_plan_kernel<<<(unsigned)((n_tiles + 7) / 8), 256, 0, st>>>(
-        cu, slots, n_reqs, tokens, set.info, set.n_slots, g.tile_tokens, n_tiles, g.max_groups, count, groups);
-    rc = launch_status("lora_plan_kernel launch");
+    rc = launch_after("lora_plan_kernel launch", lora::lora_plan_kernel, dim3((unsigned)((n_tiles + 7) / 8)),
+                      dim3(256), 0, 1, st, cu, slots, n_reqs, tokens, set.info, set.n_slots, g.tile_tokens, n_tiles,
+                      g.max_groups, count, groups);
     if (rc == 0) rc = lora::shrink_tiles(s, st);
   } else {
-    g.delta = low + low_n;
     rc = lora::shrink_by_rank(s, set.max_rank, st);
-    if (rc == 0) {
-      lora::ExpandParams e{};
-      e.up = set.up;
-      e.slot_info = set.info;
-      e.n_slots = set.n_slots;
-      e.r_pad = set.r_pad;
-      e.n_rows = w.n_rows;
-      e.tokens = tokens;
-      e.cu = cu;
-      e.slots = slots;
-      e.n_reqs = n_reqs;
-      e.low = low;
-      e.delta = low + low_n;
-      const dim3 grid((unsigned)((tokens + lora::kExpandTokens - 1) / lora::kExpandTokens),
-                      (unsigned)((w.n_rows + lora::kThreads - 1) / lora::kThreads));
-      lora::lora_expand_kernel<<<grid, lora::kThreads, 0, st>>>(e);
-      rc = launch_status("lora_expand_kernel launch");
-    }
   }
   if (rc == 0) rc = launch_b1_gemm(x, ldx, tokens, w, &seg, 1, false, st, nullptr, &g);
   scratch_free(mem, st);

@@ -324,6 +324,15 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t
                : "memory");
 }
 
+// ------------------------------------------- programmatic dependent launch
+// Wait until the grids that this one was launched behind are complete and
+// their writes visible (returns at once in an ordinary launch).
+__device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// The next grid of the stream may be launched once every CTA has said so.
+__device__ __forceinline__ void griddep_launch() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // ------------------------------------------------- UMMA descriptors (sm_100)
 // Shared-memory matrix descriptor: start address, leading / stride byte
 // offsets (all >> 4), version 1 (bits 46-47), layout type in bits 61-63
