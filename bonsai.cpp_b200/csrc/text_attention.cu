@@ -300,10 +300,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
     const int box = lane / C::HALVES, half = lane % C::HALVES;
     const bool issues = kPaged ? box < boxes : lane < C::HALVES;
     int ent = -1, ent_base = -1;
-    bool ok = true;
-    for (int j = 0; j < nkv && ok; ++j) {
+    auto load = [&](const void* map, uint8_t* ring, uint64_t* full, uint64_t* empty, int j) -> bool {
       const int s = j % RING;
-      const uint32_t ph = (j / RING) & 1;
       const int key0 = (j0 + j) * BKV;
       int page = 0;
       if constexpr (kPaged) {
@@ -314,22 +312,26 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
         }
         page = __shfl_sync(0xffffffffu, ent, (((key0 + (box << box_shift)) >> p.page_shift) - ent_base) & 31);
       }
-      auto load = [&](const void* map, uint8_t* ring, uint64_t* full, uint64_t* empty) -> bool {
-        const bool good = wait_bar(&empty[s], ph ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_TMA);
-        if (!__all_sync(0xffffffffu, good)) return false;
-        if (lane == 0) bar_arrive_expect_tx(&full[s], C::KV_BYTES);
-        __syncwarp();
-        if (issues) {
-          uint8_t* d = ring + s * C::KV_BYTES + half * C::KV_HALF;
-          if constexpr (kPaged)
-            tma_load_4d(d + (box << box_shift) * 128, map, &full[s], half * 64, kvh,
-                        (key0 + (box << box_shift)) & ((1 << p.page_shift) - 1), page);
-          else
-            tma_load_3d(d, map, &full[s], half * 64, kvh, q_begin + key0);
-        }
-        return true;
-      };
-      ok = load(&kmap, ks, k_full, k_empty) && load(&vmap, vs, v_full, v_empty);
+      const bool good = wait_bar(&empty[s], ((j / RING) & 1) ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_TMA);
+      if (!__all_sync(0xffffffffu, good)) return false;
+      if (lane == 0) bar_arrive_expect_tx(&full[s], C::KV_BYTES);
+      __syncwarp();
+      if (issues) {
+        uint8_t* d = ring + s * C::KV_BYTES + half * C::KV_HALF;
+        if constexpr (kPaged)
+          tma_load_4d(d + (box << box_shift) * 128, map, &full[s], half * 64, kvh,
+                      (key0 + (box << box_shift)) & ((1 << p.page_shift) - 1), page);
+        else
+          tma_load_3d(d, map, &full[s], half * 64, kvh, q_begin + key0);
+      }
+      return true;
+    };
+    // K runs two blocks ahead of V, as S does of P V: each load is asked for as
+    // soon as its slot is free, two blocks' time before it is needed.
+    bool ok = load(&kmap, ks, k_full, k_empty, 0) && (nkv == 1 || load(&kmap, ks, k_full, k_empty, 1));
+    for (int j = 0; j < nkv && ok; ++j) {
+      ok = load(&vmap, vs, v_full, v_empty, j);
+      if (ok && j + 2 < nkv) ok = load(&kmap, ks, k_full, k_empty, j + 2);
     }
     if (!ok) {  // let copies in flight land before the shared memory is released
       const unsigned long long w0 = globaltimer_ns();
