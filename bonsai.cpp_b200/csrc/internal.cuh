@@ -40,7 +40,7 @@ int launch_after(const char* what, void (*kern)(P...), dim3 grid, dim3 block, si
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
   return e == cudaSuccess ? launch_status(what) : cuda_status(e, what);
 }

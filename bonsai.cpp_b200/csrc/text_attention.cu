@@ -8,28 +8,35 @@
 // place (causal), or all of them.  G = n_heads / n_kv_heads query heads share
 // one key/value head.
 //
-// One CTA = one sequence x one key/value head x one tile of 128 query rows,
-// where a row is a (token, head of the group) pair: row r is token r / G, head
-// r % G.  Taking the group's heads into the rows reads every key once for G
-// heads, makes the causal triangle's diagonal G times narrower, and lets a
-// single token fill G rows.  Two such CTAs share an SM: one's softmax runs
-// beside the other's products and loads.
+// A unit of work = one sequence x one key/value head x one tile of 128 query
+// rows, where a row is a (token, head of the group) pair: row r is token r / G,
+// head r % G.  Taking the group's heads into the rows reads every key once for
+// G heads, makes the causal triangle's diagonal G times narrower, and lets a
+// single token fill G rows.  Two persistent CTAs share an SM (one's softmax runs
+// beside the other's products and loads); each walks through its units, longest
+// first over the whole launch, with the next unit's loads and first products
+// under way while the last one's rows are written.
 //   warps 0-3   softmax: thread i owns row i (TMEM lane i).  Online softmax
 //               in the log2 domain; the running max moves (and O in TMEM is
 //               rescaled) only when a block's max exceeds it by more than 8.
-//               Warps without a row (a single token has G rows) take no part.
-//   warp 4      TMA: Q once, then K and V blocks of 64 keys (128-byte
-//               swizzle, 64-dim halves); paged: one box per page and half,
-//               issued by one lane each, page indices read 32 at a time.
+//               Warps without a row (a single token has G rows) only pass on.
+//   warp 4      TMA: Q, then K and V blocks of 64 keys (128-byte swizzle,
+//               64-dim halves); paged: one box per page and half, issued by
+//               one lane each, page indices read 32 at a time.
 //   warp 5      one thread issues tcgen05.mma: S(j) = Q K_j^T (SMEM, SMEM),
 //               O += P(j) V_j (P from TMEM, V MN-major); S runs two blocks
 //               ahead (double-buffered).
-//   warps 6-7   blocks that not every row sees whole (a causal diagonal, the
+//   warp 6      blocks that not every row sees whole (a causal diagonal, the
 //               end of a sequence inside a block or page): V rows past the
 //               sequence's end are zeroed in shared memory before the
 //               product, since 0 * NaN would reach every row; V values of
 //               keys that only some rows see are zeroed where they are not
 //               finite, and the rows that do see them add them at the end.
+//   warp 7      finds the units.
+// Where the units leave CTA slots empty (a few single tokens), each unit's keys
+// are split between the CTAs of a cluster, which merge their parts through
+// distributed shared memory; a split wider than a cluster goes through global
+// memory and a second kernel.
 // TMEM (256 columns): S(even) [0, 64) S(odd) [64, 128) O [128, 128 + HD);
 // P(j) (16-bit pairs) overwrites the first 32 columns of its S.
 #include "internal.cuh"
@@ -50,11 +57,12 @@ constexpr int BQ = 128;   // query rows per CTA
 constexpr int BKV = 64;   // keys per block
 constexpr int RING = 2;   // K and V slots
 constexpr int NUM_THREADS = 256;
-constexpr int WARP_TMA = 4, WARP_MMA = 5, WARP_FIX = 6;
+constexpr int WARP_TMA = 4, WARP_MMA = 5, WARP_FIX = 6, WARP_PLAN = 7;
 constexpr int TMEM_COLS = 256;
 constexpr int S_COL = 0, O_COL = 128;
 constexpr float kRescaleThreshold = 8.0f;
-constexpr int kMaxSeqs = 8192;  // tile counts of a launch fit the K/V ring
+constexpr int kMaxSeqs = 512;     // sequences of one launch (their lengths are kept in shared memory)
+constexpr int kMaxCluster = 16;   // CTAs that split a unit's keys and merge in shared memory
 
 template <int HD>
 struct Cfg {
@@ -63,9 +71,13 @@ struct Cfg {
   static constexpr int Q_BYTES = HALVES * Q_HALF;
   static constexpr int KV_HALF = BKV * 128;
   static constexpr int KV_BYTES = HALVES * KV_HALF;
-  static constexpr int SMEM_BYTES = 1024 + Q_BYTES + 2 * RING * KV_BYTES + 256;
+  // K and V rings; once a unit's products are done they can hold its O (f32)
+  static constexpr int RINGS_BYTES = 2 * RING * KV_BYTES;
+  static_assert(RINGS_BYTES >= BQ * HD * 4, "O does not fit the rings");
+  static constexpr int SMEM_BYTES = 1024 + Q_BYTES + RINGS_BYTES + 512 + BQ * 8 + kMaxSeqs * 8;
 };
-static_assert(2 * RING * Cfg<64>::KV_BYTES >= kMaxSeqs * 4, "tile counts do not fit the ring");
+// Two CTAs per SM (228 KB, 1 KB of it reserved for each).
+static_assert(2 * (Cfg<128>::SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs per SM");
 
 struct Params {
   const int* cu;        // [n_seqs + 1] first query row of each sequence
@@ -75,6 +87,7 @@ struct Params {
   int table_width, page_shift, n_pages;
   int n_seqs, total_q, n_heads, n_kv, group, tile_tokens;
   int causal, splits;
+  int in_cluster;       // the splits of a unit are one cluster
   float scale_log2;     // softmax scale * log2(e)
   void* out;
   long long out_token, out_head;
@@ -121,46 +134,119 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const void* map, uint64_t
       : "memory");
 }
 
-// Query tile b of a launch: tiles go by level (their index within their
-// sequence), the highest level of all sequences first, so that under a causal
-// mask the tiles with the most keys start first.  count[i] = tiles of
-// sequence i (shared memory).  One warp; false where there are at most b tiles.
-__device__ bool find_tile(const int* count, int n, int b, int& seq, int& level) {
-  const int lane = (int)lane_id();
-  auto at_least = [&](int lv) {  // tiles of level >= lv
-    int c = 0;
-    for (int i = lane; i < n; i += 32) c += max(0, count[i] - lv);
-    return __reduce_add_sync(0xffffffffu, c);
-  };
-  int hi = 0;
-  for (int i = lane; i < n; i += 32) hi = max(hi, count[i]);
-  hi = __reduce_max_sync(0xffffffffu, hi);
-  if (at_least(0) <= b) return false;
-  int lo = 0, above = 0;  // at_least(lo) > b, at_least(hi) = above <= b
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    const int c = at_least(mid);
-    if (c > b) {
-      lo = mid;
-    } else {
-      hi = mid;
-      above = c;
-    }
-  }
-  int rank = b - above;
-  for (int i0 = 0; i0 < n; i0 += 32) {
-    const uint32_t has = __ballot_sync(0xffffffffu, i0 + lane < n && count[i0 + lane] > lo);
-    const int c = __popc(has);
-    if (rank < c) {
-      const bool mine = ((has >> lane) & 1u) && __popc(has & ((1u << lane) - 1u)) == rank;
-      seq = i0 + __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
-      level = lo;
-      return true;
-    }
-    rank -= c;
-  }
-  return false;
+// Packed pairs of f32 in one 64-bit register.
+__device__ __forceinline__ unsigned long long pack2(float a, float b) {
+  unsigned long long d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
 }
+__device__ __forceinline__ void unpack2(unsigned long long v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b,
+                                                   unsigned long long c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// What the roles of a CTA need to know of a unit (64 bytes in shared memory).
+struct Unit {
+  int seq, kvh, q_begin, t0, n_tok;  // tokens t0 .. t0 + n_tok of the sequence
+  int first;                         // place of token t0 in the sequence
+  int kv_len, lim_min;               // keys; keys that the first token sees
+  int j0, nkv;                       // key blocks [j0, j0 + nkv) (nkv < 0: no more units)
+  int jb;                            // blocks from jb on hold a key that some row does not see
+  int pad[5];
+};
+static_assert(sizeof(Unit) == 64, "read as four int4");
+
+// Keys [0, n) that token `tok` of a tile sees.
+__device__ __forceinline__ int keys_seen(const Unit& u, int causal, int tok) {
+  return causal ? max(0, min(u.kv_len, u.first + tok + 1)) : u.kv_len;
+}
+
+// The order of a launch's query tiles: by their key blocks, most first (ties:
+// by sequence, then latest tokens first), so that the long ones do not end up
+// alone at the end.  One warp; lens[i] = {query tokens, keys before them} of
+// sequence i.
+struct Finder {
+  const int2* lens;
+  int n, tile_tokens, causal;
+  long long room;  // keys that a sequence's pages can hold
+  int c, at_c, above_c;  // tiles of >= c blocks, of > c blocks
+
+  __device__ int kv_len(int2 s) const { return (int)max(0ll, min((long long)s.x + s.y, room)); }
+  // Tiles of a sequence with at least `blocks` key blocks: the last ones.
+  __device__ int tiles(int2 s, int blocks) const {
+    const int all = (s.x + tile_tokens - 1) / tile_tokens;
+    if (blocks <= 0 || all == 0) return all;
+    const int keys = (blocks - 1) * BKV + 1;
+    if (kv_len(s) < keys) return 0;
+    if (!causal) return all;
+    const int toks = keys - s.y;  // tokens up to the first that sees as many
+    return toks <= tile_tokens ? all : all - ((toks + tile_tokens - 1) / tile_tokens - 1);
+  }
+  __device__ int total(int blocks) const {
+    int v = 0;
+    for (int i = (int)lane_id(); i < n; i += 32) v += tiles(lens[i], blocks);
+    return __reduce_add_sync(0xffffffffu, v);
+  }
+  __device__ void init() {
+    int most = 0;
+    for (int i = (int)lane_id(); i < n; i += 32) most = max(most, kv_len(lens[i]));
+    c = (__reduce_max_sync(0xffffffffu, most) + BKV - 1) / BKV + 1;
+    at_c = above_c = 0;
+  }
+  // Tile b (b never falls from call to call): its sequence and its place among
+  // the sequence's tiles; false where there are at most b tiles.
+  __device__ bool find(int b, int& seq, int& level) {
+    if (b >= at_c) {
+      if (c == 0 || total(0) <= b) return false;
+      int lo = 0, hi = c;  // total(lo) > b >= total(hi)
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (total(mid) > b) lo = mid; else hi = mid;
+      }
+      c = lo;
+      at_c = total(c);
+      above_c = total(c + 1);
+    }
+    int rank = b - above_c;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const int i = i0 + (int)lane_id();
+      const int2 s = i < n ? lens[i] : make_int2(0, 0);
+      const int more = tiles(s, c + 1), e = tiles(s, c) - more;
+      int incl = e;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if ((int)lane_id() >= o) incl += v;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, incl > rank);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        const int before = __shfl_sync(0xffffffffu, incl - e, l);
+        const int all = (s.x + tile_tokens - 1) / tile_tokens;
+        seq = i0 + l;
+        level = __shfl_sync(0xffffffffu, all - 1 - more, l) - (rank - before);
+        return true;
+      }
+      rank -= __shfl_sync(0xffffffffu, incl, 31);
+    }
+    return false;
+  }
+};
 
 template <int HD, bool kBF16, bool kPaged>
 __global__ void __launch_bounds__(NUM_THREADS, 2)
@@ -174,8 +260,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
   uint8_t* qs = smem;
   uint8_t* ks = qs + C::Q_BYTES;
   uint8_t* vs = ks + RING * C::KV_BYTES;
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(vs + RING * C::KV_BYTES);
-  uint64_t* k_full = q_full + 1;
+  Unit* units = reinterpret_cast<Unit*>(vs + RING * C::KV_BYTES);  // [2]
+  uint64_t* unit_full = reinterpret_cast<uint64_t*>(units + 2);
+  uint64_t* unit_empty = unit_full + 2;
+  uint64_t* q_full = unit_empty + 2;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* k_full = q_empty + 1;
   uint64_t* k_empty = k_full + RING;
   uint64_t* v_full = k_empty + RING;
   uint64_t* v_empty = v_full + RING;
@@ -183,157 +273,169 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
   uint64_t* s_full = v_fixed + RING;
   uint64_t* p_ready = s_full + 2;
   uint64_t* pv_done = p_ready + 2;
-  uint64_t* drain = pv_done + 2;
+  uint64_t* o_empty = pv_done + 2;
+  uint64_t* drain = o_empty + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* nonfinite = abort_flag + 1;
-  int* found = const_cast<int*>(nonfinite) + 1;  // sequence (-1: none), level
+  volatile int* nonfinite = abort_flag + 1;  // [2] by unit
+  float2* stats = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(units) + 512);  // [BQ] log2 sum (cluster merge)
+  int2* lens = reinterpret_cast<int2*>(stats + BQ);  // [kMaxSeqs]
 
   const int warp = threadIdx.x / 32;
   const int lane = (int)lane_id();
   const int split = (int)(blockIdx.x % (unsigned)p.splits);
-  const int unit = (int)(blockIdx.x / (unsigned)p.splits);
-  const int kvh = unit % p.n_kv;
-
-  // ---- which tile
-  int* count = reinterpret_cast<int*>(ks);
-  for (int i = threadIdx.x; i < p.n_seqs; i += NUM_THREADS) {
-    const int a = max(0, min(p.cu[i], p.total_q)), b = max(a, min(p.cu[i + 1], p.total_q));
-    count[i] = (b - a + p.tile_tokens - 1) / p.tile_tokens;
-  }
-  __syncthreads();
-  if (warp == 0) {
-    int seq = -1, level = 0;
-    if (!find_tile(count, p.n_seqs, unit / p.n_kv, seq, level)) seq = -1;
-    if (lane == 0) {
-      found[0] = seq;
-      found[1] = level;
-    }
-  }
-  fence_proxy_async_smem();  // the ring's next writer is the TMA
-  __syncthreads();
-  const int seq = found[0];
-  if (seq < 0) return;
-  const int q_begin = max(0, min(p.cu[seq], p.total_q));
-  const int q_len = max(q_begin, min(p.cu[seq + 1], p.total_q)) - q_begin;
-  int kv_len = q_len;
-  if (kPaged) {
-    const long long room = (long long)p.table_width << p.page_shift;
-    kv_len = (int)max(0ll, min((long long)p.ctx[seq], room));
-  }
-  const int t0 = found[1] * p.tile_tokens;          // first token of the tile
-  const int n_tok = min(p.tile_tokens, q_len - t0);
-  const int first = kPaged ? p.ctx[seq] - q_len + t0 : t0;  // its place in the sequence
-  // Keys [0, lim) are seen by a row; lim grows by one with each token.
-  auto keys_seen = [&](int tok) {
-    return p.causal ? max(0, min(kv_len, first + tok + 1)) : kv_len;
-  };
-  const int lim_min = keys_seen(0), lim_max = keys_seen(n_tok - 1);
-  const int blocks = (lim_max + BKV - 1) / BKV;
-  const int chunk = (blocks + p.splits - 1) / p.splits;
-  const int j0 = split * chunk;
-  const int nkv = max(0, min(blocks - j0, chunk));
-  // Blocks [jb, nkv) hold a key that some row of the tile does not see.
-  const int jb = max(0, lim_min / BKV - j0);
-
-  const int row = warp * 32 + lane;  // softmax warps
-  const int tok = row / p.group;
-  const bool valid = warp < 4 && tok < n_tok && row < p.tile_tokens * p.group;
-  const int head = kvh * p.group + row - tok * p.group;
-  const size_t q_row = (size_t)(q_begin + t0 + tok);
-  uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + q_row * p.out_token + (size_t)head * p.out_head;
-  const size_t part = ((size_t)split * p.total_q + q_row) * p.n_heads + head;
-
-  if (nkv == 0) {  // no key: zeros (or a partial of weight zero)
-    if (valid) {
-      if (p.splits > 1) {
-        p.part_lse[part] = -INFINITY;
-      } else {
-        for (int i = 0; i < HD / 8; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(0, 0, 0, 0);
-      }
-    }
-    return;
-  }
-  const int active = (n_tok * p.group + 31) / 32;  // softmax warps with a row
+  const int unit0 = (int)(blockIdx.x / (unsigned)p.splits);
+  const int ustep = (int)(gridDim.x / (unsigned)p.splits);
 
   if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      bar_init(&unit_full[i], 1);
+      bar_init(&unit_empty[i], 7);  // softmax warps, TMA, MMA, fix
+      bar_init(&s_full[i], 1);
+      bar_init(&p_ready[i], 4);
+      bar_init(&pv_done[i], 1);
+      nonfinite[i] = 0;
+    }
     bar_init(q_full, 1);
+    bar_init(q_empty, 1);
     for (int s = 0; s < RING; ++s) {
       bar_init(&k_full[s], 1);
       bar_init(&k_empty[s], 1);
       bar_init(&v_full[s], 1);
       bar_init(&v_empty[s], 1);
-      bar_init(&v_fixed[s], 2);
+      bar_init(&v_fixed[s], 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      bar_init(&s_full[i], 1);
-      bar_init(&p_ready[i], active);
-      bar_init(&pv_done[i], 1);
-    }
+    bar_init(o_empty, 4);
     bar_init(drain, 1);
     *abort_flag = 0;
-    *nonfinite = 0;
     fence_barrier_init();
+    tma_prefetch_desc(&qmap);
+    tma_prefetch_desc(&kmap);
+    tma_prefetch_desc(&vmap);
   }
   if (warp == WARP_MMA) {
     tmem_alloc(tmem_slot, TMEM_COLS);
     tmem_relinquish();
+  }
+  griddep_wait();
+  griddep_launch();
+  for (int i = threadIdx.x; i < p.n_seqs; i += NUM_THREADS) {
+    const int a = max(0, min(p.cu[i], p.total_q)), b = max(a, min(p.cu[i + 1], p.total_q));
+    lens[i] = make_int2(b - a, kPaged ? p.ctx[i] - (b - a) : 0);
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == WARP_TMA) {
-    if (lane == 0) {
-      tma_prefetch_desc(&kmap);
-      tma_prefetch_desc(&vmap);
-      bar_arrive_expect_tx(q_full, (uint32_t)(p.group * p.tile_tokens * HD * 2));
-      for (int h = 0; h < C::HALVES; ++h)
-        tma_load_3d(qs + h * C::Q_HALF, &qmap, q_full, h * 64, kvh * p.group, q_begin + t0);
+  // Unit i of this CTA, as every role gets it.
+  auto next_unit = [&](int i, Unit& u) -> bool {
+    const bool good = wait_bar(&unit_full[i & 1], (i >> 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER);
+    if (!good) return false;
+    const int4* src = reinterpret_cast<const int4*>(&units[i & 1]);
+    int4* dst = reinterpret_cast<int4*>(&u);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) dst[k] = src[k];
+    return u.nkv >= 0;
+  };
+
+  if (warp == WARP_PLAN) {
+    Finder f{lens, p.n_seqs, p.tile_tokens, p.causal, kPaged ? (long long)p.table_width << p.page_shift : 0x7fffffffll};
+    f.init();
+    for (int i = 0;; ++i) {
+      // units come longest first: rounds go up and down the CTAs in turn, so
+      // that who had the longest of one round has the shortest of the next
+      const int unit = i * ustep + (i & 1 ? ustep - 1 - unit0 : unit0);
+      Unit u{};
+      u.nkv = -1;
+      int seq, level;
+      // with splits, one unit per CTA (per cluster)
+      if ((p.splits == 1 || i == 0) && f.find(unit / p.n_kv, seq, level)) {
+        const int2 s = lens[seq];
+        u.seq = seq;
+        u.kvh = unit % p.n_kv;
+        u.q_begin = max(0, min(p.cu[seq], p.total_q));
+        u.kv_len = f.kv_len(s);
+        u.t0 = level * p.tile_tokens;
+        u.n_tok = min(p.tile_tokens, s.x - u.t0);
+        u.first = s.y + u.t0;
+        u.lim_min = keys_seen(u, p.causal, 0);
+        const int blocks = (keys_seen(u, p.causal, u.n_tok - 1) + BKV - 1) / BKV;
+        const int chunk = (blocks + p.splits - 1) / p.splits;
+        u.j0 = split * chunk;
+        u.nkv = max(0, min(blocks - u.j0, chunk));
+        u.jb = max(0, u.lim_min / BKV - u.j0);
+      }
+      const bool good = wait_bar(&unit_empty[i & 1], ((i >> 1) & 1) ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER);
+      if (!__all_sync(0xffffffffu, good)) break;
+      if (lane == 0) {
+        units[i & 1] = u;
+        nonfinite[i & 1] = 0;  // the softmax warps are done with unit i - 2
+        bar_arrive(&unit_full[i & 1]);
+      }
+      if (u.nkv < 0) break;
     }
+  } else if (warp == WARP_TMA) {
     // Paged: a block of 64 keys takes 64 / page boxes (one where a page holds
     // more), and each half of the head dims its own; lane l issues box
     // l / HALVES, half l % HALVES.  `ent` = 32 consecutive page indices.
     const int box_shift = min(p.page_shift, 6);
-    const int boxes = BKV >> box_shift;
     const int box = lane / C::HALVES, half = lane % C::HALVES;
-    const bool issues = kPaged ? box < boxes : lane < C::HALVES;
-    int ent = -1, ent_base = -1;
-    auto load = [&](const void* map, uint8_t* ring, uint64_t* full, uint64_t* empty, int j) -> bool {
-      const int s = j % RING;
-      const int key0 = (j0 + j) * BKV;
-      int page = 0;
-      if constexpr (kPaged) {
-        const int want = (key0 >> p.page_shift) & ~31;
-        if (want != ent_base) {  // 64 keys never reach past 32 pages (page >= 8)
-          ent_base = want;
-          ent = want + lane < p.table_width ? p.table[(size_t)seq * p.table_ld + want + lane] : -1;
+    const bool issues = kPaged ? box < (BKV >> box_shift) : lane < C::HALVES;
+    uint32_t kn = 0, vn = 0, qn = 0;  // loads so far
+    bool ok = true;
+    Unit u;
+    for (int i = 0; ok; ++i) {
+      if (!__all_sync(0xffffffffu, next_unit(i, u))) break;
+      if (lane == 0) bar_arrive(&unit_empty[i & 1]);
+      if (u.nkv == 0) continue;
+      int ent = -1, ent_base = -1;
+      auto load = [&](const void* map, uint8_t* ring, uint64_t* full, uint64_t* empty, uint32_t& cnt, int j) -> bool {
+        const uint32_t s = cnt % RING;
+        const int key0 = (u.j0 + j) * BKV;
+        int page = 0;
+        if constexpr (kPaged) {
+          const int want = (key0 >> p.page_shift) & ~31;
+          if (want != ent_base) {  // 64 keys never reach past 32 pages (page >= 8)
+            ent_base = want;
+            ent = want + lane < p.table_width ? p.table[(size_t)u.seq * p.table_ld + want + lane] : -1;
+          }
+          page = __shfl_sync(0xffffffffu, ent, (((key0 + (box << box_shift)) >> p.page_shift) - ent_base) & 31);
         }
-        page = __shfl_sync(0xffffffffu, ent, (((key0 + (box << box_shift)) >> p.page_shift) - ent_base) & 31);
+        const bool good = wait_bar(&empty[s], ((cnt / RING) & 1) ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_TMA);
+        if (!__all_sync(0xffffffffu, good)) return false;
+        if (lane == 0) bar_arrive_expect_tx(&full[s], C::KV_BYTES);
+        __syncwarp();
+        if (issues) {
+          uint8_t* d = ring + s * C::KV_BYTES + half * C::KV_HALF;
+          if constexpr (kPaged)
+            tma_load_4d(d + (box << box_shift) * 128, map, &full[s], half * 64, u.kvh,
+                        (key0 + (box << box_shift)) & ((1 << p.page_shift) - 1), page);
+          else
+            tma_load_3d(d, map, &full[s], half * 64, u.kvh, u.q_begin + key0);
+        }
+        ++cnt;
+        return true;
+      };
+      const bool good = wait_bar(q_empty, (qn & 1) ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_TMA);
+      ok = __all_sync(0xffffffffu, good);
+      if (!ok) break;
+      if (lane == 0) {
+        bar_arrive_expect_tx(q_full, (uint32_t)(p.group * p.tile_tokens * HD * 2));
+        for (int h = 0; h < C::HALVES; ++h)
+          tma_load_3d(qs + h * C::Q_HALF, &qmap, q_full, h * 64, u.kvh * p.group, u.q_begin + u.t0);
       }
-      const bool good = wait_bar(&empty[s], ((j / RING) & 1) ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_TMA);
-      if (!__all_sync(0xffffffffu, good)) return false;
-      if (lane == 0) bar_arrive_expect_tx(&full[s], C::KV_BYTES);
       __syncwarp();
-      if (issues) {
-        uint8_t* d = ring + s * C::KV_BYTES + half * C::KV_HALF;
-        if constexpr (kPaged)
-          tma_load_4d(d + (box << box_shift) * 128, map, &full[s], half * 64, kvh,
-                      (key0 + (box << box_shift)) & ((1 << p.page_shift) - 1), page);
-        else
-          tma_load_3d(d, map, &full[s], half * 64, kvh, q_begin + key0);
+      ++qn;
+      // K runs two blocks ahead of V, as S does of P V: each load is asked for
+      // as soon as its slot is free, two blocks' time before it is needed.
+      ok = load(&kmap, ks, k_full, k_empty, kn, 0) && (u.nkv == 1 || load(&kmap, ks, k_full, k_empty, kn, 1));
+      for (int j = 0; j < u.nkv && ok; ++j) {
+        ok = load(&vmap, vs, v_full, v_empty, vn, j);
+        if (ok && j + 2 < u.nkv) ok = load(&kmap, ks, k_full, k_empty, kn, j + 2);
       }
-      return true;
-    };
-    // K runs two blocks ahead of V, as S does of P V: each load is asked for as
-    // soon as its slot is free, two blocks' time before it is needed.
-    bool ok = load(&kmap, ks, k_full, k_empty, 0) && (nkv == 1 || load(&kmap, ks, k_full, k_empty, 1));
-    for (int j = 0; j < nkv && ok; ++j) {
-      ok = load(&vmap, vs, v_full, v_empty, j);
-      if (ok && j + 2 < nkv) ok = load(&kmap, ks, k_full, k_empty, j + 2);
     }
-    if (!ok) {  // let copies in flight land before the shared memory is released
+    if (*abort_flag) {  // let copies in flight land before the shared memory is released
       const unsigned long long w0 = globaltimer_ns();
       while (globaltimer_ns() - w0 < 1000000ull) {
       }
@@ -342,42 +444,58 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
     if (elect_one()) {
       constexpr uint32_t idesc_s = make_idesc_f16(BQ, BKV, kBF16 ? 1 : 0, 0, 0);
       constexpr uint32_t idesc_o = make_idesc_f16(BQ, HD, kBF16 ? 1 : 0, 0, 1);
-      auto issue_s = [&](int j) -> bool {
-        const int s = j % RING;
-        if (!wait_bar(&k_full[s], (j / RING) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)) return false;
+      uint32_t sn = 0, gn = 0, un = 0;  // S products, P V products, units so far
+      auto issue_s = [&]() -> bool {
+        const uint32_t s = sn % RING;
+        if (!wait_bar(&k_full[s], (sn / RING) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)) return false;
         tc_fence_after();
         const uint32_t qa = smem_u32(qs), ka = smem_u32(ks + s * C::KV_BYTES);
 #pragma unroll
         for (int k16 = 0; k16 < HD / 16; ++k16)
-          mma_ss(tmem + S_COL + (j & 1) * BKV,
+          mma_ss(tmem + S_COL + (sn & 1) * BKV,
                  make_smem_desc(qa + (k16 >> 2) * C::Q_HALF + (k16 & 3) * 32, 16, 1024),
                  make_smem_desc(ka + (k16 >> 2) * C::KV_HALF + (k16 & 3) * 32, 16, 1024), idesc_s,
                  k16 > 0 ? 1u : 0u);
-        tc_commit(&s_full[j & 1]);
+        tc_commit(&s_full[sn & 1]);
         tc_commit(&k_empty[s]);
+        ++sn;
         return true;
       };
-      auto issue_pv = [&](int j) -> bool {
-        const int s = j % RING;
-        if (!wait_bar(&v_full[s], (j / RING) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)) return false;
-        if (!wait_bar(&v_fixed[s], (j / RING) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)) return false;
-        if (!wait_bar(&p_ready[j & 1], (j >> 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)) return false;
+      auto issue_pv = [&](bool fresh) -> bool {
+        const uint32_t s = gn % RING;
+        if (!wait_bar(&v_full[s], (gn / RING) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)) return false;
+        if (!wait_bar(&v_fixed[s], (gn / RING) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)) return false;
+        if (!wait_bar(&p_ready[gn & 1], (gn >> 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)) return false;
         tc_fence_after();
         const uint32_t va = smem_u32(vs + s * C::KV_BYTES);
 #pragma unroll
         for (int k16 = 0; k16 < BKV / 16; ++k16)
-          mma_ts(tmem + O_COL, tmem + S_COL + (j & 1) * BKV + k16 * 8,
-                 make_smem_desc(va + k16 * 16 * 128, C::KV_HALF, 1024), idesc_o,
-                 (j > 0 || k16 > 0) ? 1u : 0u);
-        tc_commit(&pv_done[j & 1]);
+          mma_ts(tmem + O_COL, tmem + S_COL + (gn & 1) * BKV + k16 * 8,
+                 make_smem_desc(va + k16 * 16 * 128, C::KV_HALF, 1024), idesc_o, (!fresh || k16 > 0) ? 1u : 0u);
+        tc_commit(&pv_done[gn & 1]);
         tc_commit(&v_empty[s]);
+        ++gn;
         return true;
       };
-      bool ok = wait_bar(q_full, 0, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA) && issue_s(0);
-      if (ok && nkv > 1) ok = issue_s(1);
-      for (int j = 0; j < nkv && ok; ++j) {
-        ok = issue_pv(j);
-        if (ok && j + 2 < nkv) ok = issue_s(j + 2);
+      Unit u;
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        if (!next_unit(i, u)) break;
+        bar_arrive(&unit_empty[i & 1]);
+        if (u.nkv == 0) continue;
+        ok = wait_bar(q_full, un & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA) && issue_s();
+        if (ok && u.nkv > 1) ok = issue_s();
+        if (ok && u.nkv <= 2) tc_commit(q_empty);
+        for (int j = 0; j < u.nkv && ok; ++j) {
+          // the rows of the unit before have been read out of O
+          if (j == 0) ok = wait_bar(o_empty, (un & 1) ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA);
+          if (ok) ok = issue_pv(j == 0);
+          if (ok && j + 2 < u.nkv) {
+            ok = issue_s();
+            if (ok && j + 3 == u.nkv) tc_commit(q_empty);
+          }
+        }
+        ++un;
       }
       tc_commit(drain);
       const uint32_t da = smem_u32(drain);
@@ -389,145 +507,183 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
         }
       }
     }
-  } else if (warp >= WARP_FIX) {
-    // Every block passes here, so that the two warps follow each phase of the
-    // ring; those before jb pass untouched.
-    for (int j = 0; j < nkv; ++j) {
-      const int s = j % RING;
-      const bool good = wait_bar(&v_full[s], (j / RING) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER);
-      if (!__all_sync(0xffffffffu, good)) break;
-      if (j < jb) {
-        if (lane == 0) bar_arrive(&v_fixed[s]);
-        continue;
-      }
-      const int key0 = (j0 + j) * BKV;
-      // one key per thread: row `key` of both halves (the swizzle permutes
-      // 16-byte pieces within a 128-byte row only)
-      const int r = (warp - WARP_FIX) * 32 + lane;
-      uint8_t* at = vs + s * C::KV_BYTES + r * 128;
-      if (key0 + r >= kv_len) {
-        for (int h = 0; h < C::HALVES; ++h)
+  } else if (warp == WARP_FIX) {
+    uint32_t vn = 0;
+    Unit u;
+    bool ok = true;
+    for (int i = 0; ok; ++i) {
+      if (!__all_sync(0xffffffffu, next_unit(i, u))) break;
+      if (lane == 0) bar_arrive(&unit_empty[i & 1]);
+      // Every block passes here, so that the warp follows each phase of the
+      // ring; those before jb pass untouched.
+      for (int j = 0; j < u.nkv; ++j, ++vn) {
+        const uint32_t s = vn % RING;
+        const bool good = wait_bar(&v_full[s], (vn / RING) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER);
+        ok = __all_sync(0xffffffffu, good);
+        if (!ok) break;
+        if (j >= u.jb) {
+          const int key0 = (u.j0 + j) * BKV;
+          for (int r = lane; r < BKV; r += 32) {
+            if (key0 + r < u.lim_min) continue;  // seen by every row
+            // row r of both halves (the swizzle permutes 16-byte pieces
+            // within a 128-byte row only)
+            uint8_t* at = vs + s * C::KV_BYTES + r * 128;
+            const bool past = key0 + r >= u.kv_len;
+            for (int h = 0; h < C::HALVES; ++h)
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<uint4*>(at + h * C::KV_HALF + ((i ^ r) & 7) * 16) = make_uint4(0, 0, 0, 0);
-      } else if (key0 + r >= lim_min) {
-        for (int h = 0; h < C::HALVES; ++h)
+              for (int k = 0; k < 8; ++k) {
+                uint4* q4 = reinterpret_cast<uint4*>(at + h * C::KV_HALF + ((k ^ r) & 7) * 16);
+                if (past) {
+                  *q4 = make_uint4(0, 0, 0, 0);
+                  continue;
+                }
+                uint32_t w[4] = {q4->x, q4->y, q4->z, q4->w};
+                bool bad = false;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            uint4* q4 = reinterpret_cast<uint4*>(at + h * C::KV_HALF + ((i ^ r) & 7) * 16);
-            uint32_t w[4] = {q4->x, q4->y, q4->z, q4->w};
-            bool bad = false;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const bool lo = finite16<kBF16>(w[k]), hi = finite16<kBF16>(w[k] >> 16);
-              bad |= !lo || !hi;
-              w[k] &= (lo ? 0x0000ffffu : 0u) | (hi ? 0xffff0000u : 0u);
-            }
-            if (bad) {
-              *q4 = make_uint4(w[0], w[1], w[2], w[3]);
-              *nonfinite = 1;
-            }
+                for (int m = 0; m < 4; ++m) {
+                  const bool lo = finite16<kBF16>(w[m]), hi = finite16<kBF16>(w[m] >> 16);
+                  bad |= !lo || !hi;
+                  w[m] &= (lo ? 0x0000ffffu : 0u) | (hi ? 0xffff0000u : 0u);
+                }
+                if (bad) {
+                  *q4 = make_uint4(w[0], w[1], w[2], w[3]);
+                  nonfinite[i & 1] = 1;
+                }
+              }
           }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        if (lane == 0) bar_arrive(&v_fixed[s]);
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) bar_arrive(&v_fixed[s]);
     }
-  } else if (warp < active) {
+  } else {
     const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
     const uint32_t o_addr = tmem + lane_base + O_COL;
-    const int lim = valid ? keys_seen(tok) : 0;
-    float m = -INFINITY, l = 0.0f;
+    const int row = warp * 32 + lane;
+    const int tok = row / p.group;
+    const unsigned long long sc2 = pack2(p.scale_log2, p.scale_log2);
+    uint32_t gn = 0;  // blocks so far
+    Unit u;
     bool ok = true;
-    for (int j = 0; j < nkv; ++j) {
-      const int buf = j & 1;
-      const uint32_t s_addr = tmem + lane_base + S_COL + buf * BKV;
-      bool good = wait_bar(&s_full[buf], (j >> 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_SOFTMAX);
-      if (!__all_sync(0xffffffffu, good)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      float s[BKV];
-      {
-        uint32_t r0[32], r1[32];
-        tmem_ld32(s_addr, r0);
-        tmem_ld32(s_addr + 32, r1);
-        tmem_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          s[i] = __uint_as_float(r0[i]);
-          s[32 + i] = __uint_as_float(r1[i]);
+    for (int i = 0; ok; ++i) {
+      if (!__all_sync(0xffffffffu, next_unit(i, u))) break;
+      const bool valid = tok < u.n_tok && row < p.tile_tokens * p.group;
+      const bool any = __any_sync(0xffffffffu, valid);
+      const int head = u.kvh * p.group + row - tok * p.group;
+      const size_t q_row = (size_t)(u.q_begin + u.t0 + tok);
+      uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + q_row * p.out_token + (size_t)head * p.out_head;
+      const size_t part = ((size_t)split * p.total_q + q_row) * p.n_heads + head;
+      if (u.nkv == 0) {  // no key: zeros (or a part of weight zero)
+        if (p.in_cluster) {
+          stats[row] = make_float2(-INFINITY, 0.f);
+        } else if (valid && p.splits > 1) {
+          p.part_lse[part] = -INFINITY;
+        } else if (valid) {
+          for (int k = 0; k < HD / 8; ++k) reinterpret_cast<uint4*>(dst)[k] = make_uint4(0, 0, 0, 0);
         }
+        __syncwarp();
+        if (lane == 0) bar_arrive(&unit_empty[i & 1]);
+        continue;
       }
-      if (j >= jb) {  // a key past the row's limit: whatever it gave, it counts nothing
-        const int left = lim - (j0 + j) * BKV;
-#pragma unroll
-        for (int c = 0; c < BKV; ++c)
-          if (c >= left) s[c] = -INFINITY;
-      }
-      float m8[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) m8[i] = fmaxf(s[i], s[8 + i]);
-#pragma unroll
-      for (int c = 16; c < BKV; c += 8) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m8[i] = fmaxf(m8[i], s[c + i]);
-      }
-      float mx = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])),
-                       fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])));
-      mx *= p.scale_log2;
-      float alpha = 1.0f;
-      if (mx > m + kRescaleThreshold) {
-        alpha = ex2(m - mx);
-        m = mx;
-      }
-      if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-        good = wait_bar(&pv_done[buf ^ 1], ((j - 1) >> 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_SOFTMAX);
-        if (!__all_sync(0xffffffffu, good)) {
-          ok = false;
-          break;
+      const int lim = valid ? keys_seen(u, p.causal, tok) : 0;
+      float m = -INFINITY, l = 0.0f;
+      for (int j = 0; j < u.nkv; ++j, ++gn) {
+        const uint32_t buf = gn & 1;
+        const uint32_t s_addr = tmem + lane_base + S_COL + buf * BKV;
+        bool good = wait_bar(&s_full[buf], (gn >> 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_SOFTMAX);
+        ok = __all_sync(0xffffffffu, good);
+        if (!ok) break;
+        if (!any) {  // no row here: P of these rows is never read out
+          if (lane == 0) bar_arrive(&p_ready[buf]);
+          continue;
         }
         tc_fence_after();
-#pragma unroll 1
-        for (int c = 0; c < HD / 32; ++c) {
-          uint32_t r[32];
-          tmem_ld32(o_addr + c * 32, r);
+        float s[BKV];
+        {
+          uint32_t r0[32], r1[32];
+          tmem_ld32(s_addr, r0);
+          tmem_ld32(s_addr + 32, r1);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
-          tmem_st32(o_addr + c * 32, r);
+          for (int k = 0; k < 32; ++k) {
+            s[k] = __uint_as_float(r0[k]);
+            s[32 + k] = __uint_as_float(r1[k]);
+          }
         }
-      }
-      const float mref = m == -INFINITY ? 0.0f : m;  // no key seen yet: every p is 2^-inf = 0
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        if (j >= u.jb) {  // a key past the row's limit: whatever it gave, it counts nothing
+          const int left = lim - (u.j0 + j) * BKV;
 #pragma unroll
-      for (int ch = 0; ch < BKV / 32; ++ch) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float a = ex2(fmaf(s[ch * 32 + 2 * i], p.scale_log2, -mref));
-          const float b = ex2(fmaf(s[ch * 32 + 2 * i + 1], p.scale_log2, -mref));
-          sum[i & 3] += a + b;
-          pk[i] = cvt2<kBF16>(a, b);
+          for (int c = 0; c < BKV; ++c)
+            if (c >= left) s[c] = -INFINITY;
         }
-        tmem_st16(s_addr + ch * 16, pk);
+        float m8[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m8[k] = fmaxf(s[k], s[8 + k]);
+#pragma unroll
+        for (int c = 16; c < BKV; c += 16) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) m8[k] = max3f(m8[k], s[c + k], s[c + 8 + k]);
+        }
+        const float mx = max3f(max3f(m8[0], m8[1], m8[2]), max3f(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7])) *
+                         p.scale_log2;
+        float alpha = 1.0f;
+        if (mx > m + kRescaleThreshold) {
+          alpha = ex2(m - mx);
+          m = mx;
+        }
+        if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+          good = wait_bar(&pv_done[buf ^ 1], ((gn - 1) >> 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_SOFTMAX);
+          ok = __all_sync(0xffffffffu, good);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t r[32];
+            tmem_ld32(o_addr + c * 32, r);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * alpha);
+            tmem_st32(o_addr + c * 32, r);
+          }
+        }
+        const float mref = m == -INFINITY ? 0.0f : m;  // no key seen yet: every p is 2^-inf = 0
+        const unsigned long long nm2 = pack2(-mref, -mref);
+        unsigned long long sum2[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+        for (int ch = 0; ch < BKV / 32; ++ch) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            float a, b;
+            unpack2(fma2(pack2(s[ch * 32 + 2 * k], s[ch * 32 + 2 * k + 1]), sc2, nm2), a, b);
+            a = ex2(a);
+            b = ex2(b);
+            sum2[k & 3] = add2(sum2[k & 3], pack2(a, b));
+            pk[k] = cvt2<kBF16>(a, b);
+          }
+          tmem_st16(s_addr + ch * 16, pk);
+        }
+        float a0, a1;
+        unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), a0, a1);
+        l = l * alpha + (a0 + a1);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&p_ready[buf]);
       }
-      l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive(&p_ready[buf]);
-    }
-    if (ok) {
-      const int last = nkv - 1;
-      const bool good = wait_bar(&pv_done[last & 1], (last >> 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_SOFTMAX);
-      if (__all_sync(0xffffffffu, good)) {
+      if (!ok) break;
+      const bool good = !any || wait_bar(&pv_done[(gn - 1) & 1], ((gn - 1) >> 1) & 1, abort_flag, p.err,
+                                         DEV_ERR_TIMEOUT_SOFTMAX);
+      ok = __all_sync(0xffffffffu, good);
+      if (!ok) break;
+      if (any) {
         tc_fence_after();
         const float inv_l = l == 0.0f ? 0.0f : 1.0f / l;  // no key in this range: zeros
-        const bool repair = *nonfinite != 0;
+        const bool repair = nonfinite[i & 1] != 0;
         // keys that only some rows see, within this CTA's range
-        const int from = max(lim_min, (j0 + jb) * BKV), to = min(lim, (j0 + nkv) * BKV);
+        const int from = max(u.lim_min, (u.j0 + u.jb) * BKV), to = min(lim, (u.j0 + u.nkv) * BKV);
+        if (p.in_cluster) stats[row] = make_float2(l == 0.0f ? -INFINITY : m + log2f(l), 0.f);
 #pragma unroll 1
         for (int c = 0; c < HD / 32; ++c) {
           uint32_t r[32];
@@ -536,42 +692,102 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
           if (!valid) continue;
           float o[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(r[i]) * inv_l;
+          for (int k = 0; k < 32; ++k) o[k] = __uint_as_float(r[k]) * inv_l;
           if (repair) {
             for (int key = from; key < to; ++key) {
-              const uint16_t* src = static_cast<const uint16_t*>(p.v) + (size_t)kvh * p.v_head + c * 32;
+              const uint16_t* src = static_cast<const uint16_t*>(p.v) + (size_t)u.kvh * p.v_head + c * 32;
               if constexpr (kPaged) {
-                const int page = p.table[(size_t)seq * p.table_ld + (key >> p.page_shift)];
+                const int page = p.table[(size_t)u.seq * p.table_ld + (key >> p.page_shift)];
                 if (page < 0 || page >= p.n_pages) continue;
                 src += (size_t)page * p.v_page + (size_t)(key & ((1 << p.page_shift) - 1)) * p.v_token;
               } else {
-                src += (size_t)(q_begin + key) * p.v_token;
+                src += (size_t)(u.q_begin + key) * p.v_token;
               }
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (!finite16<kBF16>(src[i])) o[i] += to_f32<kBF16>(src[i]);
+              for (int k = 0; k < 32; ++k)
+                if (!finite16<kBF16>(src[k])) o[k] += to_f32<kBF16>(src[k]);
             }
           }
           if (p.splits > 1) {
-            float4* d4 = reinterpret_cast<float4*>(p.part_o + part * HD + c * 32);
+            // global memory, or the rings (every product of the unit is done);
+            // there, 16-byte pieces are permuted within a row against conflicts
+            float* po = p.in_cluster ? reinterpret_cast<float*>(ks) + row * HD : p.part_o + part * HD;
+            const int x = p.in_cluster ? row & 7 : 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              d4[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            for (int k = 0; k < 8; ++k)
+              *reinterpret_cast<float4*>(po + ((c * 8 + k) ^ x) * 4) =
+                  make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
           } else {
             uint4* d4 = reinterpret_cast<uint4*>(dst + c * 32);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              d4[i] = make_uint4(cvt2<kBF16>(o[8 * i], o[8 * i + 1]), cvt2<kBF16>(o[8 * i + 2], o[8 * i + 3]),
-                                 cvt2<kBF16>(o[8 * i + 4], o[8 * i + 5]), cvt2<kBF16>(o[8 * i + 6], o[8 * i + 7]));
+            for (int k = 0; k < 4; ++k)
+              d4[k] = make_uint4(cvt2<kBF16>(o[8 * k], o[8 * k + 1]), cvt2<kBF16>(o[8 * k + 2], o[8 * k + 3]),
+                                 cvt2<kBF16>(o[8 * k + 4], o[8 * k + 5]), cvt2<kBF16>(o[8 * k + 6], o[8 * k + 7]));
           }
         }
-        if (valid && p.splits > 1) p.part_lse[part] = l == 0.0f ? -INFINITY : m + log2f(l);
+        if (valid && p.splits > 1 && !p.in_cluster) p.part_lse[part] = l == 0.0f ? -INFINITY : m + log2f(l);
+        tc_fence_before();
+      }
+      __syncwarp();
+      if (lane == 0) {
+        bar_arrive(o_empty);
+        bar_arrive(&unit_empty[i & 1]);
       }
     }
     tc_fence_before();
   }
   __syncthreads();
+  if (p.in_cluster) {
+    // Merge: row r of the unit by CTA r % splits, HD / 8 threads per row, the
+    // parts in the order of their keys.
+    cluster_sync_all();
+    const Unit& u = units[0];
+    if (!*abort_flag && u.nkv >= 0) {
+      const int rows = u.n_tok * p.group;
+      const int d8 = (int)(threadIdx.x % (HD / 8)) * 2;  // 16-byte pieces d8, d8 + 1
+      const uint32_t st0 = smem_u32(stats), o0 = smem_u32(ks);
+      for (int r = split + p.splits * (int)(threadIdx.x / (HD / 8)); r < rows;
+           r += p.splits * (NUM_THREADS / (HD / 8))) {
+        float lse[kMaxCluster];
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < kMaxCluster; ++c)
+          if (c < p.splits) {
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(lse[c]) : "r"(mapa_shared(st0 + r * 8u, c)) : "memory");
+          }
+#pragma unroll
+        for (int c = 0; c < kMaxCluster; ++c)
+          if (c < p.splits) top = lse[c] > top || lse[c] != lse[c] ? lse[c] : top;  // a NaN sum stays
+        float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, total = 0.f;
+#pragma unroll
+        for (int c = 0; c < kMaxCluster; ++c) {
+          if (c >= p.splits || lse[c] == -INFINITY) continue;
+          const float w = exp2f(lse[c] - top);
+          total += w;
+          const uint32_t a = mapa_shared(o0 + (uint32_t)r * (HD * 4u), c);
+          float v[8];
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(v[4 * k]), "=f"(v[4 * k + 1]), "=f"(v[4 * k + 2]), "=f"(v[4 * k + 3])
+                         : "r"(a + (uint32_t)((d8 + k) ^ (r & 7)) * 16u)
+                         : "memory");
+#pragma unroll
+          for (int k = 0; k < 8; ++k) acc[k] = fmaf(w, v[k], acc[k]);
+        }
+        const float inv = total == 0.f ? 0.f : 1.0f / total;
+        const int tk = r / p.group, head = u.kvh * p.group + r - tk * p.group;
+        uint32_t h[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) h[k] = cvt2<kBF16>(acc[2 * k] * inv, acc[2 * k + 1] * inv);
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + (size_t)(u.q_begin + u.t0 + tk) * p.out_token +
+                                  (size_t)head * p.out_head + d8 * 4) = make_uint4(h[0], h[1], h[2], h[3]);
+      }
+    }
+    cluster_sync_all();  // no CTA ends while another reads its shared memory
+  }
   if (warp == WARP_MMA) {
+    __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, TMEM_COLS);
   }
@@ -587,8 +803,12 @@ __global__ void text_combine_kernel(const float* __restrict__ part_o, const floa
   const long long idx = blockIdx.x * (long long)blockDim.x + threadIdx.x;
   const long long items = (long long)rows * n_heads;
   const long long it = idx / (HD / 8);
-  if (it >= items) return;
+  if (it >= items) {
+    griddep_wait();
+    return;
+  }
   const int d8 = (int)(idx % (HD / 8)) * 8;
+  griddep_wait();
   float top = -INFINITY;
   for (int s = 0; s < splits; ++s) {
     const float x = part_lse[s * items + it];
@@ -627,8 +847,13 @@ __global__ void paged_append_kernel(const uint16_t* __restrict__ k, const uint16
   const int pieces = n_kv * (head_dim / 8);
   const long long idx = blockIdx.x * (long long)blockDim.x + threadIdx.x;
   const long long t = idx / pieces;
-  if (t >= total) return;
+  if (t >= total) {
+    griddep_wait();
+    return;
+  }
   const int piece = (int)(idx - t * pieces);
+  griddep_wait();
+  griddep_launch();
   const int h = piece / (head_dim / 8), d = (piece - h * (head_dim / 8)) * 8;
   int lo = 0, hi = n_seqs;  // the last sequence that begins at or before t
   while (hi - lo > 1) {
@@ -670,34 +895,88 @@ int encode(CUtensorMap* map, void* base, bool bf16, int rank, const long long* d
   return 0;
 }
 
+// Largest number of co-resident clusters of `size` CTAs (a cluster lies within
+// one GPC); 0 if the query fails.  The occupancy query counts one CTA per SM
+// for a kernel that allocates TMEM; two of these fit (256 of the 512 columns,
+// half the shared memory and registers each) and do run.
 template <int HD, bool kBF16, bool kPaged>
-int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const Params& p,
-           long long ctas, cudaStream_t st) {
+int cluster_slots(int size) {
+  static int slots[64][kMaxCluster + 1];
+  static bool known[64][kMaxCluster + 1];
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lock(mu);
+  const int d = device_slot();
+  if (known[d][size]) return slots[d][size];
+  known[d][size] = true;
   auto kern = text_attention_kernel<HD, kBF16, kPaged>;
-  static std::once_flag once[64];
-  cudaError_t e = cudaSuccess;
-  std::call_once(once[device_slot()], [&] {
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD>::SMEM_BYTES);
-  });
-  if (e != cudaSuccess) return cuda_status(e, "text attention set smem attribute");
-  kern<<<(unsigned)ctas, NUM_THREADS, Cfg<HD>::SMEM_BYTES, st>>>(qm, km, vm, p);
-  int rc = launch_status("text_attention_kernel launch");
-  if (rc || p.splits == 1) return rc;
-  const long long threads = (long long)p.total_q * p.n_heads * (HD / 8);
-  text_combine_kernel<HD, kBF16><<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(
-      p.part_o, p.part_lse, p.splits, p.total_q, p.n_heads, static_cast<uint16_t*>(p.out), p.out_token,
-      p.out_head);
-  return launch_status("text_combine_kernel launch");
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD>::SMEM_BYTES) == cudaSuccess &&
+      cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) ==
+          cudaSuccess &&
+      cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)size;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)size);
+    cfg.blockDim = dim3(NUM_THREADS);
+    cfg.dynamicSmemBytes = Cfg<HD>::SMEM_BYTES;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int c = 0;
+    if (cudaOccupancyMaxActiveClusters(&c, kern, &cfg) == cudaSuccess) slots[d][size] = 2 * c;
+  }
+  cudaGetLastError();
+  return slots[d][size];
+}
+
+template <int HD, bool kBF16, bool kPaged>
+int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, Params p, long long units,
+           int max_ctx, cudaStream_t st) {
+  auto kern = text_attention_kernel<HD, kBF16, kPaged>;
+  // CTA slots; the query also prepares the kernel for its shared memory
+  const long long slots = cluster_slots<HD, kBF16, kPaged>(1);
+  if (slots < 1) return fail(-3, "text attention: the kernel cannot be scheduled on this device");
+  // Key split: where the units leave CTA slots empty, each unit's keys are cut
+  // into ranges of at least 4 blocks.  Up to kMaxCluster ranges are one
+  // cluster, as many as fit the GPU at once.
+  const long long blocks = ((long long)max_ctx + BKV - 1) / BKV;
+  long long want = kPaged ? std::max(1ll, std::min(slots / units, blocks / 4)) : 1;
+  p.splits = (int)std::min(want, 64ll);
+  if (p.splits > 1 && p.splits <= kMaxCluster) {
+    while (p.splits > 1 && cluster_slots<HD, kBF16, kPaged>(p.splits) < units) --p.splits;
+    p.in_cluster = p.splits > 1;
+  }
+  void* part = nullptr;
+  if (p.splits > 1 && !p.in_cluster) {
+    const size_t items = (size_t)p.splits * p.total_q * p.n_heads;
+    const int rc = scratch_alloc(&part, items * (HD + 1) * sizeof(float), "text attention", st);
+    if (rc) return rc;
+    p.part_o = static_cast<float*>(part);
+    p.part_lse = p.part_o + items * HD;
+  }
+  const long long ctas = p.splits > 1 ? units * p.splits : std::min(units, slots);
+  int rc = launch_after("text_attention_kernel launch", kern, dim3((unsigned)ctas), dim3(NUM_THREADS),
+                        Cfg<HD>::SMEM_BYTES, p.in_cluster ? p.splits : 1, st, qm, km, vm, p);
+  if (rc == 0 && part) {
+    const long long threads = (long long)p.total_q * p.n_heads * (HD / 8);
+    rc = launch_after("text_combine_kernel launch", text_combine_kernel<HD, kBF16>,
+                      dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, 1, st, p.part_o, p.part_lse, p.splits,
+                      p.total_q, p.n_heads, static_cast<uint16_t*>(p.out), p.out_token, p.out_head);
+  }
+  scratch_free(part, st);
+  return rc;
 }
 
 template <bool kPaged>
 int dispatch(const TextAttention& a, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm,
-             const Params& p, long long ctas, cudaStream_t st) {
+             const Params& p, long long units, cudaStream_t st) {
   if (a.head_dim == 128)
-    return a.bf16 ? launch<128, true, kPaged>(qm, km, vm, p, ctas, st)
-                  : launch<128, false, kPaged>(qm, km, vm, p, ctas, st);
-  return a.bf16 ? launch<64, true, kPaged>(qm, km, vm, p, ctas, st)
-                : launch<64, false, kPaged>(qm, km, vm, p, ctas, st);
+    return a.bf16 ? launch<128, true, kPaged>(qm, km, vm, p, units, a.max_ctx, st)
+                  : launch<128, false, kPaged>(qm, km, vm, p, units, a.max_ctx, st);
+  return a.bf16 ? launch<64, true, kPaged>(qm, km, vm, p, units, a.max_ctx, st)
+                : launch<64, false, kPaged>(qm, km, vm, p, units, a.max_ctx, st);
 }
 
 }  // namespace text
@@ -705,17 +984,13 @@ int dispatch(const TextAttention& a, const CUtensorMap& qm, const CUtensorMap& k
 int launch_text_attention(const TextAttention& a, cudaStream_t st) {
   using namespace text;
   if (a.total_q == 0 || a.n_seqs == 0) return 0;
-  if (a.n_seqs > kMaxSeqs) return fail(-2, "text attention: more than 8192 sequences in one call");
   const int group = a.n_heads / a.n_kv;
   Params p{};
-  p.cu = a.cu;
-  p.ctx = a.ctx;
-  p.table = a.table;
   p.table_ld = a.table_ld;
   p.table_width = a.table_width;
   p.page_shift = a.page_shift;
   p.n_pages = a.n_pages;
-  p.n_seqs = a.n_seqs;
+  p.splits = 1;
   p.total_q = a.total_q;
   p.n_heads = a.n_heads;
   p.n_kv = a.n_kv;
@@ -757,31 +1032,20 @@ int launch_text_attention(const TextAttention& a, cudaStream_t st) {
     if (rc) return rc;
   }
 
-  // Tiles: sum_i ceil(q_len_i / T) <= (total + n * (T - 1)) / T; CTAs past the
-  // real number of tiles end at once.
-  const long long T = p.tile_tokens;
-  const long long seqs = std::min<long long>(a.n_seqs, a.total_q);
-  const long long units = ((a.total_q + seqs * (T - 1)) / T) * a.n_kv;
-  // Key split: where the units leave CTA slots (two per SM) empty, each
-  // unit's keys are cut into ranges of at least 4 blocks.
-  const long long slots = 2ll * num_sms();
-  const long long blocks = ((long long)a.max_ctx + BKV - 1) / BKV;
-  long long splits = paged ? std::min(slots / units, blocks / 4) : 1;
-  p.splits = (int)std::max(1ll, std::min(splits, 64ll));
-  const long long ctas = units * p.splits;
-  if (ctas > 0x7fffffffll) return fail(-2, "text attention: too many tiles in one call");
-
-  void* part = nullptr;
-  if (p.splits > 1) {
-    const size_t items = (size_t)p.splits * a.total_q * a.n_heads;
-    const int rc = scratch_alloc(&part, items * (a.head_dim + 1) * sizeof(float), "text attention", st);
+  for (int s0 = 0; s0 < a.n_seqs; s0 += kMaxSeqs) {
+    p.n_seqs = std::min(kMaxSeqs, a.n_seqs - s0);
+    p.cu = a.cu + s0;
+    p.ctx = paged ? a.ctx + s0 : nullptr;
+    p.table = paged ? a.table + s0 * a.table_ld : nullptr;
+    // Tiles: sum_i ceil(q_len_i / T) <= (total + n * (T - 1)) / T; CTAs past
+    // the real number of tiles end at once.
+    const long long T = p.tile_tokens, seqs = std::min(p.n_seqs, a.total_q);
+    const long long units = (a.total_q + seqs * (T - 1)) / T * a.n_kv;
+    if (units > 0x7fffffffll / 64) return fail(-2, "text attention: too many tiles in one call");
+    const int rc = paged ? dispatch<true>(a, qm, km, vm, p, units, st) : dispatch<false>(a, qm, km, vm, p, units, st);
     if (rc) return rc;
-    p.part_o = static_cast<float*>(part);
-    p.part_lse = p.part_o + items * a.head_dim;
   }
-  const int rc = paged ? dispatch<true>(a, qm, km, vm, p, ctas, st) : dispatch<false>(a, qm, km, vm, p, ctas, st);
-  scratch_free(part, st);
-  return rc;
+  return 0;
 }
 
 int launch_paged_append(const TextTensor& k, const TextTensor& v, const TextTensor& kc, const TextTensor& vc,
@@ -792,12 +1056,11 @@ int launch_paged_append(const TextTensor& k, const TextTensor& v, const TextTens
   const long long threads = (long long)total * n_kv * (head_dim / 8);
   const long long blocks = (threads + 255) / 256;
   if (blocks > 0x7fffffffll) return fail(-2, "paged_append: too many values in one call");
-  text::paged_append_kernel<<<(unsigned)blocks, 256, 0, st>>>(
-      static_cast<const uint16_t*>(k.data), static_cast<const uint16_t*>(v.data), k.token, k.head, v.token,
-      v.head, static_cast<uint16_t*>(kc.data), static_cast<uint16_t*>(vc.data), kc.page, kc.token, kc.head,
-      vc.page, vc.token, vc.head, n_pages, page_shift, table, table_ld, table_width, cu, ctx, n_seqs, total,
-      n_kv, head_dim);
-  return launch_status("paged_append_kernel launch");
+  return launch_after("paged_append_kernel launch", text::paged_append_kernel, dim3((unsigned)blocks), dim3(256), 0, 1,
+                      st, static_cast<const uint16_t*>(k.data), static_cast<const uint16_t*>(v.data), k.token, k.head,
+                      v.token, v.head, static_cast<uint16_t*>(kc.data), static_cast<uint16_t*>(vc.data), kc.page,
+                      kc.token, kc.head, vc.page, vc.token, vc.head, n_pages, page_shift, table, table_ld, table_width,
+                      cu, ctx, n_seqs, total, n_kv, head_dim);
 }
 
 }  // namespace bonsai

@@ -302,7 +302,7 @@ typedef struct {
 
 /* Attention over whole prompts, packed one after another: sequence s has the
  * rows [cu_seqlens[s], cu_seqlens[s + 1]) of q, k, v and out (device int32
- * [n_seqs + 1], ascending; lengths may be zero; at most 8192 sequences).
+ * [n_seqs + 1], ascending; lengths may be zero).
  * Query head h reads key/value head h / (n_heads / n_kv_heads).  causal != 0:
  * a token sees its own sequence up to itself; 0: all of its sequence.
  *   out[t][h] = sum_j softmax_j(scale * q[t][h] . k[j]) v[j]

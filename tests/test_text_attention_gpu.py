@@ -360,3 +360,22 @@ def test_same_call_twice_gives_the_same_bits(gpu):
     q = randn(19, 70, 8, 128, dtype=bf16)
     a = run_paged(gpu, q, kc, vc, table, [0, 1, 70], ctx, 16)
     assert torch.equal(a, run_paged(gpu, q, kc, vc, table, [0, 1, 70], ctx, 16))
+
+
+@pytest.mark.parametrize("kv,ctx", [(1, [20000]), (1, [70]), (2, [3000, 9]), (2, [40000, 0, 17, 5000])], ids=str)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_paged_key_splits(gpu, kv, ctx, dim):
+    """Few units: their keys are split over a cluster, or more widely through
+    global memory; sequences shorter than the split leave parts without keys."""
+    kc, vc, table = make_cache(20, ctx, 64, kv, dim, bf16, fill=float("nan"))
+    n = len(ctx)
+    run_paged(gpu, randn(21, n, 8 * kv, dim, dtype=bf16), kc, vc, table, list(range(n + 1)), ctx, 64)
+
+
+def test_prompt_more_units_than_slots(gpu):
+    """Long and short sequences in one launch, several units per CTA, some of one
+    block and some of many, both masks."""
+    lens = [1, 900, 64, 3, 1500, 130, 0, 31] * 4
+    q, k, v = (randn(i, sum(lens), h, 64) for i, h in enumerate((8, 8, 8)))
+    run_prompt(gpu, q, k, v, cumulated(lens))
+    run_prompt(gpu, q, k, v, cumulated(lens), causal=False)

@@ -43,7 +43,7 @@ PAGES = [(dict(kc=None), ARG), (dict(vc=pages(size=12)), UNSUPPORTED), (dict(vc=
          (dict(ctx=None), ARG), (dict(ld=8), ARG), (dict(width=-1, ld=3), ARG)]
 
 
-@pytest.mark.parametrize("bad,code", SHAPES + ATTENTION + [(dict(cu=None), ARG), (dict(n=9000, T=9000), UNSUPPORTED),
+@pytest.mark.parametrize("bad,code", SHAPES + ATTENTION + [(dict(cu=None), ARG),
                                                            (dict(k=heads(token=1001)), ARG)], ids=str)
 def test_prompt_attention_refuses(bad, code):
     assert prompt(**bad) == code
