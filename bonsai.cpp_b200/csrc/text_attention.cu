@@ -37,8 +37,7 @@
 // are split between the CTAs of a cluster, which merge their parts through
 // distributed shared memory; a split wider than a cluster goes through global
 // memory and a second kernel.
-// TMEM (256 columns): S(even) [0, 64) S(odd) [64, 128) O [128, 128 + HD);
-// P(j) (16-bit pairs) overwrites the first 32 columns of its S.
+// TMEM: per tile S(even), S(odd) of 64 columns each, then O of each tile; P(j) (16-bit pairs) overwrites the first 32 columns of its S.
 #include "internal.cuh"
 #include "ptx.cuh"
 
@@ -53,19 +52,24 @@ PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn();
 }
 namespace text {
 
-constexpr int BQ = 128;   // query rows per CTA
+constexpr int BQ = 128;   // query rows per tile
 constexpr int BKV = 64;   // keys per block
-constexpr int RING = 2;   // K and V slots
-constexpr int NUM_THREADS = 256;
-constexpr int WARP_TMA = 4, WARP_MMA = 5, WARP_FIX = 6, WARP_PLAN = 7;
-constexpr int TMEM_COLS = 256;
-constexpr int S_COL = 0, O_COL = 128;
 constexpr float kRescaleThreshold = 8.0f;
 constexpr int kMaxSeqs = 512;     // sequences of one launch (their lengths are kept in shared memory)
 constexpr int kMaxCluster = 16;   // CTAs that split a unit's keys and merge in shared memory
 
-template <int HD>
+// A kernel form: head dims, and query tiles per CTA.  One tile (two CTAs per
+// SM) for single tokens, where K and V are read once and the number of CTAs
+// counts; two tiles (one CTA per SM) for prompts, where every 128 rows read
+// all of K and V again and the L2's bandwidth bounds the one-tile form.
+template <int HD, int NT>
 struct Cfg {
+  static constexpr int RING = NT == 1 ? 2 : 4;  // K and V slots
+  static constexpr int SOFTMAX_WARPS = 4 * NT;
+  static constexpr int WARP_TMA = 4 * NT, WARP_MMA = WARP_TMA + 1, WARP_FIX = WARP_TMA + 2, WARP_PLAN = WARP_TMA + 3;
+  static constexpr int NUM_THREADS = (WARP_PLAN + 1) * 32;
+  // TMEM: S of tile g, buffer b at g * 128 + b * 64; O of tile g after all S
+  static constexpr int TMEM_COLS = 256 * NT, O_COL = 128 * NT;
   static constexpr int HALVES = HD / 64;
   static constexpr int Q_HALF = BQ * 128;         // 128 rows x 64 dims
   static constexpr int Q_BYTES = HALVES * Q_HALF;
@@ -73,11 +77,12 @@ struct Cfg {
   static constexpr int KV_BYTES = HALVES * KV_HALF;
   // K and V rings; once a unit's products are done they can hold its O (f32)
   static constexpr int RINGS_BYTES = 2 * RING * KV_BYTES;
-  static_assert(RINGS_BYTES >= BQ * HD * 4, "O does not fit the rings");
-  static constexpr int SMEM_BYTES = 1024 + Q_BYTES + RINGS_BYTES + 512 + BQ * 8 + kMaxSeqs * 8;
+  static_assert(RINGS_BYTES >= NT * BQ * HD * 4, "O does not fit the rings");
+  static constexpr int BAR_BYTES = 512;
+  static constexpr int SMEM_BYTES = 1024 + NT * Q_BYTES + RINGS_BYTES + BAR_BYTES + NT * BQ * 8 + kMaxSeqs * 8 +
+                                    SOFTMAX_WARPS * 2048;
+  static_assert((SMEM_BYTES + 1024) * (3 - NT) <= 228 * 1024, "CTAs per SM");
 };
-// Two CTAs per SM (228 KB, 1 KB of it reserved for each).
-static_assert(2 * (Cfg<128>::SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs per SM");
 
 struct Params {
   const int* cu;        // [n_seqs + 1] first query row of each sequence
@@ -116,6 +121,13 @@ template <bool kBF16>
 __device__ __forceinline__ bool finite16(uint32_t h) {  // low 16 bits
   constexpr uint32_t e = kBF16 ? 0x7f80u : 0x7c00u;
   return (h & e) != e;
+}
+// Non-zero where one of eight values has an exponent of all ones: adding one to
+// the exponent field carries into the sign's place then, and nowhere else.
+template <bool kBF16>
+__device__ __forceinline__ uint32_t nonfinite_bits(uint4 v) {
+  constexpr uint32_t e = kBF16 ? 0x7f807f80u : 0x7c007c00u, one = kBF16 ? 0x00800080u : 0x04000400u;
+  return (((v.x & e) + one) | ((v.y & e) + one) | ((v.z & e) + one) | ((v.w & e) + one)) & 0x80008000u;
 }
 template <bool kBF16>
 __device__ __forceinline__ float to_f32(uint16_t h) {
@@ -248,17 +260,18 @@ struct Finder {
   }
 };
 
-template <int HD, bool kBF16, bool kPaged>
-__global__ void __launch_bounds__(NUM_THREADS, 2)
+template <int HD, bool kBF16, bool kPaged, int NT>
+__global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
     text_attention_kernel(const __grid_constant__ CUtensorMap qmap,
                           const __grid_constant__ CUtensorMap kmap,
                           const __grid_constant__ CUtensorMap vmap, const Params p) {
-  using C = Cfg<HD>;
+  using C = Cfg<HD, NT>;
+  constexpr int RING = C::RING;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   uint8_t* qs = smem;
-  uint8_t* ks = qs + C::Q_BYTES;
+  uint8_t* ks = qs + NT * C::Q_BYTES;
   uint8_t* vs = ks + RING * C::KV_BYTES;
   Unit* units = reinterpret_cast<Unit*>(vs + RING * C::KV_BYTES);  // [2]
   uint64_t* unit_full = reinterpret_cast<uint64_t*>(units + 2);
@@ -270,16 +283,17 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
   uint64_t* v_full = k_empty + RING;
   uint64_t* v_empty = v_full + RING;
   uint64_t* v_fixed = v_empty + RING;
-  uint64_t* s_full = v_fixed + RING;
-  uint64_t* p_ready = s_full + 2;
-  uint64_t* pv_done = p_ready + 2;
-  uint64_t* o_empty = pv_done + 2;
-  uint64_t* drain = o_empty + 1;
+  uint64_t* s_full = v_fixed + RING;      // [2 * NT] tile g, buffer b: g * 2 + b
+  uint64_t* p_ready = s_full + 2 * NT;    // [2 * NT]
+  uint64_t* pv_done = p_ready + 2 * NT;   // [2 * NT]
+  uint64_t* o_empty = pv_done + 2 * NT;   // [NT]
+  uint64_t* drain = o_empty + NT;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* nonfinite = abort_flag + 1;  // [2] by unit
-  float2* stats = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(units) + 512);  // [BQ] log2 sum (cluster merge)
-  int2* lens = reinterpret_cast<int2*>(stats + BQ);  // [kMaxSeqs]
+  float2* stats = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(units) + C::BAR_BYTES);  // [NT * BQ] log2 sum (cluster merge)
+  int2* lens = reinterpret_cast<int2*>(stats + NT * BQ);  // [kMaxSeqs]
+  uint4* stage = reinterpret_cast<uint4*>(lens + kMaxSeqs);  // 2 KB per softmax warp
 
   const int warp = threadIdx.x / 32;
   const int lane = (int)lane_id();
@@ -290,11 +304,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       bar_init(&unit_full[i], 1);
-      bar_init(&unit_empty[i], 7);  // softmax warps, TMA, MMA, fix
+      bar_init(&unit_empty[i], C::SOFTMAX_WARPS + 3);  // softmax warps, TMA, MMA, fix
+      nonfinite[i] = 0;
+    }
+    for (int i = 0; i < 2 * NT; ++i) {
       bar_init(&s_full[i], 1);
       bar_init(&p_ready[i], 4);
       bar_init(&pv_done[i], 1);
-      nonfinite[i] = 0;
     }
     bar_init(q_full, 1);
     bar_init(q_empty, 1);
@@ -305,7 +321,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
       bar_init(&v_empty[s], 1);
       bar_init(&v_fixed[s], 1);
     }
-    bar_init(o_empty, 4);
+    for (int g = 0; g < NT; ++g) bar_init(&o_empty[g], 4);
     bar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -313,13 +329,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
     tma_prefetch_desc(&kmap);
     tma_prefetch_desc(&vmap);
   }
-  if (warp == WARP_MMA) {
-    tmem_alloc(tmem_slot, TMEM_COLS);
+  if (warp == C::WARP_MMA) {
+    tmem_alloc(tmem_slot, C::TMEM_COLS);
     tmem_relinquish();
   }
   griddep_wait();
   griddep_launch();
-  for (int i = threadIdx.x; i < p.n_seqs; i += NUM_THREADS) {
+  for (int i = threadIdx.x; i < p.n_seqs; i += C::NUM_THREADS) {
     const int a = max(0, min(p.cu[i], p.total_q)), b = max(a, min(p.cu[i + 1], p.total_q));
     lens[i] = make_int2(b - a, kPaged ? p.ctx[i] - (b - a) : 0);
   }
@@ -339,8 +355,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
     return u.nkv >= 0;
   };
 
-  if (warp == WARP_PLAN) {
-    Finder f{lens, p.n_seqs, p.tile_tokens, p.causal, kPaged ? (long long)p.table_width << p.page_shift : 0x7fffffffll};
+  if (warp == C::WARP_PLAN) {
+    Finder f{lens, p.n_seqs, NT * p.tile_tokens, p.causal, kPaged ? (long long)p.table_width << p.page_shift : 0x7fffffffll};
     f.init();
     for (int i = 0;; ++i) {
       // units come longest first: rounds go up and down the CTAs in turn, so
@@ -356,8 +372,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
         u.kvh = unit % p.n_kv;
         u.q_begin = max(0, min(p.cu[seq], p.total_q));
         u.kv_len = f.kv_len(s);
-        u.t0 = level * p.tile_tokens;
-        u.n_tok = min(p.tile_tokens, s.x - u.t0);
+        u.t0 = level * NT * p.tile_tokens;
+        u.n_tok = min(NT * p.tile_tokens, s.x - u.t0);
         u.first = s.y + u.t0;
         u.lim_min = keys_seen(u, p.causal, 0);
         const int blocks = (keys_seen(u, p.causal, u.n_tok - 1) + BKV - 1) / BKV;
@@ -375,7 +391,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
       }
       if (u.nkv < 0) break;
     }
-  } else if (warp == WARP_TMA) {
+  } else if (warp == C::WARP_TMA) {
     // Paged: a block of 64 keys takes 64 / page boxes (one where a page holds
     // more), and each half of the head dims its own; lane l issues box
     // l / HALVES, half l % HALVES.  `ent` = 32 consecutive page indices.
@@ -421,9 +437,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
       ok = __all_sync(0xffffffffu, good);
       if (!ok) break;
       if (lane == 0) {
-        bar_arrive_expect_tx(q_full, (uint32_t)(p.group * p.tile_tokens * HD * 2));
-        for (int h = 0; h < C::HALVES; ++h)
-          tma_load_3d(qs + h * C::Q_HALF, &qmap, q_full, h * 64, u.kvh * p.group, u.q_begin + u.t0);
+        const int tiles = NT == 1 || u.n_tok <= p.tile_tokens ? 1 : NT;
+        bar_arrive_expect_tx(q_full, (uint32_t)(tiles * p.group * p.tile_tokens * HD * 2));
+        for (int h = 0; h < tiles * C::HALVES; ++h)
+          tma_load_3d(qs + h * C::Q_HALF, &qmap, q_full, h % C::HALVES * 64, u.kvh * p.group,
+                      u.q_begin + u.t0 + h / C::HALVES * p.tile_tokens);
       }
       __syncwarp();
       ++qn;
@@ -440,41 +458,42 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
       while (globaltimer_ns() - w0 < 1000000ull) {
       }
     }
-  } else if (warp == WARP_MMA) {
+  } else if (warp == C::WARP_MMA) {
     if (elect_one()) {
       constexpr uint32_t idesc_s = make_idesc_f16(BQ, BKV, kBF16 ? 1 : 0, 0, 0);
       constexpr uint32_t idesc_o = make_idesc_f16(BQ, HD, kBF16 ? 1 : 0, 0, 1);
-      uint32_t sn = 0, gn = 0, un = 0;  // S products, P V products, units so far
-      auto issue_s = [&]() -> bool {
-        const uint32_t s = sn % RING;
-        if (!wait_bar(&k_full[s], (sn / RING) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)) return false;
+      // Blocks and units so far, of the CTA (K and V rings, Q) and of each tile
+      // (its S buffers and O): a unit may have rows in the first tile only.
+      uint32_t nb = 0, un = 0, tb[NT] = {}, tu[NT] = {};
+      int tiles = 1;  // of the unit
+      auto issue_s = [&](int g, int j) -> bool {
+        const uint32_t n = nb + j, s = n % RING, b = (tb[g] + j) & 1;
+        if (g == 0 && !wait_bar(&k_full[s], (n / RING) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)) return false;
         tc_fence_after();
-        const uint32_t qa = smem_u32(qs), ka = smem_u32(ks + s * C::KV_BYTES);
+        const uint32_t qa = smem_u32(qs + g * C::Q_BYTES), ka = smem_u32(ks + s * C::KV_BYTES);
 #pragma unroll
         for (int k16 = 0; k16 < HD / 16; ++k16)
-          mma_ss(tmem + S_COL + (sn & 1) * BKV,
-                 make_smem_desc(qa + (k16 >> 2) * C::Q_HALF + (k16 & 3) * 32, 16, 1024),
+          mma_ss(tmem + g * 128 + b * BKV, make_smem_desc(qa + (k16 >> 2) * C::Q_HALF + (k16 & 3) * 32, 16, 1024),
                  make_smem_desc(ka + (k16 >> 2) * C::KV_HALF + (k16 & 3) * 32, 16, 1024), idesc_s,
                  k16 > 0 ? 1u : 0u);
-        tc_commit(&s_full[sn & 1]);
-        tc_commit(&k_empty[s]);
-        ++sn;
+        tc_commit(&s_full[g * 2 + b]);
+        if (g + 1 == tiles) tc_commit(&k_empty[s]);
         return true;
       };
-      auto issue_pv = [&](bool fresh) -> bool {
-        const uint32_t s = gn % RING;
-        if (!wait_bar(&v_full[s], (gn / RING) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)) return false;
-        if (!wait_bar(&v_fixed[s], (gn / RING) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)) return false;
-        if (!wait_bar(&p_ready[gn & 1], (gn >> 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)) return false;
+      auto issue_pv = [&](int g, int j) -> bool {
+        const uint32_t n = nb + j, s = n % RING, b = (tb[g] + j) & 1;
+        if (g == 0 && !(wait_bar(&v_full[s], (n / RING) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA) &&
+                        wait_bar(&v_fixed[s], (n / RING) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)))
+          return false;
+        if (!wait_bar(&p_ready[g * 2 + b], ((tb[g] + j) >> 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)) return false;
         tc_fence_after();
         const uint32_t va = smem_u32(vs + s * C::KV_BYTES);
 #pragma unroll
         for (int k16 = 0; k16 < BKV / 16; ++k16)
-          mma_ts(tmem + O_COL, tmem + S_COL + (gn & 1) * BKV + k16 * 8,
-                 make_smem_desc(va + k16 * 16 * 128, C::KV_HALF, 1024), idesc_o, (!fresh || k16 > 0) ? 1u : 0u);
-        tc_commit(&pv_done[gn & 1]);
-        tc_commit(&v_empty[s]);
-        ++gn;
+          mma_ts(tmem + C::O_COL + g * 128, tmem + g * 128 + b * BKV + k16 * 8,
+                 make_smem_desc(va + k16 * 16 * 128, C::KV_HALF, 1024), idesc_o, (j > 0 || k16 > 0) ? 1u : 0u);
+        tc_commit(&pv_done[g * 2 + b]);
+        if (g + 1 == tiles) tc_commit(&v_empty[s]);
         return true;
       };
       Unit u;
@@ -483,19 +502,33 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
         if (!next_unit(i, u)) break;
         bar_arrive(&unit_empty[i & 1]);
         if (u.nkv == 0) continue;
-        ok = wait_bar(q_full, un & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA) && issue_s();
-        if (ok && u.nkv > 1) ok = issue_s();
+        tiles = NT == 1 || u.n_tok <= p.tile_tokens ? 1 : NT;
+        ok = wait_bar(q_full, un & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA);
+        for (int j = 0; j < min(u.nkv, 2); ++j) {
+#pragma unroll
+          for (int g = 0; g < NT; ++g)
+            if (g < tiles && ok) ok = issue_s(g, j);
+        }
         if (ok && u.nkv <= 2) tc_commit(q_empty);
         for (int j = 0; j < u.nkv && ok; ++j) {
-          // the rows of the unit before have been read out of O
-          if (j == 0) ok = wait_bar(o_empty, (un & 1) ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA);
-          if (ok) ok = issue_pv(j == 0);
-          if (ok && j + 2 < u.nkv) {
-            ok = issue_s();
-            if (ok && j + 3 == u.nkv) tc_commit(q_empty);
+#pragma unroll
+          for (int g = 0; g < NT; ++g) {
+            if (g >= tiles || !ok) continue;
+            // the rows of the unit before have been read out of O
+            if (j == 0) ok = wait_bar(&o_empty[g], (tu[g] & 1) ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA);
+            if (ok) ok = issue_pv(g, j);
+            if (ok && j + 2 < u.nkv) ok = issue_s(g, j + 2);
           }
+          if (ok && j + 3 == u.nkv) tc_commit(q_empty);
         }
+        nb += (uint32_t)u.nkv;
         ++un;
+#pragma unroll
+        for (int g = 0; g < NT; ++g)
+          if (g < tiles) {
+            tb[g] += (uint32_t)u.nkv;
+            ++tu[g];
+          }
       }
       tc_commit(drain);
       const uint32_t da = smem_u32(drain);
@@ -507,7 +540,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
         }
       }
     }
-  } else if (warp == WARP_FIX) {
+  } else if (warp == C::WARP_FIX) {
     uint32_t vn = 0;
     Unit u;
     bool ok = true;
@@ -523,33 +556,29 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
         if (!ok) break;
         if (j >= u.jb) {
           const int key0 = (u.j0 + j) * BKV;
-          for (int r = lane; r < BKV; r += 32) {
-            if (key0 + r < u.lim_min) continue;  // seen by every row
-            // row r of both halves (the swizzle permutes 16-byte pieces
-            // within a 128-byte row only)
-            uint8_t* at = vs + s * C::KV_BYTES + r * 128;
-            const bool past = key0 + r >= u.kv_len;
+          // Rows from r0 on (the swizzle permutes 16-byte pieces within a
+          // 128-byte row only): to r1 they are checked, past it zeroed.
+          const int r0 = max(0, u.lim_min - key0), r1 = max(r0, min(BKV, u.kv_len - key0));
+          uint8_t* at = vs + s * C::KV_BYTES;
+          uint32_t bad = 0;
+          for (int h = 0; h < C::HALVES; ++h) {
+#pragma unroll 4
+            for (int e = r0 * 8 + lane; e < r1 * 8; e += 32)
+              bad |= nonfinite_bits<kBF16>(*reinterpret_cast<const uint4*>(at + h * C::KV_HALF + e * 16));
+            for (int e = r1 * 8 + lane; e < BKV * 8; e += 32)
+              *reinterpret_cast<uint4*>(at + h * C::KV_HALF + e * 16) = make_uint4(0, 0, 0, 0);
+          }
+          if (__any_sync(0xffffffffu, bad != 0)) {
             for (int h = 0; h < C::HALVES; ++h)
-#pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                uint4* q4 = reinterpret_cast<uint4*>(at + h * C::KV_HALF + ((k ^ r) & 7) * 16);
-                if (past) {
-                  *q4 = make_uint4(0, 0, 0, 0);
-                  continue;
-                }
+              for (int e = r0 * 8 + lane; e < r1 * 8; e += 32) {
+                uint4* q4 = reinterpret_cast<uint4*>(at + h * C::KV_HALF + e * 16);
                 uint32_t w[4] = {q4->x, q4->y, q4->z, q4->w};
-                bool bad = false;
 #pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                  const bool lo = finite16<kBF16>(w[m]), hi = finite16<kBF16>(w[m] >> 16);
-                  bad |= !lo || !hi;
-                  w[m] &= (lo ? 0x0000ffffu : 0u) | (hi ? 0xffff0000u : 0u);
-                }
-                if (bad) {
-                  *q4 = make_uint4(w[0], w[1], w[2], w[3]);
-                  nonfinite[i & 1] = 1;
-                }
+                for (int m = 0; m < 4; ++m)
+                  w[m] &= (finite16<kBF16>(w[m]) ? 0x0000ffffu : 0u) | (finite16<kBF16>(w[m] >> 16) ? 0xffff0000u : 0u);
+                *q4 = make_uint4(w[0], w[1], w[2], w[3]);
               }
+            if (lane == 0) nonfinite[i & 1] = 1;
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -558,25 +587,29 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
       }
     }
   } else {
-    const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
-    const uint32_t o_addr = tmem + lane_base + O_COL;
-    const int row = warp * 32 + lane;
-    const int tok = row / p.group;
+    const int g = warp >> 2;  // tile
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t o_addr = tmem + lane_base + C::O_COL + g * 128;
+    const int row = (warp & 3) * 32 + lane;              // of the tile
+    const int tok = g * p.tile_tokens + row / p.group;   // of the unit
     const unsigned long long sc2 = pack2(p.scale_log2, p.scale_log2);
-    uint32_t gn = 0;  // blocks so far
+    uint32_t gn = 0;  // blocks of this tile so far
     Unit u;
     bool ok = true;
     for (int i = 0; ok; ++i) {
       if (!__all_sync(0xffffffffu, next_unit(i, u))) break;
       const bool valid = tok < u.n_tok && row < p.tile_tokens * p.group;
       const bool any = __any_sync(0xffffffffu, valid);
-      const int head = u.kvh * p.group + row - tok * p.group;
+      const bool idle = g > 0 && u.n_tok <= p.tile_tokens;  // this unit has no tile g
+      const int head = u.kvh * p.group + row % p.group;
+      // The unit's rows in order: a tile has tile_tokens * group of them.
+      const int urow = g * p.tile_tokens * p.group + row;
       const size_t q_row = (size_t)(u.q_begin + u.t0 + tok);
       uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + q_row * p.out_token + (size_t)head * p.out_head;
       const size_t part = ((size_t)split * p.total_q + q_row) * p.n_heads + head;
       if (u.nkv == 0) {  // no key: zeros (or a part of weight zero)
         if (p.in_cluster) {
-          stats[row] = make_float2(-INFINITY, 0.f);
+          if (valid) stats[urow] = make_float2(-INFINITY, 0.f);
         } else if (valid && p.splits > 1) {
           p.part_lse[part] = -INFINITY;
         } else if (valid) {
@@ -586,16 +619,20 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
         if (lane == 0) bar_arrive(&unit_empty[i & 1]);
         continue;
       }
+      if (idle) {
+        if (lane == 0) bar_arrive(&unit_empty[i & 1]);
+        continue;
+      }
       const int lim = valid ? keys_seen(u, p.causal, tok) : 0;
       float m = -INFINITY, l = 0.0f;
       for (int j = 0; j < u.nkv; ++j, ++gn) {
         const uint32_t buf = gn & 1;
-        const uint32_t s_addr = tmem + lane_base + S_COL + buf * BKV;
-        bool good = wait_bar(&s_full[buf], (gn >> 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_SOFTMAX);
+        const uint32_t s_addr = tmem + lane_base + g * 128 + buf * BKV;
+        bool good = wait_bar(&s_full[g * 2 + buf], (gn >> 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_SOFTMAX);
         ok = __all_sync(0xffffffffu, good);
         if (!ok) break;
         if (!any) {  // no row here: P of these rows is never read out
-          if (lane == 0) bar_arrive(&p_ready[buf]);
+          if (lane == 0) bar_arrive(&p_ready[g * 2 + buf]);
           continue;
         }
         tc_fence_after();
@@ -633,7 +670,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
           m = mx;
         }
         if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-          good = wait_bar(&pv_done[buf ^ 1], ((gn - 1) >> 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_SOFTMAX);
+          good = wait_bar(&pv_done[g * 2 + (buf ^ 1)], ((gn - 1) >> 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_SOFTMAX);
           ok = __all_sync(0xffffffffu, good);
           if (!ok) break;
           tc_fence_after();
@@ -670,27 +707,28 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) bar_arrive(&p_ready[buf]);
+        if (lane == 0) bar_arrive(&p_ready[g * 2 + buf]);
       }
       if (!ok) break;
-      const bool good = !any || wait_bar(&pv_done[(gn - 1) & 1], ((gn - 1) >> 1) & 1, abort_flag, p.err,
+      const bool good = !any || wait_bar(&pv_done[g * 2 + ((gn - 1) & 1)], ((gn - 1) >> 1) & 1, abort_flag, p.err,
                                          DEV_ERR_TIMEOUT_SOFTMAX);
       ok = __all_sync(0xffffffffu, good);
       if (!ok) break;
       if (any) {
         tc_fence_after();
         const float inv_l = l == 0.0f ? 0.0f : 1.0f / l;  // no key in this range: zeros
-        const bool repair = nonfinite[i & 1] != 0;
+        const bool repair = nonfinite[i & 1] != 0 && valid;
+        const uint32_t vmask = __ballot_sync(0xffffffffu, valid);
         // keys that only some rows see, within this CTA's range
         const int from = max(u.lim_min, (u.j0 + u.jb) * BKV), to = min(lim, (u.j0 + u.nkv) * BKV);
-        if (p.in_cluster) stats[row] = make_float2(l == 0.0f ? -INFINITY : m + log2f(l), 0.f);
+        if (p.in_cluster && valid) stats[urow] = make_float2(l == 0.0f ? -INFINITY : m + log2f(l), 0.f);
 #pragma unroll 1
         for (int c = 0; c < HD / 32; ++c) {
           uint32_t r[32];
           tmem_ld32(o_addr + c * 32, r);
           tmem_wait_ld();
-          if (!valid) continue;
           float o[32];
+          uint4 h4[4];
 #pragma unroll
           for (int k = 0; k < 32; ++k) o[k] = __uint_as_float(r[k]) * inv_l;
           if (repair) {
@@ -711,18 +749,35 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
           if (p.splits > 1) {
             // global memory, or the rings (every product of the unit is done);
             // there, 16-byte pieces are permuted within a row against conflicts
-            float* po = p.in_cluster ? reinterpret_cast<float*>(ks) + row * HD : p.part_o + part * HD;
-            const int x = p.in_cluster ? row & 7 : 0;
+            float* po = p.in_cluster ? reinterpret_cast<float*>(ks) + urow * HD : p.part_o + part * HD;
+            const int x = p.in_cluster ? urow & 7 : 0;
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
+            for (int k = 0; k < 8 && valid; ++k)
               *reinterpret_cast<float4*>(po + ((c * 8 + k) ^ x) * 4) =
                   make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
           } else {
-            uint4* d4 = reinterpret_cast<uint4*>(dst + c * 32);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              d4[k] = make_uint4(cvt2<kBF16>(o[8 * k], o[8 * k + 1]), cvt2<kBF16>(o[8 * k + 2], o[8 * k + 3]),
+              h4[k] = make_uint4(cvt2<kBF16>(o[8 * k], o[8 * k + 1]), cvt2<kBF16>(o[8 * k + 2], o[8 * k + 3]),
                                  cvt2<kBF16>(o[8 * k + 4], o[8 * k + 5]), cvt2<kBF16>(o[8 * k + 6], o[8 * k + 7]));
+          }
+          if (p.splits == 1) {
+            // Through shared memory, so that four lanes write 64 bytes of one
+            // row together (a lane writing its own row touches 32 lines per
+            // instruction); pieces are permuted against bank conflicts.
+            uint4* st = stage + warp * 128;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) st[lane * 4 + (k ^ ((lane >> 1) & 3))] = h4[k];
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int r = k * 8 + (lane >> 2);
+              const uint4 v = st[r * 4 + ((lane & 3) ^ ((r >> 1) & 3))];
+              const unsigned long long to = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r);
+              if ((vmask >> r) & 1u)
+                *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(to) + c * 32 + (lane & 3) * 8) = v;
+            }
+            __syncwarp();
           }
         }
         if (valid && p.splits > 1 && !p.in_cluster) p.part_lse[part] = l == 0.0f ? -INFINITY : m + log2f(l);
@@ -730,7 +785,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
       }
       __syncwarp();
       if (lane == 0) {
-        bar_arrive(o_empty);
+        bar_arrive(&o_empty[g]);
         bar_arrive(&unit_empty[i & 1]);
       }
     }
@@ -747,7 +802,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
       const int d8 = (int)(threadIdx.x % (HD / 8)) * 2;  // 16-byte pieces d8, d8 + 1
       const uint32_t st0 = smem_u32(stats), o0 = smem_u32(ks);
       for (int r = split + p.splits * (int)(threadIdx.x / (HD / 8)); r < rows;
-           r += p.splits * (NUM_THREADS / (HD / 8))) {
+           r += p.splits * (C::NUM_THREADS / (HD / 8))) {
         float lse[kMaxCluster];
         float top = -INFINITY;
 #pragma unroll
@@ -786,10 +841,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
     }
     cluster_sync_all();  // no CTA ends while another reads its shared memory
   }
-  if (warp == WARP_MMA) {
+  if (warp == C::WARP_MMA) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tmem, TMEM_COLS);
+    tmem_dealloc(tmem, C::TMEM_COLS);
   }
 }
 
@@ -899,7 +954,7 @@ int encode(CUtensorMap* map, void* base, bool bf16, int rank, const long long* d
 // one GPC); 0 if the query fails.  The occupancy query counts one CTA per SM
 // for a kernel that allocates TMEM; two of these fit (256 of the 512 columns,
 // half the shared memory and registers each) and do run.
-template <int HD, bool kBF16, bool kPaged>
+template <int HD, bool kBF16, bool kPaged, int NT>
 int cluster_slots(int size) {
   static int slots[64][kMaxCluster + 1];
   static bool known[64][kMaxCluster + 1];
@@ -908,8 +963,8 @@ int cluster_slots(int size) {
   const int d = device_slot();
   if (known[d][size]) return slots[d][size];
   known[d][size] = true;
-  auto kern = text_attention_kernel<HD, kBF16, kPaged>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD>::SMEM_BYTES) == cudaSuccess &&
+  auto kern = text_attention_kernel<HD, kBF16, kPaged, NT>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD, NT>::SMEM_BYTES) == cudaSuccess &&
       cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) ==
           cudaSuccess &&
       cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) {
@@ -920,23 +975,23 @@ int cluster_slots(int size) {
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3((unsigned)size);
-    cfg.blockDim = dim3(NUM_THREADS);
-    cfg.dynamicSmemBytes = Cfg<HD>::SMEM_BYTES;
+    cfg.blockDim = dim3(Cfg<HD, NT>::NUM_THREADS);
+    cfg.dynamicSmemBytes = Cfg<HD, NT>::SMEM_BYTES;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int c = 0;
-    if (cudaOccupancyMaxActiveClusters(&c, kern, &cfg) == cudaSuccess) slots[d][size] = 2 * c;
+    if (cudaOccupancyMaxActiveClusters(&c, kern, &cfg) == cudaSuccess) slots[d][size] = (3 - NT) * c;
   }
   cudaGetLastError();
   return slots[d][size];
 }
 
-template <int HD, bool kBF16, bool kPaged>
+template <int HD, bool kBF16, bool kPaged, int NT>
 int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, Params p, long long units,
            int max_ctx, cudaStream_t st) {
-  auto kern = text_attention_kernel<HD, kBF16, kPaged>;
+  auto kern = text_attention_kernel<HD, kBF16, kPaged, NT>;
   // CTA slots; the query also prepares the kernel for its shared memory
-  const long long slots = cluster_slots<HD, kBF16, kPaged>(1);
+  const long long slots = cluster_slots<HD, kBF16, kPaged, NT>(1);
   if (slots < 1) return fail(-3, "text attention: the kernel cannot be scheduled on this device");
   // Key split: where the units leave CTA slots empty, each unit's keys are cut
   // into ranges of at least 4 blocks.  Up to kMaxCluster ranges are one
@@ -945,8 +1000,11 @@ int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, 
   long long want = kPaged ? std::max(1ll, std::min(slots / units, blocks / 4)) : 1;
   p.splits = (int)std::min(want, 64ll);
   if (p.splits > 1 && p.splits <= kMaxCluster) {
-    while (p.splits > 1 && cluster_slots<HD, kBF16, kPaged>(p.splits) < units) --p.splits;
-    p.in_cluster = p.splits > 1;
+    while (p.splits > 1 && cluster_slots<HD, kBF16, kPaged, NT>(p.splits) < units) --p.splits;
+    // Clusters pack badly where the wanted split is odd (32 units in 9 ranges:
+    // 6 fit, 196 us; 9 ranges through global memory, 168 us).
+    p.in_cluster = 5 * p.splits >= 4 * want && p.splits > 1;
+    if (!p.in_cluster) p.splits = (int)want;
   }
   void* part = nullptr;
   if (p.splits > 1 && !p.in_cluster) {
@@ -957,8 +1015,8 @@ int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, 
     p.part_lse = p.part_o + items * HD;
   }
   const long long ctas = p.splits > 1 ? units * p.splits : std::min(units, slots);
-  int rc = launch_after("text_attention_kernel launch", kern, dim3((unsigned)ctas), dim3(NUM_THREADS),
-                        Cfg<HD>::SMEM_BYTES, p.in_cluster ? p.splits : 1, st, qm, km, vm, p);
+  int rc = launch_after("text_attention_kernel launch", kern, dim3((unsigned)ctas), dim3(Cfg<HD, NT>::NUM_THREADS),
+                        Cfg<HD, NT>::SMEM_BYTES, p.in_cluster ? p.splits : 1, st, qm, km, vm, p);
   if (rc == 0 && part) {
     const long long threads = (long long)p.total_q * p.n_heads * (HD / 8);
     rc = launch_after("text_combine_kernel launch", text_combine_kernel<HD, kBF16>,
@@ -969,14 +1027,30 @@ int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, 
   return rc;
 }
 
+template <int HD, bool kBF16, bool kPaged>
+int launch_form(const TextAttention& a, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm,
+                const Params& p, cudaStream_t st) {
+  // Tiles: sum_i ceil(q_len_i / T) <= (total + n * (T - 1)) / T; CTAs past the
+  // real number of tiles end at once.
+  const long long seqs = std::min(p.n_seqs, a.total_q);
+  auto units = [&](long long T) { return (a.total_q + seqs * (T - 1)) / T * a.n_kv; };
+  const long long u1 = units(p.tile_tokens), u2 = units(2 * p.tile_tokens);
+  if (u1 > 0x7fffffffll / 64) return fail(-2, "text attention: too many tiles in one call");
+  // Two tiles per CTA where they are enough to fill the GPU and the sequences
+  // fill them: more than one tile of rows each on average.
+  if (u2 >= num_sms() && a.total_q > seqs * p.tile_tokens)
+    return launch<HD, kBF16, kPaged, 2>(qm, km, vm, p, u2, a.max_ctx, st);
+  return launch<HD, kBF16, kPaged, 1>(qm, km, vm, p, u1, a.max_ctx, st);
+}
+
 template <bool kPaged>
 int dispatch(const TextAttention& a, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm,
-             const Params& p, long long units, cudaStream_t st) {
+             const Params& p, cudaStream_t st) {
   if (a.head_dim == 128)
-    return a.bf16 ? launch<128, true, kPaged>(qm, km, vm, p, units, a.max_ctx, st)
-                  : launch<128, false, kPaged>(qm, km, vm, p, units, a.max_ctx, st);
-  return a.bf16 ? launch<64, true, kPaged>(qm, km, vm, p, units, a.max_ctx, st)
-                : launch<64, false, kPaged>(qm, km, vm, p, units, a.max_ctx, st);
+    return a.bf16 ? launch_form<128, true, kPaged>(a, qm, km, vm, p, st)
+                  : launch_form<128, false, kPaged>(a, qm, km, vm, p, st);
+  return a.bf16 ? launch_form<64, true, kPaged>(a, qm, km, vm, p, st)
+                : launch_form<64, false, kPaged>(a, qm, km, vm, p, st);
 }
 
 }  // namespace text
@@ -1037,12 +1111,7 @@ int launch_text_attention(const TextAttention& a, cudaStream_t st) {
     p.cu = a.cu + s0;
     p.ctx = paged ? a.ctx + s0 : nullptr;
     p.table = paged ? a.table + s0 * a.table_ld : nullptr;
-    // Tiles: sum_i ceil(q_len_i / T) <= (total + n * (T - 1)) / T; CTAs past
-    // the real number of tiles end at once.
-    const long long T = p.tile_tokens, seqs = std::min(p.n_seqs, a.total_q);
-    const long long units = (a.total_q + seqs * (T - 1)) / T * a.n_kv;
-    if (units > 0x7fffffffll / 64) return fail(-2, "text attention: too many tiles in one call");
-    const int rc = paged ? dispatch<true>(a, qm, km, vm, p, units, st) : dispatch<false>(a, qm, km, vm, p, units, st);
+    const int rc = paged ? dispatch<true>(a, qm, km, vm, p, st) : dispatch<false>(a, qm, km, vm, p, st);
     if (rc) return rc;
   }
   return 0;
