@@ -23,7 +23,7 @@
 //   warp 4      TMA: Q, then K and V blocks of 64 keys (128-byte swizzle,
 //               64-dim halves); paged: one box per page and half, issued by
 //               one lane each, page indices read 32 at a time.
-//   warp 5      one thread issues tcgen05.mma: S(j) = Q K_j^T (SMEM, SMEM),
+//   warp 5      issues tcgen05.mma: S(j) = Q K_j^T (SMEM, SMEM),
 //               O += P(j) V_j (P from TMEM, V MN-major); S runs two blocks
 //               ahead (double-buffered).
 //   warp 6      blocks that not every row sees whole (a causal diagonal, the
@@ -32,7 +32,7 @@
 //               product, since 0 * NaN would reach every row; V values of
 //               keys that only some rows see are zeroed where they are not
 //               finite, and the rows that do see them add them at the end.
-//   warp 7      finds the units.
+//               It also finds the units, two ahead.
 // Where the units leave CTA slots empty (a few single tokens), each unit's keys
 // are split between the CTAs of a cluster, which merge their parts through
 // distributed shared memory; a split wider than a cluster goes through global
@@ -66,8 +66,9 @@ template <int HD, int NT>
 struct Cfg {
   static constexpr int RING = NT == 1 ? 2 : 4;  // K and V slots
   static constexpr int SOFTMAX_WARPS = 4 * NT;
-  static constexpr int WARP_TMA = 4 * NT, WARP_MMA = WARP_TMA + 1, WARP_FIX = WARP_TMA + 2, WARP_PLAN = WARP_TMA + 3;
-  static constexpr int NUM_THREADS = (WARP_PLAN + 1) * 32;
+  static constexpr int WARP_MMA = 4 * NT;  // one per tile
+  static constexpr int WARP_TMA = WARP_MMA + NT, WARP_FIX = WARP_TMA + 1;
+  static constexpr int NUM_THREADS = (WARP_FIX + 1) * 32;
   // TMEM: S of tile g, buffer b at g * 128 + b * 64; O of tile g after all S
   static constexpr int TMEM_COLS = 256 * NT, O_COL = 128 * NT;
   static constexpr int HALVES = HD / 64;
@@ -260,6 +261,12 @@ struct Finder {
   }
 };
 
+// wait_bar for a phase that has usually completed already.
+__device__ __forceinline__ bool wait_fast(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err,
+                                          int code) {
+  return bar_test_wait(smem_u32(bar), parity) || wait_bar(bar, parity, abort_flag, err, code);
+}
+
 template <int HD, bool kBF16, bool kPaged, int NT>
 __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
     text_attention_kernel(const __grid_constant__ CUtensorMap qmap,
@@ -304,7 +311,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       bar_init(&unit_full[i], 1);
-      bar_init(&unit_empty[i], C::SOFTMAX_WARPS + 3);  // softmax warps, TMA, MMA, fix
+      bar_init(&unit_empty[i], C::SOFTMAX_WARPS + NT + 1);  // softmax and MMA warps, TMA
       nonfinite[i] = 0;
     }
     for (int i = 0; i < 2 * NT; ++i) {
@@ -313,16 +320,16 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
       bar_init(&pv_done[i], 1);
     }
     bar_init(q_full, 1);
-    bar_init(q_empty, 1);
+    bar_init(q_empty, NT);
     for (int s = 0; s < RING; ++s) {
       bar_init(&k_full[s], 1);
-      bar_init(&k_empty[s], 1);
+      bar_init(&k_empty[s], NT);
       bar_init(&v_full[s], 1);
-      bar_init(&v_empty[s], 1);
+      bar_init(&v_empty[s], NT);
       bar_init(&v_fixed[s], 1);
     }
     for (int g = 0; g < NT; ++g) bar_init(&o_empty[g], 4);
-    bar_init(drain, 1);
+    bar_init(drain, NT);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&qmap);
@@ -355,43 +362,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
     return u.nkv >= 0;
   };
 
-  if (warp == C::WARP_PLAN) {
-    Finder f{lens, p.n_seqs, NT * p.tile_tokens, p.causal, kPaged ? (long long)p.table_width << p.page_shift : 0x7fffffffll};
-    f.init();
-    for (int i = 0;; ++i) {
-      // units come longest first: rounds go up and down the CTAs in turn, so
-      // that who had the longest of one round has the shortest of the next
-      const int unit = i * ustep + (i & 1 ? ustep - 1 - unit0 : unit0);
-      Unit u{};
-      u.nkv = -1;
-      int seq, level;
-      // with splits, one unit per CTA (per cluster)
-      if ((p.splits == 1 || i == 0) && f.find(unit / p.n_kv, seq, level)) {
-        const int2 s = lens[seq];
-        u.seq = seq;
-        u.kvh = unit % p.n_kv;
-        u.q_begin = max(0, min(p.cu[seq], p.total_q));
-        u.kv_len = f.kv_len(s);
-        u.t0 = level * NT * p.tile_tokens;
-        u.n_tok = min(NT * p.tile_tokens, s.x - u.t0);
-        u.first = s.y + u.t0;
-        u.lim_min = keys_seen(u, p.causal, 0);
-        const int blocks = (keys_seen(u, p.causal, u.n_tok - 1) + BKV - 1) / BKV;
-        const int chunk = (blocks + p.splits - 1) / p.splits;
-        u.j0 = split * chunk;
-        u.nkv = max(0, min(blocks - u.j0, chunk));
-        u.jb = max(0, u.lim_min / BKV - u.j0);
-      }
-      const bool good = wait_bar(&unit_empty[i & 1], ((i >> 1) & 1) ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER);
-      if (!__all_sync(0xffffffffu, good)) break;
-      if (lane == 0) {
-        units[i & 1] = u;
-        nonfinite[i & 1] = 0;  // the softmax warps are done with unit i - 2
-        bar_arrive(&unit_full[i & 1]);
-      }
-      if (u.nkv < 0) break;
-    }
-  } else if (warp == C::WARP_TMA) {
+  if (warp == C::WARP_TMA) {
     // Paged: a block of 64 keys takes 64 / page boxes (one where a page holds
     // more), and each half of the head dims its own; lane l issues box
     // l / HALVES, half l % HALVES.  `ent` = 32 consecutive page indices.
@@ -458,95 +429,143 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
       while (globaltimer_ns() - w0 < 1000000ull) {
       }
     }
-  } else if (warp == C::WARP_MMA) {
-    if (elect_one()) {
-      constexpr uint32_t idesc_s = make_idesc_f16(BQ, BKV, kBF16 ? 1 : 0, 0, 0);
-      constexpr uint32_t idesc_o = make_idesc_f16(BQ, HD, kBF16 ? 1 : 0, 0, 1);
-      // Blocks and units so far, of the CTA (K and V rings, Q) and of each tile
-      // (its S buffers and O): a unit may have rows in the first tile only.
-      uint32_t nb = 0, un = 0, tb[NT] = {}, tu[NT] = {};
-      int tiles = 1;  // of the unit
-      auto issue_s = [&](int g, int j) -> bool {
-        const uint32_t n = nb + j, s = n % RING, b = (tb[g] + j) & 1;
-        if (g == 0 && !wait_bar(&k_full[s], (n / RING) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)) return false;
-        tc_fence_after();
-        const uint32_t qa = smem_u32(qs + g * C::Q_BYTES), ka = smem_u32(ks + s * C::KV_BYTES);
+  } else if (warp >= C::WARP_MMA && warp < C::WARP_MMA + NT) {
+    // One warp per tile: waits and commits of one tile's products hide behind
+    // the other's (a single warp takes 2100 clocks for the two tiles' products
+    // of a block, which run in 1300).  The whole warp runs this role, one
+    // thread of it issues: see mma_ss_if.
+    constexpr uint32_t idesc_s = make_idesc_f16(BQ, BKV, kBF16 ? 1 : 0, 0, 0);
+    constexpr uint32_t idesc_o = make_idesc_f16(BQ, HD, kBF16 ? 1 : 0, 0, 1);
+    const int g = __shfl_sync(0xffffffffu, warp - C::WARP_MMA, 0);
+    const uint32_t leader = elect_one() ? 1u : 0u;
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0) + g * 128;
+    const uint64_t q_desc = make_smem_desc(smem_u32(qs) + g * C::Q_BYTES, 16, 1024);
+    const uint64_t k_desc = make_smem_desc(smem_u32(ks), 16, 1024);
+    const uint64_t v_desc = make_smem_desc(smem_u32(vs), C::KV_HALF, 1024);
+    // Blocks and units so far, of the CTA (K and V rings, Q) and of this tile
+    // (its S buffers and O): a unit may have rows in the first tile only.
+    uint32_t nb = 0, un = 0, tb = 0, tu = 0;
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool {
+      return __all_sync(0xffffffffu, wait_fast(bar, parity, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA));
+    };
+    auto issue_s = [&](int j) -> bool {
+      const uint32_t n = nb + j, s = n % RING, b = (tb + j) & 1;
+      if (!wait_all(&k_full[s], (n / RING) & 1)) return false;
+      tc_fence_after();
 #pragma unroll
-        for (int k16 = 0; k16 < HD / 16; ++k16)
-          mma_ss(tmem + g * 128 + b * BKV, make_smem_desc(qa + (k16 >> 2) * C::Q_HALF + (k16 & 3) * 32, 16, 1024),
-                 make_smem_desc(ka + (k16 >> 2) * C::KV_HALF + (k16 & 3) * 32, 16, 1024), idesc_s,
-                 k16 > 0 ? 1u : 0u);
-        tc_commit(&s_full[g * 2 + b]);
-        if (g + 1 == tiles) tc_commit(&k_empty[s]);
-        return true;
-      };
-      auto issue_pv = [&](int g, int j) -> bool {
-        const uint32_t n = nb + j, s = n % RING, b = (tb[g] + j) & 1;
-        if (g == 0 && !(wait_bar(&v_full[s], (n / RING) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA) &&
-                        wait_bar(&v_fixed[s], (n / RING) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)))
-          return false;
-        if (!wait_bar(&p_ready[g * 2 + b], ((tb[g] + j) >> 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)) return false;
-        tc_fence_after();
-        const uint32_t va = smem_u32(vs + s * C::KV_BYTES);
+      for (int k16 = 0; k16 < HD / 16; ++k16)  // descriptors count 16 bytes
+        mma_ss_if(leader, tm + b * BKV,
+                  q_desc + (uint64_t)(((k16 >> 2) * C::Q_HALF + (k16 & 3) * 32) >> 4),
+                  k_desc + (uint64_t)(s * (C::KV_BYTES >> 4) + (((k16 >> 2) * C::KV_HALF + (k16 & 3) * 32) >> 4)),
+                  idesc_s, k16 > 0 ? 1u : 0u);
+      tc_commit_if(leader, &s_full[g * 2 + b]);
+      tc_commit_if(leader, &k_empty[s]);
+      return true;
+    };
+    auto issue_pv = [&](int j) -> bool {
+      const uint32_t n = nb + j, s = n % RING, b = (tb + j) & 1;
+      // v_fixed: the fix warp has seen the block's copy complete
+      if (!wait_all(&v_fixed[s], (n / RING) & 1) || !wait_all(&p_ready[g * 2 + b], ((tb + j) >> 1) & 1)) return false;
+      tc_fence_after();
 #pragma unroll
-        for (int k16 = 0; k16 < BKV / 16; ++k16)
-          mma_ts(tmem + C::O_COL + g * 128, tmem + g * 128 + b * BKV + k16 * 8,
-                 make_smem_desc(va + k16 * 16 * 128, C::KV_HALF, 1024), idesc_o, (j > 0 || k16 > 0) ? 1u : 0u);
-        tc_commit(&pv_done[g * 2 + b]);
-        if (g + 1 == tiles) tc_commit(&v_empty[s]);
-        return true;
-      };
-      Unit u;
-      bool ok = true;
-      for (int i = 0; ok; ++i) {
-        if (!next_unit(i, u)) break;
-        bar_arrive(&unit_empty[i & 1]);
-        if (u.nkv == 0) continue;
-        tiles = NT == 1 || u.n_tok <= p.tile_tokens ? 1 : NT;
-        ok = wait_bar(q_full, un & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA);
-        for (int j = 0; j < min(u.nkv, 2); ++j) {
-#pragma unroll
-          for (int g = 0; g < NT; ++g)
-            if (g < tiles && ok) ok = issue_s(g, j);
-        }
-        if (ok && u.nkv <= 2) tc_commit(q_empty);
-        for (int j = 0; j < u.nkv && ok; ++j) {
-#pragma unroll
-          for (int g = 0; g < NT; ++g) {
-            if (g >= tiles || !ok) continue;
-            // the rows of the unit before have been read out of O
-            if (j == 0) ok = wait_bar(&o_empty[g], (tu[g] & 1) ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA);
-            if (ok) ok = issue_pv(g, j);
-            if (ok && j + 2 < u.nkv) ok = issue_s(g, j + 2);
-          }
-          if (ok && j + 3 == u.nkv) tc_commit(q_empty);
-        }
-        nb += (uint32_t)u.nkv;
-        ++un;
-#pragma unroll
-        for (int g = 0; g < NT; ++g)
-          if (g < tiles) {
-            tb[g] += (uint32_t)u.nkv;
-            ++tu[g];
-          }
-      }
-      tc_commit(drain);
-      const uint32_t da = smem_u32(drain);
-      const unsigned long long w0 = globaltimer_ns();
-      while (!bar_try_wait(da, 0)) {
-        if (globaltimer_ns() - w0 > kWaitLimitNs) {
-          if (p.err) atomicCAS(p.err, 0, DEV_ERR_TIMEOUT_MMA);
-          break;
-        }
-      }
-    }
-  } else if (warp == C::WARP_FIX) {
-    uint32_t vn = 0;
+      for (int k16 = 0; k16 < BKV / 16; ++k16)
+        mma_ts_if(leader, tm + C::O_COL, tm + b * BKV + k16 * 8,
+                  v_desc + (uint64_t)(s * (C::KV_BYTES >> 4) + k16 * (16 * 128 >> 4)), idesc_o,
+                  (j > 0 || k16 > 0) ? 1u : 0u);
+      tc_commit_if(leader, &pv_done[g * 2 + b]);
+      tc_commit_if(leader, &v_empty[s]);
+      return true;
+    };
     Unit u;
     bool ok = true;
     for (int i = 0; ok; ++i) {
       if (!__all_sync(0xffffffffu, next_unit(i, u))) break;
-      if (lane == 0) bar_arrive(&unit_empty[i & 1]);
+      if (leader) bar_arrive(&unit_empty[i & 1]);
+      const int nkv = __shfl_sync(0xffffffffu, u.nkv, 0);
+      if (nkv == 0) continue;
+      if (g > 0 && __shfl_sync(0xffffffffu, u.n_tok, 0) <= p.tile_tokens) {
+        // no rows in this tile: only the other one uses Q, K and V
+        for (int j = 0; j < nkv && ok; ++j) {
+          const uint32_t s = (nb + j) % RING, ph = ((nb + j) / RING) & 1;
+          ok = wait_all(&k_full[s], ph);
+          if (ok && leader) bar_arrive(&k_empty[s]);
+          if (ok) ok = wait_all(&v_fixed[s], ph);
+          if (ok && leader) bar_arrive(&v_empty[s]);
+        }
+        if (ok) ok = wait_all(q_full, un & 1);
+        if (ok && leader) bar_arrive(q_empty);
+      } else {
+        ok = wait_all(q_full, un & 1);
+        for (int j = 0; j < min(nkv, 2) && ok; ++j) ok = issue_s(j);
+        if (ok && nkv <= 2) tc_commit_if(leader, q_empty);
+        // the rows of the unit before have been read out of O
+        if (ok) ok = wait_all(&o_empty[g], (tu & 1) ^ 1);
+        for (int j = 0; j < nkv && ok; ++j) {
+          ok = issue_pv(j);
+          if (ok && j + 2 < nkv) ok = issue_s(j + 2);
+          if (ok && j + 3 == nkv) tc_commit_if(leader, q_empty);
+        }
+        tb += (uint32_t)nkv;
+        ++tu;
+      }
+      nb += (uint32_t)nkv;
+      ++un;
+    }
+    tc_commit_if(leader, drain);
+    const uint32_t da = smem_u32(drain);
+    const unsigned long long w0 = globaltimer_ns();
+    while (!bar_try_wait(da, 0)) {
+      if (globaltimer_ns() - w0 > kWaitLimitNs) {
+        if (p.err) atomicCAS(p.err, 0, DEV_ERR_TIMEOUT_MMA);
+        break;
+      }
+    }
+    __syncwarp();
+  } else if (warp == C::WARP_FIX) {
+    // The units: two are out at a time, the next one is found and put in the
+    // place of one that every role has left.
+    Finder f{lens, p.n_seqs, NT * p.tile_tokens, p.causal, kPaged ? (long long)p.table_width << p.page_shift : 0x7fffffffll};
+    f.init();
+    auto publish = [&](int i, Unit& u) -> bool {
+      // units come longest first: rounds go up and down the CTAs in turn, so
+      // that who had the longest of one round has the shortest of the next
+      const int unit = i * ustep + (i & 1 ? ustep - 1 - unit0 : unit0);
+      u = Unit{};
+      u.nkv = -1;
+      int seq, level;
+      // with splits, one unit per CTA (per cluster)
+      if ((p.splits == 1 || i == 0) && f.find(unit / p.n_kv, seq, level)) {
+        const int2 s = lens[seq];
+        u.seq = seq;
+        u.kvh = unit % p.n_kv;
+        u.q_begin = max(0, min(p.cu[seq], p.total_q));
+        u.kv_len = f.kv_len(s);
+        u.t0 = level * NT * p.tile_tokens;
+        u.n_tok = min(NT * p.tile_tokens, s.x - u.t0);
+        u.first = s.y + u.t0;
+        u.lim_min = keys_seen(u, p.causal, 0);
+        const int blocks = (keys_seen(u, p.causal, u.n_tok - 1) + BKV - 1) / BKV;
+        const int chunk = (blocks + p.splits - 1) / p.splits;
+        u.j0 = split * chunk;
+        u.nkv = max(0, min(blocks - u.j0, chunk));
+        u.jb = max(0, u.lim_min / BKV - u.j0);
+      }
+      const bool good = wait_bar(&unit_empty[i & 1], ((i >> 1) & 1) ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER);
+      if (!__all_sync(0xffffffffu, good)) return false;
+      if (lane == 0) {
+        units[i & 1] = u;
+        nonfinite[i & 1] = 0;  // the softmax warps are done with unit i - 2
+        bar_arrive(&unit_full[i & 1]);
+      }
+      __syncwarp();
+      return true;
+    };
+    uint32_t vn = 0;
+    Unit u, after;
+    bool ok = publish(0, u);
+    after.nkv = -1;
+    if (ok && u.nkv >= 0) ok = publish(1, after);
+    for (int i = 0; ok && u.nkv >= 0; ++i) {
       // Every block passes here, so that the warp follows each phase of the
       // ring; those before jb pass untouched.
       for (int j = 0; j < u.nkv; ++j, ++vn) {
@@ -585,6 +604,8 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
         }
         if (lane == 0) bar_arrive(&v_fixed[s]);
       }
+      u = after;
+      if (ok && after.nkv >= 0) ok = publish(i + 2, after);
     }
   } else {
     const int g = warp >> 2;  // tile
@@ -628,7 +649,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
       for (int j = 0; j < u.nkv; ++j, ++gn) {
         const uint32_t buf = gn & 1;
         const uint32_t s_addr = tmem + lane_base + g * 128 + buf * BKV;
-        bool good = wait_bar(&s_full[g * 2 + buf], (gn >> 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_SOFTMAX);
+        bool good = wait_fast(&s_full[g * 2 + buf], (gn >> 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_SOFTMAX);
         ok = __all_sync(0xffffffffu, good);
         if (!ok) break;
         if (!any) {  // no row here: P of these rows is never read out
