@@ -45,6 +45,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 namespace bonsai {
 namespace gemm {
@@ -71,6 +72,8 @@ struct Cfg {
   static constexpr int NUM_THREADS = (WARP_FIX + 1) * 32;
   // TMEM: S of tile g, buffer b at g * 128 + b * 64; O of tile g after all S
   static constexpr int TMEM_COLS = 256 * NT, O_COL = 128 * NT;
+  // Pairs of 16 whose exponentials take the polynomial
+  static constexpr unsigned kPolyPairs = NT == 1 ? 0u : 0x8888u;
   static constexpr int HALVES = HD / 64;
   static constexpr int Q_HALF = BQ * 128;         // 128 rows x 64 dims
   static constexpr int Q_BYTES = HALVES * Q_HALF;
@@ -167,10 +170,42 @@ __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigne
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-__device__ __forceinline__ float max3f(float a, float b, float c) {
+// Maxima that pass NaN on.
+__device__ __forceinline__ float max2n(float a, float b) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
+}
+__device__ __forceinline__ float max3n(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^x for a pair on the FMA and ALU pipes, to take part of the exponentials off
+// the MUFU, which two tiles' keep busy for 1024 clocks a block, nearly as long
+// as their products take.  x = n + f with n = round(x) (the 1.5 * 2^23 shift
+// leaves n in the low mantissa bits) and f in [-0.5, 0.5]; 2^f by a degree-3
+// polynomial (Remez exchange on the relative error, max 7.5e-5: below the
+// rounding of P to 16 bits); n is added to the exponent field.  x is at most
+// the rescaling threshold; below -126 it is cut, which P does not resolve.
+// Neither 2^-inf = 0 (a key that is not seen) nor NaN comes out of it: the
+// caller keeps to ex2 for the one and looks for the other by itself.
+__device__ __forceinline__ void ex2_poly2(unsigned long long x2, float& a, float& b) {
+  constexpr float kShift = 12582912.0f;  // 1.5 * 2^23
+  float x0, x1;
+  unpack2(x2, x0, x1);
+  const unsigned long long xc = pack2(fmaxf(x0, -126.0f), fmaxf(x1, -126.0f));
+  const unsigned long long t = add2(xc, pack2(kShift, kShift));
+  const unsigned long long f = fma2(add2(t, pack2(-kShift, -kShift)), pack2(-1.0f, -1.0f), xc);
+  unsigned long long q = fma2(f, pack2(0.0551716685f, 0.0551716685f), pack2(0.2426111251f, 0.2426111251f));
+  q = fma2(q, f, pack2(0.6932609677f, 0.6932609677f));
+  q = fma2(q, f, pack2(0.9999280572f, 0.9999280572f));
+  float q0, q1, t0, t1;
+  unpack2(q, q0, q1);
+  unpack2(t, t0, t1);
+  a = __uint_as_float(__float_as_uint(q0) + (__float_as_uint(t0) << 23));
+  b = __uint_as_float(__float_as_uint(q1) + (__float_as_uint(t1) << 23));
 }
 
 // What the roles of a CTA need to know of a unit (64 bytes in shared memory).
@@ -448,10 +483,8 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
     auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool {
       return __all_sync(0xffffffffu, wait_fast(bar, parity, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA));
     };
-    auto issue_s = [&](int j) -> bool {
-      const uint32_t n = nb + j, s = n % RING, b = (tb + j) & 1;
-      if (!wait_all(&k_full[s], (n / RING) & 1)) return false;
-      tc_fence_after();
+    auto s_products = [&](int j) {
+      const uint32_t s = (nb + j) % RING, b = (tb + j) & 1;
 #pragma unroll
       for (int k16 = 0; k16 < HD / 16; ++k16)  // descriptors count 16 bytes
         mma_ss_if(leader, tm + b * BKV,
@@ -460,10 +493,13 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
                   idesc_s, k16 > 0 ? 1u : 0u);
       tc_commit_if(leader, &s_full[g * 2 + b]);
       tc_commit_if(leader, &k_empty[s]);
-      return true;
     };
-    auto issue_pv = [&](int j) -> bool {
+    // P V of block j and S of block j + 2 (where there is one).  What P does
+    // not need to wait for is waited for before it, so that both products
+    // follow P at once: softmax(j + 1) runs meanwhile, softmax(j + 2) next.
+    auto step = [&](int j, bool more) -> bool {
       const uint32_t n = nb + j, s = n % RING, b = (tb + j) & 1;
+      if (more && !wait_all(&k_full[(n + 2) % RING], ((n + 2) / RING) & 1)) return false;
       // v_fixed: the fix warp has seen the block's copy complete
       if (!wait_all(&v_fixed[s], (n / RING) & 1) || !wait_all(&p_ready[g * 2 + b], ((tb + j) >> 1) & 1)) return false;
       tc_fence_after();
@@ -472,6 +508,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
         mma_ts_if(leader, tm + C::O_COL, tm + b * BKV + k16 * 8,
                   v_desc + (uint64_t)(s * (C::KV_BYTES >> 4) + k16 * (16 * 128 >> 4)), idesc_o,
                   (j > 0 || k16 > 0) ? 1u : 0u);
+      if (more) s_products(j + 2);
       tc_commit_if(leader, &pv_done[g * 2 + b]);
       tc_commit_if(leader, &v_empty[s]);
       return true;
@@ -496,13 +533,16 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
         if (ok && leader) bar_arrive(q_empty);
       } else {
         ok = wait_all(q_full, un & 1);
-        for (int j = 0; j < min(nkv, 2) && ok; ++j) ok = issue_s(j);
+        for (int j = 0; j < min(nkv, 2) && ok; ++j) {
+          ok = wait_all(&k_full[(nb + j) % RING], ((nb + j) / RING) & 1);
+          tc_fence_after();
+          if (ok) s_products(j);
+        }
         if (ok && nkv <= 2) tc_commit_if(leader, q_empty);
         // the rows of the unit before have been read out of O
         if (ok) ok = wait_all(&o_empty[g], (tu & 1) ^ 1);
         for (int j = 0; j < nkv && ok; ++j) {
-          ok = issue_pv(j);
-          if (ok && j + 2 < nkv) ok = issue_s(j + 2);
+          ok = step(j, j + 2 < nkv);
           if (ok && j + 3 == nkv) tc_commit_if(leader, q_empty);
         }
         tb += (uint32_t)nkv;
@@ -677,13 +717,13 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
         }
         float m8[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) m8[k] = fmaxf(s[k], s[8 + k]);
+        for (int k = 0; k < 8; ++k) m8[k] = max2n(s[k], s[8 + k]);
 #pragma unroll
         for (int c = 16; c < BKV; c += 16) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) m8[k] = max3f(m8[k], s[c + k], s[c + 8 + k]);
+          for (int k = 0; k < 8; ++k) m8[k] = max3n(m8[k], s[c + k], s[c + 8 + k]);
         }
-        const float mx = max3f(max3f(m8[0], m8[1], m8[2]), max3f(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7])) *
+        const float mx = max3n(max3n(m8[0], m8[1], m8[2]), max3n(m8[3], m8[4], m8[5]), max2n(m8[6], m8[7])) *
                          p.scale_log2;
         float alpha = 1.0f;
         if (mx > m + kRescaleThreshold) {
@@ -708,23 +748,37 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
         const float mref = m == -INFINITY ? 0.0f : m;  // no key seen yet: every p is 2^-inf = 0
         const unsigned long long nm2 = pack2(-mref, -mref);
         unsigned long long sum2[4] = {0ull, 0ull, 0ull, 0ull};
+        // P and its row sum (before the rounding); bit k of poly: pair k of 16
+        // takes the polynomial.
+        auto exps = [&](auto poly) {
 #pragma unroll
-        for (int ch = 0; ch < BKV / 32; ++ch) {
-          uint32_t pk[16];
+          for (int ch = 0; ch < BKV / 32; ++ch) {
+            uint32_t pk[16];
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            float a, b;
-            unpack2(fma2(pack2(s[ch * 32 + 2 * k], s[ch * 32 + 2 * k + 1]), sc2, nm2), a, b);
-            a = ex2(a);
-            b = ex2(b);
-            sum2[k & 3] = add2(sum2[k & 3], pack2(a, b));
-            pk[k] = cvt2<kBF16>(a, b);
+            for (int k = 0; k < 16; ++k) {
+              float a, b;
+              const unsigned long long x2 = fma2(pack2(s[ch * 32 + 2 * k], s[ch * 32 + 2 * k + 1]), sc2, nm2);
+              if ((decltype(poly)::value >> k) & 1) {
+                ex2_poly2(x2, a, b);
+              } else {
+                unpack2(x2, a, b);
+                a = ex2(a);
+                b = ex2(b);
+              }
+              sum2[k & 3] = add2(sum2[k & 3], pack2(a, b));
+              pk[k] = cvt2<kBF16>(a, b);
+            }
+            tmem_st16(s_addr + ch * 16, pk);
           }
-          tmem_st16(s_addr + ch * 16, pk);
-        }
+        };
+        if (C::kPolyPairs == 0 || j >= u.jb || __any_sync(0xffffffffu, m == -INFINITY))
+          exps(std::integral_constant<unsigned, 0u>{});
+        else
+          exps(std::integral_constant<unsigned, C::kPolyPairs>{});
         float a0, a1;
         unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), a0, a1);
         l = l * alpha + (a0 + a1);
+        if (!(mx < INFINITY)) l = __int_as_float(0x7fc00000);  // a NaN or +inf score: the row is NaN
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -739,7 +793,12 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
         tc_fence_after();
         const float inv_l = l == 0.0f ? 0.0f : 1.0f / l;  // no key in this range: zeros
         const bool repair = nonfinite[i & 1] != 0 && valid;
-        const uint32_t vmask = __ballot_sync(0xffffffffu, valid);
+        // where the rows that this lane helps to write begin (null: no row)
+        uint16_t* rows_at[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          rows_at[k] = reinterpret_cast<uint16_t*>(__shfl_sync(
+              0xffffffffu, valid ? reinterpret_cast<unsigned long long>(dst) : 0ull, k * 8 + (lane >> 2)));
         // keys that only some rows see, within this CTA's range
         const int from = max(u.lim_min, (u.j0 + u.jb) * BKV), to = min(lim, (u.j0 + u.nkv) * BKV);
         if (p.in_cluster && valid) stats[urow] = make_float2(l == 0.0f ? -INFINITY : m + log2f(l), 0.f);
@@ -794,9 +853,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
             for (int k = 0; k < 4; ++k) {
               const int r = k * 8 + (lane >> 2);
               const uint4 v = st[r * 4 + ((lane & 3) ^ ((r >> 1) & 3))];
-              const unsigned long long to = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r);
-              if ((vmask >> r) & 1u)
-                *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(to) + c * 32 + (lane & 3) * 8) = v;
+              if (rows_at[k]) *reinterpret_cast<uint4*>(rows_at[k] + c * 32 + (lane & 3) * 8) = v;
             }
             __syncwarp();
           }
