@@ -65,7 +65,8 @@ constexpr int kMaxCluster = 16;   // CTAs that split a unit's keys and merge in 
 // all of K and V again and the L2's bandwidth bounds the one-tile form.
 template <int HD, int NT>
 struct Cfg {
-  static constexpr int RING = NT == 1 ? 2 : 4;  // K and V slots
+  // K and V slots (a K slot is free two blocks before a V slot)
+  static constexpr int KRING = NT == 1 ? 2 : 3, VRING = NT == 1 ? 2 : 4;
   static constexpr int SOFTMAX_WARPS = 4 * NT;
   static constexpr int WARP_MMA = 4 * NT;  // one per tile
   static constexpr int WARP_TMA = WARP_MMA + NT, WARP_FIX = WARP_TMA + 1;
@@ -79,12 +80,15 @@ struct Cfg {
   static constexpr int Q_BYTES = HALVES * Q_HALF;
   static constexpr int KV_HALF = BKV * 128;
   static constexpr int KV_BYTES = HALVES * KV_HALF;
-  // K and V rings; once a unit's products are done they can hold its O (f32)
-  static constexpr int RINGS_BYTES = 2 * RING * KV_BYTES;
-  static_assert(RINGS_BYTES >= NT * BQ * HD * 4, "O does not fit the rings");
+  // Q and the rings; once a unit's products are done they can hold its O (f32)
+  static constexpr int TILES_BYTES = NT * Q_BYTES + (KRING + VRING) * KV_BYTES;
+  static_assert(TILES_BYTES >= NT * BQ * HD * 4, "O does not fit the tiles");
   static constexpr int BAR_BYTES = 512;
-  static constexpr int SMEM_BYTES = 1024 + NT * Q_BYTES + RINGS_BYTES + BAR_BYTES + NT * BQ * 8 + kMaxSeqs * 8 +
-                                    SOFTMAX_WARPS * 2048;
+  // Columns that the epilogue takes at a time through a warp's staging rows:
+  // 128 bytes of a row (a whole line) where there is room
+  static constexpr int EC = NT == 1 ? 32 : 64;
+  static constexpr int SMEM_BYTES = 1024 + TILES_BYTES + BAR_BYTES + NT * BQ * 8 + kMaxSeqs * 8 +
+                                    SOFTMAX_WARPS * 32 * EC * 2;
   static_assert((SMEM_BYTES + 1024) * (3 - NT) <= 228 * 1024, "CTAs per SM");
 };
 
@@ -308,24 +312,24 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
                           const __grid_constant__ CUtensorMap kmap,
                           const __grid_constant__ CUtensorMap vmap, const Params p) {
   using C = Cfg<HD, NT>;
-  constexpr int RING = C::RING;
+  constexpr int KRING = C::KRING, VRING = C::VRING;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   uint8_t* qs = smem;
   uint8_t* ks = qs + NT * C::Q_BYTES;
-  uint8_t* vs = ks + RING * C::KV_BYTES;
-  Unit* units = reinterpret_cast<Unit*>(vs + RING * C::KV_BYTES);  // [2]
+  uint8_t* vs = ks + KRING * C::KV_BYTES;
+  Unit* units = reinterpret_cast<Unit*>(vs + VRING * C::KV_BYTES);  // [2]
   uint64_t* unit_full = reinterpret_cast<uint64_t*>(units + 2);
   uint64_t* unit_empty = unit_full + 2;
   uint64_t* q_full = unit_empty + 2;
   uint64_t* q_empty = q_full + 1;
   uint64_t* k_full = q_empty + 1;
-  uint64_t* k_empty = k_full + RING;
-  uint64_t* v_full = k_empty + RING;
-  uint64_t* v_empty = v_full + RING;
-  uint64_t* v_fixed = v_empty + RING;
-  uint64_t* s_full = v_fixed + RING;      // [2 * NT] tile g, buffer b: g * 2 + b
+  uint64_t* k_empty = k_full + KRING;
+  uint64_t* v_full = k_empty + KRING;
+  uint64_t* v_empty = v_full + VRING;
+  uint64_t* v_fixed = v_empty + VRING;
+  uint64_t* s_full = v_fixed + VRING;      // [2 * NT] tile g, buffer b: g * 2 + b
   uint64_t* p_ready = s_full + 2 * NT;    // [2 * NT]
   uint64_t* pv_done = p_ready + 2 * NT;   // [2 * NT]
   uint64_t* o_empty = pv_done + 2 * NT;   // [NT]
@@ -335,7 +339,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
   volatile int* nonfinite = abort_flag + 1;  // [2] by unit
   float2* stats = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(units) + C::BAR_BYTES);  // [NT * BQ] log2 sum (cluster merge)
   int2* lens = reinterpret_cast<int2*>(stats + NT * BQ);  // [kMaxSeqs]
-  uint4* stage = reinterpret_cast<uint4*>(lens + kMaxSeqs);  // 2 KB per softmax warp
+  uint4* stage = reinterpret_cast<uint4*>(lens + kMaxSeqs);  // 32 rows of EC columns per softmax warp
 
   const int warp = threadIdx.x / 32;
   const int lane = (int)lane_id();
@@ -356,9 +360,11 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
     }
     bar_init(q_full, 1);
     bar_init(q_empty, NT);
-    for (int s = 0; s < RING; ++s) {
+    for (int s = 0; s < KRING; ++s) {
       bar_init(&k_full[s], 1);
       bar_init(&k_empty[s], NT);
+    }
+    for (int s = 0; s < VRING; ++s) {
       bar_init(&v_full[s], 1);
       bar_init(&v_empty[s], NT);
       bar_init(&v_fixed[s], 1);
@@ -412,8 +418,9 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
       if (lane == 0) bar_arrive(&unit_empty[i & 1]);
       if (u.nkv == 0) continue;
       int ent = -1, ent_base = -1;
-      auto load = [&](const void* map, uint8_t* ring, uint64_t* full, uint64_t* empty, uint32_t& cnt, int j) -> bool {
-        const uint32_t s = cnt % RING;
+      auto load = [&](const void* map, uint8_t* ring, uint64_t* full, uint64_t* empty, uint32_t depth, uint32_t& cnt,
+                      int j) -> bool {
+        const uint32_t s = cnt % depth;
         const int key0 = (u.j0 + j) * BKV;
         int page = 0;
         if constexpr (kPaged) {
@@ -424,7 +431,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
           }
           page = __shfl_sync(0xffffffffu, ent, (((key0 + (box << box_shift)) >> p.page_shift) - ent_base) & 31);
         }
-        const bool good = wait_bar(&empty[s], ((cnt / RING) & 1) ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_TMA);
+        const bool good = wait_bar(&empty[s], ((cnt / depth) & 1) ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_TMA);
         if (!__all_sync(0xffffffffu, good)) return false;
         if (lane == 0) bar_arrive_expect_tx(&full[s], C::KV_BYTES);
         __syncwarp();
@@ -453,10 +460,10 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
       ++qn;
       // K runs two blocks ahead of V, as S does of P V: each load is asked for
       // as soon as its slot is free, two blocks' time before it is needed.
-      ok = load(&kmap, ks, k_full, k_empty, kn, 0) && (u.nkv == 1 || load(&kmap, ks, k_full, k_empty, kn, 1));
+      ok = load(&kmap, ks, k_full, k_empty, KRING, kn, 0) && (u.nkv == 1 || load(&kmap, ks, k_full, k_empty, KRING, kn, 1));
       for (int j = 0; j < u.nkv && ok; ++j) {
-        ok = load(&vmap, vs, v_full, v_empty, vn, j);
-        if (ok && j + 2 < u.nkv) ok = load(&kmap, ks, k_full, k_empty, kn, j + 2);
+        ok = load(&vmap, vs, v_full, v_empty, VRING, vn, j);
+        if (ok && j + 2 < u.nkv) ok = load(&kmap, ks, k_full, k_empty, KRING, kn, j + 2);
       }
     }
     if (*abort_flag) {  // let copies in flight land before the shared memory is released
@@ -484,7 +491,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
       return __all_sync(0xffffffffu, wait_fast(bar, parity, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA));
     };
     auto s_products = [&](int j) {
-      const uint32_t s = (nb + j) % RING, b = (tb + j) & 1;
+      const uint32_t s = (nb + j) % KRING, b = (tb + j) & 1;
 #pragma unroll
       for (int k16 = 0; k16 < HD / 16; ++k16)  // descriptors count 16 bytes
         mma_ss_if(leader, tm + b * BKV,
@@ -498,10 +505,10 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
     // not need to wait for is waited for before it, so that both products
     // follow P at once: softmax(j + 1) runs meanwhile, softmax(j + 2) next.
     auto step = [&](int j, bool more) -> bool {
-      const uint32_t n = nb + j, s = n % RING, b = (tb + j) & 1;
-      if (more && !wait_all(&k_full[(n + 2) % RING], ((n + 2) / RING) & 1)) return false;
+      const uint32_t n = nb + j, s = n % VRING, b = (tb + j) & 1;
+      if (more && !wait_all(&k_full[(n + 2) % KRING], ((n + 2) / KRING) & 1)) return false;
       // v_fixed: the fix warp has seen the block's copy complete
-      if (!wait_all(&v_fixed[s], (n / RING) & 1) || !wait_all(&p_ready[g * 2 + b], ((tb + j) >> 1) & 1)) return false;
+      if (!wait_all(&v_fixed[s], (n / VRING) & 1) || !wait_all(&p_ready[g * 2 + b], ((tb + j) >> 1) & 1)) return false;
       tc_fence_after();
 #pragma unroll
       for (int k16 = 0; k16 < BKV / 16; ++k16)
@@ -523,18 +530,18 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
       if (g > 0 && __shfl_sync(0xffffffffu, u.n_tok, 0) <= p.tile_tokens) {
         // no rows in this tile: only the other one uses Q, K and V
         for (int j = 0; j < nkv && ok; ++j) {
-          const uint32_t s = (nb + j) % RING, ph = ((nb + j) / RING) & 1;
-          ok = wait_all(&k_full[s], ph);
-          if (ok && leader) bar_arrive(&k_empty[s]);
-          if (ok) ok = wait_all(&v_fixed[s], ph);
-          if (ok && leader) bar_arrive(&v_empty[s]);
+          const uint32_t n = nb + j;
+          ok = wait_all(&k_full[n % KRING], (n / KRING) & 1);
+          if (ok && leader) bar_arrive(&k_empty[n % KRING]);
+          if (ok) ok = wait_all(&v_fixed[n % VRING], (n / VRING) & 1);
+          if (ok && leader) bar_arrive(&v_empty[n % VRING]);
         }
         if (ok) ok = wait_all(q_full, un & 1);
         if (ok && leader) bar_arrive(q_empty);
       } else {
         ok = wait_all(q_full, un & 1);
         for (int j = 0; j < min(nkv, 2) && ok; ++j) {
-          ok = wait_all(&k_full[(nb + j) % RING], ((nb + j) / RING) & 1);
+          ok = wait_all(&k_full[(nb + j) % KRING], ((nb + j) / KRING) & 1);
           tc_fence_after();
           if (ok) s_products(j);
         }
@@ -609,8 +616,8 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
       // Every block passes here, so that the warp follows each phase of the
       // ring; those before jb pass untouched.
       for (int j = 0; j < u.nkv; ++j, ++vn) {
-        const uint32_t s = vn % RING;
-        const bool good = wait_bar(&v_full[s], (vn / RING) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER);
+        const uint32_t s = vn % VRING;
+        const bool good = wait_bar(&v_full[s], (vn / VRING) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER);
         ok = __all_sync(0xffffffffu, good);
         if (!ok) break;
         if (j >= u.jb) {
@@ -793,27 +800,30 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
         tc_fence_after();
         const float inv_l = l == 0.0f ? 0.0f : 1.0f / l;  // no key in this range: zeros
         const bool repair = nonfinite[i & 1] != 0 && valid;
-        // where the rows that this lane helps to write begin (null: no row)
-        uint16_t* rows_at[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          rows_at[k] = reinterpret_cast<uint16_t*>(__shfl_sync(
-              0xffffffffu, valid ? reinterpret_cast<unsigned long long>(dst) : 0ull, k * 8 + (lane >> 2)));
         // keys that only some rows see, within this CTA's range
         const int from = max(u.lim_min, (u.j0 + u.jb) * BKV), to = min(lim, (u.j0 + u.nkv) * BKV);
         if (p.in_cluster && valid) stats[urow] = make_float2(l == 0.0f ? -INFINITY : m + log2f(l), 0.f);
-#pragma unroll 1
-        for (int c = 0; c < HD / 32; ++c) {
-          uint32_t r[32];
-          tmem_ld32(o_addr + c * 32, r);
-          tmem_wait_ld();
-          float o[32];
-          uint4 h4[4];
+        constexpr int EC = C::EC, PIECES = EC / 8;  // 16-byte pieces of a staged row
+        // where the rows that this lane helps to write begin (null: no row)
+        uint16_t* rows_at[PIECES];
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = __uint_as_float(r[k]) * inv_l;
+        for (int k = 0; k < PIECES; ++k)
+          rows_at[k] = reinterpret_cast<uint16_t*>(__shfl_sync(
+              0xffffffffu, valid ? reinterpret_cast<unsigned long long>(dst) : 0ull, (k * 32 + lane) / PIECES));
+#pragma unroll 1
+        for (int c = 0; c < HD; c += EC) {
+          float o[EC];
+#pragma unroll
+          for (int h = 0; h < EC; h += 32) {
+            uint32_t r[32];
+            tmem_ld32(o_addr + c + h, r);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[h + k] = __uint_as_float(r[k]) * inv_l;
+          }
           if (repair) {
             for (int key = from; key < to; ++key) {
-              const uint16_t* src = static_cast<const uint16_t*>(p.v) + (size_t)u.kvh * p.v_head + c * 32;
+              const uint16_t* src = static_cast<const uint16_t*>(p.v) + (size_t)u.kvh * p.v_head + c;
               if constexpr (kPaged) {
                 const int page = p.table[(size_t)u.seq * p.table_ld + (key >> p.page_shift)];
                 if (page < 0 || page >= p.n_pages) continue;
@@ -822,38 +832,39 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
                 src += (size_t)(u.q_begin + key) * p.v_token;
               }
 #pragma unroll
-              for (int k = 0; k < 32; ++k)
+              for (int k = 0; k < EC; ++k)
                 if (!finite16<kBF16>(src[k])) o[k] += to_f32<kBF16>(src[k]);
             }
           }
           if (p.splits > 1) {
-            // global memory, or the rings (every product of the unit is done);
-            // there, 16-byte pieces are permuted within a row against conflicts
-            float* po = p.in_cluster ? reinterpret_cast<float*>(ks) + urow * HD : p.part_o + part * HD;
+            // global memory, or this CTA's tiles (every product of the unit is
+            // done); there, 16-byte pieces are permuted within a row against conflicts
+            float* po = p.in_cluster ? reinterpret_cast<float*>(qs) + urow * HD : p.part_o + part * HD;
             const int x = p.in_cluster ? urow & 7 : 0;
 #pragma unroll
-            for (int k = 0; k < 8 && valid; ++k)
-              *reinterpret_cast<float4*>(po + ((c * 8 + k) ^ x) * 4) =
-                  make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+            for (int k = 0; k < EC / 4; ++k)
+              if (valid)
+                *reinterpret_cast<float4*>(po + ((c / 4 + k) ^ x) * 4) =
+                    make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
           } else {
+            // Through shared memory, so that neighbouring lanes write
+            // neighbouring pieces of a row (a lane writing its own row touches
+            // 32 lines per instruction, and the SM takes about 3 clocks for
+            // each); pieces are permuted against bank conflicts.
+            auto place = [](int row, int piece) {
+              return row * PIECES + (piece ^ (PIECES == 8 ? row & 7 : (row >> 1) & 3));
+            };
+            uint4* st = stage + warp * (32 * PIECES);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              h4[k] = make_uint4(cvt2<kBF16>(o[8 * k], o[8 * k + 1]), cvt2<kBF16>(o[8 * k + 2], o[8 * k + 3]),
-                                 cvt2<kBF16>(o[8 * k + 4], o[8 * k + 5]), cvt2<kBF16>(o[8 * k + 6], o[8 * k + 7]));
-          }
-          if (p.splits == 1) {
-            // Through shared memory, so that four lanes write 64 bytes of one
-            // row together (a lane writing its own row touches 32 lines per
-            // instruction); pieces are permuted against bank conflicts.
-            uint4* st = stage + warp * 128;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) st[lane * 4 + (k ^ ((lane >> 1) & 3))] = h4[k];
+            for (int k = 0; k < PIECES; ++k)
+              st[place(lane, k)] =
+                  make_uint4(cvt2<kBF16>(o[8 * k], o[8 * k + 1]), cvt2<kBF16>(o[8 * k + 2], o[8 * k + 3]),
+                             cvt2<kBF16>(o[8 * k + 4], o[8 * k + 5]), cvt2<kBF16>(o[8 * k + 6], o[8 * k + 7]));
             __syncwarp();
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int r = k * 8 + (lane >> 2);
-              const uint4 v = st[r * 4 + ((lane & 3) ^ ((r >> 1) & 3))];
-              if (rows_at[k]) *reinterpret_cast<uint4*>(rows_at[k] + c * 32 + (lane & 3) * 8) = v;
+            for (int k = 0; k < PIECES; ++k) {
+              const uint4 v = st[place((k * 32 + lane) / PIECES, lane % PIECES)];
+              if (rows_at[k]) *reinterpret_cast<uint4*>(rows_at[k] + c + lane % PIECES * 8) = v;
             }
             __syncwarp();
           }
@@ -878,7 +889,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
     if (!*abort_flag && u.nkv >= 0) {
       const int rows = u.n_tok * p.group;
       const int d8 = (int)(threadIdx.x % (HD / 8)) * 2;  // 16-byte pieces d8, d8 + 1
-      const uint32_t st0 = smem_u32(stats), o0 = smem_u32(ks);
+      const uint32_t st0 = smem_u32(stats), o0 = smem_u32(qs);
       for (int r = split + p.splits * (int)(threadIdx.x / (HD / 8)); r < rows;
            r += p.splits * (C::NUM_THREADS / (HD / 8))) {
         float lse[kMaxCluster];
