@@ -426,6 +426,7 @@ int shrink_tiles(const ShrinkParams& p, cudaStream_t st) {
   int c = 8;  // CTAs that split K: up to three per SM, each at least two stages
   while (c > 1 && (units * c > 3ll * num_sms() || p.k_in / tile::BK < 2 * c)) c /= 2;
   if (units * c > 0x7fffffffll) return fail(-2, "b1_gemm_lora: too many tokens in one call");
+  ProfScope prof("lora_shrink", 0.0, 2.0 * p.tokens * p.k_in, st);  // x; the ranks are on the device
   return launch_after("lora_shrink_tile_kernel launch", lora_shrink_tile_kernel, dim3((unsigned)(units * c)),
                       dim3(tile::NUM_THREADS), (size_t)tile::smem_bytes(p.r_pad), c, st, xmap, amap, p,
                       device_error_word());
@@ -447,6 +448,7 @@ int shrink(const ShrinkParams& p, cudaStream_t st) {
   int c = 8;
   while (c > 1 && (units * c > 2ll * num_sms() || (p.k_in / kChunk) / c < kWarps)) c /= 2;
   if (units * c > 0x7fffffffll) return fail(-2, "b1_gemm_lora: too many tokens in one call");
+  ProfScope prof("lora_shrink", 0.0, 2.0 * p.tokens * p.k_in, st);
   return launch_after("lora_shrink_kernel launch", kern, dim3((unsigned)(units * c)), dim3(kThreads), smem, c, st, p);
 }
 
@@ -513,6 +515,7 @@ int launch_b1_gemm_lora(const __half* x, long long ldx, int tokens, const B1Weig
     int* count = reinterpret_cast<int*>(groups + (size_t)n_tiles * g.max_groups);
     g.groups = groups;
     g.group_count = count;
+    ProfScope prof("lora_plan", 0.0, 0.0, st);
     rc = launch_after("lora_plan_kernel launch", lora::lora_plan_kernel, dim3((unsigned)((n_tiles + 7) / 8)),
                       dim3(256), 0, 1, st, cu, slots, n_reqs, tokens, set.info, set.n_slots, g.tile_tokens, n_tiles,
                       g.max_groups, count, groups);
