@@ -14,6 +14,8 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
+import threading
 from pathlib import Path
 
 import numpy as np
@@ -261,7 +263,7 @@ class LoraSet:
 def b1_gemm_lora(x16, w: B1Weight, mode: int, out, lora: LoraSet, cu_tokens, slots, gate=None, stream=None) -> None:
     """b1_gemm with each request's adapter beside it: request i has the tokens
     [cu_tokens[i], cu_tokens[i + 1]) and the adapter slots[i] (-1: none); cuda int32."""
-    dev, st = _text_place(x16)
+    dev, st, _ = _text_place(x16)
     n = slots.shape[0]
     if cu_tokens.shape[0] != n + 1:
         raise BonsaiError(f"cu_tokens {tuple(cu_tokens.shape)} and slots [{n}] do not match")
@@ -340,12 +342,27 @@ class PagesDesc(ctypes.Structure):
 
 
 # These calls run once per layer and token, so their checks are kept to a few
-# microseconds: plain comparisons of what the tensors say of themselves.
+# microseconds: plain comparisons of what the tensors say of themselves, and
+# descriptors packed into a buffer of the calling thread.
 _text_torch = None
+_HEADS = struct.Struct("Qqq")       # bonsai_heads_t
+_PAGES = struct.Struct("Qqqqii")    # bonsai_pages_t
+
+
+class _TextDescs(threading.local):
+    """Up to four descriptors, 40 bytes apart, and their addresses."""
+
+    def __init__(self):
+        self.buf = bytearray(160)
+        base = ctypes.addressof((ctypes.c_char * 160).from_buffer(self.buf))
+        self.at = (base, base + 40, base + 80, base + 120)
+
+
+_text_descs = _TextDescs()
 
 
 def _text_place(first):
-    """(device index of `first`, which has to be the current one, and its current stream)."""
+    """(device index of `first`, which has to be the current one, its current stream, descriptors)."""
     global _text_torch
     if _text_torch is None:
         import torch
@@ -353,7 +370,7 @@ def _text_place(first):
     dev = first.get_device()
     if dev < 0 or dev != _text_torch._C._cuda_getDevice():
         raise BonsaiError(f"tensors must be on the current cuda device, got {first.device}")
-    return dev, _text_torch._C._cuda_getCurrentRawStream(dev)
+    return dev, _text_torch._C._cuda_getCurrentRawStream(dev), _text_descs
 
 
 def _text_dtype(dtype) -> int:
@@ -370,22 +387,24 @@ def _text_ints(dev, name, t):
     return t.data_ptr()
 
 
-def _heads(t, dtype, dev, dim):
-    """bonsai_heads_t of a [token][head][dim] tensor."""
+def _heads(d, i, t, dtype, dev, dim):
+    """Descriptor i: a [token][head][dim] tensor."""
     s = t.stride()
     if len(s) != 3 or t.dtype is not dtype or t.get_device() != dev or s[2] != 1 and dim > 1:
         raise BonsaiError(f"want a [token][head][dim] tensor of {dtype} with contiguous dims on the current device, "
                           f"got {t.dtype} {tuple(t.shape)} {tuple(s)} on {t.device}")
-    return ctypes.byref(HeadsDesc(t.data_ptr(), s[0], s[1]))
+    _HEADS.pack_into(d.buf, 40 * i, t.data_ptr(), s[0], s[1])
+    return d.at[i]
 
 
-def _pages(t, dtype, dev, dim):
-    """bonsai_pages_t of a [page][slot][head][dim] tensor."""
+def _pages(d, i, t, dtype, dev, dim):
+    """Descriptor i: a [page][slot][head][dim] tensor."""
     s, n = t.stride(), t.shape
     if len(s) != 4 or t.dtype is not dtype or t.get_device() != dev or s[3] != 1 and dim > 1:
         raise BonsaiError(f"want a [page][slot][head][dim] cache of {dtype} with contiguous dims on the current device, "
                           f"got {t.dtype} {tuple(n)} {tuple(s)} on {t.device}")
-    return ctypes.byref(PagesDesc(t.data_ptr(), s[0], s[1], s[2], n[0], n[1]))
+    _PAGES.pack_into(d.buf, 40 * i, t.data_ptr(), s[0], s[1], s[2], n[0], n[1])
+    return d.at[i]
 
 
 def _same(what, a, b):
@@ -397,7 +416,7 @@ def prompt_attention(q, k, v, cu_seqlens, out, scale=None, causal=True, stream=N
     """Attention over packed prompts: q, out [T][H][D], k, v [T][Hkv][D] (f16 or
     bf16, any token / head strides that are multiples of 8), cu_seqlens cuda
     int32 [n + 1]; sequence s has the rows [cu_seqlens[s], cu_seqlens[s + 1])."""
-    dev, st = _text_place(q)
+    dev, st, d = _text_place(q)
     dtype, shape, kshape = q.dtype, q.shape, k.shape
     _same("q and out", shape, out.shape)
     _same("k and v", kshape, v.shape)
@@ -405,9 +424,9 @@ def prompt_attention(q, k, v, cu_seqlens, out, scale=None, causal=True, stream=N
     if kshape[0] != T or kshape[2] != D:
         raise BonsaiError(f"k {tuple(kshape)} does not fit q {tuple(shape)}")
     check(lib().bonsai_prompt_attention(
-        _heads(q, dtype, dev, D), _heads(k, dtype, dev, D), _heads(v, dtype, dev, D),
+        _heads(d, 0, q, dtype, dev, D), _heads(d, 1, k, dtype, dev, D), _heads(d, 2, v, dtype, dev, D),
         _text_ints(dev, "cu_seqlens", cu_seqlens), cu_seqlens.shape[0] - 1, T, H, kshape[1], D, _text_dtype(dtype),
-        1 if causal else 0, D ** -0.5 if scale is None else scale, _heads(out, dtype, dev, D),
+        1 if causal else 0, D ** -0.5 if scale is None else scale, _heads(d, 3, out, dtype, dev, D),
         st if stream is None else stream.cuda_stream), "bonsai_prompt_attention")
 
 
@@ -425,7 +444,7 @@ def paged_append(k, v, k_cache, v_cache, page_table, cu_q, ctx_lens, stream=None
     """Write new keys / values [T][Hkv][D] into the cache [pages][page_size][Hkv][D]:
     token i of sequence s (rows [cu_q[s], cu_q[s + 1])) goes to place
     ctx_lens[s] - q_len + i of its page_table row [n][width]."""
-    dev, st = _text_place(k)
+    dev, st, d = _text_place(k)
     dtype, shape, cshape = k.dtype, k.shape, k_cache.shape
     _text_dtype(dtype)
     _same("k and v", shape, v.shape)
@@ -434,8 +453,8 @@ def paged_append(k, v, k_cache, v_cache, page_table, cu_q, ctx_lens, stream=None
     if cshape[2] != Hk or cshape[3] != D:
         raise BonsaiError(f"caches {tuple(cshape)} do not fit k {tuple(shape)}")
     check(lib().bonsai_paged_append(
-        _heads(k, dtype, dev, D), _heads(v, dtype, dev, D), _pages(k_cache, dtype, dev, D),
-        _pages(v_cache, dtype, dev, D), *_table_args(dev, page_table, cu_q, ctx_lens), T, Hk, D,
+        _heads(d, 0, k, dtype, dev, D), _heads(d, 1, v, dtype, dev, D), _pages(d, 2, k_cache, dtype, dev, D),
+        _pages(d, 3, v_cache, dtype, dev, D), *_table_args(dev, page_table, cu_q, ctx_lens), T, Hk, D,
         st if stream is None else stream.cuda_stream), "bonsai_paged_append")
 
 
@@ -444,7 +463,7 @@ def paged_attention(q, k_cache, v_cache, page_table, cu_q, ctx_lens, max_ctx, ou
     """Causal attention of new tokens q [T][H][D] over the paged cache
     [pages][page_size][Hkv][D], the new tokens' own keys appended before;
     max_ctx: an upper bound of ctx_lens (only sets how the work is split)."""
-    dev, st = _text_place(q)
+    dev, st, d = _text_place(q)
     dtype, shape, cshape = q.dtype, q.shape, k_cache.shape
     _same("q and out", shape, out.shape)
     _same("the caches", cshape, v_cache.shape)
@@ -452,9 +471,9 @@ def paged_attention(q, k_cache, v_cache, page_table, cu_q, ctx_lens, max_ctx, ou
     if cshape[3] != D:
         raise BonsaiError(f"caches {tuple(cshape)} do not fit q {tuple(shape)}")
     check(lib().bonsai_paged_attention(
-        _heads(q, dtype, dev, D), _pages(k_cache, dtype, dev, D), _pages(v_cache, dtype, dev, D),
+        _heads(d, 0, q, dtype, dev, D), _pages(d, 1, k_cache, dtype, dev, D), _pages(d, 2, v_cache, dtype, dev, D),
         *_table_args(dev, page_table, cu_q, ctx_lens), T, max_ctx, H, cshape[2], D, _text_dtype(dtype),
-        D ** -0.5 if scale is None else scale, _heads(out, dtype, dev, D),
+        D ** -0.5 if scale is None else scale, _heads(d, 3, out, dtype, dev, D),
         st if stream is None else stream.cuda_stream), "bonsai_paged_attention")
 
 
