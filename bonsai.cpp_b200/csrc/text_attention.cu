@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
   if (warp == C::WARP_TMA) {
     // Paged: a block of 64 keys takes 64 / page boxes (one where a page holds
     // more), and each half of the head dims its own; lane l issues box
-    // l / HALVES, half l % HALVES.  `ent` = 32 consecutive page indices.
+    // l / HALVES, half l % HALVES.
     const int box_shift = min(p.page_shift, 6);
     const int box = lane / C::HALVES, half = lane % C::HALVES;
     const bool issues = kPaged ? box < (BKV >> box_shift) : lane < C::HALVES;
@@ -417,9 +417,10 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
       if (!__all_sync(0xffffffffu, next_unit(i, u))) break;
       if (lane == 0) bar_arrive(&unit_empty[i & 1]);
       if (u.nkv == 0) continue;
-      int ent = -1, ent_base = -1;
+      // 32 page indices each for K and V, which runs behind
+      int ent_k = -1, base_k = -1, ent_v = -1, base_v = -1;
       auto load = [&](const void* map, uint8_t* ring, uint64_t* full, uint64_t* empty, uint32_t depth, uint32_t& cnt,
-                      int j) -> bool {
+                      int& ent, int& ent_base, int j) -> bool {
         const uint32_t s = cnt % depth;
         const int key0 = (u.j0 + j) * BKV;
         int page = 0;
@@ -460,10 +461,10 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
       ++qn;
       // K runs two blocks ahead of V, as S does of P V: each load is asked for
       // as soon as its slot is free, two blocks' time before it is needed.
-      ok = load(&kmap, ks, k_full, k_empty, KRING, kn, 0) && (u.nkv == 1 || load(&kmap, ks, k_full, k_empty, KRING, kn, 1));
+      ok = load(&kmap, ks, k_full, k_empty, KRING, kn, ent_k, base_k, 0) && (u.nkv == 1 || load(&kmap, ks, k_full, k_empty, KRING, kn, ent_k, base_k, 1));
       for (int j = 0; j < u.nkv && ok; ++j) {
-        ok = load(&vmap, vs, v_full, v_empty, VRING, vn, j);
-        if (ok && j + 2 < u.nkv) ok = load(&kmap, ks, k_full, k_empty, KRING, kn, j + 2);
+        ok = load(&vmap, vs, v_full, v_empty, VRING, vn, ent_v, base_v, j);
+        if (ok && j + 2 < u.nkv) ok = load(&kmap, ks, k_full, k_empty, KRING, kn, ent_k, base_k, j + 2);
       }
     }
     if (*abort_flag) {  // let copies in flight land before the shared memory is released
@@ -501,12 +502,16 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
       tc_commit_if(leader, &s_full[g * 2 + b]);
       tc_commit_if(leader, &k_empty[s]);
     };
-    // P V of block j and S of block j + 2 (where there is one).  What P does
-    // not need to wait for is waited for before it, so that both products
-    // follow P at once: softmax(j + 1) runs meanwhile, softmax(j + 2) next.
+    // P V of block j and S of block j + 2 (where there is one).  Two tiles:
+    // what P does not need to wait for is waited for before it, so that both
+    // products follow P at once (softmax(j + 1) runs meanwhile, softmax(j + 2)
+    // next).  One tile, bound by the loads: P V first, so that its V slot is
+    // free while K is still on its way (118 us the other way around, 64
+    // sequences of 130 to 4000 keys, one token each).
     auto step = [&](int j, bool more) -> bool {
       const uint32_t n = nb + j, s = n % VRING, b = (tb + j) & 1;
-      if (more && !wait_all(&k_full[(n + 2) % KRING], ((n + 2) / KRING) & 1)) return false;
+      auto k_there = [&] { return !more || wait_all(&k_full[(n + 2) % KRING], ((n + 2) / KRING) & 1); };
+      if (NT > 1 && !k_there()) return false;
       // v_fixed: the fix warp has seen the block's copy complete
       if (!wait_all(&v_fixed[s], (n / VRING) & 1) || !wait_all(&p_ready[g * 2 + b], ((tb + j) >> 1) & 1)) return false;
       tc_fence_after();
@@ -515,9 +520,14 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
         mma_ts_if(leader, tm + C::O_COL, tm + b * BKV + k16 * 8,
                   v_desc + (uint64_t)(s * (C::KV_BYTES >> 4) + k16 * (16 * 128 >> 4)), idesc_o,
                   (j > 0 || k16 > 0) ? 1u : 0u);
-      if (more) s_products(j + 2);
+      if (NT > 1 && more) s_products(j + 2);
       tc_commit_if(leader, &pv_done[g * 2 + b]);
       tc_commit_if(leader, &v_empty[s]);
+      if (NT == 1 && more) {
+        if (!k_there()) return false;
+        tc_fence_after();
+        s_products(j + 2);
+      }
       return true;
     };
     Unit u;
