@@ -20,12 +20,12 @@
 //               in the log2 domain; the running max moves (and O in TMEM is
 //               rescaled) only when a block's max exceeds it by more than 8.
 //               Warps without a row (a single token has G rows) only pass on.
-//   warp 4      TMA: Q, then K and V blocks of 64 keys (128-byte swizzle,
-//               64-dim halves); paged: one box per page and half, issued by
-//               one lane each, page indices read 32 at a time.
-//   warp 5      issues tcgen05.mma: S(j) = Q K_j^T (SMEM, SMEM),
+//   warp 4      issues tcgen05.mma: S(j) = Q K_j^T (SMEM, SMEM),
 //               O += P(j) V_j (P from TMEM, V MN-major); S runs two blocks
 //               ahead (double-buffered).
+//   warp 5      TMA: Q, then K and V blocks of 64 keys (128-byte swizzle,
+//               64-dim halves); paged: one box per page and half, issued by
+//               one lane each, page indices read 32 at a time.
 //   warp 6      blocks that not every row sees whole (a causal diagonal, the
 //               end of a sequence inside a block or page): V rows past the
 //               sequence's end are zeroed in shared memory before the
@@ -37,7 +37,19 @@
 // are split between the CTAs of a cluster, which merge their parts through
 // distributed shared memory; a split wider than a cluster goes through global
 // memory and a second kernel.
-// TMEM: per tile S(even), S(odd) of 64 columns each, then O of each tile; P(j) (16-bit pairs) overwrites the first 32 columns of its S.
+// TMEM (256 columns): S(even) [0, 64) S(odd) [64, 128) O [128, 128 + HD);
+// P(j) (16-bit pairs) overwrites the first 32 columns of its S.
+//
+// Bounds and measurements (B200, 32 / 8 heads of 128, bf16 unless noted; a call
+// among others): single tokens by HBM, 5.0 TB/s for 64 sequences of 130 to 4000
+// keys (104 us) and 5.7 TB/s for 4 of 30000 to 65536 in f16 (149 us); long
+// prompts by the 64-key Q K^T, whose 192 bytes of shared memory per clock are
+// more than an SM reads, and by the power limit: 10007 tokens 843 us, 973
+// TFLOP/s; batches of short prompts by the start and end of each unit: 48 of 7
+// to 512 tokens 111 us.  128 rows per CTA, two CTAs per SM, because 256 rows
+// per CTA (half the reads of K and V) measured the same on long prompts (778
+// to 838 us against 760 to 804) and 10 to 20 % slower on batches of short
+// ones: 8 x 150 tokens 19.7 against 16.5 us, 48 x 80 40.5 against 33.9.
 #include "internal.cuh"
 #include "ptx.cuh"
 
@@ -45,7 +57,6 @@
 
 #include <algorithm>
 #include <mutex>
-#include <type_traits>
 
 namespace bonsai {
 namespace gemm {
@@ -55,42 +66,31 @@ namespace text {
 
 constexpr int BQ = 128;   // query rows per tile
 constexpr int BKV = 64;   // keys per block
+constexpr int RING = 2;   // K and V slots
+constexpr int WARP_MMA = 4, WARP_TMA = 5, WARP_FIX = 6;
+constexpr int NUM_THREADS = 224;
+constexpr int TMEM_COLS = 256;  // S(even), S(odd) of 64 columns each, O from 128 on
+constexpr int O_COL = 128;
+constexpr int BAR_BYTES = 512;
+constexpr int EC = 32;    // columns that the epilogue takes at a time through a warp's staging rows
 constexpr float kRescaleThreshold = 8.0f;
 constexpr int kMaxSeqs = 512;     // sequences of one launch (their lengths are kept in shared memory)
 constexpr int kMaxCluster = 16;   // CTAs that split a unit's keys and merge in shared memory
 
-// A kernel form: head dims, and query tiles per CTA.  One tile (two CTAs per
-// SM) for single tokens, where K and V are read once and the number of CTAs
-// counts; two tiles (one CTA per SM) for prompts, where every 128 rows read
-// all of K and V again and the L2's bandwidth bounds the one-tile form.
-template <int HD, int NT>
+template <int HD>
 struct Cfg {
-  // K and V slots (a K slot is free two blocks before a V slot)
-  static constexpr int KRING = NT == 1 ? 2 : 3, VRING = NT == 1 ? 2 : 4;
-  static constexpr int SOFTMAX_WARPS = 4 * NT;
-  static constexpr int WARP_MMA = 4 * NT;  // one per tile
-  static constexpr int WARP_TMA = WARP_MMA + NT, WARP_FIX = WARP_TMA + 1;
-  static constexpr int NUM_THREADS = (WARP_FIX + 1) * 32;
-  // TMEM: S of tile g, buffer b at g * 128 + b * 64; O of tile g after all S
-  static constexpr int TMEM_COLS = 256 * NT, O_COL = 128 * NT;
-  // Pairs of 16 whose exponentials take the polynomial
-  static constexpr unsigned kPolyPairs = NT == 1 ? 0u : 0x8888u;
   static constexpr int HALVES = HD / 64;
   static constexpr int Q_HALF = BQ * 128;         // 128 rows x 64 dims
   static constexpr int Q_BYTES = HALVES * Q_HALF;
   static constexpr int KV_HALF = BKV * 128;
   static constexpr int KV_BYTES = HALVES * KV_HALF;
   // Q and the rings; once a unit's products are done they can hold its O (f32)
-  static constexpr int TILES_BYTES = NT * Q_BYTES + (KRING + VRING) * KV_BYTES;
-  static_assert(TILES_BYTES >= NT * BQ * HD * 4, "O does not fit the tiles");
-  static constexpr int BAR_BYTES = 512;
-  // Columns that the epilogue takes at a time through a warp's staging rows:
-  // 128 bytes of a row (a whole line) where there is room
-  static constexpr int EC = NT == 1 ? 32 : 64;
-  static constexpr int SMEM_BYTES = 1024 + TILES_BYTES + BAR_BYTES + NT * BQ * 8 + kMaxSeqs * 8 +
-                                    SOFTMAX_WARPS * 32 * EC * 2;
-  static_assert((SMEM_BYTES + 1024) * (3 - NT) <= 228 * 1024, "CTAs per SM");
+  static constexpr int TILES_BYTES = Q_BYTES + 2 * RING * KV_BYTES;
+  static_assert(TILES_BYTES >= BQ * HD * 4, "O does not fit the tiles");
+  static constexpr int SMEM_BYTES = 1024 + TILES_BYTES + BAR_BYTES + BQ * 8 + kMaxSeqs * 8 + 4 * 32 * EC * 2;
 };
+// Two CTAs per SM (228 KB, 1 KB of it reserved for each).
+static_assert(2 * (Cfg<128>::SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs per SM");
 
 struct Params {
   const int* cu;        // [n_seqs + 1] first query row of each sequence
@@ -174,42 +174,10 @@ __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigne
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-// Maxima that pass NaN on.
-__device__ __forceinline__ float max2n(float a, float b) {
+__device__ __forceinline__ float max3f(float a, float b, float c) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
-}
-__device__ __forceinline__ float max3n(float a, float b, float c) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
-// 2^x for a pair on the FMA and ALU pipes, to take part of the exponentials off
-// the MUFU, which two tiles' keep busy for 1024 clocks a block, nearly as long
-// as their products take.  x = n + f with n = round(x) (the 1.5 * 2^23 shift
-// leaves n in the low mantissa bits) and f in [-0.5, 0.5]; 2^f by a degree-3
-// polynomial (Remez exchange on the relative error, max 7.5e-5: below the
-// rounding of P to 16 bits); n is added to the exponent field.  x is at most
-// the rescaling threshold; below -126 it is cut, which P does not resolve.
-// Neither 2^-inf = 0 (a key that is not seen) nor NaN comes out of it: the
-// caller keeps to ex2 for the one and looks for the other by itself.
-__device__ __forceinline__ void ex2_poly2(unsigned long long x2, float& a, float& b) {
-  constexpr float kShift = 12582912.0f;  // 1.5 * 2^23
-  float x0, x1;
-  unpack2(x2, x0, x1);
-  const unsigned long long xc = pack2(fmaxf(x0, -126.0f), fmaxf(x1, -126.0f));
-  const unsigned long long t = add2(xc, pack2(kShift, kShift));
-  const unsigned long long f = fma2(add2(t, pack2(-kShift, -kShift)), pack2(-1.0f, -1.0f), xc);
-  unsigned long long q = fma2(f, pack2(0.0551716685f, 0.0551716685f), pack2(0.2426111251f, 0.2426111251f));
-  q = fma2(q, f, pack2(0.6932609677f, 0.6932609677f));
-  q = fma2(q, f, pack2(0.9999280572f, 0.9999280572f));
-  float q0, q1, t0, t1;
-  unpack2(q, q0, q1);
-  unpack2(t, t0, t1);
-  a = __uint_as_float(__float_as_uint(q0) + (__float_as_uint(t0) << 23));
-  b = __uint_as_float(__float_as_uint(q1) + (__float_as_uint(t1) << 23));
 }
 
 // What the roles of a CTA need to know of a unit (64 bytes in shared memory).
@@ -306,39 +274,38 @@ __device__ __forceinline__ bool wait_fast(uint64_t* bar, uint32_t parity, volati
   return bar_test_wait(smem_u32(bar), parity) || wait_bar(bar, parity, abort_flag, err, code);
 }
 
-template <int HD, bool kBF16, bool kPaged, int NT>
-__global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
+template <int HD, bool kBF16, bool kPaged>
+__global__ void __launch_bounds__(NUM_THREADS, 2)
     text_attention_kernel(const __grid_constant__ CUtensorMap qmap,
                           const __grid_constant__ CUtensorMap kmap,
                           const __grid_constant__ CUtensorMap vmap, const Params p) {
-  using C = Cfg<HD, NT>;
-  constexpr int KRING = C::KRING, VRING = C::VRING;
+  using C = Cfg<HD>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   uint8_t* qs = smem;
-  uint8_t* ks = qs + NT * C::Q_BYTES;
-  uint8_t* vs = ks + KRING * C::KV_BYTES;
-  Unit* units = reinterpret_cast<Unit*>(vs + VRING * C::KV_BYTES);  // [2]
+  uint8_t* ks = qs + C::Q_BYTES;
+  uint8_t* vs = ks + RING * C::KV_BYTES;
+  Unit* units = reinterpret_cast<Unit*>(vs + RING * C::KV_BYTES);  // [2]
   uint64_t* unit_full = reinterpret_cast<uint64_t*>(units + 2);
   uint64_t* unit_empty = unit_full + 2;
   uint64_t* q_full = unit_empty + 2;
   uint64_t* q_empty = q_full + 1;
   uint64_t* k_full = q_empty + 1;
-  uint64_t* k_empty = k_full + KRING;
-  uint64_t* v_full = k_empty + KRING;
-  uint64_t* v_empty = v_full + VRING;
-  uint64_t* v_fixed = v_empty + VRING;
-  uint64_t* s_full = v_fixed + VRING;      // [2 * NT] tile g, buffer b: g * 2 + b
-  uint64_t* p_ready = s_full + 2 * NT;    // [2 * NT]
-  uint64_t* pv_done = p_ready + 2 * NT;   // [2 * NT]
-  uint64_t* o_empty = pv_done + 2 * NT;   // [NT]
-  uint64_t* drain = o_empty + NT;
+  uint64_t* k_empty = k_full + RING;
+  uint64_t* v_full = k_empty + RING;
+  uint64_t* v_empty = v_full + RING;
+  uint64_t* v_fixed = v_empty + RING;
+  uint64_t* s_full = v_fixed + RING;
+  uint64_t* p_ready = s_full + 2;
+  uint64_t* pv_done = p_ready + 2;
+  uint64_t* o_empty = pv_done + 2;
+  uint64_t* drain = o_empty + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* nonfinite = abort_flag + 1;  // [2] by unit
-  float2* stats = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(units) + C::BAR_BYTES);  // [NT * BQ] log2 sum (cluster merge)
-  int2* lens = reinterpret_cast<int2*>(stats + NT * BQ);  // [kMaxSeqs]
+  float2* stats = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(units) + BAR_BYTES);  // [BQ] log2 sum (cluster merge)
+  int2* lens = reinterpret_cast<int2*>(stats + BQ);  // [kMaxSeqs]
   uint4* stage = reinterpret_cast<uint4*>(lens + kMaxSeqs);  // 32 rows of EC columns per softmax warp
 
   const int warp = threadIdx.x / 32;
@@ -350,40 +317,36 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       bar_init(&unit_full[i], 1);
-      bar_init(&unit_empty[i], C::SOFTMAX_WARPS + NT + 1);  // softmax and MMA warps, TMA
+      bar_init(&unit_empty[i], 6);  // softmax warps, MMA, TMA
       nonfinite[i] = 0;
-    }
-    for (int i = 0; i < 2 * NT; ++i) {
       bar_init(&s_full[i], 1);
       bar_init(&p_ready[i], 4);
       bar_init(&pv_done[i], 1);
     }
     bar_init(q_full, 1);
-    bar_init(q_empty, NT);
-    for (int s = 0; s < KRING; ++s) {
+    bar_init(q_empty, 1);
+    for (int s = 0; s < RING; ++s) {
       bar_init(&k_full[s], 1);
-      bar_init(&k_empty[s], NT);
-    }
-    for (int s = 0; s < VRING; ++s) {
+      bar_init(&k_empty[s], 1);
       bar_init(&v_full[s], 1);
-      bar_init(&v_empty[s], NT);
+      bar_init(&v_empty[s], 1);
       bar_init(&v_fixed[s], 1);
     }
-    for (int g = 0; g < NT; ++g) bar_init(&o_empty[g], 4);
-    bar_init(drain, NT);
+    bar_init(o_empty, 4);
+    bar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&qmap);
     tma_prefetch_desc(&kmap);
     tma_prefetch_desc(&vmap);
   }
-  if (warp == C::WARP_MMA) {
-    tmem_alloc(tmem_slot, C::TMEM_COLS);
+  if (warp == WARP_MMA) {
+    tmem_alloc(tmem_slot, TMEM_COLS);
     tmem_relinquish();
   }
   griddep_wait();
   griddep_launch();
-  for (int i = threadIdx.x; i < p.n_seqs; i += C::NUM_THREADS) {
+  for (int i = threadIdx.x; i < p.n_seqs; i += NUM_THREADS) {
     const int a = max(0, min(p.cu[i], p.total_q)), b = max(a, min(p.cu[i + 1], p.total_q));
     lens[i] = make_int2(b - a, kPaged ? p.ctx[i] - (b - a) : 0);
   }
@@ -403,7 +366,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
     return u.nkv >= 0;
   };
 
-  if (warp == C::WARP_TMA) {
+  if (warp == WARP_TMA) {
     // Paged: a block of 64 keys takes 64 / page boxes (one where a page holds
     // more), and each half of the head dims its own; lane l issues box
     // l / HALVES, half l % HALVES.
@@ -451,20 +414,18 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
       ok = __all_sync(0xffffffffu, good);
       if (!ok) break;
       if (lane == 0) {
-        const int tiles = NT == 1 || u.n_tok <= p.tile_tokens ? 1 : NT;
-        bar_arrive_expect_tx(q_full, (uint32_t)(tiles * p.group * p.tile_tokens * HD * 2));
-        for (int h = 0; h < tiles * C::HALVES; ++h)
-          tma_load_3d(qs + h * C::Q_HALF, &qmap, q_full, h % C::HALVES * 64, u.kvh * p.group,
-                      u.q_begin + u.t0 + h / C::HALVES * p.tile_tokens);
+        bar_arrive_expect_tx(q_full, (uint32_t)(p.group * p.tile_tokens * HD * 2));
+        for (int h = 0; h < C::HALVES; ++h)
+          tma_load_3d(qs + h * C::Q_HALF, &qmap, q_full, h * 64, u.kvh * p.group, u.q_begin + u.t0);
       }
       __syncwarp();
       ++qn;
       // K runs two blocks ahead of V, as S does of P V: each load is asked for
       // as soon as its slot is free, two blocks' time before it is needed.
-      ok = load(&kmap, ks, k_full, k_empty, KRING, kn, ent_k, base_k, 0) && (u.nkv == 1 || load(&kmap, ks, k_full, k_empty, KRING, kn, ent_k, base_k, 1));
+      ok = load(&kmap, ks, k_full, k_empty, RING, kn, ent_k, base_k, 0) && (u.nkv == 1 || load(&kmap, ks, k_full, k_empty, RING, kn, ent_k, base_k, 1));
       for (int j = 0; j < u.nkv && ok; ++j) {
-        ok = load(&vmap, vs, v_full, v_empty, VRING, vn, ent_v, base_v, j);
-        if (ok && j + 2 < u.nkv) ok = load(&kmap, ks, k_full, k_empty, KRING, kn, ent_k, base_k, j + 2);
+        ok = load(&vmap, vs, v_full, v_empty, RING, vn, ent_v, base_v, j);
+        if (ok && j + 2 < u.nkv) ok = load(&kmap, ks, k_full, k_empty, RING, kn, ent_k, base_k, j + 2);
       }
     }
     if (*abort_flag) {  // let copies in flight land before the shared memory is released
@@ -472,62 +433,48 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
       while (globaltimer_ns() - w0 < 1000000ull) {
       }
     }
-  } else if (warp >= C::WARP_MMA && warp < C::WARP_MMA + NT) {
-    // One warp per tile: waits and commits of one tile's products hide behind
-    // the other's (a single warp takes 2100 clocks for the two tiles' products
-    // of a block, which run in 1300).  The whole warp runs this role, one
-    // thread of it issues: see mma_ss_if.
+  } else if (warp == WARP_MMA) {
+    // The whole warp runs this role, one thread of it issues: see mma_ss_if.
     constexpr uint32_t idesc_s = make_idesc_f16(BQ, BKV, kBF16 ? 1 : 0, 0, 0);
     constexpr uint32_t idesc_o = make_idesc_f16(BQ, HD, kBF16 ? 1 : 0, 0, 1);
-    const int g = __shfl_sync(0xffffffffu, warp - C::WARP_MMA, 0);
     const uint32_t leader = elect_one() ? 1u : 0u;
-    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0) + g * 128;
-    const uint64_t q_desc = make_smem_desc(smem_u32(qs) + g * C::Q_BYTES, 16, 1024);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint64_t q_desc = make_smem_desc(smem_u32(qs), 16, 1024);
     const uint64_t k_desc = make_smem_desc(smem_u32(ks), 16, 1024);
     const uint64_t v_desc = make_smem_desc(smem_u32(vs), C::KV_HALF, 1024);
-    // Blocks and units so far, of the CTA (K and V rings, Q) and of this tile
-    // (its S buffers and O): a unit may have rows in the first tile only.
-    uint32_t nb = 0, un = 0, tb = 0, tu = 0;
+    uint32_t nb = 0, un = 0;  // blocks and units so far
     auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool {
       return __all_sync(0xffffffffu, wait_fast(bar, parity, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA));
     };
-    auto s_products = [&](int j) {
-      const uint32_t s = (nb + j) % KRING, b = (tb + j) & 1;
+    auto issue_s = [&](int j) -> bool {
+      const uint32_t n = nb + j, s = n % RING, b = n & 1;
+      if (!wait_all(&k_full[s], (n / RING) & 1)) return false;
+      tc_fence_after();
 #pragma unroll
       for (int k16 = 0; k16 < HD / 16; ++k16)  // descriptors count 16 bytes
         mma_ss_if(leader, tm + b * BKV,
                   q_desc + (uint64_t)(((k16 >> 2) * C::Q_HALF + (k16 & 3) * 32) >> 4),
                   k_desc + (uint64_t)(s * (C::KV_BYTES >> 4) + (((k16 >> 2) * C::KV_HALF + (k16 & 3) * 32) >> 4)),
                   idesc_s, k16 > 0 ? 1u : 0u);
-      tc_commit_if(leader, &s_full[g * 2 + b]);
+      tc_commit_if(leader, &s_full[b]);
       tc_commit_if(leader, &k_empty[s]);
+      return true;
     };
-    // P V of block j and S of block j + 2 (where there is one).  Two tiles:
-    // what P does not need to wait for is waited for before it, so that both
-    // products follow P at once (softmax(j + 1) runs meanwhile, softmax(j + 2)
-    // next).  One tile, bound by the loads: P V first, so that its V slot is
-    // free while K is still on its way (118 us the other way around, 64
-    // sequences of 130 to 4000 keys, one token each).
-    auto step = [&](int j, bool more) -> bool {
-      const uint32_t n = nb + j, s = n % VRING, b = (tb + j) & 1;
-      auto k_there = [&] { return !more || wait_all(&k_full[(n + 2) % KRING], ((n + 2) / KRING) & 1); };
-      if (NT > 1 && !k_there()) return false;
+    // P V first, then S: its V slot is free while K may still be on its way
+    // (the other way around 118 us instead of 111, 64 sequences of 130 to 4000
+    // keys, one token each).
+    auto issue_pv = [&](int j) -> bool {
+      const uint32_t n = nb + j, s = n % RING, b = n & 1;
       // v_fixed: the fix warp has seen the block's copy complete
-      if (!wait_all(&v_fixed[s], (n / VRING) & 1) || !wait_all(&p_ready[g * 2 + b], ((tb + j) >> 1) & 1)) return false;
+      if (!wait_all(&v_fixed[s], (n / RING) & 1) || !wait_all(&p_ready[b], (n >> 1) & 1)) return false;
       tc_fence_after();
 #pragma unroll
       for (int k16 = 0; k16 < BKV / 16; ++k16)
-        mma_ts_if(leader, tm + C::O_COL, tm + b * BKV + k16 * 8,
+        mma_ts_if(leader, tm + O_COL, tm + b * BKV + k16 * 8,
                   v_desc + (uint64_t)(s * (C::KV_BYTES >> 4) + k16 * (16 * 128 >> 4)), idesc_o,
                   (j > 0 || k16 > 0) ? 1u : 0u);
-      if (NT > 1 && more) s_products(j + 2);
-      tc_commit_if(leader, &pv_done[g * 2 + b]);
+      tc_commit_if(leader, &pv_done[b]);
       tc_commit_if(leader, &v_empty[s]);
-      if (NT == 1 && more) {
-        if (!k_there()) return false;
-        tc_fence_after();
-        s_products(j + 2);
-      }
       return true;
     };
     Unit u;
@@ -537,33 +484,15 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
       if (leader) bar_arrive(&unit_empty[i & 1]);
       const int nkv = __shfl_sync(0xffffffffu, u.nkv, 0);
       if (nkv == 0) continue;
-      if (g > 0 && __shfl_sync(0xffffffffu, u.n_tok, 0) <= p.tile_tokens) {
-        // no rows in this tile: only the other one uses Q, K and V
-        for (int j = 0; j < nkv && ok; ++j) {
-          const uint32_t n = nb + j;
-          ok = wait_all(&k_full[n % KRING], (n / KRING) & 1);
-          if (ok && leader) bar_arrive(&k_empty[n % KRING]);
-          if (ok) ok = wait_all(&v_fixed[n % VRING], (n / VRING) & 1);
-          if (ok && leader) bar_arrive(&v_empty[n % VRING]);
-        }
-        if (ok) ok = wait_all(q_full, un & 1);
-        if (ok && leader) bar_arrive(q_empty);
-      } else {
-        ok = wait_all(q_full, un & 1);
-        for (int j = 0; j < min(nkv, 2) && ok; ++j) {
-          ok = wait_all(&k_full[(nb + j) % KRING], ((nb + j) / KRING) & 1);
-          tc_fence_after();
-          if (ok) s_products(j);
-        }
-        if (ok && nkv <= 2) tc_commit_if(leader, q_empty);
-        // the rows of the unit before have been read out of O
-        if (ok) ok = wait_all(&o_empty[g], (tu & 1) ^ 1);
-        for (int j = 0; j < nkv && ok; ++j) {
-          ok = step(j, j + 2 < nkv);
-          if (ok && j + 3 == nkv) tc_commit_if(leader, q_empty);
-        }
-        tb += (uint32_t)nkv;
-        ++tu;
+      ok = wait_all(q_full, un & 1);
+      for (int j = 0; j < min(nkv, 2) && ok; ++j) ok = issue_s(j);
+      if (ok && nkv <= 2) tc_commit_if(leader, q_empty);
+      // the rows of the unit before have been read out of O
+      if (ok) ok = wait_all(o_empty, (un & 1) ^ 1);
+      for (int j = 0; j < nkv && ok; ++j) {
+        ok = issue_pv(j);
+        if (ok && j + 2 < nkv) ok = issue_s(j + 2);
+        if (ok && j + 3 == nkv) tc_commit_if(leader, q_empty);
       }
       nb += (uint32_t)nkv;
       ++un;
@@ -578,10 +507,10 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
       }
     }
     __syncwarp();
-  } else if (warp == C::WARP_FIX) {
+  } else if (warp == WARP_FIX) {
     // The units: two are out at a time, the next one is found and put in the
     // place of one that every role has left.
-    Finder f{lens, p.n_seqs, NT * p.tile_tokens, p.causal, kPaged ? (long long)p.table_width << p.page_shift : 0x7fffffffll};
+    Finder f{lens, p.n_seqs, p.tile_tokens, p.causal, kPaged ? (long long)p.table_width << p.page_shift : 0x7fffffffll};
     f.init();
     auto publish = [&](int i, Unit& u) -> bool {
       // units come longest first: rounds go up and down the CTAs in turn, so
@@ -597,8 +526,8 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
         u.kvh = unit % p.n_kv;
         u.q_begin = max(0, min(p.cu[seq], p.total_q));
         u.kv_len = f.kv_len(s);
-        u.t0 = level * NT * p.tile_tokens;
-        u.n_tok = min(NT * p.tile_tokens, s.x - u.t0);
+        u.t0 = level * p.tile_tokens;
+        u.n_tok = min(p.tile_tokens, s.x - u.t0);
         u.first = s.y + u.t0;
         u.lim_min = keys_seen(u, p.causal, 0);
         const int blocks = (keys_seen(u, p.causal, u.n_tok - 1) + BKV - 1) / BKV;
@@ -626,8 +555,8 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
       // Every block passes here, so that the warp follows each phase of the
       // ring; those before jb pass untouched.
       for (int j = 0; j < u.nkv; ++j, ++vn) {
-        const uint32_t s = vn % VRING;
-        const bool good = wait_bar(&v_full[s], (vn / VRING) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER);
+        const uint32_t s = vn % RING;
+        const bool good = wait_bar(&v_full[s], (vn / RING) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER);
         ok = __all_sync(0xffffffffu, good);
         if (!ok) break;
         if (j >= u.jb) {
@@ -665,29 +594,25 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
       if (ok && after.nkv >= 0) ok = publish(i + 2, after);
     }
   } else {
-    const int g = warp >> 2;  // tile
-    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t o_addr = tmem + lane_base + C::O_COL + g * 128;
-    const int row = (warp & 3) * 32 + lane;              // of the tile
-    const int tok = g * p.tile_tokens + row / p.group;   // of the unit
+    const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+    const uint32_t o_addr = tmem + lane_base + O_COL;
+    const int row = warp * 32 + lane;
+    const int tok = row / p.group;
     const unsigned long long sc2 = pack2(p.scale_log2, p.scale_log2);
-    uint32_t gn = 0;  // blocks of this tile so far
+    uint32_t gn = 0;  // blocks so far
     Unit u;
     bool ok = true;
     for (int i = 0; ok; ++i) {
       if (!__all_sync(0xffffffffu, next_unit(i, u))) break;
       const bool valid = tok < u.n_tok && row < p.tile_tokens * p.group;
       const bool any = __any_sync(0xffffffffu, valid);
-      const bool idle = g > 0 && u.n_tok <= p.tile_tokens;  // this unit has no tile g
-      const int head = u.kvh * p.group + row % p.group;
-      // The unit's rows in order: a tile has tile_tokens * group of them.
-      const int urow = g * p.tile_tokens * p.group + row;
+      const int head = u.kvh * p.group + row - tok * p.group;
       const size_t q_row = (size_t)(u.q_begin + u.t0 + tok);
       uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + q_row * p.out_token + (size_t)head * p.out_head;
       const size_t part = ((size_t)split * p.total_q + q_row) * p.n_heads + head;
       if (u.nkv == 0) {  // no key: zeros (or a part of weight zero)
         if (p.in_cluster) {
-          if (valid) stats[urow] = make_float2(-INFINITY, 0.f);
+          if (valid) stats[row] = make_float2(-INFINITY, 0.f);
         } else if (valid && p.splits > 1) {
           p.part_lse[part] = -INFINITY;
         } else if (valid) {
@@ -697,20 +622,16 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
         if (lane == 0) bar_arrive(&unit_empty[i & 1]);
         continue;
       }
-      if (idle) {
-        if (lane == 0) bar_arrive(&unit_empty[i & 1]);
-        continue;
-      }
       const int lim = valid ? keys_seen(u, p.causal, tok) : 0;
       float m = -INFINITY, l = 0.0f;
       for (int j = 0; j < u.nkv; ++j, ++gn) {
         const uint32_t buf = gn & 1;
-        const uint32_t s_addr = tmem + lane_base + g * 128 + buf * BKV;
-        bool good = wait_fast(&s_full[g * 2 + buf], (gn >> 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_SOFTMAX);
+        const uint32_t s_addr = tmem + lane_base + buf * BKV;
+        bool good = wait_fast(&s_full[buf], (gn >> 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_SOFTMAX);
         ok = __all_sync(0xffffffffu, good);
         if (!ok) break;
         if (!any) {  // no row here: P of these rows is never read out
-          if (lane == 0) bar_arrive(&p_ready[g * 2 + buf]);
+          if (lane == 0) bar_arrive(&p_ready[buf]);
           continue;
         }
         tc_fence_after();
@@ -734,13 +655,13 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
         }
         float m8[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) m8[k] = max2n(s[k], s[8 + k]);
+        for (int k = 0; k < 8; ++k) m8[k] = fmaxf(s[k], s[8 + k]);
 #pragma unroll
         for (int c = 16; c < BKV; c += 16) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) m8[k] = max3n(m8[k], s[c + k], s[c + 8 + k]);
+          for (int k = 0; k < 8; ++k) m8[k] = max3f(m8[k], s[c + k], s[c + 8 + k]);
         }
-        const float mx = max3n(max3n(m8[0], m8[1], m8[2]), max3n(m8[3], m8[4], m8[5]), max2n(m8[6], m8[7])) *
+        const float mx = max3f(max3f(m8[0], m8[1], m8[2]), max3f(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7])) *
                          p.scale_log2;
         float alpha = 1.0f;
         if (mx > m + kRescaleThreshold) {
@@ -748,7 +669,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
           m = mx;
         }
         if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-          good = wait_bar(&pv_done[g * 2 + (buf ^ 1)], ((gn - 1) >> 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_SOFTMAX);
+          good = wait_bar(&pv_done[buf ^ 1], ((gn - 1) >> 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_SOFTMAX);
           ok = __all_sync(0xffffffffu, good);
           if (!ok) break;
           tc_fence_after();
@@ -765,44 +686,31 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
         const float mref = m == -INFINITY ? 0.0f : m;  // no key seen yet: every p is 2^-inf = 0
         const unsigned long long nm2 = pack2(-mref, -mref);
         unsigned long long sum2[4] = {0ull, 0ull, 0ull, 0ull};
-        // P and its row sum (before the rounding); bit k of poly: pair k of 16
-        // takes the polynomial.
-        auto exps = [&](auto poly) {
+        // P, and its row sum before the rounding
 #pragma unroll
-          for (int ch = 0; ch < BKV / 32; ++ch) {
-            uint32_t pk[16];
+        for (int ch = 0; ch < BKV / 32; ++ch) {
+          uint32_t pk[16];
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              float a, b;
-              const unsigned long long x2 = fma2(pack2(s[ch * 32 + 2 * k], s[ch * 32 + 2 * k + 1]), sc2, nm2);
-              if ((decltype(poly)::value >> k) & 1) {
-                ex2_poly2(x2, a, b);
-              } else {
-                unpack2(x2, a, b);
-                a = ex2(a);
-                b = ex2(b);
-              }
-              sum2[k & 3] = add2(sum2[k & 3], pack2(a, b));
-              pk[k] = cvt2<kBF16>(a, b);
-            }
-            tmem_st16(s_addr + ch * 16, pk);
+          for (int k = 0; k < 16; ++k) {
+            float a, b;
+            unpack2(fma2(pack2(s[ch * 32 + 2 * k], s[ch * 32 + 2 * k + 1]), sc2, nm2), a, b);
+            a = ex2(a);
+            b = ex2(b);
+            sum2[k & 3] = add2(sum2[k & 3], pack2(a, b));
+            pk[k] = cvt2<kBF16>(a, b);
           }
-        };
-        if (C::kPolyPairs == 0 || j >= u.jb || __any_sync(0xffffffffu, m == -INFINITY))
-          exps(std::integral_constant<unsigned, 0u>{});
-        else
-          exps(std::integral_constant<unsigned, C::kPolyPairs>{});
+          tmem_st16(s_addr + ch * 16, pk);
+        }
         float a0, a1;
         unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), a0, a1);
         l = l * alpha + (a0 + a1);
-        if (!(mx < INFINITY)) l = __int_as_float(0x7fc00000);  // a NaN or +inf score: the row is NaN
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) bar_arrive(&p_ready[g * 2 + buf]);
+        if (lane == 0) bar_arrive(&p_ready[buf]);
       }
       if (!ok) break;
-      const bool good = !any || wait_bar(&pv_done[g * 2 + ((gn - 1) & 1)], ((gn - 1) >> 1) & 1, abort_flag, p.err,
+      const bool good = !any || wait_bar(&pv_done[(gn - 1) & 1], ((gn - 1) >> 1) & 1, abort_flag, p.err,
                                          DEV_ERR_TIMEOUT_SOFTMAX);
       ok = __all_sync(0xffffffffu, good);
       if (!ok) break;
@@ -812,8 +720,8 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
         const bool repair = nonfinite[i & 1] != 0 && valid;
         // keys that only some rows see, within this CTA's range
         const int from = max(u.lim_min, (u.j0 + u.jb) * BKV), to = min(lim, (u.j0 + u.nkv) * BKV);
-        if (p.in_cluster && valid) stats[urow] = make_float2(l == 0.0f ? -INFINITY : m + log2f(l), 0.f);
-        constexpr int EC = C::EC, PIECES = EC / 8;  // 16-byte pieces of a staged row
+        if (p.in_cluster && valid) stats[row] = make_float2(l == 0.0f ? -INFINITY : m + log2f(l), 0.f);
+        constexpr int PIECES = EC / 8;  // 16-byte pieces of a staged row
         // where the rows that this lane helps to write begin (null: no row)
         uint16_t* rows_at[PIECES];
 #pragma unroll
@@ -849,8 +757,8 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
           if (p.splits > 1) {
             // global memory, or this CTA's tiles (every product of the unit is
             // done); there, 16-byte pieces are permuted within a row against conflicts
-            float* po = p.in_cluster ? reinterpret_cast<float*>(qs) + urow * HD : p.part_o + part * HD;
-            const int x = p.in_cluster ? urow & 7 : 0;
+            float* po = p.in_cluster ? reinterpret_cast<float*>(qs) + row * HD : p.part_o + part * HD;
+            const int x = p.in_cluster ? row & 7 : 0;
 #pragma unroll
             for (int k = 0; k < EC / 4; ++k)
               if (valid)
@@ -862,7 +770,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
             // 32 lines per instruction, and the SM takes about 3 clocks for
             // each); pieces are permuted against bank conflicts.
             auto place = [](int row, int piece) {
-              return row * PIECES + (piece ^ (PIECES == 8 ? row & 7 : (row >> 1) & 3));
+              return row * PIECES + (piece ^ ((row >> 1) & 3));
             };
             uint4* st = stage + warp * (32 * PIECES);
 #pragma unroll
@@ -884,7 +792,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
       }
       __syncwarp();
       if (lane == 0) {
-        bar_arrive(&o_empty[g]);
+        bar_arrive(o_empty);
         bar_arrive(&unit_empty[i & 1]);
       }
     }
@@ -901,7 +809,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
       const int d8 = (int)(threadIdx.x % (HD / 8)) * 2;  // 16-byte pieces d8, d8 + 1
       const uint32_t st0 = smem_u32(stats), o0 = smem_u32(qs);
       for (int r = split + p.splits * (int)(threadIdx.x / (HD / 8)); r < rows;
-           r += p.splits * (C::NUM_THREADS / (HD / 8))) {
+           r += p.splits * (NUM_THREADS / (HD / 8))) {
         float lse[kMaxCluster];
         float top = -INFINITY;
 #pragma unroll
@@ -940,10 +848,10 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::NUM_THREADS, 3 - NT)
     }
     cluster_sync_all();  // no CTA ends while another reads its shared memory
   }
-  if (warp == C::WARP_MMA) {
+  if (warp == WARP_MMA) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tmem, C::TMEM_COLS);
+    tmem_dealloc(tmem, TMEM_COLS);
   }
 }
 
@@ -1069,7 +977,7 @@ int encode(CUtensorMap* map, void* base, bool bf16, int rank, const long long* d
 // one GPC); 0 if the query fails.  The occupancy query counts one CTA per SM
 // for a kernel that allocates TMEM; two of these fit (256 of the 512 columns,
 // half the shared memory and registers each) and do run.
-template <int HD, bool kBF16, bool kPaged, int NT>
+template <int HD, bool kBF16, bool kPaged>
 int cluster_slots(int size) {
   static int slots[64][kMaxCluster + 1];
   static bool known[64][kMaxCluster + 1];
@@ -1078,8 +986,8 @@ int cluster_slots(int size) {
   const int d = device_slot();
   if (known[d][size]) return slots[d][size];
   known[d][size] = true;
-  auto kern = text_attention_kernel<HD, kBF16, kPaged, NT>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD, NT>::SMEM_BYTES) == cudaSuccess &&
+  auto kern = text_attention_kernel<HD, kBF16, kPaged>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD>::SMEM_BYTES) == cudaSuccess &&
       cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) ==
           cudaSuccess &&
       cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) {
@@ -1090,23 +998,23 @@ int cluster_slots(int size) {
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3((unsigned)size);
-    cfg.blockDim = dim3(Cfg<HD, NT>::NUM_THREADS);
-    cfg.dynamicSmemBytes = Cfg<HD, NT>::SMEM_BYTES;
+    cfg.blockDim = dim3(NUM_THREADS);
+    cfg.dynamicSmemBytes = Cfg<HD>::SMEM_BYTES;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int c = 0;
-    if (cudaOccupancyMaxActiveClusters(&c, kern, &cfg) == cudaSuccess) slots[d][size] = (3 - NT) * c;
+    if (cudaOccupancyMaxActiveClusters(&c, kern, &cfg) == cudaSuccess) slots[d][size] = 2 * c;
   }
   cudaGetLastError();
   return slots[d][size];
 }
 
-template <int HD, bool kBF16, bool kPaged, int NT>
+template <int HD, bool kBF16, bool kPaged>
 int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, Params p, long long units,
            int max_ctx, cudaStream_t st) {
-  auto kern = text_attention_kernel<HD, kBF16, kPaged, NT>;
+  auto kern = text_attention_kernel<HD, kBF16, kPaged>;
   // CTA slots; the query also prepares the kernel for its shared memory
-  const long long slots = cluster_slots<HD, kBF16, kPaged, NT>(1);
+  const long long slots = cluster_slots<HD, kBF16, kPaged>(1);
   if (slots < 1) return fail(-3, "text attention: the kernel cannot be scheduled on this device");
   // Key split: where the units leave CTA slots empty, each unit's keys are cut
   // into ranges.  Up to kMaxCluster of them are one cluster, as many as fit
@@ -1120,7 +1028,7 @@ int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, 
   want = std::min<long long>(want, kMaxSplits);
   p.splits = (int)want;
   if (p.splits > 1 && p.splits <= kMaxCluster) {
-    while (p.splits > 1 && cluster_slots<HD, kBF16, kPaged, NT>(p.splits) < units) --p.splits;
+    while (p.splits > 1 && cluster_slots<HD, kBF16, kPaged>(p.splits) < units) --p.splits;
     // Clusters pack badly where the wanted split is odd (32 units in 9 ranges:
     // 6 fit, 196 us; 9 ranges through global memory, 168 us).
     p.in_cluster = 5 * p.splits >= 4 * want && p.splits > 1;
@@ -1140,8 +1048,8 @@ int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, 
   const double keys = kPaged ? (double)p.n_seqs * max_ctx : (double)p.total_q;
   ProfScope prof(kPaged ? "paged_attention" : "prompt_attention", 0.0,
                  2.0 * HD * (2.0 * p.total_q * p.n_heads + 2.0 * keys * p.n_kv), st);
-  int rc = launch_after("text_attention_kernel launch", kern, dim3((unsigned)ctas), dim3(Cfg<HD, NT>::NUM_THREADS),
-                        Cfg<HD, NT>::SMEM_BYTES, p.in_cluster ? p.splits : 1, st, qm, km, vm, p);
+  int rc = launch_after("text_attention_kernel launch", kern, dim3((unsigned)ctas), dim3(NUM_THREADS),
+                        Cfg<HD>::SMEM_BYTES, p.in_cluster ? p.splits : 1, st, qm, km, vm, p);
   if (rc == 0 && part) {
     rc = launch_after("text_combine_kernel launch", text_combine_kernel<HD, kBF16>,
                       dim3((unsigned)(p.total_q * p.n_heads)), dim3(256), 0, 1, st, p.part_o, p.part_lse, p.splits,
@@ -1151,30 +1059,14 @@ int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, 
   return rc;
 }
 
-template <int HD, bool kBF16, bool kPaged>
-int launch_form(const TextAttention& a, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm,
-                const Params& p, cudaStream_t st) {
-  // Tiles: sum_i ceil(q_len_i / T) <= (total + n * (T - 1)) / T; CTAs past the
-  // real number of tiles end at once.
-  const long long seqs = std::min(p.n_seqs, a.total_q);
-  auto units = [&](long long T) { return (a.total_q + seqs * (T - 1)) / T * a.n_kv; };
-  const long long u1 = units(p.tile_tokens), u2 = units(2 * p.tile_tokens);
-  if (u1 > 0x7fffffffll / 64) return fail(-2, "text attention: too many tiles in one call");
-  // Two tiles per CTA where they are enough to fill the GPU and the sequences
-  // fill them: more than one tile of rows each on average.
-  if (u2 >= num_sms() && a.total_q > seqs * p.tile_tokens)
-    return launch<HD, kBF16, kPaged, 2>(qm, km, vm, p, u2, a.max_ctx, st);
-  return launch<HD, kBF16, kPaged, 1>(qm, km, vm, p, u1, a.max_ctx, st);
-}
-
 template <bool kPaged>
 int dispatch(const TextAttention& a, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm,
-             const Params& p, cudaStream_t st) {
+             const Params& p, long long units, cudaStream_t st) {
   if (a.head_dim == 128)
-    return a.bf16 ? launch_form<128, true, kPaged>(a, qm, km, vm, p, st)
-                  : launch_form<128, false, kPaged>(a, qm, km, vm, p, st);
-  return a.bf16 ? launch_form<64, true, kPaged>(a, qm, km, vm, p, st)
-                : launch_form<64, false, kPaged>(a, qm, km, vm, p, st);
+    return a.bf16 ? launch<128, true, kPaged>(qm, km, vm, p, units, a.max_ctx, st)
+                  : launch<128, false, kPaged>(qm, km, vm, p, units, a.max_ctx, st);
+  return a.bf16 ? launch<64, true, kPaged>(qm, km, vm, p, units, a.max_ctx, st)
+                : launch<64, false, kPaged>(qm, km, vm, p, units, a.max_ctx, st);
 }
 
 }  // namespace text
@@ -1235,7 +1127,12 @@ int launch_text_attention(const TextAttention& a, cudaStream_t st) {
     p.cu = a.cu + s0;
     p.ctx = paged ? a.ctx + s0 : nullptr;
     p.table = paged ? a.table + s0 * a.table_ld : nullptr;
-    const int rc = paged ? dispatch<true>(a, qm, km, vm, p, st) : dispatch<false>(a, qm, km, vm, p, st);
+    // Tiles: sum_i ceil(q_len_i / T) <= (total + n * (T - 1)) / T; CTAs past
+    // the real number of tiles end at once.
+    const long long T = p.tile_tokens, seqs = std::min(p.n_seqs, a.total_q);
+    const long long units = (a.total_q + seqs * (T - 1)) / T * a.n_kv;
+    if (units > 0x7fffffffll / kMaxSplits) return fail(-2, "text attention: too many tiles in one call");
+    const int rc = paged ? dispatch<true>(a, qm, km, vm, p, units, st) : dispatch<false>(a, qm, km, vm, p, units, st);
     if (rc) return rc;
   }
   return 0;
