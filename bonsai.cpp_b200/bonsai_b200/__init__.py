@@ -382,8 +382,8 @@ def _text_dtype(dtype) -> int:
 
 
 def _text_ints(dev, name, t):
-    if t.dtype is not _text_torch.int32 or t.get_device() != dev or t.stride(-1) != 1 and t.shape[-1] > 1:
-        raise BonsaiError(f"{name} must be int32 with unit stride on the current device")
+    if t.dtype is not _text_torch.int32 or t.get_device() != dev or not t.is_contiguous():
+        raise BonsaiError(f"{name} must be contiguous int32 on the current device")
     return t.data_ptr()
 
 
@@ -432,12 +432,14 @@ def prompt_attention(q, k, v, cu_seqlens, out, scale=None, causal=True, stream=N
 
 def _table_args(dev, page_table, cu_q, ctx_lens):
     """(page_table, row stride, width, cu_q, ctx_lens, sequences) as the C calls take them."""
-    n = ctx_lens.shape[0]
-    if cu_q.shape[0] != n + 1 or page_table.dim() != 2 or page_table.shape[0] != n:
-        raise BonsaiError(f"page_table {tuple(page_table.shape)}, cu_q {tuple(cu_q.shape)} and ctx_lens [{n}] do not match")
-    width = page_table.shape[1]
-    return (_text_ints(dev, "page_table", page_table), page_table.stride(0) if n > 1 else width, width,
-            _text_ints(dev, "cu_q", cu_q), _text_ints(dev, "ctx_lens", ctx_lens), n)
+    shape, s = page_table.shape, page_table.stride()
+    n = ctx_lens.numel()
+    if len(shape) != 2 or shape[0] != n or cu_q.numel() != n + 1:
+        raise BonsaiError(f"page_table {tuple(shape)}, cu_q {tuple(cu_q.shape)} and ctx_lens [{n}] do not match")
+    if page_table.dtype is not _text_torch.int32 or page_table.get_device() != dev or s[1] != 1 and shape[1] > 1:
+        raise BonsaiError("page_table must be int32 with unit stride along a row on the current device")
+    return (page_table.data_ptr(), s[0] if n > 1 else shape[1], shape[1], _text_ints(dev, "cu_q", cu_q),
+            _text_ints(dev, "ctx_lens", ctx_lens), n)
 
 
 def paged_append(k, v, k_cache, v_cache, page_table, cu_q, ctx_lens, stream=None) -> None:
