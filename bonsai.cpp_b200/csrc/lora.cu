@@ -222,7 +222,6 @@ __global__ void __launch_bounds__(tile::NUM_THREADS)
   const int csize = (int)cluster.num_blocks(), crank = (int)cluster.block_rank();
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   griddep_wait();
-  griddep_launch();
   if (warp == 0) {
     int req = -1, tl = 0;
     if (!find_request(p.cu, p.n_reqs, p.tokens, BM, (int)blockIdx.x / csize, req, tl)) req = -1;
@@ -260,6 +259,7 @@ __global__ void __launch_bounds__(tile::NUM_THREADS)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  griddep_launch();  // after the TMEM allocation: a dependent's could block it, and waits for this grid
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0) {

@@ -345,14 +345,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
     tmem_relinquish();
   }
   griddep_wait();
-  griddep_launch();
   for (int i = threadIdx.x; i < p.n_seqs; i += NUM_THREADS) {
     const int a = max(0, min(p.cu[i], p.total_q)), b = max(a, min(p.cu[i + 1], p.total_q));
-    lens[i] = make_int2(b - a, kPaged ? p.ctx[i] - (b - a) : 0);
+    lens[i] = make_int2(b - a, kPaged ? max(0, p.ctx[i]) - (b - a) : 0);
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  griddep_launch();  // after the TMEM allocation: a dependent's could block it, and waits for this grid
   const uint32_t tmem = *tmem_slot;
 
   // Unit i of this CTA, as every role gets it.

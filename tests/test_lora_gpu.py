@@ -243,3 +243,29 @@ def test_lora_refusals(gpu):
         p.lora.set(0, d.float(), u, 1.0)
     with pytest.raises(bb.BonsaiError):
         p.lora.set(0, d, u[:63].contiguous(), 1.0)
+
+
+@pytest.mark.parametrize("per", [1, 20])
+def test_lora_more_tiles_than_sms(gpu, per):
+    """Both forms with several tiles per CTA."""
+    n = 400 // per * (1 if per == 1 else 4)
+    p = Problem(gpu, 4096, 128, [16, 5, 0, 33])
+    cu = [i * per for i in range(n + 1)]
+    check_f32(p, p.x(cu[-1]), cu, [i % 5 - 1 for i in range(n)])
+
+
+@pytest.mark.parametrize("lens", [[1, 1, 1], [100, 30]], ids=str)
+def test_lora_in_a_graph(gpu, lens):
+    p = Problem(gpu, 512, 1024, [16, 64])
+    cu, slots = np.cumsum([0] + lens).tolist(), [1, 0, 1][:len(lens)]
+    x, c, s = p.x(cu[-1]), ints(cu), ints(slots)
+    want = p.run(x, cu, slots, gpu.BONSAI_EPI_F32, torch.empty(cu[-1], 512, device="cuda"))
+    out = torch.zeros_like(want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gpu.b1_gemm_lora(x, p.w, gpu.BONSAI_EPI_F32, out, p.lora, c, s)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)

@@ -379,3 +379,28 @@ def test_prompt_more_units_than_slots(gpu):
     q, k, v = (randn(i, sum(lens), h, 64) for i, h in enumerate((8, 8, 8)))
     run_prompt(gpu, q, k, v, cumulated(lens))
     run_prompt(gpu, q, k, v, cumulated(lens), causal=False)
+
+
+def test_paged_negative_lengths_see_nothing(gpu):
+    kc, vc, table = make_cache(22, [40, 40], 16, 2, 128, f16)
+    q = randn(23, 4, 8, 128)
+    out = torch.full_like(q, 7.0)
+    gpu.paged_attention(q, kc, vc, table, ints([0, 2, 4]), ints([-2147483648, 40]), 40, out)
+    assert (out[:2] == 0).all()
+    check(out[2:], *ref_rows(q[2:], gather(kc, table[1], 40, 16), gather(vc, table[1], 40, 16), 38, 128 ** -0.5))
+
+
+def test_wide_split_in_a_graph(gpu):
+    """A split that goes through scratch: its allocation belongs to the graph."""
+    kc, vc, table = make_cache(24, [30000], 64, 1, 128, f16)
+    q, cu, ctx = randn(25, 1, 8, 128), ints([0, 1]), ints([30000])
+    want = run_paged(gpu, q, kc, vc, table, [0, 1], [30000], 64)
+    out = torch.zeros_like(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gpu.paged_attention(q, kc, vc, table, cu, ctx, 30000, out)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
