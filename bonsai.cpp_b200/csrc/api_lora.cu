@@ -59,23 +59,25 @@ int bonsai_lora_set(bonsai_lora_t h, int slot, const uint16_t* down, const uint1
   if (dev != s.device) return fail(BONSAI_ERR_ARG, "lora_set: the adapters live on device " + std::to_string(s.device));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const LoraSlot info{rank, scale};
-  if (rank > 0) {
-    __half* d = s.down + (size_t)slot * s.r_pad * s.k_in;
-    const size_t d_bytes = (size_t)rank * s.k_in * sizeof(__half), u_bytes = (size_t)rank * s.n_rows * sizeof(__half);
-    e = cudaMemsetAsync(d, 0, (size_t)s.r_pad * s.k_in * sizeof(__half), st);
-    if (e == cudaSuccess) e = cudaMemcpyAsync(d, down, d_bytes, cudaMemcpyDefault, st);
-    if (e != cudaSuccess) return cuda_status(e, "lora_set: copy");
-    void* staged = nullptr;
-    int rc = scratch_alloc(&staged, u_bytes, "lora_set", st);
-    if (rc) return rc;
-    e = cudaMemcpyAsync(staged, up, u_bytes, cudaMemcpyDefault, st);
-    rc = e == cudaSuccess ? launch_lora_retile(static_cast<const __half*>(staged), rank, s, slot, st)
-                          : cuda_status(e, "lora_set: copy");
-    scratch_free(staged, st);
-    if (rc) return rc;
-  }
-  if (e == cudaSuccess) e = cudaMemcpyAsync(s.info + slot, &info, sizeof(info), cudaMemcpyDefault, st);
-  return cuda_status(e, "lora_set: copy");
+  if (rank == 0) return launch_lora_retile(nullptr, info, s, slot, st);
+  __half* d = s.down + (size_t)slot * s.r_pad * s.k_in;
+  const size_t row = (size_t)s.k_in * sizeof(__half), u_bytes = (size_t)rank * s.n_rows * sizeof(__half);
+  e = cudaMemcpyAsync(d, down, rank * row, cudaMemcpyDefault, st);
+  if (e == cudaSuccess && rank < s.r_pad)
+    e = cudaMemsetAsync(d + (size_t)rank * s.k_in, 0, (s.r_pad - rank) * row, st);
+  if (e != cudaSuccess) return cuda_status(e, "lora_set: copy");
+  cudaPointerAttributes at{};
+  if (cudaPointerGetAttributes(&at, up) == cudaSuccess && at.type == cudaMemoryTypeDevice && at.device == dev)
+    return launch_lora_retile(reinterpret_cast<const __half*>(up), info, s, slot, st);
+  cudaGetLastError();
+  void* staged = nullptr;
+  int rc = scratch_alloc(&staged, u_bytes, "lora_set", st);
+  if (rc) return rc;
+  e = cudaMemcpyAsync(staged, up, u_bytes, cudaMemcpyDefault, st);
+  rc = e == cudaSuccess ? launch_lora_retile(static_cast<const __half*>(staged), info, s, slot, st)
+                        : cuda_status(e, "lora_set: copy");
+  scratch_free(staged, st);
+  return rc;
 }
 
 int bonsai_lora_free(bonsai_lora_t h) {

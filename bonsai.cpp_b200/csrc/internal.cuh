@@ -183,8 +183,8 @@ struct LoraDevice {
   __half* up = nullptr;
   LoraSlot* info = nullptr;
 };
-// B [out][rank] (device memory) into the chunks of a slot.
-int launch_lora_retile(const __half* up, int rank, const LoraDevice& set, int slot, cudaStream_t st);
+// B [out][rank] (device memory) into the chunks of a slot, and its info.
+int launch_lora_retile(const __half* up, const LoraSlot& info, const LoraDevice& set, int slot, cudaStream_t st);
 // cu: device [n_reqs + 1] first token of each request; slots: device
 // [n_reqs] its adapter (outside [0, n_slots): none).
 int launch_b1_gemm_lora(const __half* x, long long ldx, int tokens, const B1Weight& w, const EpiSeg& seg,

@@ -343,11 +343,14 @@ __global__ void __launch_bounds__(tile::NUM_THREADS)
   }
 }
 
-// B [out][rank] into the chunks of a slot (LoraDevice::up).  Rows
-// [swiglu_from, out) go to alternating device rows, gate then value, as those
-// of the B1_0 weight.
-__global__ void lora_retile_kernel(const __half* __restrict__ src, int rank, int n_rows, int n_ftiles, int r_pad,
-                                   int swiglu_from, __half* __restrict__ dst) {
+// B [out][rank] into the chunks of a slot (LoraDevice::up), and the slot's rank
+// and scale.  Rows [swiglu_from, out) go to alternating device rows, gate then
+// value, as those of the B1_0 weight.
+__global__ void lora_retile_kernel(const __half* __restrict__ src, LoraSlot info, int n_rows, int n_ftiles, int r_pad,
+                                   int swiglu_from, __half* __restrict__ dst, LoraSlot* slot) {
+  const int rank = info.rank;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *slot = info;
+  if (rank == 0) return;
   const long long total = (long long)n_ftiles * 128 * r_pad;
   for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total;
        i += (long long)gridDim.x * blockDim.x) {
@@ -464,10 +467,11 @@ int shrink_by_rank(const ShrinkParams& p, int max_rank, cudaStream_t st) {
 
 }  // namespace lora
 
-int launch_lora_retile(const __half* up, int rank, const LoraDevice& set, int slot, cudaStream_t st) {
+int launch_lora_retile(const __half* up, const LoraSlot& info, const LoraDevice& set, int slot, cudaStream_t st) {
   const size_t n = (size_t)set.n_ftiles * 128 * set.r_pad;
-  lora::lora_retile_kernel<<<(unsigned)std::min<size_t>((n + 255) / 256, 148 * 16), 256, 0, st>>>(
-      up, rank, set.n_rows, set.n_ftiles, set.r_pad, set.swiglu_from, set.up + (size_t)slot * n);
+  const unsigned blocks = info.rank == 0 ? 1u : (unsigned)std::min<size_t>((n + 255) / 256, 148 * 16);
+  lora::lora_retile_kernel<<<blocks, 256, 0, st>>>(up, info, set.n_rows, set.n_ftiles, set.r_pad, set.swiglu_from,
+                                                   set.up + (size_t)slot * n, set.info + slot);
   return launch_status("lora_retile_kernel launch");
 }
 

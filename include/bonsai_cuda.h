@@ -185,8 +185,8 @@ int bonsai_lora_create(int out_dim, int in_dim, int max_rank, int n_slots, int s
 /* Put an adapter into a slot: down f16 [rank][in_dim], up f16
  * [out_dim][rank] (host or device memory), y += scale * up (down x).
  * rank 0 empties the slot (down, up may be NULL).  Ordered on the stream, as
- * its copies are: pinned host memory must keep its contents until they are
- * done. */
+ * its copies are: device and pinned host memory must keep its contents until
+ * they are done. */
 int bonsai_lora_set(bonsai_lora_t set, int slot, const uint16_t* down, const uint16_t* up, int rank,
                     float scale, void* stream);
 int bonsai_lora_free(bonsai_lora_t set);
