@@ -408,7 +408,7 @@ __global__ void lora_plan_kernel(const int* __restrict__ cu, const int* __restri
         groups[(size_t)tile * max_groups + at + j] =
             make_int4(j < n16 ? slot : slot | (1 << 30), (j < n16 ? j : j - n16) * 16, a, b);
     base += __shfl_sync(0xffffffffu, incl, 31);
-    // past the tile once a request of this round begins at or after its end
+    // past the tile once one of these 32 requests begins at or after its end
     if (__any_sync(0xffffffffu, i < n_reqs && cu[i] >= t1)) break;
   }
   if (lane == 0) group_count[tile] = min(base, max_groups);
