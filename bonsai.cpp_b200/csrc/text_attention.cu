@@ -41,12 +41,12 @@
 // P(j) (16-bit pairs) overwrites the first 32 columns of its S.
 //
 // Bounds and measurements (B200, 32 / 8 heads of 128, bf16 unless noted; a call
-// among others): single tokens by HBM, 5.0 TB/s for 64 sequences of 130 to 4000
-// keys (104 us) and 5.7 TB/s for 4 of 30000 to 65536 in f16 (149 us); long
+// among others): single tokens by HBM, 5.1 TB/s for 64 sequences of 130 to 4000
+// keys (102 us) and 5.7 TB/s for 4 of 30000 to 65536 in f16 (149 us); long
 // prompts by the 64-key Q K^T, whose 192 bytes of shared memory per clock are
 // more than an SM reads, and by the power limit: 10007 tokens 843 us, 973
 // TFLOP/s; batches of short prompts by the start and end of each unit: 48 of 7
-// to 512 tokens 111 us.  128 rows per CTA, two CTAs per SM, because 256 rows
+// to 512 tokens 100 us.  128 rows per CTA, two CTAs per SM, because 256 rows
 // per CTA (half the reads of K and V) measured the same on long prompts (778
 // to 838 us against 760 to 804) and 10 to 20 % slower on batches of short
 // ones: 8 x 150 tokens 19.7 against 16.5 us, 48 x 80 40.5 against 33.9.
@@ -74,7 +74,7 @@ constexpr int O_COL = 128;
 constexpr int BAR_BYTES = 512;
 constexpr int EC = 32;    // columns that the epilogue takes at a time through a warp's staging rows
 constexpr float kRescaleThreshold = 8.0f;
-constexpr int kMaxSeqs = 512;     // sequences of one launch (their lengths are kept in shared memory)
+constexpr int kMaxSeqs = 256;     // sequences of one launch (16 bytes each in shared memory)
 constexpr int kMaxCluster = 16;   // CTAs that split a unit's keys and merge in shared memory
 
 template <int HD>
@@ -87,7 +87,7 @@ struct Cfg {
   // Q and the rings; once a unit's products are done they can hold its O (f32)
   static constexpr int TILES_BYTES = Q_BYTES + 2 * RING * KV_BYTES;
   static_assert(TILES_BYTES >= BQ * HD * 4, "O does not fit the tiles");
-  static constexpr int SMEM_BYTES = 1024 + TILES_BYTES + BAR_BYTES + BQ * 8 + kMaxSeqs * 8 + 4 * 32 * EC * 2;
+  static constexpr int SMEM_BYTES = 1024 + TILES_BYTES + BAR_BYTES + BQ * 8 + kMaxSeqs * 16 + 4 * 32 * EC * 2;
 };
 // Two CTAs per SM (228 KB, 1 KB of it reserved for each).
 static_assert(2 * (Cfg<128>::SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs per SM");
@@ -196,73 +196,96 @@ __device__ __forceinline__ int keys_seen(const Unit& u, int causal, int tok) {
   return causal ? max(0, min(u.kv_len, u.first + tok + 1)) : u.kv_len;
 }
 
+// What the search for units keeps of a sequence (shared memory).
+struct Seq {
+  int q_len, before;  // query tokens, keys before them
+  int kv_len, tiles;  // keys, query tiles
+};
+static_assert(sizeof(Seq) == 16, "read as one int4");
+
 // The order of a launch's query tiles: by their key blocks, most first (ties:
 // by sequence, then latest tokens first), so that the long ones do not end up
-// alone at the end.  One warp; lens[i] = {query tokens, keys before them} of
-// sequence i.
+// alone at the end.  One warp, for every unit again, so what it does per
+// sequence is kept small: lengths and tile counts are computed once per launch
+// (divided out at every look instead, 256 single tokens over 100-900 keys took
+// 166 us, not 117, and 250 prompts of 40 tokens 78, not 66), and a launch takes
+// at most 256 sequences (with 512, before that, 512 single tokens took 377 us
+// against 328, 500 prompts of 40 tokens 177 against 152).
 struct Finder {
-  const int2* lens;
+  const Seq* seqs;
   int n, tile_tokens, causal;
-  long long room;  // keys that a sequence's pages can hold
   int c, at_c, above_c;  // tiles of >= c blocks, of > c blocks
 
-  __device__ int kv_len(int2 s) const { return (int)max(0ll, min((long long)s.x + s.y, room)); }
+  __device__ Seq seq(int i) const {
+    Seq s;
+    *reinterpret_cast<int4*>(&s) = *reinterpret_cast<const int4*>(seqs + i);
+    return s;
+  }
   // Tiles of a sequence with at least `blocks` key blocks: the last ones.
-  __device__ int tiles(int2 s, int blocks) const {
-    const int all = (s.x + tile_tokens - 1) / tile_tokens;
-    if (blocks <= 0 || all == 0) return all;
-    const int keys = (blocks - 1) * BKV + 1;
-    if (kv_len(s) < keys) return 0;
-    if (!causal) return all;
-    const int toks = keys - s.y;  // tokens up to the first that sees as many
-    return toks <= tile_tokens ? all : all - ((toks + tile_tokens - 1) / tile_tokens - 1);
+  __device__ int tiles(const Seq& s, int blocks) const {
+    const int keys = (blocks - 1) * BKV + 1;  // blocks <= 0: any tile
+    if (s.kv_len < keys) return blocks > 0 ? 0 : s.tiles;
+    if (!causal || s.tiles <= 1 || blocks <= 0) return s.tiles;
+    const int toks = keys - s.before;  // tokens up to the first that sees as many
+    return toks <= tile_tokens ? s.tiles : s.tiles - ((toks + tile_tokens - 1) / tile_tokens - 1);
   }
   __device__ int total(int blocks) const {
     int v = 0;
-    for (int i = (int)lane_id(); i < n; i += 32) v += tiles(lens[i], blocks);
+    for (int i = (int)lane_id(); i < n; i += 32) v += tiles(seq(i), blocks);
     return __reduce_add_sync(0xffffffffu, v);
   }
   __device__ void init() {
     int most = 0;
-    for (int i = (int)lane_id(); i < n; i += 32) most = max(most, kv_len(lens[i]));
+    for (int i = (int)lane_id(); i < n; i += 32) most = max(most, seqs[i].kv_len);
     c = (__reduce_max_sync(0xffffffffu, most) + BKV - 1) / BKV + 1;
     at_c = above_c = 0;
   }
   // Tile b (b never falls from call to call): its sequence and its place among
   // the sequence's tiles; false where there are at most b tiles.
-  __device__ bool find(int b, int& seq, int& level) {
+  __device__ bool find(int b, int& at, int& level) {
     if (b >= at_c) {
       if (c == 0 || total(0) <= b) return false;
-      int lo = 0, hi = c;  // total(lo) > b >= total(hi)
+      int lo = 0, hi = c;  // total(lo) = n_lo > b >= n_hi = total(hi)
+      int n_lo = -1, n_hi = at_c;
       while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (total(mid) > b) lo = mid; else hi = mid;
+        const int mid = (lo + hi) / 2, v = total(mid);
+        if (v > b) {
+          lo = mid;
+          n_lo = v;
+        } else {
+          hi = mid;
+          n_hi = v;
+        }
       }
       c = lo;
-      at_c = total(c);
-      above_c = total(c + 1);
+      at_c = n_lo >= 0 ? n_lo : total(lo);
+      above_c = n_hi;
     }
     int rank = b - above_c;
     for (int i0 = 0; i0 < n; i0 += 32) {
       const int i = i0 + (int)lane_id();
-      const int2 s = i < n ? lens[i] : make_int2(0, 0);
-      const int more = tiles(s, c + 1), e = tiles(s, c) - more;
+      int more = 0, e = 0, all = 0;
+      if (i < n) {
+        const Seq s = seq(i);
+        more = tiles(s, c + 1);
+        e = tiles(s, c) - more;
+        all = s.tiles;
+      }
+      const int here = __reduce_add_sync(0xffffffffu, e);
+      if (rank >= here) {
+        rank -= here;
+        continue;
+      }
       int incl = e;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, incl, o);
         if ((int)lane_id() >= o) incl += v;
       }
-      const uint32_t past = __ballot_sync(0xffffffffu, incl > rank);
-      if (past) {
-        const int l = __ffs(past) - 1;
-        const int before = __shfl_sync(0xffffffffu, incl - e, l);
-        const int all = (s.x + tile_tokens - 1) / tile_tokens;
-        seq = i0 + l;
-        level = __shfl_sync(0xffffffffu, all - 1 - more, l) - (rank - before);
-        return true;
-      }
-      rank -= __shfl_sync(0xffffffffu, incl, 31);
+      const int l = __ffs(__ballot_sync(0xffffffffu, incl > rank)) - 1;
+      at = i0 + l;
+      level = __shfl_sync(0xffffffffu, all - 1 - more + incl - e, l) - rank;
+      return true;
     }
     return false;
   }
@@ -305,8 +328,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* nonfinite = abort_flag + 1;  // [2] by unit
   float2* stats = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(units) + BAR_BYTES);  // [BQ] log2 sum (cluster merge)
-  int2* lens = reinterpret_cast<int2*>(stats + BQ);  // [kMaxSeqs]
-  uint4* stage = reinterpret_cast<uint4*>(lens + kMaxSeqs);  // 32 rows of EC columns per softmax warp
+  Seq* seqs = reinterpret_cast<Seq*>(stats + BQ);  // [kMaxSeqs]
+  uint4* stage = reinterpret_cast<uint4*>(seqs + kMaxSeqs);  // 32 rows of EC columns per softmax warp
 
   const int warp = threadIdx.x / 32;
   const int lane = (int)lane_id();
@@ -347,7 +370,17 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
   griddep_wait();
   for (int i = threadIdx.x; i < p.n_seqs; i += NUM_THREADS) {
     const int a = max(0, min(p.cu[i], p.total_q)), b = max(a, min(p.cu[i + 1], p.total_q));
-    lens[i] = make_int2(b - a, kPaged ? max(0, p.ctx[i]) - (b - a) : 0);
+    Seq s;
+    s.q_len = b - a;
+    s.kv_len = b - a;
+    s.before = 0;
+    if constexpr (kPaged) {  // a length past the table is cut to it
+      const int ctx = max(0, p.ctx[i]);
+      s.kv_len = (int)min((long long)ctx, (long long)p.table_width << p.page_shift);
+      s.before = ctx - s.q_len;
+    }
+    s.tiles = (s.q_len + p.tile_tokens - 1) / p.tile_tokens;
+    *reinterpret_cast<int4*>(seqs + i) = *reinterpret_cast<const int4*>(&s);
   }
   tc_fence_before();
   __syncthreads();
@@ -510,7 +543,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
   } else if (warp == WARP_FIX) {
     // The units: two are out at a time, the next one is found and put in the
     // place of one that every role has left.
-    Finder f{lens, p.n_seqs, p.tile_tokens, p.causal, kPaged ? (long long)p.table_width << p.page_shift : 0x7fffffffll};
+    Finder f{seqs, p.n_seqs, p.tile_tokens, p.causal};
     f.init();
     auto publish = [&](int i, Unit& u) -> bool {
       // units come longest first: rounds go up and down the CTAs in turn, so
@@ -521,14 +554,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
       int seq, level;
       // with splits, one unit per CTA (per cluster)
       if ((p.splits == 1 || i == 0) && f.find(unit / p.n_kv, seq, level)) {
-        const int2 s = lens[seq];
+        const Seq s = f.seq(seq);
         u.seq = seq;
         u.kvh = unit % p.n_kv;
         u.q_begin = max(0, min(p.cu[seq], p.total_q));
-        u.kv_len = f.kv_len(s);
+        u.kv_len = s.kv_len;
         u.t0 = level * p.tile_tokens;
-        u.n_tok = min(p.tile_tokens, s.x - u.t0);
-        u.first = s.y + u.t0;
+        u.n_tok = min(p.tile_tokens, s.q_len - u.t0);
+        u.first = s.before + u.t0;
         u.lim_min = keys_seen(u, p.causal, 0);
         const int blocks = (keys_seen(u, p.causal, u.n_tok - 1) + BKV - 1) / BKV;
         const int chunk = (blocks + p.splits - 1) / p.splits;

@@ -236,6 +236,15 @@ def test_paged_chunks(gpu, lens, ctx, heads, kv, dim, page):
     run_paged(gpu, randn(3, sum(lens), heads, dim, dtype=bf16), kc, vc, table, cumulated(lens), ctx, page)
 
 
+@pytest.mark.parametrize("n", [255, 256, 257, 600])
+def test_paged_many_sequences(gpu, n):
+    """More sequences than one launch takes; single tokens, chunks and empty ones mixed."""
+    lens = [(1, 1, 0, 5, 1, 40)[i % 6] for i in range(n)]
+    ctx = [max(m, (i * 61) % 330) for i, m in enumerate(lens)]
+    kc, vc, table = make_cache(21, ctx, 16, 2, 64, f16, fill=float("nan"))
+    run_paged(gpu, randn(22, sum(lens), 8, 64), kc, vc, table, cumulated(lens), ctx, 16)
+
+
 @pytest.mark.parametrize("max_ctx", [0, 1, 100, 100000])
 def test_paged_max_ctx_only_sets_the_split(gpu, max_ctx):
     ctx = [5000, 3, 777]
