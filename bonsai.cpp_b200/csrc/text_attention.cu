@@ -894,19 +894,23 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
 // read.  HD / 8 threads take a range's row, the block's groups of them every
 // 256 / (HD / 8)-th range, so that the few rows of single tokens do not wait
 // for one range after the other (one token over 30000 keys of 8 heads: 36 us against 51); the
-// groups' sums meet in a fixed order.
+// groups' sums meet in a fixed order.  Only the rows of this launch's own
+// sequences have parts: the others (of another launch of the call, or of no
+// sequence at all) are left alone.
 constexpr int kMaxSplits = 64;
 template <int HD, bool kBF16>
 __global__ void __launch_bounds__(256) text_combine_kernel(const float* __restrict__ part_o,
                                                            const float* __restrict__ part_lse, int splits, int rows,
-                                                           int n_heads, uint16_t* out, long long out_token,
-                                                           long long out_head) {
+                                                           int n_heads, const int* __restrict__ cu, int n_seqs,
+                                                           uint16_t* out, long long out_token, long long out_head) {
   constexpr int LANES = HD / 8, GROUPS = 256 / LANES;
   __shared__ float lse[kMaxSplits];
   __shared__ float sums[GROUPS][HD + 4];
   const size_t items = (size_t)rows * n_heads, it = blockIdx.x;
   const int grp = threadIdx.x / LANES, d = (threadIdx.x % LANES) * 8;
   griddep_wait();
+  const int row = (int)(it / n_heads);
+  if (row < cu[0] || row >= cu[n_seqs]) return;
   if (threadIdx.x < splits) lse[threadIdx.x] = __ldcg(part_lse + threadIdx.x * items + it);
   __syncthreads();
   float top = -INFINITY;
@@ -940,7 +944,7 @@ __global__ void __launch_bounds__(256) text_combine_kernel(const float* __restri
       x += sums[k][2 * threadIdx.x];
       y += sums[k][2 * threadIdx.x + 1];
     }
-    reinterpret_cast<uint32_t*>(out + (it / n_heads) * out_token + (it % n_heads) * out_head)[threadIdx.x] =
+    reinterpret_cast<uint32_t*>(out + (size_t)row * out_token + (it % n_heads) * out_head)[threadIdx.x] =
         cvt2<kBF16>(x * inv, y * inv);
   }
 }
@@ -1086,7 +1090,7 @@ int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, 
   if (rc == 0 && part) {
     rc = launch_after("text_combine_kernel launch", text_combine_kernel<HD, kBF16>,
                       dim3((unsigned)(p.total_q * p.n_heads)), dim3(256), 0, 1, st, p.part_o, p.part_lse, p.splits,
-                      p.total_q, p.n_heads, static_cast<uint16_t*>(p.out), p.out_token, p.out_head);
+                      p.total_q, p.n_heads, p.cu, p.n_seqs, static_cast<uint16_t*>(p.out), p.out_token, p.out_head);
   }
   scratch_free(part, st);
   return rc;

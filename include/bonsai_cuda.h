@@ -338,7 +338,8 @@ int bonsai_paged_append(const bonsai_heads_t* k, const bonsai_heads_t* v,
 /* Causal attention of the new tokens of each sequence (packed as in
  * bonsai_paged_append, one token or a chunk) over its ctx_lens[s] cached
  * tokens, the new ones included (append them first): new token i sees the
- * places up to ctx_lens[s] - q_len + i.  A row that sees nothing is zero.
+ * places up to ctx_lens[s] - q_len + i.  A row that sees nothing is zero; rows
+ * of out that belong to no sequence are not written.
  * Cache contents past a sequence's length are never used, whatever they are;
  * page indices outside [0, n_pages) read as zeros; ctx_lens past the table
  * are cut to it.  max_ctx: an upper bound of ctx_lens, which only sets how
