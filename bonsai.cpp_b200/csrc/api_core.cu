@@ -256,6 +256,21 @@ long long bonsai_launch_count(void) {
   return n;
 }
 
+int bonsai_debug_tmem_shares(int* smem, int* cols, int cap) {
+  if (cap < 0 || (cap > 0 && (!smem || !cols))) return fail(BONSAI_ERR_ARG, "debug_tmem_shares: null output");
+  int n = 0;
+  for (auto part : {attention_tmem_shares, conv_tmem_shares, gemm_tmem_shares, lora_tmem_shares, text_tmem_shares}) {
+    TmemShare s[kMaxTmemShares];
+    const int k = part(s);
+    for (int i = 0; i < k; ++i, ++n)
+      if (n < cap) {
+        smem[n] = s[i].smem + kSmemReserved;
+        cols[n] = s[i].cols;
+      }
+  }
+  return n;
+}
+
 int bonsai_init(int device) {
   cudaError_t e = cudaSetDevice(device);
   if (e != cudaSuccess) return cuda_status(e, "cudaSetDevice");

@@ -1201,6 +1201,12 @@ int choose_kv_split(long long units, int slots, int nkv, int* chunk) {
 }
 }  // namespace
 
+int attention_tmem_shares(TmemShare* s) {
+  s[0] = {attn::SMEM_BYTES, attn::TMEM_COLS};
+  s[1] = {attn::v2::SMEM_BYTES, attn::TMEM_COLS};
+  return 2;
+}
+
 int launch_attention(const __half* q, const __half* k, const __half* v, int n_heads, int seq,
                      int head_dim, float scale, __half* out, long long ld_out, cudaStream_t st,
                      const RowRoutes* routes) {

@@ -76,7 +76,7 @@ constexpr int DELTA_AHEAD = 12;
 constexpr int SMEM_DELTA_BYTES = 1024 + DELTA_STAGES * (DELTA_BN * BK * 2 + RAW_STAGE_BYTES) + 256 +
                                  DELTA_BN * BM * 4 + DELTA_BN * 8 + DELTA_BN * 128 * 4 +
                                  EPI_WARPS * DELTA_AHEAD * 1024;
-static_assert(SMEM_DELTA_BYTES <= 232448 && SMEM_BLOCKS_BYTES <= 232448, "shared memory of one CTA");
+static_assert(SMEM_DELTA_BYTES <= kSmemMax && SMEM_BLOCKS_BYTES <= kSmemMax, "shared memory of one CTA");
 
 // Barrier of the epilogue warps alone.
 __device__ __forceinline__ void epi_sync() {
@@ -1485,6 +1485,12 @@ bool prefer_pair(long long tiles1, long long tiles2, int ksplit, int slots) {
   return t2 < t1;
 }
 }  // namespace
+
+int gemm_tmem_shares(TmemShare* s) {
+  s[0] = {gemm::pair::SMEM_BYTES, gemm::pair::TMEM_COLS};
+  s[1] = {gemm::SMEM_DELTA_BYTES, gemm::TMEM_COLS};
+  return 2;
+}
 
 int b1_gemm_tile_tokens(int tokens, const B1Weight& w, int epi_mode) {
   // sums in parts take the one-CTA kernel: a pair's 256-token tile leaves no

@@ -62,6 +62,27 @@ class ProfScope {
 int scratch_alloc(void** ptr, size_t bytes, const char* what, cudaStream_t st);
 void scratch_free(void* ptr, cudaStream_t st);
 int* device_error_word();
+
+// Tensor memory and clusters.  tcgen05.alloc waits until the columns are free,
+// and a CTA of a cluster frees its columns only after its peers have come to
+// the cluster's last barrier.  Two clusters that each hold columns the other's
+// CTAs wait for, on two SMs, would wait for ever, whether they are of one
+// launch or of two streams.  So no set of such CTAs that an SM's shared memory
+// admits may need more than its 512 columns; what a CTA of each of these
+// kernels takes is listed here, and a test adds up every set.
+constexpr int kSmemPerSm = 228 * 1024, kSmemReserved = 1024;  // per CTA, by the system
+constexpr int kSmemMax = kSmemPerSm - kSmemReserved;          // dynamic, of a CTA alone on its SM
+constexpr int kTmemColumns = 512;
+struct TmemShare {
+  int smem;  // dynamic shared memory of a CTA
+  int cols;
+};
+constexpr int kMaxTmemShares = 8;  // of one file
+int attention_tmem_shares(TmemShare* s);
+int conv_tmem_shares(TmemShare* s);
+int gemm_tmem_shares(TmemShare* s);
+int lora_tmem_shares(TmemShare* s);
+int text_tmem_shares(TmemShare* s);
 long long launch_counter();           // launches counted on this thread so far
 void launch_counter_add(long long n);  // account for kernels replayed from a CUDA graph
 bool profiling_active();              // bonsai_profile_start() in effect on this thread  // device address of the per-device error word (lazily resolved)

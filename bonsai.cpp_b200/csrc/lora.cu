@@ -192,10 +192,15 @@ constexpr int kMaxRank = 128;
 inline __host__ __device__ int tmem_cols(int r_pad) { return r_pad <= 16 ? 64 : r_pad <= 32 ? 128 : r_pad <= 64 ? 256 : 512; }
 
 // Shared memory of a launch: stages of x and A; the partial sums (f32
-// [r_pad][128 tokens]) take the stages' place once the products are done.
+// [r_pad][128 tokens]) take the stages' place once the products are done.  A
+// CTA that takes all of the tensor memory takes all of the shared memory too,
+// so that none waits for its columns (see TmemShare).
 inline int smem_bytes(int r_pad) {
+  if (tmem_cols(r_pad) == kTmemColumns) return kSmemMax;
   return 1024 + std::max(STAGES * (X_BYTES + r_pad * BK * 2), r_pad * BM * 4) + 256;
 }
+static_assert(1024 + STAGES * (X_BYTES + kMaxRank * BK * 2) + 256 <= kSmemMax && kMaxRank * BM * 4 <= kSmemMax - 1280,
+              "shared memory of one CTA");
 }  // namespace tile
 
 // low of one 128-token tile of one request: x (128 x K) times A^T (K x rank) on
@@ -429,7 +434,7 @@ int shrink_tiles(const ShrinkParams& p, cudaStream_t st) {
   if (e != cudaSuccess) return cuda_status(e, "lora shrink set smem attribute");
   const long long seqs = std::min(p.n_reqs, p.tokens);
   const long long units = (p.tokens + seqs * (tile::BM - 1)) / tile::BM;
-  int c = 8;  // CTAs that split K: up to three per SM, each at least two stages
+  int c = 8;  // CTAs that split K: about three per SM's worth of them, each at least two stages
   while (c > 1 && (units * c > 3ll * num_sms() || p.k_in / tile::BK < 2 * c)) c /= 2;
   if (units * c > 0x7fffffffll) return fail(-2, "b1_gemm_lora: too many tokens in one call");
   ProfScope prof("lora_shrink", 0.0, 2.0 * p.tokens * p.k_in, st);  // x; the ranks are on the device
@@ -466,6 +471,13 @@ int shrink_by_rank(const ShrinkParams& p, int max_rank, cudaStream_t st) {
 }
 
 }  // namespace lora
+
+int lora_tmem_shares(TmemShare* s) {
+  int n = 0;
+  for (int r = 16; r <= lora::tile::kMaxRank; r += 16)
+    s[n++] = {lora::tile::smem_bytes(r), lora::tile::tmem_cols(r)};
+  return n;
+}
 
 int launch_lora_retile(const __half* up, const LoraSlot& info, const LoraDevice& set, int slot, cudaStream_t st) {
   const size_t n = (size_t)set.n_ftiles * 128 * set.r_pad;

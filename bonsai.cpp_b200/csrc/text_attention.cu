@@ -87,10 +87,13 @@ struct Cfg {
   // Q and the rings; once a unit's products are done they can hold its O (f32)
   static constexpr int TILES_BYTES = Q_BYTES + 2 * RING * KV_BYTES;
   static_assert(TILES_BYTES >= BQ * HD * 4, "O does not fit the tiles");
-  static constexpr int SMEM_BYTES = 1024 + TILES_BYTES + BAR_BYTES + BQ * 8 + kMaxSeqs * 16 + 4 * 32 * EC * 2;
+  // As much for 64 dims as for 128: a CTA takes half of the tensor memory, and
+  // so no less of the shared memory than that leaves to others (see TmemShare).
+  static constexpr int SMEM_BYTES = 1024 + 2 * Q_HALF + 2 * RING * 2 * KV_HALF + BAR_BYTES + BQ * 8 + kMaxSeqs * 16 +
+                                    4 * 32 * EC * 2;
+  static_assert(SMEM_BYTES >= 1024 + TILES_BYTES + BAR_BYTES + BQ * 8 + kMaxSeqs * 16 + 4 * 32 * EC * 2, "layout");
 };
-// Two CTAs per SM (228 KB, 1 KB of it reserved for each).
-static_assert(2 * (Cfg<128>::SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs per SM");
+static_assert(2 * (Cfg<128>::SMEM_BYTES + kSmemReserved) <= kSmemPerSm, "two CTAs per SM");
 
 struct Params {
   const int* cu;        // [n_seqs + 1] first query row of each sequence
@@ -1107,6 +1110,12 @@ int dispatch(const TextAttention& a, const CUtensorMap& qm, const CUtensorMap& k
 }
 
 }  // namespace text
+
+int text_tmem_shares(TmemShare* s) {
+  s[0] = {text::Cfg<64>::SMEM_BYTES, text::TMEM_COLS};
+  s[1] = {text::Cfg<128>::SMEM_BYTES, text::TMEM_COLS};
+  return 2;
+}
 
 int launch_text_attention(const TextAttention& a, cudaStream_t st) {
   using namespace text;

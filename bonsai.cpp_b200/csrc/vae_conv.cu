@@ -645,6 +645,11 @@ int conv_pair_slots() {
 
 }  // namespace
 
+int conv_tmem_shares(TmemShare* s) {
+  s[0] = {vconv::SMEM_BYTES, vconv::TMEM_COLS};
+  return 1;
+}
+
 int launch_vae_conv(const VaeConvArgs& a, cudaStream_t st) {
   using namespace vconv;
   const int phases = a.phases == 4 ? 4 : 1;

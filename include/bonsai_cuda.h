@@ -88,6 +88,13 @@ int bonsai_count_nonfinite(const float* x, long long n, long long* count, void* 
  * the code with bonsai_device_error().  The launch's output is not written. */
 int bonsai_debug_stall_next_gemm(void);
 
+/* Testing hook: what a CTA of each kernel takes of its SM whose CTAs hold
+ * tensor memory while they wait for one another (clusters): shared memory in
+ * bytes, the system's 1 KB included, and tensor memory columns, the first cap
+ * entries.  Any of them that fit an SM's 228 KB together must fit its 512
+ * columns.  Returns the number of entries. */
+int bonsai_debug_tmem_shares(int* smem, int* cols, int cap);
+
 /* Number of kernel launches this library has issued on the current thread
  * since the last call (launch accounting for benchmarks); resets to 0. */
 long long bonsai_launch_count(void);
