@@ -1492,18 +1492,18 @@ int gemm_tmem_shares(TmemShare* s) {
   return 2;
 }
 
+// Set by bonsai_debug_stall_next_gemm, consumed by the next launch on the thread.
+thread_local bool g_stall_next_gemm = false;
+
 int b1_gemm_tile_tokens(int tokens, const B1Weight& w, int epi_mode) {
   // sums in parts take the one-CTA kernel: a pair's 256-token tile leaves no
-  // shared memory for them
-  if (lora_part(w, epi_mode) < w.k_blocks) return gemm::BN;
+  // shared memory for them; and so does a launch with the test hook
+  if (lora_part(w, epi_mode) < w.k_blocks || g_stall_next_gemm) return gemm::BN;
   const long long tt1 = (tokens + gemm::BN - 1) / gemm::BN, tt2 = (tokens + gemm::pair::BN - 1) / gemm::pair::BN;
   return prefer_pair(w.n_ftiles * tt1, (w.n_ftiles + 1) / 2 * tt2, 1, pair_cluster_slots(false, LORA_BLOCKS))
              ? gemm::pair::BN
              : gemm::BN;
 }
-
-// Set by bonsai_debug_stall_next_gemm, consumed by the next launch on the thread.
-thread_local bool g_stall_next_gemm = false;
 
 bool b1_gemv_supported(const B1Weight& w) {
   return w.swiglu_from < 0 && w.k_blocks >= 1 && w.k_blocks <= gemm::kGemvMaxKBlocks;
