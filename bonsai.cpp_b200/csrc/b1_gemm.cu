@@ -153,52 +153,78 @@ __device__ __forceinline__ uint32_t bf16_from_f16_scale(uint32_t s16) {
 // LORA_BLOCKS (many tokens per request): extra k-blocks whose weight columns
 // are columns of the adapters' B and whose activations are the low-rank
 // values of the tokens of one request (zero for the tile's others):
-//   [W | B_a B_a B_b ...] [x; low_a hi; low_a lo; low_b hi; ...].
-// The f32 low-rank values enter as two f16 (value and remainder), which keeps
-// 22 bits of them.
+//   [W | B1_a B1_a ... B2_a ... B1_b ...] [x; l1_a; l2_a; ...; l1_a; ...; l1_b; ...],
+// both as bf16 pieces (kLowPieces).
 // LORA_DELTA (few tokens per request): the epilogue warps compute B low for
 // their rows and tokens in f32 while the products of W x run, reading each
 // adapter's rows once; a tile's k-blocks are split between the CTAs of a
 // cluster, since few tokens make few tiles (128 weight rows x all tokens).
 // The parts meet in shared memory, token by token, in a fixed order.
 
-// 16-column groups of the extra k-blocks of token tile `ttile`.
+// 16-column steps of the extra k-blocks of token tile `ttile`.
 template <int kLora>
-__device__ __forceinline__ int lora_groups(const LoraGemm& l, int ttile) {
-  return kLora == LORA_BLOCKS ? __ldg(l.group_count + ttile) : 0;
+__device__ __forceinline__ int lora_steps(const LoraGemm& l, int ttile) {
+  return kLora == LORA_BLOCKS ? kLowPieces * __ldg(l.group_count + ttile) : 0;
 }
 // 128 weight rows x 16 ranks of an adapter's B, contiguous (LoraDevice::up).
 __device__ __forceinline__ const __half* lora_chunk(const LoraGemm& l, int slot, int ftile, int r0) {
   return l.up + (((size_t)slot * l.n_ftiles + ftile) * (l.r_pad / 16) + r0 / 16) * (BM * 16);
 }
-// One 16-column group: this thread's weight row (8 words of two columns) and
-// its token's activations (8 words), zero where they are none of the group's.
-__device__ __forceinline__ void lora_group(const LoraGemm& l, const int4 e, int ftile, int r, int tok,
-                                           uint32_t* w, uint32_t* x) {
-  const int slot = e.x & 0x3fffffff;
-  const bool lo = (e.x & 0x40000000) != 0;
-  const uint4* wsrc = reinterpret_cast<const uint4*>(lora_chunk(l, slot, ftile, e.y) + r * 16);
-  const uint4 b0 = __ldg(wsrc), b1 = __ldg(wsrc + 1);
-  w[0] = b0.x; w[1] = b0.y; w[2] = b0.z; w[3] = b0.w;
-  w[4] = b1.x; w[5] = b1.y; w[6] = b1.z; w[7] = b1.w;
+// B1 or B2 of two f16 values.
+__device__ __forceinline__ uint32_t b_pieces(uint32_t h, bool second) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  __nv_bfloat162 b = __floats2bfloat162_rn(f.x, f.y);
+  if (second) {
+    const float2 g = __bfloat1622float2(b);
+    b = __floats2bfloat162_rn(f.x - g.x, f.y - g.y);
+  }
+  return *reinterpret_cast<const uint32_t*>(&b);
+}
+// This thread's part of a k-block of low-rank steps [step, step + 4) of token
+// tile `ttile`: its weight row of the two groups at most that they belong to,
+// its token's pieces (zeros where the token is none of the group's).  All loads
+// are under way together and, a piece's tokens being contiguous, coalesced
+// (pieces cut here from f32 rows: 410 us for the images of four requests, not
+// 322; rows of pieces token by token 350).
+struct LowBlock {
+  uint4 b[4], x[8];
+  int n, first, left;  // steps that exist; piece of the first; steps of its group
+};
+__device__ __forceinline__ void lora_load(const LoraGemm& l, int ttile, int step, int steps, int ftile, int r, int tok,
+                                          LowBlock& v) {
+  const int4* list = l.groups + (size_t)ttile * l.max_groups + step / kLowPieces;
+  v.first = step % kLowPieces;
+  v.left = kLowPieces - v.first;
+  v.n = min(4, steps - step);
+  const int4 e0 = __ldg(list);
+  const int4 e1 = v.left < v.n ? __ldg(list + 1) : e0;
+  const uint4* w0 = reinterpret_cast<const uint4*>(lora_chunk(l, e0.x, ftile, e0.y) + r * 16);
+  const uint4* w1 = reinterpret_cast<const uint4*>(lora_chunk(l, e1.x, ftile, e1.y) + r * 16);
+  v.b[0] = __ldg(w0);
+  v.b[1] = __ldg(w0 + 1);
+  v.b[2] = __ldg(w1);
+  v.b[3] = __ldg(w1 + 1);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = 0u;
-  if (tok >= e.z && tok < e.w) {
-    const float4* src = reinterpret_cast<const float4*>(l.low + (size_t)tok * l.r_pad + e.y);
+  for (int i = 0; i < 4; ++i) {
+    const int piece = i < v.left ? v.first + i : i - v.left, part = piece < 3 ? piece : piece - 3;
+    const int4 e = i < v.left ? e0 : e1;
+    const bool own = i < v.n && tok >= e.z && tok < e.w;
+    const uint4* src = l.low_pieces + ((size_t)(e.y / 16 * kLowParts + part) * l.tokens + tok) * 2;
+    v.x[2 * i] = own ? __ldcg(src) : make_uint4(0, 0, 0, 0);
+    v.x[2 * i + 1] = own ? __ldcg(src + 1) : make_uint4(0, 0, 0, 0);
+  }
+}
+// The 8 words (of two columns) of step i of the thread's weight row.
+__device__ __forceinline__ void lora_weights(const LowBlock& v, int i, uint32_t* w) {
+  const bool one = i < v.left;
+  const bool second = (one ? v.first + i : i - v.left) >= 3;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 f = __ldcg(src + i);
-      const __half2 h0 = __floats2half2_rn(f.x, f.y), h1 = __floats2half2_rn(f.z, f.w);
-      if (!lo) {
-        x[2 * i] = *reinterpret_cast<const uint32_t*>(&h0);
-        x[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&h1);
-      } else {
-        const float2 g0 = __half22float2(h0), g1 = __half22float2(h1);
-        const __half2 r0 = __floats2half2_rn(f.x - g0.x, f.y - g0.y), r1 = __floats2half2_rn(f.z - g1.x, f.w - g1.y);
-        x[2 * i] = *reinterpret_cast<const uint32_t*>(&r0);
-        x[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&r1);
-      }
-    }
+  for (int k = 0; k < 2; ++k) {
+    const uint4 h = one ? v.b[k] : v.b[2 + k];
+    w[4 * k] = b_pieces(h.x, second);
+    w[4 * k + 1] = b_pieces(h.y, second);
+    w[4 * k + 2] = b_pieces(h.z, second);
+    w[4 * k + 3] = b_pieces(h.w, second);
   }
 }
 
@@ -415,7 +441,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         const int ttile = tile / p.nf;
         const int ftile = sel_ftile(tile - ttile * p.nf, p.fcount, p.fbase);
         const uint32_t* wsrc = p.chunks + (size_t)ftile * k_blocks * kChunkWords;
-        const int nkb = kr1 + (lora_groups<kLora>(p.lora, ttile) + 3) / 4;
+        const int nkb = kr1 + (lora_steps<kLora>(p.lora, ttile) + 3) / 4;
         for (int kb = kr0; kb < nkb; ++kb, ++it) {
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1;
@@ -445,11 +471,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   } else if (warp == WARP_MMA) {
     if (elect_one()) {
       constexpr uint32_t idesc = make_idesc_f16(BM, BN, kBF16 ? 1 : 0, 0, 0);
+      constexpr uint32_t idesc_low = make_idesc_f16(BM, BN, 1, 0, 0);
       uint32_t it = 0, lt = 0;
       bool ok = true;
       for (int tile = tile0; tile < p.num_tiles && ok; tile += tstep) {
-        const int groups = lora_groups<kLora>(p.lora, tile / p.nf);
-        const int nkb = kr1 + (groups + 3) / 4;
+        const int steps = lora_steps<kLora>(p.lora, tile / p.nf);
+        const int nkb = kr1 + (steps + 3) / 4;
         for (int part = 0; part < parts && ok; ++part, ++lt) {
         const int kb0 = kr0 + (kLora != LORA_NONE ? part * p.kpart : 0);
         const int kb1 = part + 1 < parts ? kb0 + p.kpart : nkb;
@@ -472,10 +499,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           const uint32_t xaddr = smem_u32(xs + s * X_STAGE_BYTES);
 #pragma unroll
           for (int k16 = 0; k16 < BK / 16; ++k16) {
-            if (kLora == LORA_BLOCKS && kb >= k_blocks && (kb - k_blocks) * 4 + k16 >= groups) break;
+            if (kLora == LORA_BLOCKS && kb >= k_blocks && (kb - k_blocks) * 4 + k16 >= steps) break;
             const uint32_t a_tmem = tmem + A_COL0 + s * 32 + k16 * 8;
             const uint64_t bdesc = make_smem_desc(xaddr + k16 * 32, 16, 1024);
-            mma_ts(d_tmem, a_tmem, bdesc, idesc, kb != kb0 || k16 != 0 ? 1u : 0u);
+            mma_ts(d_tmem, a_tmem, bdesc, kLora == LORA_BLOCKS && kb >= k_blocks ? idesc_low : idesc, kb != kb0 || k16 != 0 ? 1u : 0u);
           }
           tc_commit(&empty[s]);
         }
@@ -505,15 +532,33 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const uint32_t slot = (uint32_t)((warp - WARP_EXP0) >> 2);
     uint32_t it = 0;
     int pending = -1;  // stage whose tcgen05.st is in flight
+    auto publish = [&]() {
+      if (pending < 0) return;
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(&full[pending]);
+      pending = -1;
+    };
     bool ok = true;
     for (int tile = tile0; tile < p.num_tiles && ok; tile += tstep) {
       const int ttile = tile / p.nf;
-      const int groups = lora_groups<kLora>(p.lora, ttile);
-      const int nkb = kr1 + (groups + 3) / 4;
+      const int steps = lora_steps<kLora>(p.lora, ttile);
+      const int nkb = kr1 + (steps + 3) / 4;
       for (int kb = kr0; kb < nkb; ++kb, ++it) {
         if (it % EXP_PER_Q != slot) continue;
         const int s = it % STAGES;
         const uint32_t ph = (it / STAGES) & 1;
+        // An extra block's loads are under way while its stage is waited for, and
+        // the block before it does not wait for them.
+        const bool extra = kLora == LORA_BLOCKS && kb >= k_blocks;
+        LowBlock low_block;
+        if (extra) {
+          publish();
+          griddep_wait();  // the low-rank values
+          lora_load(p.lora, ttile, (kb - k_blocks) * 4, steps, sel_ftile(tile - ttile * p.nf, p.fcount, p.fbase), r,
+                    ttile * BN + r, low_block);
+        }
         bool good = wait_bar(&rawfull[s], ph, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER) &&
                     wait_bar(&empty[s], ph ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER);
         // tcgen05.st below is warp-collective: every lane must take the same path.
@@ -522,20 +567,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           break;
         }
         uint32_t v[32];
-        if (kLora == LORA_BLOCKS && kb >= k_blocks) {
-          griddep_wait();  // the low-rank values
-          const int ftile = sel_ftile(tile - ttile * p.nf, p.fcount, p.fbase);
+        if (extra) {
           const uint32_t xrow = smem_u32(xs + s * X_STAGE_BYTES) + (uint32_t)r * 128u;
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int gi = (kb - k_blocks) * 4 + g;
-            if (gi >= groups) break;  // its columns are not multiplied
-            const int4 e = __ldg(p.lora.groups + (size_t)ttile * p.lora.max_groups + gi);
-            uint32_t x[8];
-            lora_group(p.lora, e, ftile, r, ttile * BN + r, v + 8 * g, x);
-            st_shared_v4(xrow + (((2u * g) ^ (r & 7)) << 4), x[0], x[1], x[2], x[3]);
-            st_shared_v4(xrow + (((2u * g + 1u) ^ (r & 7)) << 4), x[4], x[5], x[6], x[7]);
-          }
+          for (int i = 0; i < 8; ++i)  // columns of steps past n are not multiplied
+            if (i / 2 < low_block.n)
+              st_shared_v4(xrow + (((uint32_t)i ^ (r & 7)) << 4), low_block.x[i].x, low_block.x[i].y,
+                           low_block.x[i].z, low_block.x[i].w);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) lora_weights(low_block, i, v + 8 * i);
           fence_proxy_async_smem();
         } else {
           const uint32_t* rs = raw + s * kChunkWords;
@@ -545,24 +585,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           expand_group(p0, bf16_from_f16_scale<kBF16>(sc & 0xFFFFu), v);
           expand_group(p1, bf16_from_f16_scale<kBF16>(sc >> 16), v + 16);
         }
-        if (pending >= 0) {
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) bar_arrive(&full[pending]);
-        }
+        publish();
         tmem_st32(tmem + lane_base + A_COL0 + s * 32, v);
         pending = s;
       }
     }
-    if (pending >= 0) {
-      // Publish the last stage (also on the abort path: the MMA side is
-      // bounded and ignores it).
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive(&full[pending]);
-    }
+    publish();  // the last stage (also on the abort path: the MMA side is bounded and ignores it)
     if constexpr (kLora != LORA_NONE) griddep_wait();  // the grid ends after the ones before it
   } else if (warp >= WARP_EPI0 && warp < WARP_EPI0 + EPI_WARPS) {
     const int q = warp & 3;
@@ -855,7 +883,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         const int fidx = min(2 * pf + (int)rank, p.nf - 1);
         const int ftile = sel_ftile(fidx, p.fcount, p.fbase);
         const uint32_t* wsrc = p.chunks + (size_t)ftile * k_blocks * kChunkWords;
-        const int nkb = kb1 + (lora_groups<kLora>(p.lora, ttile) + 3) / 4;
+        const int nkb = kb1 + (lora_steps<kLora>(p.lora, ttile) + 3) / 4;
         for (int kb = kb0; kb < nkb; ++kb, ++it) {
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1;
@@ -886,10 +914,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     if (elect_one()) {
       if (rank == 0) {
         constexpr uint32_t idesc = make_idesc_f16(2 * BM, BN, kBF16 ? 1 : 0, 0, 0);
+        constexpr uint32_t idesc_low = make_idesc_f16(2 * BM, BN, 1, 0, 0);
         uint32_t it = 0, lt = 0;
         bool ok = true;
         for (int tile = cid; tile < p.num_tiles && ok; tile += ncl, ++lt) {
-          const int groups = lora_groups<kLora>(p.lora, tile / p.ksplit / p.npf);
+          const int steps = lora_steps<kLora>(p.lora, tile / p.ksplit / p.npf);
           const uint32_t b = lt & 1;
           const uint32_t dph = (lt >> 1) & 1;
           if (!wait_bar(&dempty[b], dph ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA)) {
@@ -899,7 +928,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           tc_fence_after();
           const uint32_t d_tmem = tmem + b * BN;
           const int kb0 = (tile % p.ksplit) * p.kchunk;
-          const int kb1 = min(k_blocks, kb0 + p.kchunk) + (groups + 3) / 4;
+          const int kb1 = min(k_blocks, kb0 + p.kchunk) + (steps + 3) / 4;
           for (int kb = kb0; kb < kb1; ++kb, ++it) {
             const int s = it % STAGES;
             const uint32_t ph = (it / STAGES) & 1;
@@ -912,10 +941,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             const uint32_t xaddr = smem_u32(xs + s * X_STAGE_BYTES);
 #pragma unroll
             for (int k16 = 0; k16 < BK / 16; ++k16) {
-              if (kLora == LORA_BLOCKS && kb >= k_blocks && (kb - k_blocks) * 4 + k16 >= groups) break;
+              if (kLora == LORA_BLOCKS && kb >= k_blocks && (kb - k_blocks) * 4 + k16 >= steps) break;
               const uint64_t adesc = make_smem_desc(aaddr + k16 * 32, 16, 1024);
               const uint64_t bdesc = make_smem_desc(xaddr + k16 * 32, 16, 1024);
-              mma_ss_pair(d_tmem, adesc, bdesc, idesc, (kb != kb0 || k16 != 0) ? 1u : 0u);
+              mma_ss_pair(d_tmem, adesc, bdesc, kLora == LORA_BLOCKS && kb >= k_blocks ? idesc_low : idesc, (kb != kb0 || k16 != 0) ? 1u : 0u);
             }
             tc_commit_pair(&empty[s], 0x3);
           }
@@ -948,8 +977,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const int kb0 = (tile % p.ksplit) * p.kchunk;
       const int kb1 = min(k_blocks, kb0 + p.kchunk);
       const int ttile = tile / p.ksplit / p.npf;
-      const int groups = lora_groups<kLora>(p.lora, ttile);
-      const int nkb = kb1 + (groups + 3) / 4;
+      const int steps = lora_steps<kLora>(p.lora, ttile);
+      const int nkb = kb1 + (steps + 3) / 4;
       for (int kb = kb0; kb < nkb; ++kb, ++it) {
         if (it % EXP_PER_G != slot) continue;
         const int s = it % STAGES;
@@ -964,21 +993,22 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if (kLora == LORA_BLOCKS && kb >= k_blocks) {
           griddep_wait();  // the low-rank values
           const int fidx = min(2 * (tile - ttile * p.npf) + (int)rank, p.nf - 1);
-          const int ftile = sel_ftile(fidx, p.fcount, p.fbase);
+          LowBlock low_block;
+          lora_load(p.lora, ttile, (kb - k_blocks) * 4, steps, sel_ftile(fidx, p.fcount, p.fbase), r,
+                    ttile * BN + (int)rank * BNH + r, low_block);
           const uint32_t arow = smem_u32(as + s * A_STAGE_BYTES) + row_off;
           const uint32_t xrow = smem_u32(xs + s * X_STAGE_BYTES) + row_off;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int gi = (kb - k_blocks) * 4 + q;
-            if (gi >= groups) break;  // its columns are not multiplied
-            const int4 e = __ldg(p.lora.groups + (size_t)ttile * p.lora.max_groups + gi);
-            uint32_t w[8], x[8];
-            lora_group(p.lora, e, ftile, r, ttile * BN + (int)rank * BNH + r, w, x);
-            const uint32_t c0 = ((2u * q) ^ sw) << 4, c1 = ((2u * q + 1u) ^ sw) << 4;
+          for (int i = 0; i < 4; ++i) {
+            if (i >= low_block.n) break;  // its columns are not multiplied
+            const uint32_t c0 = ((2u * i) ^ sw) << 4, c1 = ((2u * i + 1u) ^ sw) << 4;
+            const uint4 x0 = low_block.x[2 * i], x1 = low_block.x[2 * i + 1];
+            uint32_t w[8];
+            lora_weights(low_block, i, w);
             st_shared_v4(arow + c0, w[0], w[1], w[2], w[3]);
             st_shared_v4(arow + c1, w[4], w[5], w[6], w[7]);
-            st_shared_v4(xrow + c0, x[0], x[1], x[2], x[3]);
-            st_shared_v4(xrow + c1, x[4], x[5], x[6], x[7]);
+            st_shared_v4(xrow + c0, x0.x, x0.y, x0.z, x0.w);
+            st_shared_v4(xrow + c1, x1.x, x1.y, x1.z, x1.w);
           }
         } else {
           const uint32_t* rs = raw + s * kChunkWords;

@@ -162,12 +162,18 @@ struct LoraSlot {
   float scale = 0.f;
 };
 enum LoraMode : int { LORA_NONE = 0, LORA_DELTA = 1, LORA_BLOCKS = 2 };
+// LORA_BLOCKS: B low as products of bf16 pieces, which have f32's range: B
+// (f16) is exactly B1 + B2, low (f32) exactly l1 + l2 + l3, and the sum takes
+// B1 l1, B1 l2, B1 l3, B2 l1, B2 l2; the one left out, B2 l3, is below 2^-24 of
+// B low.  (Two f16 values of low, with B as it is, keep 22 bits of it above 2^-3
+// only and end at 65504.)
+constexpr int kLowPieces = 5, kLowParts = 3;
 struct LoraGemm {
   int mode = LORA_NONE;
-  // LORA_BLOCKS: extra k-blocks of four 16-column groups, laid out for tiles
-  // of tile_tokens (b1_gemm_tile_tokens).  Token tile i has
-  // group_count[i] groups {slot | remainder << 30, first rank, first token,
-  // end token} at groups + i * max_groups.
+  // LORA_BLOCKS: extra k-blocks, laid out for tiles of tile_tokens
+  // (b1_gemm_tile_tokens).  Token tile i has group_count[i] groups of 16 ranks
+  // {slot, first rank, first token, end token} at groups + i * max_groups,
+  // each of which takes kLowPieces steps of 16 columns.
   const int* group_count = nullptr;
   const int4* groups = nullptr;
   int tile_tokens = 0, max_groups = 0;
@@ -176,10 +182,14 @@ struct LoraGemm {
   const int* slots = nullptr;
   const LoraSlot* info = nullptr;
   int n_reqs = 0, n_slots = 0;
-  // both: the adapters' B (LoraDevice::up), low-rank values f32 [tokens][r_pad]
+  // both: the adapters' B (LoraDevice::up)
   int r_pad = 0, n_ftiles = 0;
   const __half* up = nullptr;
+  // the low-rank values: LORA_DELTA f32 [tokens][r_pad], LORA_BLOCKS bf16
+  // [r_pad / 16][l1, l2, l3][tokens][16]
+  int tokens = 0;
   const float* low = nullptr;
+  const uint4* low_pieces = nullptr;
 };
 
 // Launch the tcgen05 B1_0 GEMM: for every token t < tokens and weight row n,

@@ -16,9 +16,9 @@
 // Measured (B200, a call among others): 64 requests of one token, 3072 -> 9216,
 // ranks 8 to 64: 35 us; 4 requests of about 1100 tokens, 3072 -> 12288: 312 us,
 // 1.11 PFLOP/s, 20 of them the shrink.
-// low stays in f32; as a tensor-core operand low is two f16 values
-// (22 bits), so nothing between x and the epilogue's own rounding is rounded
-// further.
+// low stays in f32, and the tensor cores take it and B in pieces that keep all
+// of it (kLowPieces), so nothing between x and the epilogue's own rounding is
+// rounded further, whatever its magnitude.
 #include "internal.cuh"
 
 #include "ptx.cuh"
@@ -59,8 +59,18 @@ struct ShrinkParams {
   const int* cu;              // [n_reqs + 1]
   const int* slots;           // [n_reqs]
   int n_reqs;
-  float* low;                 // [tokens][r_pad]
+  float* low;                 // [tokens][r_pad] (few tokens per request)
+  uint32_t* low_pieces;       // bf16 [r_pad / 16][kLowParts][tokens][16] (many)
 };
+
+// The upper 8 bits of an f32 value's 24, as an f32 value; what is left of it is
+// exact, and after three times nothing (the pieces l1, l2, l3).  All of a value
+// that is not finite is in its first piece.
+__device__ __forceinline__ float cut_piece(float& rest) {
+  const float piece = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
+  rest = (__float_as_uint(piece) & 0x7f800000u) == 0x7f800000u ? 0.f : rest - piece;
+  return piece;
+}
 
 // Tile u of the requests' token tiles (tiles of `size` tokens that do not
 // cross requests).  One warp; false where there are at most u tiles.
@@ -333,12 +343,22 @@ __global__ void __launch_bounds__(tile::NUM_THREADS)
     tc_fence_before();
   }
   cluster.sync();
-  const int n = n16 * 16;
+  const int n = n16 * 8;  // pairs of ranks
   for (int e = crank * NUM_THREADS + threadIdx.x; e < n * BM; e += csize * NUM_THREADS) {
-    const int t = t0 + e % BM, r = e / BM;
-    float s = 0.f;
-    for (int c = 0; c < csize; ++c) s += cluster.map_shared_rank(sums, c)[e];
-    if (t < end) p.low[(size_t)t * p.r_pad + r] = info.scale * s;
+    const int row = e % BM, t = t0 + row, r = e / BM * 2;
+    float a = 0.f, b = 0.f;
+    for (int c = 0; c < csize; ++c) {
+      const float* part = cluster.map_shared_rank(sums, c) + r * BM + row;
+      a += part[0];
+      b += part[BM];
+    }
+    if (t >= end) continue;
+    a *= info.scale;
+    b *= info.scale;
+    uint32_t* dst = p.low_pieces + ((size_t)(r / 16 * kLowParts) * p.tokens + t) * 8 + r % 16 / 2;
+#pragma unroll
+    for (int k = 0; k < kLowParts; ++k)
+      dst[(size_t)k * p.tokens * 8] = __byte_perm(__float_as_uint(cut_piece(a)), __float_as_uint(cut_piece(b)), 0x7632);
   }
   cluster.sync();  // no CTA ends while another reads its shared memory
   if (warp == 1) {
@@ -377,7 +397,7 @@ __global__ void lora_retile_kernel(const __half* __restrict__ src, LoraSlot info
 
 // Lists the extra k-blocks of each token tile of the GEMM (LoraGemm): for
 // every request with an adapter that has tokens in the tile, its ranks in
-// groups of 16, first the values, then the remainders.  One warp per tile.
+// groups of 16.  One warp per tile.
 __global__ void lora_plan_kernel(const int* __restrict__ cu, const int* __restrict__ slots, int n_reqs, int tokens,
                                  const LoraSlot* __restrict__ slot_info, int n_slots, int tile_tokens, int n_tiles,
                                  int max_groups, int* __restrict__ group_count, int4* __restrict__ groups) {
@@ -401,17 +421,15 @@ __global__ void lora_plan_kernel(const int* __restrict__ cu, const int* __restri
       slot = slots[i];
       if (a < b && slot >= 0 && slot < n_slots) n16 = (slot_info[slot].rank + 15) / 16;
     }
-    int incl = 2 * n16;
+    int incl = n16;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
     }
-    const int at = base + incl - 2 * n16;
-    for (int j = 0; j < 2 * n16; ++j)
-      if (at + j < max_groups)
-        groups[(size_t)tile * max_groups + at + j] =
-            make_int4(j < n16 ? slot : slot | (1 << 30), (j < n16 ? j : j - n16) * 16, a, b);
+    const int at = base + incl - n16;
+    for (int j = 0; j < n16; ++j)
+      if (at + j < max_groups) groups[(size_t)tile * max_groups + at + j] = make_int4(slot, j * 16, a, b);
     base += __shfl_sync(0xffffffffu, incl, 31);
     // past the tile once one of these 32 requests begins at or after its end
     if (__any_sync(0xffffffffu, i < n_reqs && cu[i] >= t1)) break;
@@ -497,14 +515,15 @@ int launch_b1_gemm_lora(const __half* x, long long ldx, int tokens, const B1Weig
   // 23, 64 x 32 464 / 129: the few-form reads B once per token, the other
   // takes extra k-blocks per request.
   g.mode = tokens > 8ll * n_reqs ? LORA_BLOCKS : LORA_DELTA;
-  // scratch: low, then the lists of extra blocks
-  const size_t low_n = ((size_t)tokens * set.r_pad + 3) / 4 * 4;
+  // scratch: low (or its pieces), then the lists of extra blocks
+  const size_t low_bytes = (size_t)tokens * set.r_pad * (g.mode == LORA_BLOCKS ? 2 * kLowParts : sizeof(float));
+  const size_t low_n = (low_bytes + 15) / 16 * 4;
   size_t more = 0;
   int n_tiles = 0;
   if (g.mode == LORA_BLOCKS) {
     g.tile_tokens = b1_gemm_tile_tokens(tokens, w, seg.mode);
     n_tiles = (tokens + g.tile_tokens - 1) / g.tile_tokens;
-    g.max_groups = 2 * (set.r_pad / 16) * std::min(n_reqs, g.tile_tokens);
+    g.max_groups = set.r_pad / 16 * std::min(n_reqs, g.tile_tokens);
     more = (size_t)n_tiles * (g.max_groups * sizeof(int4) + sizeof(int));
   }
   void* mem = nullptr;
@@ -524,6 +543,7 @@ int launch_b1_gemm_lora(const __half* x, long long ldx, int tokens, const B1Weig
   s.slots = slots;
   s.n_reqs = n_reqs;
   s.low = low;
+  s.low_pieces = reinterpret_cast<uint32_t*>(low);
   g.cu = cu;
   g.slots = slots;
   g.info = set.info;
@@ -533,6 +553,8 @@ int launch_b1_gemm_lora(const __half* x, long long ldx, int tokens, const B1Weig
   g.n_ftiles = set.n_ftiles;
   g.up = set.up;
   g.low = low;
+  g.tokens = tokens;
+  g.low_pieces = reinterpret_cast<const uint4*>(low);
   if (g.mode == LORA_BLOCKS) {
     int4* groups = reinterpret_cast<int4*>(low + low_n);
     int* count = reinterpret_cast<int*>(groups + (size_t)n_tiles * g.max_groups);
