@@ -206,7 +206,7 @@ __device__ __forceinline__ void lora_load(const LoraGemm& l, int ttile, int step
   v.b[3] = __ldg(w1 + 1);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int piece = i < v.left ? v.first + i : i - v.left, part = piece < 3 ? piece : piece - 3;
+    const int part = low_part(i < v.left ? v.first + i : i - v.left);
     const int4 e = i < v.left ? e0 : e1;
     const bool own = i < v.n && tok >= e.z && tok < e.w;
     const uint4* src = l.low_pieces + ((size_t)(e.y / 16 * kLowParts + part) * l.tokens + tok) * 2;
@@ -549,16 +549,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if (it % EXP_PER_Q != slot) continue;
         const int s = it % STAGES;
         const uint32_t ph = (it / STAGES) & 1;
-        // An extra block's loads are under way while its stage is waited for, and
-        // the block before it does not wait for them.
         const bool extra = kLora == LORA_BLOCKS && kb >= k_blocks;
-        LowBlock low_block;
-        if (extra) {
-          publish();
-          griddep_wait();  // the low-rank values
-          lora_load(p.lora, ttile, (kb - k_blocks) * 4, steps, sel_ftile(tile - ttile * p.nf, p.fcount, p.fbase), r,
-                    ttile * BN + r, low_block);
-        }
         bool good = wait_bar(&rawfull[s], ph, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER) &&
                     wait_bar(&empty[s], ph ^ 1, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER);
         // tcgen05.st below is warp-collective: every lane must take the same path.
@@ -568,6 +559,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
         uint32_t v[32];
         if (extra) {
+          griddep_wait();  // the low-rank values
+          publish();       // the block before this one does not wait for the loads
+          LowBlock low_block;
+          lora_load(p.lora, ttile, (kb - k_blocks) * 4, steps, sel_ftile(tile - ttile * p.nf, p.fcount, p.fbase), r,
+                    ttile * BN + r, low_block);
           const uint32_t xrow = smem_u32(xs + s * X_STAGE_BYTES) + (uint32_t)r * 128u;
 #pragma unroll
           for (int i = 0; i < 8; ++i)  // columns of steps past n are not multiplied

@@ -167,7 +167,12 @@ enum LoraMode : int { LORA_NONE = 0, LORA_DELTA = 1, LORA_BLOCKS = 2 };
 // B1 l1, B1 l2, B1 l3, B2 l1, B2 l2; the one left out, B2 l3, is below 2^-24 of
 // B low.  (Two f16 values of low, with B as it is, keep 22 bits of it above 2^-3
 // only and end at 65504.)
-constexpr int kLowPieces = 5, kLowParts = 3;
+constexpr int kLowPieces = 5;
+// The parts of low that are kept: l1, l2, l3, and the l1 that B2 is multiplied
+// with, zero where low is not finite (an infinite low times a B2 of zero would
+// make a NaN of what is infinite).
+constexpr int kLowParts = 4;
+__host__ __device__ constexpr int low_part(int piece) { return piece < 3 ? piece : piece == 3 ? 3 : 1; }
 struct LoraGemm {
   int mode = LORA_NONE;
   // LORA_BLOCKS: extra k-blocks, laid out for tiles of tile_tokens
@@ -186,7 +191,7 @@ struct LoraGemm {
   int r_pad = 0, n_ftiles = 0;
   const __half* up = nullptr;
   // the low-rank values: LORA_DELTA f32 [tokens][r_pad], LORA_BLOCKS bf16
-  // [r_pad / 16][l1, l2, l3][tokens][16]
+  // [r_pad / 16][kLowParts][tokens][16]
   int tokens = 0;
   const float* low = nullptr;
   const uint4* low_pieces = nullptr;

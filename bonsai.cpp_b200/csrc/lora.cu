@@ -64,8 +64,8 @@ struct ShrinkParams {
 };
 
 // The upper 8 bits of an f32 value's 24, as an f32 value; what is left of it is
-// exact, and after three times nothing (the pieces l1, l2, l3).  All of a value
-// that is not finite is in its first piece.
+// exact, and after three times nothing (the parts l1, l2, l3).  All of a value
+// that is not finite is in its first part.
 __device__ __forceinline__ float cut_piece(float& rest) {
   const float piece = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
   rest = (__float_as_uint(piece) & 0x7f800000u) == 0x7f800000u ? 0.f : rest - piece;
@@ -185,7 +185,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const ShrinkPa
     const int t = t0 + e / R, r = e % R;
     float s = 0.f;
     for (int q = 0; q < csize; ++q) s += cluster.map_shared_rank(red, q)[e];
-    if (r < p.r_pad) p.low[(size_t)t * p.r_pad + r] = info.scale * s;
+    if (r < p.r_pad)  // what x leaves of A's rows past the rank (0 * inf) is no value
+      p.low[(size_t)t * p.r_pad + r] = r < info.rank ? info.scale * s : 0.f;
   }
   cluster.sync();  // no CTA ends while another reads its shared memory
 }
@@ -353,12 +354,16 @@ __global__ void __launch_bounds__(tile::NUM_THREADS)
       b += part[BM];
     }
     if (t >= end) continue;
-    a *= info.scale;
-    b *= info.scale;
+    a = r < info.rank ? a * info.scale : 0.f;  // what x leaves of A's rows past the rank (0 * inf) is no value
+    b = r + 1 < info.rank ? b * info.scale : 0.f;
     uint32_t* dst = p.low_pieces + ((size_t)(r / 16 * kLowParts) * p.tokens + t) * 8 + r % 16 / 2;
-#pragma unroll
-    for (int k = 0; k < kLowParts; ++k)
-      dst[(size_t)k * p.tokens * 8] = __byte_perm(__float_as_uint(cut_piece(a)), __float_as_uint(cut_piece(b)), 0x7632);
+    const size_t part = (size_t)p.tokens * 8;
+    const uint32_t l1 = __byte_perm(__float_as_uint(cut_piece(a)), __float_as_uint(cut_piece(b)), 0x7632);
+    dst[0] = l1;
+    dst[part] = __byte_perm(__float_as_uint(cut_piece(a)), __float_as_uint(cut_piece(b)), 0x7632);
+    dst[2 * part] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+    dst[3 * part] = l1 & (((l1 & 0x7f80u) != 0x7f80u ? 0x0000ffffu : 0u) |
+                          ((l1 & 0x7f800000u) != 0x7f800000u ? 0xffff0000u : 0u));
   }
   cluster.sync();  // no CTA ends while another reads its shared memory
   if (warp == 1) {
