@@ -164,11 +164,15 @@ __device__ __forceinline__ uint32_t bf16_from_f16_scale(uint32_t s16) {
 // 16-column steps of the extra k-blocks of token tile `ttile`.
 template <int kLora>
 __device__ __forceinline__ int lora_steps(const LoraGemm& l, int ttile) {
-  return kLora == LORA_BLOCKS ? kLowPieces * __ldg(l.group_count + ttile) : 0;
+  return kLora == LORA_BLOCKS ? kLowPieces * (__ldg(l.group_count + ttile) & ~kNonfinite) : 0;
 }
 // 128 weight rows x 16 ranks of an adapter's B, contiguous (LoraDevice::up).
 __device__ __forceinline__ const __half* lora_chunk(const LoraGemm& l, int slot, int ftile, int r0) {
   return l.up + (((size_t)slot * l.n_ftiles + ftile) * (l.r_pad / 16) + r0 / 16) * (BM * 16);
+}
+// Which of two f16 values are finite, as a mask.
+__device__ __forceinline__ uint32_t finite_mask(uint32_t h) {
+  return ((h & 0x7c00u) != 0x7c00u ? 0x0000ffffu : 0u) | ((h & 0x7c000000u) != 0x7c000000u ? 0xffff0000u : 0u);
 }
 // B1 or B2 of two f16 values.
 __device__ __forceinline__ uint32_t b_pieces(uint32_t h, bool second) {
@@ -198,12 +202,21 @@ __device__ __forceinline__ void lora_load(const LoraGemm& l, int ttile, int step
   v.n = min(4, steps - step);
   const int4 e0 = __ldg(list);
   const int4 e1 = v.left < v.n ? __ldg(list + 1) : e0;
-  const uint4* w0 = reinterpret_cast<const uint4*>(lora_chunk(l, e0.x, ftile, e0.y) + r * 16);
-  const uint4* w1 = reinterpret_cast<const uint4*>(lora_chunk(l, e1.x, ftile, e1.y) + r * 16);
+  const uint4* w0 = reinterpret_cast<const uint4*>(lora_chunk(l, e0.x & ~kNonfinite, ftile, e0.y) + r * 16);
+  const uint4* w1 = reinterpret_cast<const uint4*>(lora_chunk(l, e1.x & ~kNonfinite, ftile, e1.y) + r * 16);
   v.b[0] = __ldg(w0);
   v.b[1] = __ldg(w0 + 1);
   v.b[2] = __ldg(w1);
   v.b[3] = __ldg(w1 + 1);
+  if ((e0.x | e1.x) & kNonfinite) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v.b[i].x &= finite_mask(v.b[i].x);
+      v.b[i].y &= finite_mask(v.b[i].y);
+      v.b[i].z &= finite_mask(v.b[i].z);
+      v.b[i].w &= finite_mask(v.b[i].w);
+    }
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int part = low_part(i < v.left ? v.first + i : i - v.left);
@@ -226,6 +239,43 @@ __device__ __forceinline__ void lora_weights(const LowBlock& v, int i, uint32_t*
     w[4 * k + 2] = b_pieces(h.z, second);
     w[4 * k + 3] = b_pieces(h.w, second);
   }
+}
+
+// What the products left out: B's values of row `r` that are not finite, for the
+// tokens t0 .. t0 + 31 of their requests.  Off the common path, and kept out of
+// its registers.
+__device__ __noinline__ void lora_add_left_out(const int4* list, int count, const __half* up, int n_ftiles,
+                                               int r_groups, const __nv_bfloat16* low, int tokens, int ftile, int r,
+                                               int t0, float* v) {
+  griddep_wait();  // the low-rank values
+  for (int g = 0; g < count; ++g) {
+    const int4 e = __ldg(list + g);
+    if (!(e.x & kNonfinite)) continue;
+    const __half* b =
+        up + (((size_t)(e.x & ~kNonfinite) * n_ftiles + ftile) * r_groups + e.y / 16) * (BM * 16) + r * 16;
+    for (int c = 0; c < 16; ++c) {
+      const float f = __half2float(b[c]);
+      if (isfinite(f)) continue;
+      for (int t = max(e.z, t0); t < min(e.w, t0 + 32); ++t) {
+        float x = 0.f;
+        for (int part = 2; part >= 0; --part)
+          x += __bfloat162float(__ldcg(low + ((size_t)(e.y / 16 * kLowParts + part) * tokens + t) * 16 + c));
+        v[t - t0] = fmaf(f, x, v[t - t0]);
+      }
+    }
+  }
+}
+__device__ __forceinline__ void lora_add_nonfinite(const LoraGemm& l, int ttile, int ftile, int r, int t0,
+                                                   uint32_t (&v)[32]) {
+  const int count = __ldg(l.group_count + ttile);
+  if (!(count & kNonfinite)) return;
+  float sums[32];
+#pragma unroll
+  for (int j = 0; j < 32; ++j) sums[j] = __uint_as_float(v[j]);
+  lora_add_left_out(l.groups + (size_t)ttile * l.max_groups, count & ~kNonfinite, l.up, l.n_ftiles, l.r_pad / 16,
+                    reinterpret_cast<const __nv_bfloat16*>(l.low_pieces), l.tokens, ftile, r, t0, sums);
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(sums[j]);
 }
 
 // Adapter slot of token t (-1: none).
@@ -698,6 +748,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + ps[j * 128]);
           }
+          lora_add_nonfinite(p.lora, ttile, ftile, q * 32 + (int)lane, t0, v);
         }
         if (warp_swiglu) {
           // Rows are stored gate/value interleaved; the even lane owns the pair.
@@ -1088,6 +1139,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         tmem_wait_ld();
         const int t0 = ttile * BN + c * 32;
         const int nt = min(32, p.tokens - t0);
+        if constexpr (kLora == LORA_BLOCKS)
+          lora_add_nonfinite(p.lora, ttile, row / BM, q * 32 + (int)lane, t0, v);
         if (warp_swiglu) {
           __half* dst = reinterpret_cast<__half*>(sg.dst) + base + (size_t)t0 * stride;
           const bool own = mode == EPI_SWIGLU_F16 && (rr & 1) == 0;

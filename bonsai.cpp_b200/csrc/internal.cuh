@@ -160,6 +160,7 @@ struct TileSel {
 struct LoraSlot {
   int rank = 0;  // 0: no adapter in this slot
   float scale = 0.f;
+  int nonfinite = 0;  // B has a value that is not finite
 };
 enum LoraMode : int { LORA_NONE = 0, LORA_DELTA = 1, LORA_BLOCKS = 2 };
 // LORA_BLOCKS: B low as products of bf16 pieces, which have f32's range: B
@@ -173,12 +174,17 @@ constexpr int kLowPieces = 5;
 // make a NaN of what is infinite).
 constexpr int kLowParts = 4;
 __host__ __device__ constexpr int low_part(int piece) { return piece < 3 ? piece : piece == 3 ? 3 : 1; }
+// B's values that are not finite are zeros to the products, since the zeros of
+// the tile's other requests would not keep them out; the epilogue adds them for
+// the tokens of their own request.  Tiles and groups that have some carry this bit.
+constexpr int kNonfinite = 1 << 30;
 struct LoraGemm {
   int mode = LORA_NONE;
   // LORA_BLOCKS: extra k-blocks, laid out for tiles of tile_tokens
-  // (b1_gemm_tile_tokens).  Token tile i has group_count[i] groups of 16 ranks
-  // {slot, first rank, first token, end token} at groups + i * max_groups,
-  // each of which takes kLowPieces steps of 16 columns.
+  // (b1_gemm_tile_tokens).  Token tile i has group_count[i] (| kNonfinite)
+  // groups of 16 ranks {slot (| kNonfinite), first rank, first token, end token}
+  // at groups + i * max_groups, each of which takes kLowPieces steps of 16
+  // columns.
   const int* group_count = nullptr;
   const int4* groups = nullptr;
   int tile_tokens = 0, max_groups = 0;

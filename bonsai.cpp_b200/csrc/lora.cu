@@ -379,8 +379,12 @@ __global__ void __launch_bounds__(tile::NUM_THREADS)
 __global__ void lora_retile_kernel(const __half* __restrict__ src, LoraSlot info, int n_rows, int n_ftiles, int r_pad,
                                    int swiglu_from, __half* __restrict__ dst, LoraSlot* slot) {
   const int rank = info.rank;
-  if (blockIdx.x == 0 && threadIdx.x == 0) *slot = info;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {  // nonfinite is zero before this kernel
+    slot->rank = rank;
+    slot->scale = info.scale;
+  }
   if (rank == 0) return;
+  bool bad = false;
   const long long total = (long long)n_ftiles * 128 * r_pad;
   for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total;
        i += (long long)gridDim.x * blockDim.x) {
@@ -395,9 +399,11 @@ __global__ void lora_retile_kernel(const __half* __restrict__ src, LoraSlot info
         s = swiglu_from + ((j & 1) ? (n_rows - swiglu_from) / 2 + (j >> 1) : (j >> 1));
       }
       v = src[(size_t)s * rank + r];
+      bad |= (__half_as_ushort(v) & 0x7c00) == 0x7c00;
     }
     dst[i] = v;
   }
+  if (bad) atomicOr(&slot->nonfinite, 1);
 }
 
 // Lists the extra k-blocks of each token tile of the GEMM (LoraGemm): for
@@ -416,15 +422,18 @@ __global__ void lora_plan_kernel(const int* __restrict__ cu, const int* __restri
     const int mid = (lo + hi) / 2;
     if (cu[mid] <= t0) lo = mid; else hi = mid;
   }
-  int base = 0;
+  int base = 0, any_bad = 0;
   for (int i0 = lo; i0 < n_reqs; i0 += 32) {
     const int i = i0 + lane;
-    int slot = -1, n16 = 0, a = t1, b = t1;
+    int slot = -1, n16 = 0, a = t1, b = t1, bad = 0;
     if (i < n_reqs) {
       a = max(t0, cu[i]);
       b = min(t1, cu[i + 1]);
       slot = slots[i];
-      if (a < b && slot >= 0 && slot < n_slots) n16 = (slot_info[slot].rank + 15) / 16;
+      if (a < b && slot >= 0 && slot < n_slots) {
+        n16 = (slot_info[slot].rank + 15) / 16;
+        if (n16 > 0 && slot_info[slot].nonfinite) bad = kNonfinite;
+      }
     }
     int incl = n16;
 #pragma unroll
@@ -434,12 +443,13 @@ __global__ void lora_plan_kernel(const int* __restrict__ cu, const int* __restri
     }
     const int at = base + incl - n16;
     for (int j = 0; j < n16; ++j)
-      if (at + j < max_groups) groups[(size_t)tile * max_groups + at + j] = make_int4(slot, j * 16, a, b);
+      if (at + j < max_groups) groups[(size_t)tile * max_groups + at + j] = make_int4(slot | bad, j * 16, a, b);
     base += __shfl_sync(0xffffffffu, incl, 31);
+    any_bad |= __reduce_or_sync(0xffffffffu, bad);
     // past the tile once one of these 32 requests begins at or after its end
     if (__any_sync(0xffffffffu, i < n_reqs && cu[i] >= t1)) break;
   }
-  if (lane == 0) group_count[tile] = min(base, max_groups);
+  if (lane == 0) group_count[tile] = min(base, max_groups) | any_bad;
 }
 
 int shrink_tiles(const ShrinkParams& p, cudaStream_t st) {
@@ -505,8 +515,11 @@ int lora_tmem_shares(TmemShare* s) {
 int launch_lora_retile(const __half* up, const LoraSlot& info, const LoraDevice& set, int slot, cudaStream_t st) {
   const size_t n = (size_t)set.n_ftiles * 128 * set.r_pad;
   const unsigned blocks = info.rank == 0 ? 1u : (unsigned)std::min<size_t>((n + 255) / 256, 148 * 16);
+  LoraSlot* slot_info = set.info + slot;
+  const cudaError_t e = cudaMemsetAsync(&slot_info->nonfinite, 0, sizeof(int), st);
+  if (e != cudaSuccess) return cuda_status(e, "lora_retile_kernel clear");
   lora::lora_retile_kernel<<<blocks, 256, 0, st>>>(up, info, set.n_rows, set.n_ftiles, set.r_pad, set.swiglu_from,
-                                                   set.up + (size_t)slot * n, set.info + slot);
+                                                   set.up + (size_t)slot * n, slot_info);
   return launch_status("lora_retile_kernel launch");
 }
 

@@ -204,7 +204,9 @@ int bonsai_lora_free(bonsai_lora_t set);
  * [n_reqs + 1], ascending) and the adapter slots[i] (device int32 [n_reqs]);
  * a value outside [0, n_slots) or an empty slot is no adapter, as are tokens
  * of no request.  The low-rank products are held in f32 up to the epilogue's
- * own rounding, over f32's range.  Scratch is stream-ordered. */
+ * own rounding, over f32's range.  A non-finite value of x reaches its own
+ * token only, one of an adapter the tokens of its requests.  Scratch is
+ * stream-ordered. */
 int bonsai_b1_gemm_lora(const uint16_t* x, long long ldx, int tokens, bonsai_b1_t w, int mode,
                         void* out, long long ld_out, const float* gate, bonsai_lora_t set,
                         const int* cu_tokens, const int* slots, int n_reqs, void* stream);
