@@ -74,6 +74,12 @@ constexpr int O_COL = 128;
 constexpr int BAR_BYTES = 512;
 constexpr int EC = 32;    // columns that the epilogue takes at a time through a warp's staging rows
 constexpr float kRescaleThreshold = 8.0f;
+// P is 2^(s - m + kLift): an f16 P reaches 2^15 then, with the threshold, and is
+// zero below 2^-32 of the row's maximum, not 2^-25 (65536 keys of 2^-25.4 beside
+// one of 1 are 0.15 % of the sum).  The factor is in the row's sum too, and the
+// same in every part of a split.
+template <bool kBF16>
+constexpr float kLift = kBF16 ? 0.0f : 7.0f;
 constexpr int kMaxSeqs = 256;     // sequences of one launch (16 bytes each in shared memory)
 constexpr int kMaxCluster = 16;   // CTAs that split a unit's keys and merge in shared memory
 
@@ -719,7 +725,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
             tmem_st32(o_addr + c * 32, r);
           }
         }
-        const float mref = m == -INFINITY ? 0.0f : m;  // no key seen yet: every p is 2^-inf = 0
+        // no key seen yet: every p is 2^-inf = 0
+        const float mref = (m == -INFINITY ? 0.0f : m) - kLift<kBF16>;
         const unsigned long long nm2 = pack2(-mref, -mref);
         unsigned long long sum2[4] = {0ull, 0ull, 0ull, 0ull};
         // P, and its row sum before the rounding
