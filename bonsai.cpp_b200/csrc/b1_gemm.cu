@@ -1463,15 +1463,13 @@ auto single_kernel(bool bf16, int lora) {
 // Largest number of co-resident clusters of `size` CTAs of the LORA_DELTA
 // kernel (a cluster lies within one GPC); 0 if the query fails.
 int delta_cluster_slots(int size) {
-  static int slots[64][9];
-  static bool known[64][9];
-  static std::mutex mu;
-  std::lock_guard<std::mutex> lock(mu);
-  const int d = device_slot();
-  if (known[d][size]) return slots[d][size];
-  known[d][size] = true;
-  auto kern = single_kernel(false, LORA_DELTA);
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, gemm::SMEM_DELTA_BYTES) == cudaSuccess) {
+  static DeviceMemo<9> memo;
+  int slots = 0;
+  memo.get(size, &slots, [&](int* n) {
+    auto kern = single_kernel(false, LORA_DELTA);
+    const cudaError_t e =
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, gemm::SMEM_DELTA_BYTES);
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1483,11 +1481,9 @@ int delta_cluster_slots(int size) {
     cfg.dynamicSmemBytes = gemm::SMEM_DELTA_BYTES;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    int c = 0;
-    if (cudaOccupancyMaxActiveClusters(&c, kern, &cfg) == cudaSuccess) slots[d][size] = c;
-  }
-  cudaGetLastError();
-  return slots[d][size];
+    return cudaOccupancyMaxActiveClusters(n, kern, &cfg);
+  });
+  return slots;
 }
 
 // With a low-rank product, an f32 result of a long K is accumulated in parts
@@ -1505,37 +1501,26 @@ int lora_part(const B1Weight& w, int epi_mode) {
 // Largest number of co-resident pair clusters (one per TPC when every SM
 // takes one CTA of the pair kernel); 0 if the query fails.
 int pair_cluster_slots(bool bf16, int lora) {
-  struct Slots {
-    int n[3] = {-1, -1, -1};
-  };
-  static Slots slots[64];
-  static std::mutex mu;
-  std::lock_guard<std::mutex> lock(mu);
-  int& n = slots[device_slot()].n[lora == LORA_BLOCKS ? 2 : bf16 ? 1 : 0];
-  if (n >= 0) return n;
-  auto k2 = pair_kernel(bf16, lora);
-  n = 0;
-  if (cudaFuncSetAttribute(k2, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           gemm::pair::SMEM_BYTES) != cudaSuccess)
-    return n;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(2 * std::max(1, num_sms() / 2));
-  cfg.blockDim = dim3(gemm::pair::NUM_THREADS);
-  cfg.dynamicSmemBytes = gemm::pair::SMEM_BYTES;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  int c = 0;
-  if (cudaOccupancyMaxActiveClusters(&c, k2, &cfg) != cudaSuccess) {
-    cudaGetLastError();
-    return n;
-  }
-  n = c;
-  return n;
+  static DeviceMemo<3> memo;
+  int slots = 0;
+  memo.get(lora == LORA_BLOCKS ? 2 : bf16 ? 1 : 0, &slots, [&](int* n) {
+    auto k2 = pair_kernel(bf16, lora);
+    const cudaError_t e = cudaFuncSetAttribute(k2, cudaFuncAttributeMaxDynamicSharedMemorySize, gemm::pair::SMEM_BYTES);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(2 * std::max(1, num_sms() / 2));
+    cfg.blockDim = dim3(gemm::pair::NUM_THREADS);
+    cfg.dynamicSmemBytes = gemm::pair::SMEM_BYTES;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaOccupancyMaxActiveClusters(n, k2, &cfg);
+  });
+  return slots;
 }
 
 }  // namespace

@@ -8,6 +8,7 @@
 #include <cstdint>
 #include <cstdio>
 #include <map>
+#include <mutex>
 #include <string>
 #include <vector>
 
@@ -91,6 +92,34 @@ int num_sms();
 // (shared-memory attributes, cluster occupancy) are kept per device, since a
 // process may drive several GPUs.
 int device_slot();
+
+// What a query of the runtime says of a kernel on the current device, asked once
+// per key (< kKeys) and device.  An answer is kept once the query has
+// succeeded; after an error the next call asks again.
+template <int kKeys>
+class DeviceMemo {
+ public:
+  template <typename Query>  // cudaError_t query(int* value)
+  cudaError_t get(int key, int* value, Query query) {
+    std::lock_guard<std::mutex> lock(mu_);
+    const int d = device_slot();
+    if (!known_[d][key]) {
+      const cudaError_t e = query(&value_[d][key]);
+      if (e != cudaSuccess) {
+        cudaGetLastError();  // reported here, not by the next launch
+        return e;
+      }
+      known_[d][key] = true;
+    }
+    *value = value_[d][key];
+    return cudaSuccess;
+  }
+
+ private:
+  std::mutex mu_;
+  bool known_[64][kKeys] = {};
+  int value_[64][kKeys] = {};
+};
 
 // ------------------------------------------------------- B1_0 device weights
 // Device layout ("chunked"): the packed reference layout [N][K/32][6 bytes]

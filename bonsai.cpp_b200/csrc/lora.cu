@@ -27,7 +27,6 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
-#include <mutex>
 
 namespace cg = cooperative_groups;
 
@@ -458,11 +457,11 @@ int shrink_tiles(const ShrinkParams& p, cudaStream_t st) {
   if (!rc)
     rc = encode_tmap_2d_16b(&amap, p.down, (long long)p.n_slots * p.r_pad, p.k_in, p.k_in, tile::BK, 16, false);
   if (rc) return rc;
-  static std::once_flag once[64];
-  cudaError_t e = cudaSuccess;
-  std::call_once(once[device_slot()], [&] {
-    e = cudaFuncSetAttribute(lora_shrink_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             tile::smem_bytes(tile::kMaxRank));
+  static DeviceMemo<1> memo;
+  int set = 0;
+  const cudaError_t e = memo.get(0, &set, [](int*) {
+    return cudaFuncSetAttribute(lora_shrink_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                tile::smem_bytes(tile::kMaxRank));
   });
   if (e != cudaSuccess) return cuda_status(e, "lora shrink set smem attribute");
   const long long seqs = std::min(p.n_reqs, p.tokens);
@@ -481,10 +480,11 @@ int shrink(const ShrinkParams& p, cudaStream_t st) {
   auto kern = lora_shrink_kernel<NT>;
   constexpr int TM = 16;
   constexpr int smem = kWarps * TM * NT * 8 * (int)sizeof(float);
-  static std::once_flag once[64];
-  cudaError_t e = cudaSuccess;
-  std::call_once(once[device_slot()],
-                 [&] { e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+  static DeviceMemo<1> memo;
+  int set = 0;
+  const cudaError_t e = memo.get(0, &set, [&](int*) {
+    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  });
   if (e != cudaSuccess) return cuda_status(e, "lora shrink set smem attribute");
   const long long seqs = std::min(p.n_reqs, p.tokens);
   const long long units = (p.tokens + seqs * (TM - 1)) / TM;

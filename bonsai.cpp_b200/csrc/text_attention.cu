@@ -56,7 +56,6 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
-#include <mutex>
 
 namespace bonsai {
 namespace gemm {
@@ -1021,23 +1020,19 @@ int encode(CUtensorMap* map, void* base, bool bf16, int rank, const long long* d
 }
 
 // Largest number of co-resident clusters of `size` CTAs (a cluster lies within
-// one GPC); 0 if the query fails.  The occupancy query counts one CTA per SM
-// for a kernel that allocates TMEM; two of these fit (256 of the 512 columns,
-// half the shared memory and registers each) and do run.
+// one GPC).  The occupancy query counts one CTA per SM for a kernel that
+// allocates TMEM; two of these fit (256 of the 512 columns, half the shared
+// memory and registers each) and do run.
 template <int HD, bool kBF16, bool kPaged>
-int cluster_slots(int size) {
-  static int slots[64][kMaxCluster + 1];
-  static bool known[64][kMaxCluster + 1];
-  static std::mutex mu;
-  std::lock_guard<std::mutex> lock(mu);
-  const int d = device_slot();
-  if (known[d][size]) return slots[d][size];
-  known[d][size] = true;
-  auto kern = text_attention_kernel<HD, kBF16, kPaged>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD>::SMEM_BYTES) == cudaSuccess &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) ==
-          cudaSuccess &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) {
+cudaError_t cluster_slots(int size, int* slots) {
+  static DeviceMemo<kMaxCluster + 1> memo;
+  return memo.get(size, slots, [&](int* n) {
+    auto kern = text_attention_kernel<HD, kBF16, kPaged>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD>::SMEM_BYTES);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1050,10 +1045,10 @@ int cluster_slots(int size) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int c = 0;
-    if (cudaOccupancyMaxActiveClusters(&c, kern, &cfg) == cudaSuccess) slots[d][size] = 2 * c;
-  }
-  cudaGetLastError();
-  return slots[d][size];
+    e = cudaOccupancyMaxActiveClusters(&c, kern, &cfg);
+    *n = std::min(2 * c, 2 * num_sms() / size);
+    return e;
+  });
 }
 
 template <int HD, bool kBF16, bool kPaged>
@@ -1061,7 +1056,10 @@ int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, 
            int max_ctx, cudaStream_t st) {
   auto kern = text_attention_kernel<HD, kBF16, kPaged>;
   // CTA slots; the query also prepares the kernel for its shared memory
-  const long long slots = cluster_slots<HD, kBF16, kPaged>(1);
+  int one = 0;
+  const cudaError_t e = cluster_slots<HD, kBF16, kPaged>(1, &one);
+  if (e != cudaSuccess) return cuda_status(e, "text attention: occupancy query");
+  const long long slots = one;
   if (slots < 1) return fail(-3, "text attention: the kernel cannot be scheduled on this device");
   // Key split: where the units leave CTA slots empty, each unit's keys are cut
   // into ranges.  Up to kMaxCluster of them are one cluster, as many as fit
@@ -1075,7 +1073,8 @@ int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, 
   want = std::min<long long>(want, kMaxSplits);
   p.splits = (int)want;
   if (p.splits > 1 && p.splits <= kMaxCluster) {
-    while (p.splits > 1 && cluster_slots<HD, kBF16, kPaged>(p.splits) < units) --p.splits;
+    int fit = 0;  // an error counts as none: the split goes through global memory then
+    while (p.splits > 1 && (cluster_slots<HD, kBF16, kPaged>(p.splits, &fit) != cudaSuccess || fit < units)) --p.splits;
     // Clusters pack badly where the wanted split is odd (32 units in 9 ranges:
     // 6 fit, 196 us; 9 ranges through global memory, 168 us).
     p.in_cluster = 5 * p.splits >= 4 * want && p.splits > 1;
