@@ -861,7 +861,6 @@ struct Params {
   EpiSeg seg[kMaxSegs];
   int* err;
   int fence_sys;  // a segment stores to other GPUs: fence.sys after the epilogue's stores
-  int n_rows;
   LoraGemm lora;  // LORA_BLOCKS (ksplit is 1)
 };
 
@@ -1714,7 +1713,6 @@ int launch_b1_gemm(const void* x, long long ldx, int tokens, const B1Weight& w, 
     for (int i = 0; i < nseg; ++i) q.seg[i] = segs[i];
     q.err = device_error_word();
     q.fence_sys = routed ? 1 : 0;
-    q.n_rows = w.n_rows;
     if (lora) q.lora = *lora;
     auto k2 = pair_kernel(x_bf16, lmode);
     cudaLaunchConfig_t cfg = {};

@@ -528,10 +528,23 @@ int launch_b1_gemm_lora(const __half* x, long long ldx, int tokens, const B1Weig
   if (tokens == 0) return 0;
   if (n_reqs == 0) return launch_b1_gemm(x, ldx, tokens, w, &seg, 1, false, st);
   LoraGemm g;
-  // Both forms, 3072 -> 9216, rank 32 (us, few / many): 64 x 1 token 26 / 98,
-  // 1 x 8 18 / 26, 16 x 8 35 / 41, 64 x 4 65 / 61, 16 x 16 63 / 37, 1 x 64 25 /
-  // 23, 64 x 32 464 / 129: the few-form reads B once per token, the other
-  // takes extra k-blocks per request.
+  // The few-form reads B once per token, the other takes extra k-blocks per
+  // request and rank.  Both, few / many in us (calls of a graph), adapters of
+  // its own for each request:
+  //                    3072 -> 9216, f16               3072 -> 3072  9216 -> 3072, f32
+  //   rank             8         32         128        32            32
+  //   64 x 1 token     23 / 89   27 / 149   60 / 616   21 / 147      27 / 182
+  //   64 x 4           52 / 60   65 / 88    166 / 346  37 / 88       81 / 124
+  //   16 x 8           30 / 41   36 / 56    83 / 158   25 / 51       42 / 81
+  //   64 x 8           93 / 63   122 / 92   307 / 304  65 / 60       158 / 98
+  //   16 x 16          51 / 37   64 / 44    153 / 98   36 / 42       76 / 75
+  //   1 x 64           21 / 24   25 / 25    50 / 32    19 / 25       25 / 55
+  //   64 x 32          345 / 116 463 / 152  1159 / 358 179 / 83      438 / 192
+  //   1 x 300, 63 x 1  72 / 91   93 / 146   237 / 550  38 / 144      82 / 183
+  //   1 x 900, 127 x 1 185 / 164 248 / 283  617 / 1060 95 / 254      236 / 370
+  // The average decides, at 8.  Around it either may be the faster, by up to
+  // 1.9 times: the point where they cross falls with the number of requests
+  // and the outputs, which the rule does not look at.
   g.mode = tokens > 8ll * n_reqs ? LORA_BLOCKS : LORA_DELTA;
   // scratch: low (or its pieces), then the lists of extra blocks
   const size_t low_bytes = (size_t)tokens * set.r_pad * (g.mode == LORA_BLOCKS ? 2 * kLowParts : sizeof(float));
