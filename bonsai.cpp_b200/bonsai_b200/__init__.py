@@ -277,6 +277,10 @@ def b1_gemm_lora(x16, w: B1Weight, mode: int, out, lora: LoraSet, cu_tokens, slo
     if out.dtype is not (_text_torch.float16 if f16 else _text_torch.float32) or out.shape != (T, width) \
             or out.get_device() != dev or width > 1 and so[1] != 1:
         raise BonsaiError(f"out {out.dtype} {tuple(out.shape)} does not fit the mode, {T} tokens and {width} outputs")
+    if gate is not None and (gate.dtype is not _text_torch.float32 or gate.get_device() != dev
+                             or gate.numel() < w.out_dim or not gate.is_contiguous()):
+        raise BonsaiError(f"gate must be contiguous f32 of {w.out_dim} values on the current device, "
+                          f"got {gate.dtype} {tuple(gate.shape)} on {gate.device}")
     check(lib().bonsai_b1_gemm_lora(
         x16.data_ptr(), sx[0] if T > 1 else K, T, w.handle, mode, out.data_ptr(), so[0] if T > 1 else width,
         gate.data_ptr() if gate is not None else None, lora.handle, _text_ints(dev, "cu_tokens", cu_tokens),

@@ -542,9 +542,10 @@ int launch_b1_gemm_lora(const __half* x, long long ldx, int tokens, const B1Weig
   //   64 x 32          345 / 116 463 / 152  1159 / 358 179 / 83      438 / 192
   //   1 x 300, 63 x 1  72 / 91   93 / 146   237 / 550  38 / 144      82 / 183
   //   1 x 900, 127 x 1 185 / 164 248 / 283  617 / 1060 95 / 254      236 / 370
-  // The average decides, at 8.  Around it either may be the faster, by up to
-  // 1.9 times: the point where they cross falls with the number of requests
-  // and the outputs, which the rule does not look at.
+  // The average decides, at 8.  Near it either may be the faster, for 64 x 8 by
+  // 1.6 times and for the last row, whose average is 8.03, by 2.7 times the one
+  // that is not taken: the rule does not look at ranks, shapes or the longest
+  // request.
   g.mode = tokens > 8ll * n_reqs ? LORA_BLOCKS : LORA_DELTA;
   // scratch: low (or its pieces), then the lists of extra blocks
   const size_t low_bytes = (size_t)tokens * set.r_pad * (g.mode == LORA_BLOCKS ? 2 * kLowParts : sizeof(float));
