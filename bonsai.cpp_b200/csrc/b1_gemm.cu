@@ -292,10 +292,10 @@ __device__ __forceinline__ int lora_slot(const LoraGemm& l, int t) {
 // LORA_DELTA's first half of the epilogue, for the tokens t = rank + ncta * i
 // of a tile that this CTA finishes: delta[t] = sum_r B[row][r] low[t][r] (f32)
 // into psum [token][128 rows], zeros for the tokens of other CTAs.  Each half
-// of the 256 threads (one row each) takes every second token.  Bound by
-// reading B: every warp keeps DELTA_AHEAD pieces (its rows, 16 ranks of one
-// token) in flight across tokens, as asynchronous copies into a ring of its
-// own.  (Loads into registers, four ahead, were waited for together and took
+// of the 256 threads (one row each) takes every second token.  Bound by the
+// latency of reading B (22 % of DRAM's rate for 64 requests of one token): every
+// warp keeps DELTA_AHEAD pieces (its rows, 16 ranks of one token) in flight
+// across tokens, as asynchronous copies into a ring of its own.  (Loads into registers, four ahead, were waited for together and took
 // three times as long, and so did bulk copies issued by one thread.)
 __device__ __forceinline__ void lora_delta(const LoraGemm& l, float* psum, int2* adapter, float* low, uint8_t* ring,
                                            int rank, int ncta, int et, int ftile, int t0, int nt) {

@@ -8,14 +8,16 @@
 // Two forms, chosen by the tokens per request:
 //   few (decoding): low[t][r] = scale_a * sum_k A_a[r][k] x[t][k] by
 //     lora_shrink_kernel, and the B1_0 GEMM's epilogue warps compute
-//     B_a low while its products run (LORA_DELTA): both are bound by reading
-//     the adapters once.
+//     B_a low while its products run (LORA_DELTA).  Each reads the adapters
+//     once, and both are bound by latency: for the 64 tokens below 15 and 22 % of
+//     DRAM's rate.
 //   many (prompts, images): low by lora_shrink_tile_kernel (tcgen05), and
 //     the B1_0 GEMM takes scale_a B_a low as extra k-blocks of its own
 //     products, listed by lora_plan_kernel: no second pass over y.
 // Measured (B200, a call among others): 64 requests of one token, 3072 -> 9216,
-// ranks 8 to 64: 35 us; 4 requests of about 1100 tokens, 3072 -> 12288: 312 us,
-// 1.11 PFLOP/s, 20 of them the shrink.
+// ranks 8 to 64: 35 us; 4 requests of about 1100 tokens, 3072 -> 12288: 322-328
+// us, 1.06 PFLOP/s, 20 of them the shrink; 24 of 5 to 160 tokens, 9216 -> 3072,
+// f32: 172 us.
 // low stays in f32, and the tensor cores take it and B in pieces that keep all
 // of it (kLowPieces), so nothing between x and the epilogue's own rounding is
 // rounded further, whatever its magnitude.
@@ -105,7 +107,9 @@ __device__ bool find_request(const int* cu, int n, int tokens, int size, int u, 
 // K between them, and their warps split the CTA's share.  x and A go from global memory straight into
 // the fragments of mma.m16n8k16: the order of k within a step is free as long
 // as both operands share it, so each thread takes 8 consecutive k of its row
-// (one 16-byte load) for two steps.  Bound by reading A.  Partial sums meet in shared memory, then across the cluster, in a
+// (one 16-byte load) for two steps.  Bound by latency (12 us, 15 % of DRAM's rate for
+// 64 requests): request, slot, A and x one behind the other, then two barriers of
+// the cluster.  Partial sums meet in shared memory, then across the cluster, in a
 // fixed order.
 template <int NT>  // 8-rank tiles held
 __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const ShrinkParams p) {
@@ -216,7 +220,8 @@ static_assert(1024 + STAGES * (X_BYTES + kMaxRank * BK * 2) + 256 <= kSmemMax &&
 // low of one 128-token tile of one request: x (128 x K) times A^T (K x rank) on
 // the tensor cores.  A cluster's CTAs split K (the tiles of a batch of prompts
 // are too few to fill the GPU otherwise) and add their parts through
-// distributed shared memory in a fixed order.  Bound by reading x.
+// distributed shared memory in a fixed order.  Bound by latency (20-23 us; 15-22 %
+// of DRAM's rate, 6-12 % of the tensor pipe).
 __global__ void __launch_bounds__(tile::NUM_THREADS)
     lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap amap,
                             const ShrinkParams p, int* err) {

@@ -41,10 +41,10 @@
 // P(j) (16-bit pairs) overwrites the first 32 columns of its S.
 //
 // Bounds and measurements (B200, 32 / 8 heads of 128, bf16 unless noted; a call
-// among others): single tokens by HBM, 5.1 TB/s for 64 sequences of 130 to 4000
-// keys (102 us) and 5.7 TB/s for 4 of 30000 to 65536 in f16 (149 us); long
-// prompts by the 64-key Q K^T, whose 192 bytes of shared memory per clock are
-// more than an SM reads, and by the power limit: 10007 tokens 843 us, 973
+// among others, over several boxes): single tokens by HBM, 4.9-5.1 TB/s for 64
+// sequences of 130 to 4000 keys (102-107 us) and 5.4-5.7 TB/s for 4 of 30000 to
+// 65536 in f16 (149-158 us); long prompts by the 64-key Q K^T, whose 192 bytes of shared memory per clock are
+// more than an SM reads, and by the power limit: 10007 tokens 843-853 us, 962-973
 // TFLOP/s; batches of short prompts by the start and end of each unit: 48 of 7
 // to 512 tokens 100 us.  128 rows per CTA, two CTAs per SM, because 256 rows
 // per CTA (half the reads of K and V) measured the same on long prompts (778
