@@ -214,9 +214,9 @@ def _prepare_store(c, g):
 def _prepare_sample(c, g):
     n, v = c["rows"], c["vocab"]
     logits = _randn(g, n, v, std=c["spread"])
-    # a few likely tokens above the bulk; of two at one place the larger, whatever their order
+    # a few likely tokens above the bulk
     at = torch.randint(0, v, (n, 24), device=DEV, generator=g)
-    logits.scatter_reduce_(1, at, _randn(g, n, 24, std=1.5) + 4.5 * c["spread"], "amax")
+    logits.scatter_(1, at, _randn(g, n, 24, std=1.5) + 4.5 * c["spread"])
     if c["masked"]:
         logits[torch.rand(n, v, device=DEV, generator=g) < c["masked"]] = float("-inf")
     t, k, p, m = _settings(c)
