@@ -5,7 +5,10 @@
 //
 // over the cached places j that token t sees.  The codes are turned into exact
 // 16-bit values on their way to the tensor core; scores, statistics and sums are
-// f32, P is rounded to the tensors' type for its product.
+// f32.  P goes to its product as two 16-bit values, its rounding and the rounding of what
+// that leaves (bf16: within 2^-16 of P, f16: 2^-22), so that the output's rounding is the only
+// one to 16 bits (half as many products again: 78 us in place of 74 for 64 single tokens, 89 in
+// place of 85 for long contexts).
 //
 // Few rows (single tokens): the codes decide, every one is read once for all rows
 // of a key/value head, and the products are small: 16 keys x 8 rows of mma.sync per
@@ -21,9 +24,9 @@
 // turn, each through its own ring of asynchronous copies and with its own softmax;
 // they meet once per unit.
 //
-// Measured (B200, 32 / 8 heads of 128): 64 tokens over 130 to 4000 keys, bf16, 8 bits 74 us,
-// 3.7 TB/s (the same over a 16-bit cache 102); 4 over 30000 to 65536, f16, 4 bits 85 us,
-// 2.5 TB/s, and of 8 bits 87, 4.8 TB/s.  Without any arithmetic the same loads take 56,
+// Measured (B200, 32 / 8 heads of 128): 64 tokens over 130 to 4000 keys, bf16, 8 bits 78 us,
+// 3.5 TB/s (the same over a 16-bit cache 102); 4 over 30000 to 65536, f16, 4 bits 89 us,
+// 2.4 TB/s, and of 8 bits 87, 4.8 TB/s.  Without any arithmetic the same loads take 56,
 // 64 and 81 us: 64-byte rows of one head are read 128 bytes at a time (1.6 times the bytes
 // of 4 bits; two heads to a CTA read each once and took 98 us), the rest is 640 (8 bits) and 440 (4 bits)
 // instructions per 16 keys and warp on 16 warps per SM, which issue 0.6 of a cycle, and
@@ -535,7 +538,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) quant_decode_kernel(
               }
             }
         }
-        uint32_t pb[SUBS][NT][2];
+        uint32_t pb[SUBS][NT][2], pl[SUBS][NT][2];  // P rounded, and what that leaves
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           // no key seen yet: every p is 2^-inf = 0
@@ -548,8 +551,11 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) quant_decode_kernel(
             l[n][0] += p0 + p2;
             l[n][1] += p1 + p3;
             // P^T: keys 2t, 2t + 1 (+ 8) of column g
-            pb[b][n][0] = transpose8x8(pack16<kBF16>(p0, p1));
-            pb[b][n][1] = transpose8x8(pack16<kBF16>(p2, p3));
+            const uint32_t x0 = pack16<kBF16>(p0, p1), x1 = pack16<kBF16>(p2, p3);
+            pb[b][n][0] = transpose8x8(x0);
+            pb[b][n][1] = transpose8x8(x1);
+            pl[b][n][0] = transpose8x8(pack16<kBF16>(p0 - low_f32<kBF16>(x0), p1 - high_f32<kBF16>(x0)));
+            pl[b][n][1] = transpose8x8(pack16<kBF16>(p2 - low_f32<kBF16>(x1), p3 - high_f32<kBF16>(x1)));
           }
         }
 
@@ -598,13 +604,19 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) quant_decode_kernel(
                   const uint32_t a0 = sa.template pair<0>(za), a1 = sa.template pair<1>(za);
                   const uint32_t a2 = sb.template pair<0>(zb), a3 = sb.template pair<1>(zb);
 #pragma unroll
-                  for (int n = 0; n < NT; ++n) mma16816<kBF16>(o[n][mt], a0, a1, a2, a3, pb[b][n][0], pb[b][n][1]);
+                  for (int n = 0; n < NT; ++n) {
+                    mma16816<kBF16>(o[n][mt], a0, a1, a2, a3, pb[b][n][0], pb[b][n][1]);
+                    mma16816<kBF16>(o[n][mt], a0, a1, a2, a3, pl[b][n][0], pl[b][n][1]);
+                  }
                 }
                 if constexpr (kFmt == kI4) {
                   const uint32_t a0 = sa.template pair<2>(za), a1 = sa.template pair<3>(za);
                   const uint32_t a2 = sb.template pair<2>(zb), a3 = sb.template pair<3>(zb);
 #pragma unroll
-                  for (int n = 0; n < NT; ++n) mma16816<kBF16>(o[n][mt + 1], a0, a1, a2, a3, pb[b][n][0], pb[b][n][1]);
+                  for (int n = 0; n < NT; ++n) {
+                    mma16816<kBF16>(o[n][mt + 1], a0, a1, a2, a3, pb[b][n][0], pb[b][n][1]);
+                    mma16816<kBF16>(o[n][mt + 1], a0, a1, a2, a3, pl[b][n][0], pl[b][n][1]);
+                  }
                 }
               }
           }

@@ -41,11 +41,14 @@
 // them into the 16-bit tiles that TMA would have brought, warp 8 issues the products,
 // and warp 9 finds the units and asks for Q; every CTA takes an even share of the
 // blocks (Shares) and a second kernel joins the parts of the units that the shares cut.
-// 6 chunks of 33 to 512 tokens over 1000 to 8192 keys take 273 us against 215 over 16 bits:
-// a block of 64 keys and 128 rows costs 3600 instructions (a CTA converts a tile for its
-// own rows only), 50 to 60 % of what the partitions issue in its time.
+// 6 chunks of 33 to 512 tokens over 1000 to 8192 keys take 317 us against 215 over 16 bits:
+// 277 of it with a P of one 16-bit value (the same in its products alone 307, without the second
+// half's products 295), and a block of 64 keys and 128 rows cost 3600 instructions then (a
+// CTA converts a tile for its own rows only), 50 to 60 % of what the partitions issue in its time.
 // TMEM (256 columns): S(even) [0, 64) S(odd) [64, 128) O [128, 128 + HD);
-// P(j) (16-bit pairs) overwrites the first 32 columns of its S.
+// P(j) (16-bit pairs) overwrites the first 32 columns of its S.  Over codes P is two 16-bit
+// values, its rounding and the rounding of what that leaves (within 2^-16 of it in bf16, 2^-22
+// in f16), and has all 64 columns: of each 16 scores the 8 of the one, then the 8 of the other.
 //
 // Bounds and measurements (B200, 32 / 8 heads of 128, bf16 unless noted; a call
 // among others, over several boxes): single tokens by HBM, 4.9-5.1 TB/s for 64
@@ -763,10 +766,12 @@ __global__ void __launch_bounds__(threads_of(kSrc), 2)
       if (!wait_all(&v_fixed[s], (n / RING) & 1) || !wait_all(&p_ready[b], (n >> 1) & 1)) return false;
       tc_fence_after();
 #pragma unroll
-      for (int k16 = 0; k16 < BKV / 16; ++k16)
-        mma_ts_if(leader, tm + O_COL, tm + b * BKV + k16 * 8,
-                  v_desc + (uint64_t)(s * (C::KV_BYTES >> 4) + k16 * (16 * 128 >> 4)), idesc_o,
-                  (j > 0 || k16 > 0) ? 1u : 0u);
+      for (int k16 = 0; k16 < BKV / 16; ++k16) {
+        const uint32_t at = tm + b * BKV + k16 * (kQuant ? 16 : 8);
+        const uint64_t v = v_desc + (uint64_t)(s * (C::KV_BYTES >> 4) + k16 * (16 * 128 >> 4));
+        mma_ts_if(leader, tm + O_COL, at, v, idesc_o, (j > 0 || k16 > 0) ? 1u : 0u);
+        if constexpr (kQuant) mma_ts_if(leader, tm + O_COL, at + 8, v, idesc_o, 1u);
+      }
       tc_commit_if(leader, &pv_done[b]);
       tc_commit_if(leader, &v_empty[s]);
       return true;
@@ -1137,17 +1142,31 @@ __global__ void __launch_bounds__(threads_of(kSrc), 2)
                 if (ch * 32 + c >= left) s[c] = -INFINITY;
             }
           }
-          uint32_t pk[16];
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            float a, b;
+          auto two = [&](int k, float& a, float& b) -> uint32_t {  // scores 2k, 2k + 1 of the half
             unpack2(fma2(pack2(s[ch * AT + 2 * k], s[ch * AT + 2 * k + 1]), sc2, nm2), a, b);
             a = ex2(a);
             b = ex2(b);
             sum2[k & 3] = add2(sum2[k & 3], pack2(a, b));
-            pk[k] = cvt2<kBF16>(a, b);
+            return cvt2<kBF16>(a, b);
+          };
+          uint32_t pk[16];
+          float a, b;
+          if constexpr (kQuant) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                pk[k] = two(8 * h + k, a, b);
+                unpack2(fma2(pack2(quant::low_f32<kBF16>(pk[k]), quant::high_f32<kBF16>(pk[k])), pack2(-1.0f, -1.0f), pack2(a, b)), a, b);
+                pk[8 + k] = cvt2<kBF16>(a, b);
+              }
+              tmem_st16(s_addr + ch * 32 + h * 16, pk);
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) pk[k] = two(k, a, b);
+            tmem_st16(s_addr + ch * 16, pk);
           }
-          tmem_st16(s_addr + ch * 16, pk);
         }
         float a0, a1;
         unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), a0, a1);
