@@ -8,10 +8,12 @@
 //   token: the first index (in the order of indices) whose sum of kept w up to and
 //   with it exceeds u * (sum of kept w)
 //
-// A choice next to a border goes by sums over the whole row, so sums and the weights
-// at borders are f64 (e^z by a table of 2^(j/64) and a polynomial of degree 4, relative
+// A choice next to a border goes by sums over the whole row, so weights and sums
+// are f64 (e^z by a table of 2^(j/64) and a polynomial of degree 4, relative
 // error below 1e-13; f32 weights would move the choice of a flat row of 150000 tokens
-// about once in a hundred), and every sum has a fixed order: results do not depend on the run.
+// about once in a hundred; pairs of f32 within 1e-9 would by some 6e-5 of a token's weight
+// and were no faster, 62 and 67 us in place of 60 and 64 below), and every sum has a fixed
+// order: results do not depend on the run.
 //
 // A cluster of CTAs takes a row, each a range of its tokens, which it reads from
 // memory once and keeps in shared memory for the passes that follow where all rows'
@@ -30,8 +32,8 @@
 // Bounds and measurements (B200): one row of 150001, top-k 50 and top-p 0.9, 18 us
 // (0.1 us of memory): five meetings of a cluster of 16, four passes over 9400
 // tokens a CTA, and code that runs once; 64 rows of 128000 with settings of their own
-// 59 us (5 of memory), 256 rows of 32000 46 us (2.5): the instructions of
-// the passes; 32 flat rows of 150001 cut by p alone 67 us (1.5): two passes with
+// 60 us (5 of memory), 256 rows of 32000 45 us (2.5): the instructions of
+// the passes; 32 flat rows of 150001 cut by p alone 64 us (1.5): two passes with
 // weights.  With every border found in the general way these took 45, 137, 101 and 85 us.
 #include "internal.cuh"
 #include "ptx.cuh"
@@ -348,25 +350,6 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p, int 
     const double sc = __hiloint2double(__double2hiint(s) + ((k >> 6) << 20), __double2loint(s));
     return x == top ? 1.0 : fma(sc, q, sc);
   };
-  // The same for sums of many, within 5e-10 of it: the exponent's fraction in f32
-  // (the difference and its product with 64 / (T ln 2) as pairs of f32), its
-  // polynomial too, the table's value and the sum in f64.  Errors of single weights,
-  // which do not agree in sign, are lost in a sum; f64 throughout takes 14 operations of the pipe that
-  // bounds a pass over flat rows, this three.
-  const float c_hi = (float)per_step, c_lo = (float)(per_step - (double)c_hi);
-  const bool in_f32 = top < INFINITY && top - low < FLT_MAX && c_hi < 1e30f && c_hi > 1e-30f;
-  auto weight_f32 = [&](float x) -> double {
-    const float d = x - top, back = d - x, rest = (x - (d - back)) + (-top - back);
-    const float prod = d * c_hi, more = fmaf(d, c_hi, -prod) + fmaf(d, c_lo, rest * c_hi);
-    const float tk = prod + 12582912.0f;  // rounds to a whole number
-    const int k = __float_as_int(tk) - 0x4b400000;
-    const float f = (prod - (tk - 12582912.0f)) + more;
-    // e^(f ln 2 / 64) - 1
-    const float q = fmaf(fmaf(fmaf(5.7326e-10f, f, 2.11731e-7f), f, 5.8649049e-5f), f, 0.0108304247f) * f;
-    const double s = table[k & 63];
-    const double sc = __hiloint2double(__double2hiint(s) + ((k >> 6) << 20), __double2loint(s));
-    return fma(sc, (double)q, sc);
-  };
   // bins from the top down; the last one also takes what rounding puts past it
   const float span = fminf(top - low, (float)(kDepth * t64));
   const float per_unit = span > 0.0f && top < INFINITY ? fminf((float)NB / span, 1e37f) : 0.0f;
@@ -594,21 +577,16 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p, int 
       int* counter = const_cast<int*>(in_cta(&n_list, 0));
       double m[3] = {0.0, 0.0, 0.0};
       int c[2] = {0, 0};
-      auto gather = [&](auto of) {
+      if (mass_bins)
         for_each([&](float x, int i) {
           const bool in = x >= least_x;
           const int b = in ? bin_of(x) : NB;
           const bool taken = b >= lo_bin && b <= last_bin;
           if (taken) to[atomicAdd(counter, 1)] = composite(x, begin + i);
-          const double w = of(fmaxf(x, least_x));
+          const double w = weight(fmaxf(x, least_x));
           m[0] += b < lo_bin ? w : 0.0;
           m[1] += in && b > last_bin ? w : 0.0;
         });
-      };
-      if (mass_bins && in_f32)
-        gather(weight_f32);
-      else if (mass_bins)
-        gather(weight);
       else
         for_each([&](float x, int i) {
           if (x >= least_x && bin_of(x) <= last_bin) to[atomicAdd(counter, 1)] = composite(x, begin + i);
@@ -1082,13 +1060,10 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p, int 
   // ---- the sum of what stays, and the token
   const float cut_x = cut ? value_of(cut) : -INFINITY;  // the last that is in, and its place
   const int cut_i = cut ? index_of(cut) - begin : 0;
-  auto stays = [&](float x, int i, double& w, auto of) {
+  auto stays = [&](float x, int i, double& w) {
     bool in = x >= least_x && (x > cut_x || (x == cut_x && i <= cut_i));
     if (bin_cut < NB - 1) in = in && bin_of(x) <= bin_cut;
-    const float xx = fmaxf(x, least_x);
-    w = of(xx);
-    // min-p is decided by the f64 weight
-    if (m_cuts && in && !(w < least * (1.0 - 1e-8)) && w < least * (1.0 + 1e-8)) w = weight(xx);
+    w = weight(fmaxf(x, least_x));
     in = in && (!(w < least) || (x == top && begin + i == index_of(best)));
     w = in ? w : 0.0;
     return in;
@@ -1096,20 +1071,14 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p, int 
   // Tokens [i0, i1) of this CTA's, 32 neighbours at a time: the sum of their weights.
   auto mass_of = [&](int i0, int i1) {
     double a[4] = {0.0, 0.0, 0.0, 0.0};
-    auto pass = [&](auto of) {
-      for (int i = i0 + lane; i < i1; i += 128) {
+    for (int i = i0 + lane; i < i1; i += 128) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          double w;
-          stays(i + 32 * k < i1 ? at(i + 32 * k) : -INFINITY, i + 32 * k, w, of);
-          a[k] += w;
-        }
+      for (int k = 0; k < 4; ++k) {
+        double w;
+        stays(i + 32 * k < i1 ? at(i + 32 * k) : -INFINITY, i + 32 * k, w);
+        a[k] += w;
       }
-    };
-    if (in_f32)
-      pass(weight_f32);
-    else
-      pass(weight);
+    }
     return warp_sum((a[0] + a[1]) + (a[2] + a[3]));
   };
   // The first of WARPS parts in which the sum passes the target (from `from` on, which
@@ -1181,7 +1150,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p, int 
     double pick_w = 0.0;
     for (int i = i0; i < i1; i += 32) {
       double w = 0.0;
-      const bool in = i + lane < i1 && stays(at(i + lane), i + lane, w, weight);
+      const bool in = i + lane < i1 && stays(at(i + lane), i + lane, w);
       if (!in) w = 0.0;
       double incl = w;
 #pragma unroll

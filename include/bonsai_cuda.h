@@ -440,10 +440,9 @@ int bonsai_paged_attention_quant(const bonsai_heads_t* q, const bonsai_quant_pag
  *   tokens[r] = the first index, in the order of indices, at which the sum of the
  *   kept w, its own included, exceeds u[r] * (their whole sum), u in [0, 1] (the
  *   last one kept where none does); probs[r] = its w / that sum.
- * Sums are f64 and in a fixed order; weights are f64 at a border and within 5e-10
- * of that where many are summed.  T <= 0 or NaN: the
- * largest logit, the lowest index of equals, probs 1.  A row with nothing above
- * -inf: token -1, probs 0.
+ * Weights are f64, within 1e-13 of e^z, and so are all sums, in a fixed order.
+ * T <= 0 or NaN: the largest logit, the lowest index of equals, probs 1.  A row
+ * with nothing above -inf: token -1, probs 0.
  * temperature, top_k, top_p, min_p: device arrays [rows], NULL: 1, 0, 1, 0 for
  * every row; u: device [rows], NULL: 0; probs may be NULL.  Nothing is allocated. */
 int bonsai_sample_tokens(const void* logits, long long ld, int rows, int vocab, int dtype,
