@@ -529,8 +529,10 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p, int 
       for (int k = 0; k < each_bins; ++k) {
         // (the lowest of several, should rounding make there be any: every CTA has to find the same)
         if (k_cuts && c < (uint32_t)top_k && c + cn[k] >= (uint32_t)top_k) atomicMin(&edge[0], tid * each_bins + k);
-        // a border this near to a bin's end may lie in the next one by the f64 sums
-        const float near = m_total * 0x1p-13f;
+        // A border this near to a bin's end may lie in the next one by the f64 sums: a bin's mass
+        // falls short by up to a unit for each of its tokens, which are 0.97 of `unit` units
+        // or more each, on both sides of the comparison, and f32 adds 2^-16 of it at most.
+        const float near = m_total * fminf(1.0f, 8.0f / unit);
         if (mass_bins && cn[k] && m + ma[k] >= want32 - near) atomicMin(&edge[1], tid * each_bins + k);
         if (mass_bins && cn[k] && m + ma[k] >= want32 + near) atomicMin(&edge[2], tid * each_bins + k);
         c += cn[k];
