@@ -9,7 +9,7 @@
 // largest, so a value is off by at most half of 2^(e - 127), the block's largest
 // by less than one.  e is at least 1, for f16 at least 103: a step of 2^-24, f16's
 // own.  A block of zeros has e = 0 (memory of zeros therefore reads as zeros),
-// one that holds a NaN or an infinity e = 255 and n = 0, and reads as NaN.
+// one that holds a NaN or an infinity e = 255 and n = 0; it reads as NaN, whatever n.
 // A power of two as the scale, because n * 2^k is then exact in f16 and bf16: what
 // a code stands for is the same number in a product of f16, of bf16, or in f32.
 #pragma once
@@ -65,23 +65,23 @@ __device__ __forceinline__ uint32_t lift_exponents(uint32_t e4) {
   const uint32_t some = (((e4 & 0x7f7f7f7fu) + 0x7f7f7f7fu) | e4) & 0x80808080u & ~bytes_of_ones(e4);
   return e4 + (some >> 7) * (kFmt == kI8 ? 6u : 2u);
 }
-// The scales of two (lifted) exponents as a pair of 16-bit values; 0 gives zero,
-// 255 infinity (times n = 0: NaN).
+// The scales of two (lifted) exponents as a pair of 16-bit values; 0 gives zero, 255
+// NaN: in f16 by the lowest bit of the f32, which the rounding of a number takes off.
 template <bool kBF16>
 __device__ __forceinline__ uint32_t scale_pair(uint32_t ea, uint32_t eb) {
   if constexpr (kBF16)
-    return (ea << 7) | (eb << 23);
+    return (ea == 255u ? 0x7fc0u : ea << 7) | (eb == 255u ? 0x7fc00000u : eb << 23);
   else
-    return pack16<false>(__uint_as_float(ea << 23), __uint_as_float(eb << 23));
+    return pack16<false>(__uint_as_float(ea << 23 | 1u), __uint_as_float(eb << 23 | 1u));
 }
-// The same from byte `at` of two words.
+// The same from byte `at` of two words, but infinity for 255 in bf16.
 template <bool kBF16>
 __device__ __forceinline__ uint32_t scale_pair_at(uint32_t wa, uint32_t wb, uint32_t at) {
   if constexpr (kBF16) {
     return (__byte_perm(wa, wb, 0x0400u + at * 0x0101u) & 0x00ff00ffu) << 7;
   } else {
-    const uint32_t top = at * 0x1000u + 0x0444u;  // the byte at the top, zeros below
-    return pack16<false>(__uint_as_float(__byte_perm(wa, 0u, top) >> 1), __uint_as_float(__byte_perm(wb, 0u, top) >> 1));
+    const uint32_t top = at * 0x1000u + 0x0554u;  // the byte at the top, zeros below and the lowest bit
+    return pack16<false>(__uint_as_float(__byte_perm(wa, 2u, top) >> 1), __uint_as_float(__byte_perm(wb, 2u, top) >> 1));
   }
 }
 

@@ -494,6 +494,21 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) quant_decode_kernel(
         else
           scores(std::bool_constant<!kBF16>{});
 
+        // A key or value that is not a number is rare: one look at all of the step's exponents.
+        const bool odd = plain && __any_sync(0xffffffffu, (bytes_of_ones(ek) | (STEP == 32 ? bytes_of_ones(ev) : 0u)) != 0);
+        if (kBF16 && odd) {
+#pragma unroll
+          for (int b = 0; b < SUBS; ++b) {
+            const bool na = bytes_of_ones(__shfl_sync(0xffffffffu, ek, 16 * b + g)) != 0;
+            const bool nb = bytes_of_ones(__shfl_sync(0xffffffffu, ek, 16 * b + g + 8)) != 0;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (k < 2 ? na : nb) sc[b][n][k] = __int_as_float(0x7fffffff);
+          }
+        }
+
         // ---- softmax over the keys: a key past a column's limit counts nothing, whatever it gave
         if (k0 + STEP > lim_min) {
           __syncwarp();  // a branch, not a selection in every step
@@ -562,22 +577,19 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) quant_decode_kernel(
         // ---- O^T += V^T P^T: this lane's dims are [g HD/8, (g + 1) HD/8)
         // A value that is not a number reaches only the columns that see its key: it
         // is zero to the product, 0 * NaN would reach them all.
-        if (plain) {
-          const uint32_t ones = bytes_of_ones(ev);
-          if (__any_sync(0xffffffffu, ones != 0 && (STEP == 32 || lane >= 16))) {
-            for (int k = 0; k < STEP; ++k) {
-              const uint32_t e1 = (__shfl_sync(0xffffffffu, ev, STEP == 32 ? k : 16 + k) >> (8 * v_block)) & 255u;
-              if (e1 == 255u)
+        if (odd) {
+          for (int k = 0; k < STEP; ++k) {
+            const uint32_t e1 = (__shfl_sync(0xffffffffu, ev, STEP == 32 ? k : 16 + k) >> (8 * v_block)) & 255u;
+            if (e1 == 255u)
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+              for (int n = 0; n < NT; ++n)
 #pragma unroll
-                  for (int c = 0; c < 2; ++c)
-                    if (k0 + k < lim[n][c])
+                for (int c = 0; c < 2; ++c)
+                  if (k0 + k < lim[n][c])
 #pragma unroll
-                      for (int i2 = 0; i2 < MT; ++i2) o[n][i2][c] = o[n][i2][c + 2] = __int_as_float(0x7fffffff);
-            }
-            ev &= ~((ones >> 7) * 255u);
+                    for (int i2 = 0; i2 < MT; ++i2) o[n][i2][c] = o[n][i2][c + 2] = __int_as_float(0x7fffffff);
           }
+          ev &= ~((bytes_of_ones(ev) >> 7) * 255u);
         }
         auto values = [&](auto small) {
           constexpr bool kSmall = decltype(small)::value;

@@ -372,8 +372,9 @@ int bonsai_paged_attention(const bonsai_heads_t* q, const bonsai_pages_t* k_cach
  * or 2 (I4), at least 1, for f16 at least 103; n = x * 2^(127 - e), rounded to
  * the nearest (ties to even) and cut to the largest.  A block of zeros has
  * e = 0, so that zeroed memory reads as zeros; a block that holds a NaN or an
- * infinity has e = 255 and reads as NaN.  What is read back is exact in the type
- * that was written (f16 or bf16); a cache is read in the type it was written in. */
+ * infinity has e = 255 and n = 0, and reads as NaN, whatever its n.  What is read
+ * back is exact in the type that was written (f16 or bf16); a cache is read in the
+ * type it was written in. */
 #define BONSAI_CACHE_I8 0
 #define BONSAI_CACHE_I4 1
 
