@@ -148,6 +148,10 @@ struct Scale {
   }
 };
 
+// Blocks of a unit (one where there is no key).  A place may be up to 2^31 - 2: sums with
+// places in them are unsigned.
+__device__ __forceinline__ int blocks_of(int keys) { return max(1, (int)(((unsigned)keys + BLOCK - 1) / BLOCK)); }
+
 // A CTA's run of keys inside one unit, and the unit's shape.
 struct Unit {
   int seq, tile, kvh;
@@ -180,6 +184,7 @@ template <int HD, int kFmt, bool kBF16, int NT>
 __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) quant_decode_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const Params p) {
   using C = Cfg<HD, kFmt, kBF16, NT>;
   constexpr int RB = C::RB, ROWS = C::ROWS, S = C::STAGES, STEP = C::STEP, SUBS = C::SUBS;
+  constexpr unsigned STRIDE = WARPS * STEP;  // keys from a warp's step to its next
   constexpr int KW = RB / 16, VW = RB / 32;  // words of a key that a lane takes of K, of V
   constexpr int KL = KW > 4 ? 4 : KW, KN = KW / KL;  // words of a load, loads
   constexpr int MT = HD / 16;                // steps of the contraction over dims, tiles of O's dims
@@ -226,7 +231,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) quant_decode_kernel(
         x.w = ctx - x.y;
         seq_shape[s] = x;
         if (x.y <= p.max_tokens)
-          v = ((long long)x.y * p.group + ROWS - 1) / ROWS * max(1, (x.z + BLOCK - 1) / BLOCK);
+          v = ((long long)x.y * p.group + ROWS - 1) / ROWS * blocks_of(x.z);
       }
       long long incl = v;
 #pragma unroll
@@ -268,7 +273,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) quant_decode_kernel(
     u.rows = x.y * p.group;
     u.kv_len = x.z;
     u.first = x.w;
-    const int blocks = max(1, (u.kv_len + BLOCK - 1) / BLOCK);
+    const int blocks = blocks_of(u.kv_len);
     const long long base = seq_before[lo] * p.n_kv;
     const int no = (int)((b - base) / blocks);
     u.tile = no / p.n_kv;
@@ -276,14 +281,14 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) quant_decode_kernel(
     const long long begin = base + (long long)no * blocks;
     const int end = (int)min((long long)blocks, b1 - begin);
     u.from = (int)(b - begin) * BLOCK;
-    u.to = min(u.kv_len, end * BLOCK);
+    u.to = (int)min((unsigned)u.kv_len, (unsigned)end * BLOCK);
     u.ends = end == blocks;
     u.last = u.ends ? (int)blockIdx.x : (int)(((begin + blocks) * shares - 1) / all);
     b = begin + end;
     return u;
   };
 
-  // ---- what the warp reads: steps of keys first_key + i WARPS STEP, of the unit in
+  // ---- what the warp reads: steps of keys first_key + i STRIDE, of the unit in
   // hand or, from its last step on, of the next one
   const int mask = (1 << p.c.page_shift) - 1;
   const int boxes = STEP / p.box, my_box = lane % boxes;  // a step is `boxes` copies of each side; lane l has the page of box l % boxes
@@ -292,11 +297,12 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) quant_decode_kernel(
   const bool of_v = STEP == 16 && lane >= 16;
   const long long ke_page = of_v ? p.c.v.s_page : p.c.k.s_page;
   const int ke_token = (int)(of_v ? p.c.v.s_token : p.c.k.s_token);
-  int first_key = 0, to = 0, steps = 0, kvh = 0;
+  unsigned first_key = 0, to = 0;
+  int steps = 0, kvh = 0;
   const int* table = nullptr;
   const uint8_t *ke = nullptr, *ve = nullptr;
   auto pages = [&](int i) -> int {
-    const int k = first_key + i * (WARPS * STEP) + my_box * p.box;
+    const unsigned k = first_key + i * STRIDE + my_box * p.box;
     return k < to ? __ldg(table + (k >> p.c.page_shift)) : -1;
   };
   auto read_exps = [&](const uint8_t* src) -> uint32_t {
@@ -308,7 +314,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) quant_decode_kernel(
   // Asks for the codes of step i.  A page outside the cache reads as zeros.
   auto ask = [&](int i, int page) {
     if (i < steps) {
-      const int slot = (first_key + i * (WARPS * STEP)) & mask;
+      const int slot = (int)(first_key + i * STRIDE) & mask;
       const uint32_t dst = ring + put * (2 * C::TILE);
       if (boxes == 1) {  // the page is lane 0's own
         if (lane == 0) {
@@ -332,10 +338,10 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) quant_decode_kernel(
   // The lane's exponents of step i (of K, and of V where it has both).
   auto ask_exps = [&](int i, int page, uint32_t& e0, uint32_t& e1) {
     e0 = e1 = 0;
-    const int k = first_key + i * (WARPS * STEP) + e_row;
+    const unsigned k = first_key + i * STRIDE + e_row;
     const int pg = __shfl_sync(0xffffffffu, page, e_box);
     if (k < to && (unsigned)pg < (unsigned)p.c.n_pages) {
-      const int slot = k & mask;
+      const int slot = (int)k & mask;
       e0 = read_exps(ke + pg * ke_page + (long long)slot * ke_token);
       if (STEP == 32) e1 = read_exps(ve + pg * p.c.v.s_page + (long long)slot * (int)p.c.v.s_token);
     }
@@ -347,7 +353,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) quant_decode_kernel(
     first_key = u.from + warp * STEP;
     to = u.to;
     kvh = u.kvh;
-    steps = to > first_key ? (to - first_key + WARPS * STEP - 1) / (WARPS * STEP) : 0;
+    steps = to > first_key ? (int)((to - first_key + STRIDE - 1) / STRIDE) : 0;
     table = p.c.table + (size_t)u.seq * p.c.table_ld;
     ke = of_v ? p.c.v.scales + kvh * p.c.v.s_head : p.c.k.scales + kvh * p.c.k.s_head;
     ve = p.c.v.scales + kvh * p.c.v.s_head;
@@ -438,7 +444,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) quant_decode_kernel(
 #pragma unroll 1
     for (int i = 0; i < steps; ++i) {
       {
-        const int k0 = first_key + i * (WARPS * STEP);
+        const unsigned k0 = first_key + i * STRIDE;
         const uint32_t kt = ring + got * (2 * C::TILE) + k_at, vt = ring + got * (2 * C::TILE) + C::TILE + v_at;
         const uint32_t ek = lift_exponents<kFmt, kBF16>(ex0);
         uint32_t ev = STEP == 32 ? lift_exponents<kFmt, kBF16>(ex1) : ek;
@@ -510,7 +516,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) quant_decode_kernel(
         }
 
         // ---- softmax over the keys: a key past a column's limit counts nothing, whatever it gave
-        if (k0 + STEP > lim_min) {
+        if (k0 + STEP > (unsigned)lim_min) {
           __syncwarp();  // a branch, not a selection in every step
 #pragma unroll
           for (int b = 0; b < SUBS; ++b)
@@ -518,7 +524,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) quant_decode_kernel(
             for (int n = 0; n < NT; ++n)
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                if (k0 + 16 * b + g + (k >> 1) * 8 >= lim[n][k & 1]) sc[b][n][k] = -INFINITY;
+                if (k0 + 16 * b + g + (k >> 1) * 8 >= (unsigned)lim[n][k & 1]) sc[b][n][k] = -INFINITY;
         }
         float mx[NT][2];
         bool move = false;
@@ -585,7 +591,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) quant_decode_kernel(
               for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
-                  if (k0 + k < lim[n][c])
+                  if (k0 + k < (unsigned)lim[n][c])
 #pragma unroll
                     for (int i2 = 0; i2 < MT; ++i2) o[n][i2][c] = o[n][i2][c + 2] = __int_as_float(0x7fffffff);
           }

@@ -843,7 +843,7 @@ __global__ void __launch_bounds__(threads_of(kSrc), 2)
         u.n_tok = min(p.tile_tokens, s.q_len - u.t0);
         u.first = s.before + u.t0;
         u.lim_min = keys_seen(u, p.causal, 0);
-        const int blocks = (keys_seen(u, p.causal, u.n_tok - 1) + BKV - 1) / BKV;
+        const int blocks = (int)(((unsigned)keys_seen(u, p.causal, u.n_tok - 1) + BKV - 1) / BKV);
         if constexpr (kQuant) {
           const int taken = min(shares.length - shares.at, shares.left), past = shares.length - shares.at - taken;
           u.j0 = max(0, shares.at - kStart);
@@ -1186,7 +1186,7 @@ __global__ void __launch_bounds__(threads_of(kSrc), 2)
         const float inv_l = l == 0.0f ? 0.0f : 1.0f / l;  // no key in this range: zeros
         const bool repair = nonfinite[i & 1] != 0 && valid;
         // keys that only some rows see, within this CTA's range
-        const int from = kQuant ? u.j0 * BKV : max(u.lim_min, (u.j0 + u.jb) * BKV), to = min(lim, (u.j0 + u.nkv) * BKV);
+        const int from = kQuant ? u.j0 * BKV : max(u.lim_min, (u.j0 + u.jb) * BKV), to = (int)min((unsigned)lim, (unsigned)(u.j0 + u.nkv) * BKV);
         if (!kQuant && p.in_cluster && valid) stats[row] = make_float2(l == 0.0f ? -INFINITY : m + log2f(l), 0.f);
         constexpr int PIECES = EC / 8;  // 16-byte pieces of a staged row
         // where the rows that this lane helps to write begin (null: no row)
