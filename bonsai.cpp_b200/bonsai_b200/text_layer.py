@@ -118,7 +118,8 @@ def generate(layer, embedding, head, prompts, steps, u, temperature=None, top_k=
     """Tokens int32 [requests][steps] that follow the prompts (lists of tokens): each
     prompt as a whole, then one token at a time behind the cache.  embedding f16
     [vocab][hidden], head a B1Weight [vocab][hidden], u f32 [steps][requests] the
-    random numbers, settings as ``sample_tokens`` takes them."""
+    random numbers, settings as ``sample_tokens`` takes them.  A request whose logits leave
+    nothing to choose (token -1) has -1 from there on."""
     import torch
     n, lens = len(prompts), [len(x) for x in prompts]
     if n == 0 or min(lens) == 0 or steps < 1:
@@ -141,9 +142,11 @@ def generate(layer, embedding, head, prompts, steps, u, temperature=None, top_k=
     for i in range(steps):
         bb.b1_gemm(h.half().contiguous(), head, bb.BONSAI_EPI_F32, logits)
         bb.sample_tokens(logits, u[i], tokens[i], temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        if i:
+            tokens[i].masked_fill_(tokens[i - 1] < 0, -1)
         if i + 1 < steps:
             ctx = ctx + 1
-            h = layer.forward(embedding[tokens[i].long()].float(), ones, ctx, table, slots, max_ctx=max(lens) + steps, max_q=1)
+            h = layer.forward(embedding[tokens[i].clamp(min=0).long()].float(), ones, ctx, table, slots, max_ctx=max(lens) + steps, max_q=1)
     return tokens.t().contiguous()
 
 
