@@ -129,6 +129,12 @@ def generate(layer, embedding, head, prompts, steps, u, temperature=None, top_k=
         raise bb.BonsaiError(f"{n} requests of up to {max(lens) + steps} tokens need {need} pages, not {layer.k_cache.shape[0]}")
     if tuple(u.shape) != (steps, n):
         raise bb.BonsaiError(f"u must be [{steps}][{n}], got {tuple(u.shape)}")
+    # a row past the embedding's end would be a fault on the device
+    rows = embedding.shape[0]
+    if embedding.dim() != 2 or embedding.shape[1] != layer.hidden or rows < head.out_dim or head.in_dim != layer.hidden:
+        raise bb.BonsaiError(f"embedding {tuple(embedding.shape)} and head [{head.out_dim}][{head.in_dim}] do not fit a layer of {layer.hidden}")
+    if not all(0 <= t < rows for x in prompts for t in x):
+        raise bb.BonsaiError(f"a prompt has a token outside the embedding's {rows}")
     ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
     per = -(-(max(lens) + steps) // layer.page_size)
     table = torch.arange(n * per, dtype=torch.int32, device="cuda").view(n, per)
