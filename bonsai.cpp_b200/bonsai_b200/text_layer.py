@@ -135,6 +135,9 @@ def generate(layer, embedding, head, prompts, steps, u, temperature=None, top_k=
         raise bb.BonsaiError(f"embedding {tuple(embedding.shape)} and head [{head.out_dim}][{head.in_dim}] do not fit a layer of {layer.hidden}")
     if not all(0 <= t < rows for x in prompts for t in x):
         raise bb.BonsaiError(f"a prompt has a token outside the embedding's {rows}")
+    if u.dtype is not torch.float32 or not u.is_cuda:  # found by the first choice only when the prompts are in the cache
+        raise bb.BonsaiError(f"u must be f32 on the device, got {u.dtype} on {u.device}")
+    u = u.contiguous()
     ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
     per = -(-(max(lens) + steps) // layer.page_size)
     table = torch.arange(n * per, dtype=torch.int32, device="cuda").view(n, per)
