@@ -842,6 +842,9 @@ int launch_quant_attention(const QuantAttention& a, cudaStream_t st) {
   p.out_token = a.out.token * 2;
   p.out_head = a.out.head * 2;
   p.err = device_error_word();
+  const double row = (a.format == kI8 ? a.head_dim : a.head_dim / 2) + a.head_dim / kBlock;
+  ProfScope prof("paged_attention_quant", 0.0,
+                 2.0 * a.n_kv * a.n_seqs * (double)a.max_ctx * row + 4.0 * a.head_dim * a.total_q * a.n_heads, st);
   // Sequences of up to kFewRows rows (tokens x heads of the group) go to the
   // kernel above; the longer ones, where the caller's bound lets there be any, to
   // the tiles of 128 rows of text_attention.cu.
@@ -875,9 +878,6 @@ int launch_quant_attention(const QuantAttention& a, cudaStream_t st) {
     const int rc = launch_text_attention(t, st);
     if (rc) return rc;
   }
-  const double row = (a.format == kI8 ? a.head_dim : a.head_dim / 2) + a.head_dim / kBlock;
-  ProfScope prof("paged_attention_quant", 0.0,
-                 2.0 * a.n_kv * a.n_seqs * (double)a.max_ctx * row + 4.0 * a.head_dim * a.total_q * a.n_heads, st);
   for (int s0 = 0; s0 < a.n_seqs; s0 += kMaxSeqs) {
     p.n_seqs = std::min(kMaxSeqs, a.n_seqs - s0);
     p.cu = a.cu + s0;

@@ -67,6 +67,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <optional>
 
 namespace bonsai {
 namespace gemm {
@@ -1592,10 +1593,12 @@ int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, 
   }
   // Work as far as the host knows it: the lengths are on the device, so the
   // products are not counted, and a cache counts as max_ctx keys per sequence.
+  // Over codes launch_quant_attention counts the call as a whole.
   const double keys = kPaged ? (double)p.n_seqs * max_ctx : (double)p.total_q;
-  const double row = kSrc == kCodes8 ? HD + HD / 32 : kSrc == kCodes4 ? HD / 2 + HD / 32 : 2 * HD;
-  ProfScope prof(from_codes(kSrc) ? "paged_attention_quant" : kPaged ? "paged_attention" : "prompt_attention", 0.0,
-                 4.0 * HD * p.total_q * p.n_heads + 2.0 * row * keys * p.n_kv, st);
+  std::optional<ProfScope> prof;
+  if (!from_codes(kSrc))
+    prof.emplace(kPaged ? "paged_attention" : "prompt_attention", 0.0,
+                 4.0 * HD * p.total_q * p.n_heads + 2.0 * (2 * HD) * keys * p.n_kv, st);
   int rc = launch_after("text_attention_kernel launch", kern, dim3((unsigned)ctas), dim3(threads_of(kSrc)),
                         smem_of<HD>(kSrc), p.in_cluster ? p.splits : 1, st, qm, km, vm, p);
   if (rc == 0 && from_codes(kSrc)) {
