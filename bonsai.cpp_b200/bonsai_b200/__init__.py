@@ -604,7 +604,7 @@ def paged_attention_quant(q, k_cache: QuantPages, v_cache: QuantPages, page_tabl
 def sample_tokens(logits, u, tokens, probs=None, temperature=None, top_k=None, top_p=None, min_p=None,
                   stream=None) -> None:
     """The next token of each row of logits [rows][vocab] (f16, bf16 or f32, rows
-    with any stride): tokens int32 [rows], probs f32 [rows] or None.  u f32 [rows]
+    that do not overlap): tokens int32 [rows], probs f32 [rows] or None.  u f32 [rows]
     are the random numbers; temperature, top_p, min_p f32 [rows] and top_k int32
     [rows] the rows' settings (None: 1, 1, 0, 0).  The rule, ties and special values
     are at bonsai_sample_tokens in include/bonsai_cuda.h."""
