@@ -16,8 +16,8 @@
 // order: results do not depend on the run.
 //
 // A cluster of CTAs takes a row, each a range of its tokens, which it reads from
-// memory once and keeps in shared memory for the passes that follow where all rows'
-// CTAs find room at once; what a pass finds meets through distributed shared memory.
+// memory once and keeps in shared memory for the passes that follow where that leaves
+// room for a second CTA or none is needed; what a pass finds meets through distributed shared memory.
 // Nothing is sorted but the few candidates at a border.  A histogram over l (2048 bins
 // between the largest and the smallest logit that counts) gives the bin in which the
 // k-th token (by counts, exactly), the mass p (by f32 masses, verified against the f64
@@ -1236,11 +1236,14 @@ int launch_sample_tokens(const Sampling& a, cudaStream_t st) {
   while (ctas < kMaxCluster && ((long long)a.rows * ctas * 2 <= 2 * num_sms() && a.vocab / (2 * ctas) >= 1024)) ctas *= 2;
   while (ctas < kMaxCluster && (long long)share(ctas) * width + 32 > kMaxKept) ctas *= 2;
   p.per = share(ctas);
-  // Rows stay in shared memory where that leaves all CTAs room at once, or where
-  // they would not have it without, either.
+  // Rows stay in shared memory where that leaves an SM room for two CTAs, or each CTA has an SM
+  // to itself: one row of 150001 (top-k 40, top-p 0.9 / p alone) 22.5 / 43 us, read from L2 again for
+  // every pass 24.6 / 47; 400 of 32000, f16, 49.1 / 113 and 49.2 / 115.  Where the row takes the
+  // second CTA's room, the other way around: 64 rows of 128000 53 / 113 kept and 41 / 90 not, 400 of
+  // 50000, f16, 80 / 199 and 68 / 168, 1000 of 32000 148 / 322 and 117 / 252.
   const long long bytes = (long long)p.per * width + 32, all = (long long)a.rows * ctas;
-  const long long fit = std::min<long long>(2, kSmemPerSm / (FIXED + bytes + 4096));
-  const bool kept = bytes <= kMaxKept && (all <= fit * num_sms() || all > 2ll * num_sms());
+  const bool two = 2 * (FIXED + bytes + 4096) <= kSmemPerSm;
+  const bool kept = bytes <= kMaxKept && (two || all <= num_sms());
   const size_t smem = FIXED + (kept ? (size_t)bytes : 0);
   ProfScope prof("sample_tokens", 0.0, (double)a.rows * a.vocab * width, st);
   if (a.rows > 0x7fffffff / kMaxCluster) return fail(-2, "sample_tokens: too many rows in one call");
