@@ -28,12 +28,14 @@
 // 3.5 TB/s (the same over a 16-bit cache 102); 4 over 30000 to 65536, f16, 4 bits 89 us,
 // 2.4 TB/s, and of 8 bits 87, 4.8 TB/s.  Without any arithmetic the same loads take 56,
 // 64 and 81 us: 64-byte rows of one head are read 128 bytes at a time (1.6 times the bytes
-// of 4 bits; two heads to a CTA read each once and took 98 us), the rest is 640 (8 bits) and 440 (4 bits)
-// instructions per 16 keys and warp on 16 warps per SM, which issue 0.6 of a cycle, and
-// 3 to 5 us from one unit to the next.  Tried and not kept: asynchronous copies of 16 bytes in TMA's
+// of 4 bits; two heads to a CTA read each once and took 98 us).  The rest is what waits for them
+// more than instructions, 640 (8 bits) and 440 (4 bits) per 16 keys and warp: without the conversion
+// of the codes, 30 and 42 % of all, 71 in place of 74 and 74 in place of 85, without the exponents'
+// reading or the softmax (an eighth) 69 (P of one 16-bit value in all of these); and 3 to 5 us
+// from one unit to the next.  Tried and not kept: asynchronous copies of 16 bytes in TMA's
 // place (91 and 86), three stages unrolled (111 and 101), unequal shares for the two CTAs of an
 // SM (79 to 89), two chains of products per score (75 and 87), Q asked for before the warps
-// meet (83 and 94: it spills).
+// meet (83 and 94).
 #include "quant.cuh"
 #include "ptx.cuh"
 
@@ -51,7 +53,11 @@ namespace quant {
 constexpr int WARPS = 8, THREADS = WARPS * 32;
 constexpr int BLOCK = 128;            // keys: the grain of the cut
 constexpr int kMaxSeqs = 512;         // sequences of one launch (24 bytes each in shared memory)
-constexpr int kFewRows = 16;          // rows of a sequence that this kernel takes beside the other
+// Rows (tokens x heads of a group) of a sequence that this kernel takes where there are longer ones,
+// two tiles of 8: 64 sequences of 16 rows over 1000 keys 83 us, by the other kernel 98, 8 over 8000
+// 67 and 91; of 32 rows 134 and 98, 105 and 90.  (A call of one sequence of 32 rows over 900 keys
+// would be better off here, 23 and 34.)
+constexpr int kFewRows = 16;
 constexpr float kRescaleThreshold = 8.0f;
 // P is 2^(s - m + kLift): an f16 P uses the type's range (with the threshold it
 // reaches 2^15), so that weights down to 2^-32 of the largest count.

@@ -83,7 +83,7 @@ constexpr int WARP_MMA = 4, WARP_TMA = 5, WARP_FIX = 6;
 enum Source : int { kPacked = 0, kPages = 1, kCodes8 = 2, kCodes4 = 3 };
 // Codes are turned into 16-bit tiles by four warps (Q is left to the warp that finds the
 // units), one on each of the SM's partitions, which have the warps by number modulo 4
-// (six chunks of 33 to 512 tokens over 1000 to 8192: 273 us; 325 with two of them on one
+// (six chunks of 33 to 512 tokens over 1000 to 8192, P of one 16-bit value: 277 us; 325 with two of them on one
 // partition and none on another, which issued 71 and 24 % of their cycles).  Ten warps to a
 // CTA leave 96 registers a thread, so the softmax reads its scores twice, for the maximum
 // and for the exponentials; two such warps and 128 registers were slower yet (330 against 306
@@ -346,8 +346,10 @@ struct Finder {
 // CTAs waited for those with the longest: 3 chunks of 100 to 400 tokens beside 37 single ones, 75
 // blocks where an even share is 25, 176 to 205 us against 132, 3 x 64 tokens over 30000
 // 287 against 172, 6 chunks of 33 to 512 336 against 270.  Where there is no more than a
-// unit for a CTA and none is much longer than a share, units stay whole (8 x 40 to 200
-// tokens over 200 to 500: 30 us, cut 36).
+// unit for a CTA and none is much longer than a share, units stay whole.
+// Measured for both constants (us, L2 flushed): kStart 1, 3, 6: 4 x 128 tokens over 2000
+// keys 65, 65, 67, 16 x 32 over 1500 59, 59, 63, 3 x 64 over 30000 200, 196, 202; kCut 0, 6, 12, 30: 8 x 40 to
+// 200 over 200 to 500 49, 40, 40, 40, 2 x 64 over 300 34, 30, 30, 30, 4 x 128 over 2000 65, 65, 65, 75.
 constexpr int kStart = 3;  // what a unit's beginning and end cost, in blocks
 constexpr int kCut = 6;    // and a cut, with the second kernel
 struct Shares {
