@@ -418,7 +418,8 @@ int bonsai_paged_read_quant(const bonsai_quant_pages_t* k_cache,
  * (dtype).  max_q: an upper bound of the new tokens of a sequence; like max_ctx
  * it only sets how the work is done, a wrong one costs time, not correctness.  A
  * block of values that is not a number reaches only the rows that see its
- * token.  Everything else as there. */
+ * token.  Weights enter their product within 2^-16 (bf16) or 2^-22 (f16); only the
+ * output is rounded to dtype.  Everything else as there. */
 int bonsai_paged_attention_quant(const bonsai_heads_t* q, const bonsai_quant_pages_t* k_cache,
                                  const bonsai_quant_pages_t* v_cache, const int* page_table,
                                  long long table_ld, int table_width, const int* cu_q,
