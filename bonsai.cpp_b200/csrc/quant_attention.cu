@@ -360,6 +360,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) quant_decode_kernel(
     to = u.to;
     kvh = u.kvh;
     steps = to > first_key ? (int)((to - first_key + STRIDE - 1) / STRIDE) : 0;
+    if (__any_sync(0xffffffffu, *abort_flag)) steps = 0;  // a stage may still be on its way: it is not asked for again
     table = p.c.table + (size_t)u.seq * p.c.table_ld;
     ke = of_v ? p.c.v.scales + kvh * p.c.v.s_head : p.c.k.scales + kvh * p.c.k.s_head;
     ve = p.c.v.scales + kvh * p.c.v.s_head;
