@@ -7,7 +7,7 @@
 // 16-bit values on their way to the tensor core; scores, statistics and sums are
 // f32.  P goes to its product as two 16-bit values, its rounding and the rounding of what
 // that leaves (bf16: within 2^-16 of P, f16: 2^-22), so that the output's rounding is the only
-// one to 16 bits (half as many products again: 78 us in place of 74 for 64 single tokens, 89 in
+// one to 16 bits (half as many products again: 78 us in place of 74 for 64 single tokens, 90 in
 // place of 85 for long contexts).
 //
 // Few rows (single tokens): the codes decide, every one is read once for all rows
@@ -25,7 +25,7 @@
 // they meet once per unit.
 //
 // Measured (B200, 32 / 8 heads of 128): 64 tokens over 130 to 4000 keys, bf16, 8 bits 78 us,
-// 3.5 TB/s (the same over a 16-bit cache 102); 4 over 30000 to 65536, f16, 4 bits 89 us,
+// 3.5 TB/s (the same over a 16-bit cache 102); 4 over 30000 to 65536, f16, 4 bits 90 us,
 // 2.4 TB/s, and of 8 bits 87, 4.8 TB/s.  Without any arithmetic the same loads take 56,
 // 64 and 81 us: 64-byte rows of one head are read 128 bytes at a time (1.6 times the bytes
 // of 4 bits; two heads to a CTA read each once and took 98 us).  The rest is what waits for them
