@@ -26,7 +26,7 @@
 //
 // Measured (B200, 32 / 8 heads of 128): 64 tokens over 130 to 4000 keys, bf16, 8 bits 78 us,
 // 3.5 TB/s (the same over a 16-bit cache 102); 4 over 30000 to 65536, f16, 4 bits 90 us,
-// 2.4 TB/s, and of 8 bits 87, 4.8 TB/s.  Without any arithmetic the same loads take 56,
+// 2.4 TB/s, and of 8 bits 96, 4.4 TB/s.  Without any arithmetic the same loads take 56,
 // 64 and 81 us: 64-byte rows of one head are read 128 bytes at a time (1.6 times the bytes
 // of 4 bits; two heads to a CTA read each once and took 98 us).  The rest is what waits for them
 // more than instructions, 640 (8 bits) and 440 (4 bits) per 16 keys and warp: without the conversion
